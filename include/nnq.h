@@ -69,7 +69,8 @@ typedef enum nnq_format {
     NNQ_FMT_Q8_0 = 8,
     NNQ_FMT_Q4_K = 12,
     NNQ_FMT_Q6_K = 14,
-    NNQ_FMT_MXFP4 = 39
+    NNQ_FMT_MXFP4 = 39,
+    NNQ_FMT_INT4G = 1000 /* 4-bit codes with group scales (nnq_weight_create_int4); no GGUF type */
 } nnq_format;
 
 /* Byte layouts.  The reference carries more than one decoder per format:
@@ -81,12 +82,14 @@ typedef enum nnq_format {
  *                     the HIGH nibble = even element, E8M0 scales in a separate array, byte 0 -> 2^-126.
  *  NNQ_LAYOUT_OCP     nn-core Mxfp4Block (crates/nn-core/src/layers/quantized/mxfp4.rs:70-84,177-244):
  *                     17-byte blocks [shared_exp][16 packed] along the flattened order, the LOW nibble =
- *                     even element, scale 2^(shared_exp - 127) with byte 0 -> 2^-127. */
+ *                     even element, scale 2^(shared_exp - 127) with byte 0 -> 2^-127.
+ *  NNQ_LAYOUT_GROUPS  NNQ_FMT_INT4G: codes, scales and zero points in arrays of their own. */
 typedef enum nnq_layout {
     NNQ_LAYOUT_GGUF = 0,
     NNQ_LAYOUT_NN_GGUF = 1,
     NNQ_LAYOUT_GPTOSS = 2,
-    NNQ_LAYOUT_OCP = 3
+    NNQ_LAYOUT_OCP = 3,
+    NNQ_LAYOUT_GROUPS = 4
 } nnq_layout;
 
 typedef enum nnq_dtype {
@@ -140,6 +143,20 @@ int nnq_release_capture_workspaces(void);
  * block storage (crates/nn-core/src/layers/quantized/linear.rs:309-346). */
 int nnq_weight_create(nnq_format fmt, nnq_layout layout, const uint8_t *bytes, size_t nbytes, int64_t n,
                       int64_t k, nnq_weight **out);
+
+/* Upload 4-bit codes with a scale (and optionally a zero point) for every `group`
+ * consecutive weights of a row, the form of 4-bit checkpoints outside GGUF:
+ *   W[r][j] = (code[r][j] - zero[r][j / group]) * scale[r][j / group].
+ * Host arrays, row-major: codes [n, k / 2], two to a byte with the even column in the low
+ * half; scales [n, k / group], NNQ_F16 or NNQ_BF16 bits; zeros [n, k / group], one byte
+ * each from 0 to 16, or NULL for 8 throughout (symmetric codes).  group is 32, 64 or 128 and
+ * k a multiple of it (NNQ_ERR_INVALID_SHAPE); a zero point over 16 is
+ * NNQ_ERR_INVALID_ARGUMENT, a scale that is not finite NNQ_ERR_NON_FINITE.  Columns are in
+ * order (an activation-ordered checkpoint is sorted, and its input permuted, by the caller).
+ * The weight works in every call that takes an nnq_weight.  No counterpart in the
+ * reference, whose 4-bit weights are Q4_K blocks. */
+int nnq_weight_create_int4(const uint8_t *codes, const void *scales, nnq_dtype scale_dtype, const uint8_t *zeros,
+                           int64_t n, int64_t k, int64_t group, nnq_weight **out);
 
 int nnq_weight_destroy(nnq_weight *w);
 
@@ -231,6 +248,34 @@ int nnq_linear_sample(const nnq_weight *w, const float *x, int64_t k, const floa
 int nnq_linear_sample_noalloc(const nnq_weight *w, const float *x, int64_t k, const float *bias, int64_t bias_len,
                               float *logits, const uint32_t *past_tokens, int64_t n_past, const nnq_sampling *cfg,
                               uint32_t *token, void *stream);
+
+/* ---- log probabilities ------------------------------------------------------------ */
+
+/* For each row r of logits (element r * row_stride, n of them; NNQ_F32, NNQ_BF16 or NNQ_F16)
+ * and token tokens[r] (device i64), on the device and in f32:
+ *   logprobs[r]      log(softmax(row)[token]);
+ *   entropy[r]       -sum p log p, in nats (may be NULL);
+ *   ranks[r]         how many logits come before the token's in descending order, equal
+ *                    logits in index order: 0 for the most likely token (may be NULL);
+ *   top_ids, top_logprobs [m, top_n]  the top_n most likely tokens in that order (top_n from
+ *                    0 to 32 and at most n: NNQ_ERR_INVALID_SHAPE otherwise).
+ * A logit of -inf (a masked token) has probability 0 and is never among the alternatives;
+ * places that no token fills get id -1 and log probability -inf.  A row that holds NaN or
+ * +inf, or nothing above -inf, has NaN for every log probability and the entropy, as
+ * log_softmax gives.  A token outside [0, n) (padding) has log probability NaN; where that
+ * is NaN the rank is -1.  Rows may overlap or repeat (row_stride 0).  m = 0 is a no-op.
+ * Stands beside nnq_sample_token; no counterpart in the reference, which returns tokens
+ * only. */
+int nnq_token_logprobs(const void *logits, nnq_dtype dtype, int64_t m, int64_t n, int64_t row_stride,
+                       const int64_t *tokens, int top_n, float *logprobs, float *entropy, int64_t *ranks,
+                       float *top_logprobs, int64_t *top_ids, void *stream);
+
+/* nnq_token_logprobs of logits = x[m, k] @ W^T (+ bias), the linear as nnq_linear with f32
+ * output: the scoring of a prompt through the LM head, for any weight.  logits (f32 [m, n],
+ * contiguous) may be NULL: then only chunks of rows exist, in the workspace (up to 160 MB). */
+int nnq_linear_logprobs(const nnq_weight *w, const void *x, nnq_dtype x_dtype, int64_t m, int64_t k, const float *bias,
+                        int64_t bias_len, const int64_t *tokens, int top_n, float *logits, float *logprobs,
+                        float *entropy, int64_t *ranks, float *top_logprobs, int64_t *top_ids, void *stream);
 
 /* ---- Qwen3 SwiGLU MLP ----------------------------------------------------------- */
 

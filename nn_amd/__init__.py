@@ -7,7 +7,9 @@ operator surface in Python.
 """
 from .quantized import (  # noqa: F401
     BiasMismatch, DataLengthMismatch, InvalidShape, Layout, NonFiniteData, NotQuantized, QuantizedMatmulError,
-    QuantizedMLP, QuantizedMoE, QuantizedWeight, QuantType, RankMismatch, ShapeMismatch, TensorError, Unsupported, WeightRank,
-    WrongQuantType, argmax, dequantize_mxfp4_ocp, device_count, init, linear_argmax, linear_sample, sample_token,
+    QuantizedMLP, QuantizedMoE, QuantizedWeight, QuantType, RankMismatch, ShapeMismatch, TensorError, TokenLogprobs,
+    Unsupported, WeightRank,
+    WrongQuantType, argmax, dequantize_mxfp4_ocp, device_count, init, linear_argmax, linear_logprobs, linear_sample,
+    sample_token, token_logprobs,
     quantize_mxfp4, quantize_mxfp4_ocp, quantize_q4_k, quantize_q6_k, quantize_q8_0, quantized_linear, quantized_matmul_q4_k, quantized_matmul_q6_k, quantized_matmul_q8_0,
     synth_normal)

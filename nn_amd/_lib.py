@@ -79,6 +79,12 @@ SIGNATURES = {
                                   ctypes.POINTER(c_i64), ctypes.POINTER(c_double), ctypes.POINTER(ctypes.c_char_p),
                                   ctypes.POINTER(ctypes.c_uint32), ctypes.POINTER(c_u64)]),
     "nnq_gguf_weight_create": (c_int, [c_void_p, ctypes.c_char_p, c_int, c_int, ctypes.POINTER(c_void_p)]),
+    "nnq_weight_create_int4": (c_int, [c_void_p, c_void_p, c_int, c_void_p, c_i64, c_i64, c_i64,
+                                       ctypes.POINTER(c_void_p)]),
+    "nnq_token_logprobs": (c_int, [c_void_p, c_int, c_i64, c_i64, c_i64, c_void_p, c_int, c_void_p, c_void_p, c_void_p,
+                                   c_void_p, c_void_p, c_void_p]),
+    "nnq_linear_logprobs": (c_int, [c_void_p, c_void_p, c_int, c_i64, c_i64, c_void_p, c_i64, c_void_p, c_int, c_void_p,
+                                    c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p]),
     "nnq_quantize_q4_k": (c_int, [c_void_p, c_sz, c_void_p]),
     "nnq_quantize_mxfp4": (c_int, [c_void_p, c_sz, c_void_p, c_void_p]),
     "nnq_quantize_q8_0": (c_int, [c_void_p, c_sz, c_void_p]),

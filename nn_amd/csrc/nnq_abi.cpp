@@ -417,6 +417,49 @@ int nnq_weight_create(nnq_format fmt, nnq_layout layout, const uint8_t *bytes, s
     return NNQ_OK;
 }
 
+int nnq_weight_create_int4(const uint8_t *codes, const void *scales, nnq_dtype scale_dtype, const uint8_t *zeros,
+                           int64_t n, int64_t k, int64_t group, nnq_weight **out) {
+    if (!out) return fail(NNQ_ERR_INVALID_ARGUMENT, "out is null");
+    *out = nullptr;
+    if (n <= 0 || k <= 0) return fail(NNQ_ERR_INVALID_ARGUMENT, "weight shape [%lld, %lld]", (long long)n, (long long)k);
+    if (scale_dtype != NNQ_F16 && scale_dtype != NNQ_BF16)
+        return fail(NNQ_ERR_UNSUPPORTED, "scale dtype %d (f16 or bf16)", (int)scale_dtype);
+    Layout L;
+    const char *err = nullptr;
+    if (!make_layout_int4(n, k, group, zeros != nullptr, scale_dtype == NNQ_BF16, &L, &err))
+        return fail(NNQ_ERR_INVALID_SHAPE, "%s (in_features %lld, group %lld)", err, (long long)k, (long long)group);
+    if (!codes || !scales) return fail(NNQ_ERR_INVALID_ARGUMENT, "codes or scales is null");
+    size_t bytes = 0;
+    if (!array_bytes(n + kTile, k + kInt4Unit, 1, &bytes) || bytes > (size_t)INT64_MAX) return size_fail();
+    const uint16_t *sc = reinterpret_cast<const uint16_t *>(scales);
+    const uint16_t ex = scale_dtype == NNQ_BF16 ? 0x7F80 : 0x7C00;
+    const int64_t groups = n * (k / group);
+    for (int64_t i = 0; i < groups; i++)
+        if ((sc[i] & ex) == ex) return fail(NNQ_ERR_NON_FINITE, "scale %lld is not finite", (long long)i);
+    for (int64_t i = 0; zeros && i < groups; i++)
+        if (zeros[i] > 16) return fail(NNQ_ERR_INVALID_ARGUMENT, "zero point %lld is %d (0 to 16)", (long long)i, zeros[i]);
+    std::vector<uint8_t> host;
+    nnq_weight *w = nullptr;
+    try {
+        host.resize(L.total());
+        parallel_for(L.ntile, [&](int64_t lo, int64_t hi) { repack_int4(codes, sc, zeros, L, lo, hi, host.data()); });
+        w = new nnq_weight;
+    } catch (const std::exception &ex) {  // no memory, no thread
+        return fail(NNQ_ERR_OUT_OF_MEMORY, "weight repack: %s", ex.what());
+    }
+    w->L = L;
+    hipGetDevice(&w->device);
+    hipError_t e = hipMalloc(&w->dev, L.total());
+    if (e == hipSuccess) e = hipMemcpy(w->dev, host.data(), L.total(), hipMemcpyHostToDevice);
+    if (e != hipSuccess) {
+        if (w->dev) hipFree(w->dev);
+        delete w;
+        return hip_fail(e, "weight upload");
+    }
+    *out = w;
+    return NNQ_OK;
+}
+
 int nnq_weight_destroy(nnq_weight *w) {
     if (!w) return NNQ_OK;
     if (w->dev) hipFree(w->dev);
@@ -437,8 +480,10 @@ int nnq_weight_info(const nnq_weight *w, int *fmt, int *layout, int64_t *n, int6
 int nnq_dequant(const nnq_weight *w, float *out, void *stream) {
     if (!w) return fail(NNQ_ERR_NOT_QUANTIZED, "weight handle is null");
     if (!out) return fail(NNQ_ERR_INVALID_ARGUMENT, "out is null");
-    int e = launch_dequant(w->L.fmt, w->dev, w->dev + w->L.qs_bytes, w->L.n, w->L.k, w->L.ntile, w->L.nblk, out,
-                           stream);
+    int e = w->L.fmt == NNQ_FMT_INT4G
+                ? launch_int4_dequant(w->L, w->dev, out, stream)
+                : launch_dequant(w->L.fmt, w->dev, w->dev + w->L.qs_bytes, w->L.n, w->L.k, w->L.ntile, w->L.nblk, out,
+                                 stream);
     if (e) return hip_fail((hipError_t)e, "dequant launch");
     return NNQ_OK;
 }
@@ -521,6 +566,7 @@ static size_t few_call_scratch(const nnq_weight *w, int64_t m, nnq_dtype x_dtype
 
 static size_t linear_scratch_bytes(const nnq_weight *w, int64_t m, nnq_dtype x_dtype, const void *y,
                                    int swiglu_out = 0) {
+    if (w->L.fmt == NNQ_FMT_INT4G) return 0;
     if (few_batch(w, m, x_dtype)) return few_call_scratch(w, m, x_dtype);
     if (!gemm_batch(w, m, x_dtype)) return 0;
     return gemm_call_scratch(w, m, x_dtype, y, swiglu_out);
@@ -535,10 +581,50 @@ static bool prefill_swiglu(const nnq_weight *w, int64_t m, nnq_dtype x_dtype) {
     return gemm_wide_swiglu(g);
 }
 
+// a validated linear call over 4-bit codes with group scales, in launches of kInt4Rows rows
+static Int4Args int4_args(const nnq_weight *w, const void *x, nnq_dtype x_dtype, int64_t m, const float *bias, void *y,
+                          nnq_dtype y_dtype) {
+    const Layout &L = w->L;
+    Int4Args a{};
+    a.w = w->dev;
+    a.x = x;
+    a.bias = bias;
+    a.y = y;
+    a.x_bf16 = x_dtype == NNQ_BF16;
+    a.y_bf16 = y_dtype == NNQ_BF16;
+    a.group = L.group;
+    a.zeros = L.zeros;
+    a.scale_bf16 = L.scale_bf16;
+    a.n = L.n;
+    a.k = L.k;
+    a.m = m;
+    a.ntile = L.ntile;
+    a.units = L.nblk;
+    return a;
+}
+
+static int dispatch_int4(const nnq_weight *w, const void *x, nnq_dtype x_dtype, int64_t m, const float *bias, void *y,
+                         nnq_dtype y_dtype, void *stream) {
+    const size_t xe = x_dtype == NNQ_BF16 ? 2 : 4, ye = y_dtype == NNQ_BF16 ? 2 : 4;
+    for (int64_t m0 = 0; m0 < m; m0 += kInt4Rows) {
+        int e = launch_int4_rows(int4_args(w, (const uint8_t *)x + (size_t)m0 * w->L.k * xe, x_dtype,
+                                           std::min<int64_t>(kInt4Rows, m - m0), bias,
+                                           (uint8_t *)y + (size_t)m0 * w->L.n * ye, y_dtype),
+                                 stream);
+        if (e) return hip_fail((hipError_t)e, "int4 linear launch");
+    }
+    return NNQ_OK;
+}
+
 static int dispatch_linear(const nnq_weight *w, const void *x, nnq_dtype x_dtype, int64_t m, const float *bias,
                            void *y, nnq_dtype y_dtype, void *stream, int x_swiglu = 0, int32_t *status = nullptr,
                            int status_mode = 0, void *ext_scratch = nullptr, int swiglu_out = 0) {
     if (m == 0) return NNQ_OK;
+    if (w->L.fmt == NNQ_FMT_INT4G) {
+        if (x_swiglu || status || swiglu_out)
+            return fail(NNQ_ERR_INVALID_ARGUMENT, "a SwiGLU input or output or a status needs a GGUF block weight");
+        return dispatch_int4(w, x, x_dtype, m, bias, y, y_dtype, stream);
+    }
     if (swiglu_out && (w->L.fmt != NNQ_FMT_Q4_K || (m > 2 && !prefill_swiglu(w, m, x_dtype)) || x_swiglu || bias ||
                        w->L.n % 16))
         return fail(NNQ_ERR_INVALID_ARGUMENT, "SwiGLU epilogue needs a Q4_K decode GEMV or wide GEMM over whole tiles");
@@ -681,23 +767,32 @@ static int linear_argmax(const nnq_weight *w, const float *x, int64_t k, const f
                 "stage x");
         x = reinterpret_cast<const float *>(reinterpret_cast<uint8_t *>(s.p) + off[1]);
     }
-    GemvArgs a{};
-    a.qs = w->dev;
-    a.hdr = w->dev + L.qs_bytes;
-    a.x = x;
-    a.bias = bias;
-    a.y = logits;
-    a.n = L.n;
-    a.k = L.k;
-    a.m = 1;
-    a.ntile = L.ntile;
-    a.nblk = L.nblk;
-    a.argmax_partial = (unsigned long long *)s.p;
+    unsigned long long *keys = (unsigned long long *)s.p;
     int64_t nkeys = L.ntile;  // the launch lowers it when it writes one key per workgroup
-    a.argmax_count = &nkeys;
-    int e = launch_gemv(L.fmt, a, stream);
+    int e;
+    if (L.fmt == NNQ_FMT_INT4G) {
+        Int4Args a = int4_args(w, x, NNQ_F32, 1, bias, logits, NNQ_F32);
+        a.argmax_partial = keys;
+        a.argmax_count = &nkeys;
+        e = launch_int4_rows(a, stream);
+    } else {
+        GemvArgs a{};
+        a.qs = w->dev;
+        a.hdr = w->dev + L.qs_bytes;
+        a.x = x;
+        a.bias = bias;
+        a.y = logits;
+        a.n = L.n;
+        a.k = L.k;
+        a.m = 1;
+        a.ntile = L.ntile;
+        a.nblk = L.nblk;
+        a.argmax_partial = keys;
+        a.argmax_count = &nkeys;
+        e = launch_gemv(L.fmt, a, stream);
+    }
     if (e) return hip_fail((hipError_t)e, "gemv launch");
-    e = launch_argmax_final(a.argmax_partial, nkeys, idx, idx64, status_dev, stream);
+    e = launch_argmax_final(keys, nkeys, idx, idx64, status_dev, stream);
     if (e) return hip_fail((hipError_t)e, "argmax launch");
     return NNQ_OK;
 }
@@ -1223,6 +1318,91 @@ int nnq_linear_sample_noalloc(const nnq_weight *w, const float *x, int64_t k, co
     rc = dispatch_linear(w, x, NNQ_F32, 1, bias, logits, NNQ_F32, stream);
     if (rc) return rc;
     return run_sample(logits, w->L.n, past_tokens, n_past, cfg, token, stream, scr);
+}
+
+// ---- log probabilities ----------------------------------------------------------------
+
+static int check_logprobs(int64_t m, int64_t n, int top_n, const int64_t *tokens, const float *logprobs,
+                          const float *entropy, const int64_t *ranks, const float *top_logprobs,
+                          const int64_t *top_ids) {
+    if (m < 0) return fail(NNQ_ERR_INVALID_ARGUMENT, "m = %lld", (long long)m);
+    if (n <= 0) return fail(NNQ_ERR_INVALID_SHAPE, "log probabilities over a zero-length dimension");
+    if (n > kLogprobMaxVocab) return fail(NNQ_ERR_UNSUPPORTED, "%lld logits in a row (at most 2^31 - 1)", (long long)n);
+    if (top_n < 0 || top_n > n || top_n > kLogprobTop)
+        return fail(NNQ_ERR_INVALID_SHAPE, "top_n %d out of range (0 to %d, at most the %lld logits)", top_n, kLogprobTop,
+                    (long long)n);
+    if (m == 0) return NNQ_OK;
+    if (!tokens || !logprobs || (top_n && (!top_logprobs || !top_ids)))
+        return fail(NNQ_ERR_INVALID_ARGUMENT, "null pointer");
+    if (((uintptr_t)tokens | (uintptr_t)ranks | (uintptr_t)top_ids) & 7 ||
+        ((uintptr_t)logprobs | (uintptr_t)entropy | (uintptr_t)top_logprobs) & 3)
+        return fail(NNQ_ERR_INVALID_ARGUMENT, "tokens, ranks and ids must be 8-byte, floats 4-byte aligned");
+    return NNQ_OK;
+}
+
+int nnq_token_logprobs(const void *logits, nnq_dtype dtype, int64_t m, int64_t n, int64_t row_stride,
+                       const int64_t *tokens, int top_n, float *logprobs, float *entropy, int64_t *ranks,
+                       float *top_logprobs, int64_t *top_ids, void *stream) {
+    if (dtype != NNQ_F32 && dtype != NNQ_BF16 && dtype != NNQ_F16)
+        return fail(NNQ_ERR_UNSUPPORTED, "logits dtype %d (f32, bf16 or f16)", (int)dtype);
+    int rc = check_logprobs(m, n, top_n, tokens, logprobs, entropy, ranks, top_logprobs, top_ids);
+    if (rc || m == 0) return rc;
+    if (!logits) return fail(NNQ_ERR_INVALID_ARGUMENT, "logits is null");
+    if (row_stride < 0) return fail(NNQ_ERR_INVALID_ARGUMENT, "row stride %lld", (long long)row_stride);
+    const int elem = dtype == NNQ_F32 ? 4 : 2;
+    if ((uintptr_t)logits % elem) return fail(NNQ_ERR_INVALID_ARGUMENT, "logits are not aligned to their type");
+    Scratch s;
+    HIP_TRY(s.alloc(logprob_plan(m, n, top_n, elem).bytes, (hipStream_t)stream), "scratch alloc");
+    int e = launch_logprobs(LogprobArgs{logits, (int)dtype, n, row_stride, tokens, top_n, logprobs, entropy, ranks,
+                                        top_logprobs, top_ids},
+                            m, s.p, stream);
+    if (e) return hip_fail((hipError_t)e, "log probability launch");
+    return NNQ_OK;
+}
+
+int nnq_linear_logprobs(const nnq_weight *w, const void *x, nnq_dtype x_dtype, int64_t m, int64_t k, const float *bias,
+                        int64_t bias_len, const int64_t *tokens, int top_n, float *logits, float *logprobs,
+                        float *entropy, int64_t *ranks, float *top_logprobs, int64_t *top_ids, void *stream) {
+    // (logits may be null: then they stay in the workspace; any non-null pointer passes the check)
+    int rc = check_linear(w, x, x_dtype, m, k, bias, bias_len, logits ? (void *)logits : (void *)&m, NNQ_F32);
+    if (rc) return rc;
+    const int64_t n = w->L.n;
+    rc = check_logprobs(m, n, top_n, tokens, logprobs, entropy, ranks, top_logprobs, top_ids);
+    if (rc || m == 0) return rc;
+    if (logits && misaligned_out(logits)) return fail(NNQ_ERR_INVALID_ARGUMENT, "logits must be 4-byte aligned");
+    const int64_t mc = head_chunk_rows(m, n), tail = m % mc;
+    const size_t xe = x_dtype == NNQ_BF16 ? 2 : 4;
+    const bool xm = misaligned_in(x);
+    size_t xbytes = 0, lbytes = 0;
+    if (!array_bytes(m, k, xe, &xbytes) || !array_bytes(mc, n, 4, &lbytes)) return size_fail();
+    // a chunk's first row lies as the first chunk's: chunks are whole 16-row tiles, or all of m
+    size_t lin = linear_scratch_bytes(w, mc, x_dtype, logits);
+    if (tail) lin = std::max(lin, linear_scratch_bytes(w, tail, x_dtype, logits));
+    // workspace: [a chunk's logits][the linear's scratch][the log probabilities' scratch][staged x]
+    const size_t sizes[4] = {logits ? 0 : lbytes, lin, logprob_plan(mc, n, top_n, 4).bytes, xm ? xbytes : 0};
+    size_t off[4], total = 0;
+    if (!plan_regions(sizes, 4, off, &total)) return size_fail();
+    Scratch s;
+    HIP_TRY(s.alloc(total, (hipStream_t)stream), "scratch alloc");
+    uint8_t *base = reinterpret_cast<uint8_t *>(s.p);
+    if (xm) {
+        HIP_TRY(hipMemcpyAsync(base + off[3], x, xbytes, hipMemcpyDeviceToDevice, (hipStream_t)stream), "stage x");
+        x = base + off[3];
+    }
+    for (int64_t m0 = 0; m0 < m; m0 += mc) {
+        const int64_t rows = std::min(mc, m - m0);
+        float *lg = logits ? logits + m0 * n : reinterpret_cast<float *>(base);
+        rc = dispatch_linear(w, (const uint8_t *)x + (size_t)m0 * k * xe, x_dtype, rows, bias, lg, NNQ_F32, stream, 0,
+                             nullptr, 0, lin ? base + off[1] : nullptr);
+        if (rc) return rc;
+        int e = launch_logprobs(LogprobArgs{lg, NNQ_F32, n, n, tokens + m0, top_n, logprobs + m0,
+                                            entropy ? entropy + m0 : nullptr, ranks ? ranks + m0 : nullptr,
+                                            top_n ? top_logprobs + m0 * top_n : nullptr,
+                                            top_n ? top_ids + m0 * top_n : nullptr},
+                                rows, base + off[2], stream);
+        if (e) return hip_fail((hipError_t)e, "log probability launch");
+    }
+    return NNQ_OK;
 }
 
 }  // extern "C"

@@ -1,0 +1,437 @@
+// Linear over 4-bit codes with group scales on gfx950, one to sixteen token rows per launch:
+//   y[t][r] = sum_g s[r][g] * sum_{k in g} (q[r][k] - z[r][g]) * x[t][k]  (+ bias[r]),
+// g the groups of 32, 64 or 128 columns of row r, z = 8 where no zero points are stored.
+//
+// Bound: the weight stream from HBM (n * k / 2 bytes of codes, 2 or 3 bytes per group), so the
+// weight is read once for all token rows and everything else is kept small beside it:
+//  * A workgroup of up to 16 waves owns blocks of R 16-row tiles; wave w takes units w,
+//    w + waves, ... of 128 k.  One 16-byte load per lane is a unit of a tile, and exactly the
+//    B operands of four 16x16x32 f16 MFMAs.  The next step's loads are in flight while the
+//    current one is computed.
+//  * x of a unit is scaled by a power of two per token row (its largest magnitude into
+//    [2^14, 2^15)) to f16 (bf16 x; exact but for values below 2^-31 of that magnitude) or to an
+//    f16 hi + lo pair (f32 x, ~22 bits), and passes through a wave-private LDS buffer into A
+//    operands.  With K in one pass they stay in registers for all the workgroup's tiles.
+//  * A code becomes an exact f16 integer: (w & 0x000F000F) | 0x6400.. is 1024 + q, and
+//    (w & 0x00F000F0) | 0x5400.. is 64 + q in place, without a shift; one packed add takes off
+//    1024 + z (64 + z), exactly.  Nine instructions make eight operands.  The integers are kept
+//    normal: as f16 subnormals they would cost the matrix core's aligned sums low bits.
+//  * Every product is exact in f32; a group's sum is scaled in f32 (one rounding for the scale,
+//    one per addition).  The waves' sums meet in LDS, one barrier per block of tiles.
+#include <algorithm>
+
+#include "nnq_device.h"
+#include "nnq_internal.h"
+
+namespace nnq {
+
+namespace {
+
+typedef _Float16 half2v __attribute__((ext_vector_type(2)));
+
+// The raw bytes of one unit of a tile in the lane that holds row lane % 16.
+template <int GS, bool Z>
+struct Unit {
+    u32x4 q;
+    uint32_t s[(GS + 1) / 2];  // GS scales (16 bits each)
+    uint32_t z;                // GS zero points (8 bits each)
+};
+
+template <int GS, bool Z>
+__device__ __forceinline__ void load_unit(const uint8_t *rec, int lane, Unit<GS, Z> &u) {
+    u.q = ldg128(rec + 16 * lane);
+    const int r = lane & 15;
+    const uint8_t *sp = rec + 1024 + 2 * GS * r, *zp = rec + 1024 + 32 * GS + GS * r;
+    if constexpr (GS == 1) {
+        u.s[0] = *reinterpret_cast<const uint16_t *>(sp);
+        if constexpr (Z) u.z = *zp;
+    } else if constexpr (GS == 2) {
+        u.s[0] = *reinterpret_cast<const uint32_t *>(sp);
+        if constexpr (Z) u.z = *reinterpret_cast<const uint16_t *>(zp);
+    } else {
+        const u32x2 s = *reinterpret_cast<const u32x2 *>(sp);
+        u.s[0] = s[0];
+        u.s[1] = s[1];
+        if constexpr (Z) u.z = *reinterpret_cast<const uint32_t *>(zp);
+    }
+}
+
+template <int GS, bool Z>
+__device__ __forceinline__ float unit_scale(const Unit<GS, Z> &u, int g, int bf16) {
+    const uint32_t h = (u.s[g >> 1] >> (16 * (g & 1))) & 0xFFFFu;
+    return bf16 ? bf16_to_f32(h) : f16_to_f32(h);
+}
+
+__device__ __forceinline__ uint32_t pk_add(uint32_t a, uint32_t b) {
+    return __builtin_bit_cast(uint32_t, __builtin_bit_cast(half2v, a) + __builtin_bit_cast(half2v, b));
+}
+
+// eight codes of one word -> q - z as f16, in column order; c1 = -(1024 + z), c2 = -(64 + z), packed
+__device__ __forceinline__ u32x4 codes_f16(uint32_t w, uint32_t c1, uint32_t c2) {
+    const uint32_t v = w >> 8;
+    return u32x4{pk_add((w & 0x000F000Fu) | 0x64006400u, c1), pk_add((w & 0x00F000F0u) | 0x54005400u, c2),
+                 pk_add((v & 0x000F000Fu) | 0x64006400u, c1), pk_add((v & 0x00F000F0u) | 0x54005400u, c2)};
+}
+
+__device__ __forceinline__ void wave_fence() {
+    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+}
+
+template <int CTRL>
+__device__ __forceinline__ uint32_t umax_row(uint32_t v) {
+    const uint32_t o = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, CTRL, 0xF, 0xF, true);
+    return v > o ? v : o;
+}
+
+__device__ __forceinline__ uint32_t pack_f16(float a, float b) {
+    return f32_to_f16_bits(a) | (f32_to_f16_bits(b) << 16);
+}
+
+// token rows and A operand planes: bf16 x, 16 rows; f32 x, 8 tokens as row pairs (hi, lo); f32 x, 16
+// tokens as two planes (lo, hi)
+enum { XBF16 = 0, XPAIR = 1, XPLANES = 2 };
+constexpr int planes(int xf) { return xf == XPLANES ? 2 : 1; }
+
+// x[0..m) of unit u -> A operands of the unit's four MFMAs (per plane) and the rows' powers of two
+// back; `buf` (4 KB) and `bk` (16 floats) are the wave's own.  Lane 16i + c takes columns 8c ..
+// 8c + 7 of row t0 + i.  A unit past K leaves zeros and back = 0.
+template <int XF>
+__device__ __forceinline__ void stage_unit(const Int4Args &a, int64_t u, int lane, uint16_t *buf, float *bk,
+                                           u32x4 (&A)[planes(XF)][4], float (&back)[4]) {
+    const int c = lane & 15, i4 = lane >> 4;
+    const int64_t k0 = u * kInt4Unit + 8 * c;
+    const bool in = k0 < a.k;  // K is a multiple of 32, so a lane's 8 columns are all in or all out
+    const int m = (int)a.m;
+    constexpr int kPass = planes(XF);
+#pragma unroll
+    for (int pl = 0; pl < kPass; pl++) {
+        for (int t0 = 0; t0 < m; t0 += 4) {
+            const int t = t0 + i4;
+            float v[8];
+#pragma unroll
+            for (int e = 0; e < 8; e++) v[e] = 0.f;
+            if (in && t < m) {
+                if constexpr (XF == XBF16) {
+                    const u32x4 r = *reinterpret_cast<const u32x4 *>(reinterpret_cast<const uint16_t *>(a.x) + t * a.k + k0);
+#pragma unroll
+                    for (int e = 0; e < 4; e++) {
+                        v[2 * e] = __uint_as_float(r[e] << 16);
+                        v[2 * e + 1] = __uint_as_float(r[e] & 0xFFFF0000u);
+                    }
+                } else {
+                    const floatx4 *p = reinterpret_cast<const floatx4 *>(reinterpret_cast<const float *>(a.x) + t * a.k + k0);
+                    const floatx4 r0 = p[0], r1 = p[1];
+#pragma unroll
+                    for (int e = 0; e < 4; e++) {
+                        v[e] = r0[e];
+                        v[4 + e] = r1[e];
+                    }
+                }
+            }
+            // largest |x| of the row's 128 columns as bits (NaN above infinity above every number)
+            uint32_t mx = 0;
+#pragma unroll
+            for (int e = 0; e < 8; e++) mx = max(mx, __float_as_uint(v[e]) & 0x7FFFFFFFu);
+            mx = umax_row<0xB1>(mx);
+            mx = umax_row<0x4E>(mx);
+            mx = umax_row<0x141>(mx);
+            mx = umax_row<0x140>(mx);
+            float s, b;
+            f16_prescale(__uint_as_float(mx), s, b);
+            u32x4 hi, lo;
+#pragma unroll
+            for (int e = 0; e < 4; e++) {
+                const float p = v[2 * e] * s, q = v[2 * e + 1] * s;
+                hi[e] = pack_f16(p, q);
+                if constexpr (XF != XBF16)
+                    lo[e] = pack_f16(p - f16_to_f32(hi[e] & 0xFFFFu), q - f16_to_f32(hi[e] >> 16));
+            }
+            // operand (j, p) of row r at 16-byte slot (4j + p) * 16 + r: c = 4j + p
+            u32x4 *slot = reinterpret_cast<u32x4 *>(buf) + c * 16;
+            if (t < m) {
+                if constexpr (XF == XPAIR) {
+                    slot[2 * t] = hi;
+                    slot[2 * t + 1] = lo;
+                } else if constexpr (XF == XPLANES) {
+                    slot[t] = pl == 0 ? lo : hi;
+                } else {
+                    slot[t] = hi;
+                }
+                if (c == 0) {
+                    if constexpr (XF == XPAIR) {
+                        bk[2 * t] = b;
+                        bk[2 * t + 1] = b;
+                    } else {
+                        bk[t] = b;
+                    }
+                }
+            }
+        }
+        wave_fence();
+        // rows past the tokens read what the buffer holds: MFMA rows are independent, theirs are not stored
+#pragma unroll
+        for (int j = 0; j < 4; j++) A[pl][j] = reinterpret_cast<const u32x4 *>(buf)[(4 * j + i4) * 16 + c];
+        if (pl == kPass - 1) {
+            const floatx4 b4 = *reinterpret_cast<const floatx4 *>(bk + 4 * i4);
+#pragma unroll
+            for (int e = 0; e < 4; e++) back[e] = b4[e];
+        }
+        wave_fence();
+    }
+}
+
+__device__ __forceinline__ uint64_t int4_argmax_key(float v, uint32_t idx) {
+    if (v != v) return ~0ull;
+    const uint32_t b = __float_as_uint(v);
+    return ((uint64_t)((b & 0x80000000u) ? ~b : (b | 0x80000000u)) << 32) | (0xFFFFFFFFu - idx);
+}
+
+// Blocks b = blockIdx.x, + gridDim.x, ... of R tiles; passes over K of waves * UPW units.
+template <int XF, int GS, bool Z, int R, int UPW>
+__global__ __launch_bounds__(1024) void int4_rows_kernel(Int4Args a) {
+    constexpr int P = planes(XF);
+    constexpr int UB = int4_unit_bytes(kInt4Unit / GS, Z);
+    const int tid = threadIdx.x, lane = tid & 63;
+    const int wv = __builtin_amdgcn_readfirstlane(tid >> 6), waves = (int)(blockDim.x >> 6);
+    // LDS: per wave a 4 KB staging buffer and 16 floats, then two reduction buffers
+    extern __shared__ __attribute__((aligned(16))) uint8_t lds[];
+    uint16_t *buf = reinterpret_cast<uint16_t *>(lds + wv * 4096);
+    float *bk = reinterpret_cast<float *>(lds + waves * 4096 + wv * 64);
+    float *red = reinterpret_cast<float *>(lds + waves * (4096 + 64));
+    const int m = (int)a.m, units = (int)a.units;
+    const int npass = (units + waves * UPW - 1) / (waves * UPW);
+    const int nblock = (int)((a.ntile + R - 1) / R);
+    const int c = lane & 15, p4 = lane >> 4;
+
+    u32x4 A[UPW][P][4];
+    float back[UPW][4];
+    float sum[R][4];
+    Unit<GS, Z> W[R][UPW], N[R][UPW];
+    // a tile or a unit that does not exist is read at the last that does: its A operands are zeros,
+    // its outputs are not stored
+    auto load = [&](Unit<GS, Z>(&w)[R][UPW], int b, int pass) {
+#pragma unroll
+        for (int r = 0; r < R; r++)
+#pragma unroll
+            for (int j = 0; j < UPW; j++) {
+                const int64_t tile = min((int64_t)b * R + r, a.ntile - 1);
+                const int u = min((pass * UPW + j) * waves + wv, units - 1);
+                load_unit<GS, Z>(a.w + (size_t)(tile * units + u) * UB, lane, w[r][j]);
+            }
+    };
+    uint64_t key = 0;
+    int b = blockIdx.x, par = 0;
+    if (b < nblock) load(W, b, 0);
+    bool first = true;
+    for (; b < nblock; b += gridDim.x) {
+#pragma unroll
+        for (int r = 0; r < R; r++)
+#pragma unroll
+            for (int i = 0; i < 4; i++) sum[r][i] = 0.f;
+        for (int pass = 0; pass < npass; pass++) {
+            // the next step's loads: the next pass, or the next block's first
+            const bool last = pass + 1 == npass;
+            const int nb = last ? b + (int)gridDim.x : b;
+            if (nb < nblock) load(N, nb, last ? 0 : pass + 1);
+            if (npass > 1 || first) {
+#pragma unroll
+                for (int j = 0; j < UPW; j++) {
+                    const int u = (pass * UPW + j) * waves + wv;
+                    if (u < units) {
+                        stage_unit<XF>(a, u, lane, buf, bk, A[j], back[j]);
+                    } else {
+#pragma unroll
+                        for (int pl = 0; pl < P; pl++)
+#pragma unroll
+                            for (int q = 0; q < 4; q++) A[j][pl][q] = u32x4{0, 0, 0, 0};
+#pragma unroll
+                        for (int i = 0; i < 4; i++) back[j][i] = 0.f;
+                    }
+                }
+                first = false;
+            }
+#pragma unroll
+            for (int r = 0; r < R; r++)
+#pragma unroll
+                for (int j = 0; j < UPW; j++) {
+                    float tot[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                    for (int g = 0; g < GS; g++) {
+                        uint32_t c1 = 0xE408E408u, c2 = 0xD480D480u;  // -(1024 + 8), -(64 + 8)
+                        if constexpr (Z) {
+                            const uint32_t z = ((W[r][j].z >> (8 * g)) & 0xFFu) * 0x00010001u;
+                            c1 = 0xE400E400u | z;
+                            c2 = 0xD400D400u | (z << 4);
+                        }
+                        u32x4 B[4 / GS];
+#pragma unroll
+                        for (int h = 0; h < 4 / GS; h++) B[h] = codes_f16(W[r][j].q[g * (4 / GS) + h], c1, c2);
+                        floatx4 acc = {0.f, 0.f, 0.f, 0.f};
+                        // (the lo plane first: added to a finished hi sum its low bits would be cut off)
+#pragma unroll
+                        for (int pl = 0; pl < P; pl++)
+#pragma unroll
+                            for (int h = 0; h < 4 / GS; h++)
+                                acc = mfma16x16x32_f16(A[j][pl][g * (4 / GS) + h], B[h], acc);
+                        const float s = unit_scale<GS, Z>(W[r][j], g, a.scale_bf16);
+#pragma unroll
+                        for (int i = 0; i < 4; i++) tot[i] = fmaf(s, acc[i], tot[i]);
+                    }
+#pragma unroll
+                    for (int i = 0; i < 4; i++) sum[r][i] = fmaf(back[j][i], tot[i], sum[r][i]);
+                }
+#pragma unroll
+            for (int r = 0; r < R; r++)
+#pragma unroll
+                for (int j = 0; j < UPW; j++) W[r][j] = N[r][j];
+        }
+        // lane 16p + c: rows 4p .. 4p + 3 of output column c, for each tile -> [wave][tile][token][16]
+        float *rb = red + par * waves * R * 256;
+#pragma unroll
+        for (int r = 0; r < R; r++) {
+            float *o = rb + (wv * R + r) * 256 + c;
+            if constexpr (XF == XPAIR) {
+                if (2 * p4 < m) o[(2 * p4) * 16] = sum[r][0] + sum[r][1];
+                if (2 * p4 + 1 < m) o[(2 * p4 + 1) * 16] = sum[r][2] + sum[r][3];
+            } else {
+#pragma unroll
+                for (int i = 0; i < 4; i++)
+                    if (4 * p4 + i < m) o[(4 * p4 + i) * 16] = sum[r][i];
+            }
+        }
+        __syncthreads();  // also: every wave is past its reads of the other buffer
+        for (int o = tid; o < R * 256; o += (int)blockDim.x) {
+            const int r = o >> 8, t = (o >> 4) & 15, col = o & 15;
+            if (t >= m) continue;
+            const int64_t row = ((int64_t)b * R + r) * kTile + col;
+            float v = 0.f;
+            for (int w = 0; w < waves; w++) v += rb[(w * R + r) * 256 + t * 16 + col];
+            if (row < a.n) {
+                if (a.bias) v += a.bias[row];
+                if (a.y_bf16)
+                    reinterpret_cast<uint16_t *>(a.y)[t * a.n + row] = (uint16_t)f32_to_bf16_bits(v);
+                else
+                    reinterpret_cast<float *>(a.y)[t * a.n + row] = v;
+                if (a.argmax_partial) key = max(key, int4_argmax_key(v, (uint32_t)row));
+            }
+        }
+        par ^= 1;
+    }
+    if (a.argmax_partial) {
+        // m = 1: threads r * 256 + col hold keys (0 elsewhere); one key per workgroup
+        __syncthreads();
+        unsigned long long *kr = reinterpret_cast<unsigned long long *>(red);
+        for (int o = 32; o > 0; o >>= 1) {
+            const uint64_t other = __shfl_xor((unsigned long long)key, o, 64);
+            key = other > key ? other : key;
+        }
+        if (lane == 0) kr[wv] = key;
+        __syncthreads();
+        if (tid == 0) {
+            for (int w = 1; w < waves; w++) key = max(key, (uint64_t)kr[w]);
+            a.argmax_partial[blockIdx.x] = key;
+        }
+    }
+}
+
+int cus() {
+    static int n[64] = {0};
+    int dev = 0;
+    if (hipGetDevice(&dev) != hipSuccess || dev < 0 || dev >= 64) return 256;
+    if (n[dev] == 0) {
+        int c = 0;
+        if (hipDeviceGetAttribute(&c, hipDeviceAttributeMultiprocessorCount, dev) != hipSuccess || c <= 0) c = 256;
+        n[dev] = c;  // concurrent first calls store the same value
+    }
+    return n[dev];
+}
+
+template <int XF, int GS, bool Z, int R, int UPW>
+int launch_rows_t(const Int4Args &a, void *stream) {
+    // a wave for every unit, up to 16; the chip holds 16 / waves workgroups per CU
+    int waves = 16;
+    while (waves > 4 && waves / 2 >= a.units) waves /= 2;
+    const int64_t blocks = (a.ntile + R - 1) / R;
+    const int64_t grid = std::min<int64_t>(blocks, (int64_t)cus() * (16 / waves));
+    const size_t lds = (size_t)waves * (4096 + 64 + 2 * R * 1024);
+    if (a.argmax_count) *a.argmax_count = grid;
+    auto *kernel = int4_rows_kernel<XF, GS, Z, R, UPW>;
+    static bool big[64] = {false};
+    int dev = 0;
+    hipError_t e = hipGetDevice(&dev);
+    if (e != hipSuccess) return (int)e;
+    if (dev < 0 || dev >= 64 || !big[dev]) {
+        e = hipFuncSetAttribute(reinterpret_cast<const void *>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize,
+                                16 * (4096 + 64 + 2 * R * 1024));
+        if (e != hipSuccess) return (int)e;
+        if (dev >= 0 && dev < 64) big[dev] = true;
+    }
+    hipLaunchKernelGGL(kernel, dim3((unsigned)grid), dim3(waves * 64), lds, (hipStream_t)stream, a);
+    return (int)hipGetLastError();
+}
+
+template <int XF, int GS, bool Z>
+int launch_rows_r(const Int4Args &a, void *stream) {
+    if constexpr (XF == XPLANES) return launch_rows_t<XF, GS, Z, 1, 1>(a, stream);
+    else return a.ntile > 2 * (int64_t)cus() ? launch_rows_t<XF, GS, Z, 2, 2>(a, stream)
+                                             : launch_rows_t<XF, GS, Z, 1, 2>(a, stream);
+}
+
+template <int XF>
+int launch_rows_x(const Int4Args &a, void *stream) {
+    if (a.zeros) {
+        if (a.group == 128) return launch_rows_r<XF, 1, true>(a, stream);
+        if (a.group == 64) return launch_rows_r<XF, 2, true>(a, stream);
+        return launch_rows_r<XF, 4, true>(a, stream);
+    }
+    if (a.group == 128) return launch_rows_r<XF, 1, false>(a, stream);
+    if (a.group == 64) return launch_rows_r<XF, 2, false>(a, stream);
+    return launch_rows_r<XF, 4, false>(a, stream);
+}
+
+// Bit-exact decode: (q - z) has at most 5 bits and the scale 11, so the product is exact in f32.
+// One wave per (tile, unit).
+__global__ __launch_bounds__(256) void dequant_int4_kernel(const uint8_t *w, int64_t n, int64_t k, int64_t units,
+                                                           int64_t jobs, int group, int zeros, int scale_bf16,
+                                                           float *out) {
+    const int64_t job = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
+    if (job >= jobs) return;
+    const int lane = threadIdx.x & 63, r = lane & 15, p = lane >> 4;
+    const int gs = kInt4Unit / group;
+    const uint8_t *rec = w + (size_t)job * int4_unit_bytes(group, zeros);
+    const int64_t row = job / units * kTile + r;
+    if (row >= n) return;
+    const u32x4 q = ldg128(rec + 16 * lane);
+    for (int j = 0; j < 4; j++) {
+        const int64_t k0 = job % units * kInt4Unit + 32 * j + 8 * p;
+        if (k0 >= k) break;
+        const int g = 32 * j / group;
+        const uint32_t h = reinterpret_cast<const uint16_t *>(rec + 1024)[r * gs + g];
+        const float s = scale_bf16 ? bf16_to_f32(h) : f16_to_f32(h);
+        const int z = zeros ? rec[1024 + 32 * gs + r * gs + g] : 8;
+        for (int e = 0; e < 8; e++) {
+            const int code = (int)((q[j] >> (4 * (e / 2) + 16 * (e & 1))) & 0xFu);
+            out[row * k + k0 + e] = (float)(code - z) * s;
+        }
+    }
+}
+
+}  // namespace
+
+int launch_int4_rows(const Int4Args &a, void *stream) {
+    if (a.m < 1 || a.m > kInt4Rows || a.units < 1 || a.ntile < 1 || (a.argmax_partial && a.m != 1))
+        return (int)hipErrorInvalidValue;
+    if (a.x_bf16) return launch_rows_x<XBF16>(a, stream);
+    return a.m <= 8 ? launch_rows_x<XPAIR>(a, stream) : launch_rows_x<XPLANES>(a, stream);
+}
+
+int launch_int4_dequant(const Layout &L, const uint8_t *w, float *out, void *stream) {
+    const int64_t jobs = L.ntile * L.nblk;
+    hipLaunchKernelGGL(dequant_int4_kernel, dim3((unsigned)((jobs + 3) / 4)), dim3(256), 0, (hipStream_t)stream, w, L.n,
+                       L.k, L.nblk, jobs, L.group, L.zeros, L.scale_bf16, out);
+    return (int)hipGetLastError();
+}
+
+}  // namespace nnq

@@ -30,6 +30,9 @@ struct Layout {
     size_t qs_bytes = 0;   // bytes of the quant plane
     size_t hdr_bytes = 0;  // bytes of the scale/header plane
     size_t aux_bytes = 0;  // bytes of the derived plane (Q4_K: min-term operands of the GEMM)
+    int group = 0;         // INT4G: weights per scale (32, 64 or 128)
+    int zeros = 0;         //   1: a zero point per group is stored (else 8 throughout)
+    int scale_bf16 = 0;    //   scales are bf16 (else f16)
     size_t total() const { return qs_bytes + hdr_bytes + aux_bytes; }
 };
 
@@ -44,12 +47,22 @@ struct Layout {
 // Q8_0: per (tile, block pair): qs 1024 B; per (tile, 8 blocks): 16 rows x 8 f16 scales.
 // Q6_K: per (tile, block of 256): qs 3072 B (four 64-k chunks x 64 lanes x 12 B),
 //       header 16 rows x 16 int8 scales + 16 rows x f16 d (288 B).
+// INT4G: everything in the quant plane, per (tile, unit of 128 k) one record of
+//       int4_unit_bytes: codes 1024 B (lane 16p + r holds 4 words, word j = row r's columns
+//       32j + 8p .. + 7 of the unit: columns 2i, 2i + 1 at bits 4i and 16 + 4i), then 16 rows x
+//       (128 / group) scales, then with zero points 16 rows x (128 / group) bytes.
 bool make_layout(int fmt, int layout, int64_t n, int64_t k, Layout *out, const char **err);
+bool make_layout_int4(int64_t n, int64_t k, int64_t group, int zeros, int scale_bf16, Layout *out, const char **err);
+constexpr int kInt4Unit = 128;  // k of one unit
+constexpr int int4_unit_bytes(int group, int zeros) { return 1024 + kTile * (kInt4Unit / group) * (zeros ? 3 : 2); }
 
 // Host repack: source block bytes (format/layout as given) -> device image (Layout::total bytes).
 void repack_q4k(const uint8_t *src, int legacy, const Layout &L, uint8_t *dst);
 void repack_q8_0(const uint8_t *src, const Layout &L, uint8_t *dst);
 void repack_q6k(const uint8_t *src, const Layout &L, uint8_t *dst);
+// (tiles [t0, t1) of the image at dst, which starts at tile 0; zeros may be null)
+void repack_int4(const uint8_t *codes, const uint16_t *scales, const uint8_t *zeros, const Layout &L, int64_t t0,
+                 int64_t t1, uint8_t *dst);
 
 // nn-gguf legacy Q4_K block -> GGUF-spec (BlockQ4K) block with identical decoded values.
 void q4k_legacy_to_gguf(const uint8_t *legacy, uint8_t *gguf);
@@ -218,6 +231,50 @@ int launch_gemm_finalize(const float *ys, int ks, const float *bias, void *y, in
 // the staging scratch of a GEMM call (base null: sizes only) and the staging kernel
 GemmScratch gemm_carve(void *base, const GemmArgs &a, size_t *bytes);
 int launch_gemm_prep(const GemmArgs &a, const GemmScratch &sc, void *stream);
+
+// ---- 4-bit codes with group scales (nnq_int4.hip) ----------------------------------
+struct Int4Args {
+    const uint8_t *w;  // the image (Layout::qs_bytes)
+    const void *x;     // [m, k] f32 or bf16, 16-byte aligned
+    const float *bias; // [n] or null
+    void *y;           // [m, n] f32 or bf16
+    int x_bf16, y_bf16;
+    int group, zeros, scale_bf16;
+    int64_t n, k, m;
+    int64_t ntile, units;
+    unsigned long long *argmax_partial;  // optional (m = 1): argmax keys, at most ntile of them
+    int64_t *argmax_count;               //   and how many the launch writes
+};
+constexpr int kInt4Rows = 16;  // token rows of one launch_int4_rows
+int launch_int4_rows(const Int4Args &a, void *stream);
+int launch_int4_dequant(const Layout &L, const uint8_t *w, float *out, void *stream);
+
+// ---- log probabilities (nnq_logprobs.hip) -------------------------------------------
+struct LogprobArgs {
+    const void *logits;     // row r at element r * stride, n of them
+    int dtype;              // nnq_dtype
+    int64_t n, stride;
+    const int64_t *tokens;  // [m]
+    int top;                // alternatives per row (0 .. kLogprobTop)
+    float *logprob;         // [m]
+    float *entropy;         // [m] or null
+    int64_t *rank;          // [m] or null
+    float *top_lp;          // [m][top]
+    int64_t *top_id;
+};
+constexpr int kLogprobTop = 32;
+constexpr int64_t kLogprobMaxVocab = 0x7FFFFFFF;
+// how m rows run (nnq_plan.cpp): segments of a row, candidate slots of a segment, rows per launch,
+// scratch bytes
+struct LogprobPlan {
+    int64_t nseg, rows;
+    int slots;
+    size_t bytes;
+};
+LogprobPlan logprob_plan(int64_t m, int64_t n, int top, int elem);
+int launch_logprobs(const LogprobArgs &a, int64_t m, void *scratch, void *stream);
+// rows of hidden states whose logits linear_logprobs holds at a time
+int64_t head_chunk_rows(int64_t m, int64_t n);
 
 // MoE (GPT-OSS MXFP4).  Expert weights [E][K][N] with 32-element blocks along N
 // (Mxfp4Tensor of the flat tensor) are repacked per (expert, 32-column block nb,

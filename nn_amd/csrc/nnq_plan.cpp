@@ -49,6 +49,28 @@ int64_t gemm_chunk_rows(int64_t m, int64_t k) {
     return std::min(m, std::max<int64_t>(1, rows));
 }
 
+// Rows of 2048-logit segments (one wave each, four to a workgroup; a row that does not start at a
+// 16-byte address begins inside its first segment, by up to 16 / elem - 1 logits).  The candidate
+// slots leave room over the 1.1 to 1.4 top that continuous logits fill.  A launch takes at most
+// 65535 rows (its grid's second dimension) and its scratch stays near 64 MiB, whatever m.
+LogprobPlan logprob_plan(int64_t m, int64_t n, int top, int elem) {
+    LogprobPlan p{};
+    const int64_t seg = (n + 16 / elem - 1 + 2047) / 2048;
+    p.nseg = (seg + 3) / 4 * 4;
+    p.slots = top ? std::min(64, (top + top / 2 + 6 + 3) / 4 * 4) : 0;
+    const int64_t per = p.nseg * (20 + 8 * (int64_t)p.slots);
+    p.rows = std::max<int64_t>(1, std::min({m, ((int64_t)64 << 20) / per, (int64_t)65535}));
+    p.bytes = (size_t)(p.rows * per);
+    return p;
+}
+
+// Logits of one chunk: at most 160 MB of f32, which the 256 MB last-level cache holds from the GEMM
+// that writes them to the log probabilities that read them, and whole 16-row MFMA tiles.
+int64_t head_chunk_rows(int64_t m, int64_t n) {
+    const int64_t fit = ((int64_t)160 << 20) / (4 * n) / 16 * 16;
+    return std::min(m, std::max<int64_t>(16, fit));
+}
+
 // ---- dispatch rules ----------------------------------------------------------------
 
 // The path of a linear call of m tokens, by measured crossovers on MI355X (us, x f32 / bf16):

@@ -3,6 +3,7 @@
 // Every transform here is a bijection on the block bytes (plus zero padding of
 // the last row tile and, for Q8_0, of the last group of 8 blocks), so the
 // algorithmic bytes a kernel streams equal the bytes of the source blocks.
+#include <algorithm>
 #include <cmath>
 #include <cstring>
 #include <vector>
@@ -63,6 +64,61 @@ bool make_layout(int fmt, int layout, int64_t n, int64_t k, Layout *L, const cha
         *err = "unsupported block format for a linear weight";
         return false;
     }
+}
+
+bool make_layout_int4(int64_t n, int64_t k, int64_t group, int zeros, int scale_bf16, Layout *L, const char **err) {
+    *L = Layout{};
+    if (group != 32 && group != 64 && group != 128) {
+        *err = "4-bit groups are of 32, 64 or 128 weights";
+        return false;
+    }
+    if (k % group) {
+        *err = "in_features must be a multiple of the group size";
+        return false;
+    }
+    L->fmt = NNQ_FMT_INT4G;
+    L->layout = NNQ_LAYOUT_GROUPS;
+    L->n = n;
+    L->k = k;
+    L->ntile = (n + kTile - 1) / kTile;
+    L->nblk = (k + kInt4Unit - 1) / kInt4Unit;
+    L->group = (int)group;
+    L->zeros = zeros;
+    L->scale_bf16 = scale_bf16;
+    L->qs_bytes = (size_t)L->ntile * L->nblk * int4_unit_bytes((int)group, zeros);
+    return true;
+}
+
+// A pair of columns (2i, 2i + 1) of a lane's 8 sits at bits 4i and 16 + 4i, so that masking a
+// word, or the word shifted right by 8, with 0x000F000F or 0x00F000F0 leaves one pair as the
+// low mantissa bits of two f16.  Columns past k and rows past n have codes, scales and zero
+// points of 0.
+void repack_int4(const uint8_t *codes, const uint16_t *scales, const uint8_t *zeros, const Layout &L, int64_t t0,
+                 int64_t t1, uint8_t *dst) {
+    const int ub = int4_unit_bytes(L.group, L.zeros), gpu = kInt4Unit / L.group;
+    const int64_t ngroup = L.k / L.group;
+    for (int64_t t = t0; t < t1; t++)
+        for (int64_t u = 0; u < L.nblk; u++) {
+            uint8_t *rec = dst + (size_t)(t * L.nblk + u) * ub;
+            std::memset(rec, 0, ub);
+            for (int r = 0; r < kTile; r++) {
+                const int64_t row = t * kTile + r;
+                if (row >= L.n) break;
+                const uint8_t *src = codes + (size_t)row * (L.k / 2) + u * (kInt4Unit / 2);
+                const int chunks = (int)std::min<int64_t>(16, (L.k - u * kInt4Unit) / 8);  // 8 columns each
+                for (int c = 0; c < chunks; c++) {
+                    uint32_t s, w = 0;
+                    std::memcpy(&s, src + 4 * c, 4);  // column e at bits 4e
+                    for (int i = 0; i < 4; i++)
+                        w |= ((s >> (8 * i)) & 0xFu) << (4 * i) | ((s >> (8 * i + 4)) & 0xFu) << (16 + 4 * i);
+                    std::memcpy(rec + 16 * (16 * (c % 4) + r) + 4 * (c / 4), &w, 4);
+                }
+                for (int g = 0; g < gpu && u * gpu + g < ngroup; g++) {
+                    std::memcpy(rec + 1024 + 2 * (r * gpu + g), &scales[row * ngroup + u * gpu + g], 2);
+                    if (L.zeros) rec[1024 + 32 * gpu + r * gpu + g] = zeros[row * ngroup + u * gpu + g];
+                }
+            }
+        }
 }
 
 // Byte order inside each 4-byte word of the quant plane: source bytes (e0,e1,e2,e3)

@@ -14,9 +14,10 @@ no CPU fallback: without the library or a GPU these functions raise.
 """
 from __future__ import annotations
 
+import contextlib
 import ctypes
 import enum
-from typing import Optional, Sequence
+from typing import NamedTuple, Optional, Sequence
 
 import numpy as np
 import torch
@@ -113,6 +114,7 @@ class QuantType(enum.IntEnum):
     Q4_K = 12
     Q6_K = 14
     MXFP4 = 39
+    INT4G = 1000  # 4-bit codes with group scales (QuantizedWeight.from_int4_groups); no GGUF type
 
     def block_size(self) -> int:
         return 32 if self in (QuantType.Q8_0, QuantType.MXFP4) else 256
@@ -134,6 +136,7 @@ class Layout(enum.IntEnum):
     NN_GGUF = 1    # nn-gguf's own Q4_K / Q6_K decoders
     GPTOSS = 2     # GPT-OSS Mxfp4Tensor
     OCP = 3        # nn-core Mxfp4Block / Mxfp4Tensor (17-byte blocks, low nibble first)
+    GROUPS = 4     # INT4G: codes, scales and zero points in arrays of their own
 
 
 _DTYPE = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}
@@ -220,6 +223,8 @@ class QuantizedWeight:
     def from_quantized(cls, data, quant_type: QuantType, shape: Sequence[int], layout: Layout = Layout.GGUF,
                        device: int = 0) -> "QuantizedWeight":
         quant_type = QuantType(quant_type)
+        if quant_type == QuantType.INT4G:
+            raise WrongQuantType("INT4G weights come from QuantizedWeight.from_int4_groups")
         shape = tuple(int(s) for s in shape)
         if len(shape) != 2:
             raise WeightRank(f"quantized weight must be 2-D [out_features, in_features], got rank {len(shape)}")
@@ -238,6 +243,49 @@ class QuantizedWeight:
             _check(_lib.load().nnq_weight_create(int(quant_type), int(layout), buf.ctypes.data_as(ctypes.c_void_p),
                                                  buf.size, n, k, ctypes.byref(h)))
         return cls(h, quant_type, layout, shape, device)
+
+    @classmethod
+    def from_int4_groups(cls, codes: torch.Tensor, scales: torch.Tensor, zeros: Optional[torch.Tensor] = None,
+                         group_size: int = 128, device: int = 0) -> "QuantizedWeight":
+        """W[r, j] = (code[r, j] - zero[r, j // group_size]) * scale[r, j // group_size], the form of
+        4-bit checkpoints outside GGUF (no counterpart in the reference).
+
+        codes: uint8 [out_features, in_features / 2], two to a byte with the even column in the
+        low half; scales: float16 or bfloat16 [out_features, in_features / group_size]; zeros:
+        integers from 0 to 16 of the same shape, or None for 8 throughout; group_size 32, 64 or
+        128.  The tensors may be on the host or a device and are copied."""
+        for t, what in ((codes, "codes"), (scales, "scales")):
+            if not isinstance(t, torch.Tensor):
+                raise Unsupported(f"{what} must be a tensor")
+        if codes.dtype != torch.uint8:
+            raise Unsupported(f"codes must be uint8 (two to a byte), got {codes.dtype}")
+        if scales.dtype not in (torch.float16, torch.bfloat16):
+            raise Unsupported(f"scales must be float16 or bfloat16, got {scales.dtype}")
+        if codes.dim() != 2:
+            raise WeightRank(f"codes must be 2-D [out_features, in_features / 2], got rank {codes.dim()}")
+        n, k, group = codes.shape[0], 2 * codes.shape[1], int(group_size)
+        if group not in (32, 64, 128) or n == 0 or k == 0 or k % group:
+            raise InvalidShape(f"weight [{n}, {k}] in groups of {group} (32, 64 or 128 that divide in_features)")
+        if tuple(scales.shape) != (n, k // group):
+            raise ShapeMismatch(f"scales must be [{n}, {k // group}], got {list(scales.shape)}")
+        z = None
+        if zeros is not None:
+            if tuple(zeros.shape) != (n, k // group):
+                raise ShapeMismatch(f"zeros must be [{n}, {k // group}], got {list(zeros.shape)}")
+            if zeros.is_floating_point() or zeros.is_complex() or zeros.dtype == torch.bool:
+                raise Unsupported(f"zeros must be integers, got {zeros.dtype}")
+            zh = zeros.detach().cpu()
+            if zh.dtype != torch.uint8 and (int(zh.min()) < 0 or int(zh.max()) > 16):
+                raise TensorError("zero points must be from 0 to 16")
+            z = zh.to(torch.uint8).contiguous()
+        c = codes.detach().cpu().contiguous()
+        s = scales.detach().cpu().contiguous()
+        init(device)
+        with torch.cuda.device(device):
+            h = ctypes.c_void_p()
+            _check(_lib.load().nnq_weight_create_int4(c.data_ptr(), s.data_ptr(), _DTYPE[s.dtype], _ptr(z), n, k, group,
+                                                      ctypes.byref(h)))
+        return cls(h, QuantType.INT4G, Layout.GROUPS, (n, k), device)
 
     def __del__(self):
         h = getattr(self, "_h", None)
@@ -410,6 +458,101 @@ def linear_sample(x: torch.Tensor, weight: QuantizedWeight, bias: Optional[torch
     _check(_lib.load().nnq_linear_sample(weight.handle, _ptr(xv), k, _ptr(bias), n if bias is not None else 0,
                                          _ptr(logits), _ptr(past), n_past, ctypes.byref(cfg), _ptr(tok), _stream(xv)))
     return logits, tok.view(torch.int32)[0].to(torch.int64)
+
+
+# ---------------------------------------------------------------------------------
+# log probabilities
+# ---------------------------------------------------------------------------------
+
+
+class TokenLogprobs(NamedTuple):
+    """Log probabilities of given tokens, one per row of logits (see ``token_logprobs``)."""
+    logprobs: torch.Tensor                         # f32
+    entropy: torch.Tensor                          # f32, nats
+    ranks: Optional[torch.Tensor] = None           # int64, 0 for the most likely token
+    top_logprobs: Optional[torch.Tensor] = None    # f32 [..., top_n], descending
+    top_ids: Optional[torch.Tensor] = None         # int64 [..., top_n]
+    logits: Optional[torch.Tensor] = None          # f32 [..., n] (linear_logprobs with return_logits)
+
+
+def _logprob_outputs(rows, batch, n, top_n, ranks, device):
+    if not 0 <= int(top_n) <= min(32, n):
+        raise InvalidShape(f"top_n {top_n} out of range (0 to 32, at most the {n} logits)")
+    lp = torch.empty(2, rows, dtype=torch.float32, device=device)
+    ids = torch.empty(rows * (int(bool(ranks)) + int(top_n)), dtype=torch.int64, device=device)
+    rk = ids[:rows] if ranks else None
+    ti = ids[rows * int(bool(ranks)):] if top_n else None
+    tl = torch.empty(rows * int(top_n), dtype=torch.float32, device=device) if top_n else None
+    ptrs = (_ptr(lp), lp.data_ptr() + 4 * rows, _ptr(rk), _ptr(tl), _ptr(ti))
+    view = lambda t, *more: None if t is None else t.view((*batch, *more))  # noqa: E731
+    return ptrs, TokenLogprobs(view(lp[0]), view(lp[1]), view(rk), view(tl, int(top_n)), view(ti, int(top_n)))
+
+
+def _token_ids(tokens, batch, device):
+    if not isinstance(tokens, torch.Tensor):
+        tokens = torch.as_tensor(tokens)
+    if tuple(tokens.shape) != tuple(batch):
+        raise ShapeMismatch(f"tokens must be {list(batch)}, one per row of logits, got {list(tokens.shape)}")
+    if tokens.is_floating_point() or tokens.is_complex() or tokens.dtype == torch.bool:
+        raise Unsupported(f"tokens must be integers, got {tokens.dtype}")
+    return tokens.to(device=device, dtype=torch.int64).contiguous()
+
+
+def _on_device(t: torch.Tensor):
+    """Make the device of `t` current for a launch (nothing to do on the current one)."""
+    return contextlib.nullcontext() if t.device.index == torch.cuda.current_device() else torch.cuda.device(t.device)
+
+
+def token_logprobs(logits: torch.Tensor, tokens, top_n: int = 0, ranks: bool = False) -> TokenLogprobs:
+    """For each row of device logits [..., n] (f32, bf16 or f16; rows may be strided) and its token:
+    the token's log probability, the entropy of the distribution, with ``ranks`` the token's place
+    in descending order and with ``top_n`` (up to 32) the most likely tokens with their log
+    probabilities, equal logits in index order.  No host synchronisation.
+
+    A logit of -inf has probability 0 and is no alternative (places left over: id -1, -inf).  A row
+    with NaN, +inf or nothing above -inf gives NaN, a token outside [0, n) (padding) NaN and rank -1."""
+    _device_input(logits, "logits")
+    if logits.dim() < 1 or logits.shape[-1] == 0:
+        raise InvalidShape("logits must have a non-empty last dimension")
+    if logits.dtype not in _DTYPE:
+        logits = logits.float()
+    batch, n = logits.shape[:-1], logits.shape[-1]
+    tok = _token_ids(tokens, batch, logits.device)
+    v = logits if logits.dim() <= 2 else logits.reshape(-1, n)
+    if v.stride(-1) != 1 and n > 1:
+        v = v.contiguous()
+    rows = tok.numel()
+    stride = v.stride(0) if v.dim() == 2 else n
+    ptrs, out = _logprob_outputs(rows, batch, n, top_n, ranks, v.device)
+    with _on_device(v):
+        _check(_lib.load().nnq_token_logprobs(_ptr(v), _DTYPE[v.dtype], rows, n, stride, _ptr(tok), int(top_n), *ptrs,
+                                              _stream(v)))
+    return out
+
+
+def linear_logprobs(x: torch.Tensor, weight: QuantizedWeight, tokens, bias: Optional[torch.Tensor] = None,
+                    top_n: int = 0, ranks: bool = False, return_logits: bool = False) -> TokenLogprobs:
+    """``token_logprobs`` of the logits x @ W^T (+ bias) for hidden states x [..., in_features] (f32 or
+    bf16) and one token per row: a prompt scored through the LM head.  The logits are f32 and, unless
+    ``return_logits`` asks for them, exist a chunk of rows at a time."""
+    if not isinstance(weight, QuantizedWeight):
+        raise NotQuantized("linear_logprobs: weight is not quantized")
+    n, k = weight.shape
+    xv = _validate_input(x, k, weight.device)
+    if bias is not None:
+        if bias.dim() != 1 or bias.shape[0] != n:
+            raise BiasMismatch(f"bias shape mismatch: expected [{n}], got {list(bias.shape)}")
+        bias = _side_input(bias, xv)
+    batch = xv.shape[:-1]
+    tok = _token_ids(tokens, batch, xv.device)
+    rows = tok.numel()
+    ptrs, out = _logprob_outputs(rows, batch, n, top_n, ranks, xv.device)
+    logits = xv.new_empty((*batch, n), dtype=torch.float32) if return_logits else None
+    with _on_device(xv):
+        _check(_lib.load().nnq_linear_logprobs(weight.handle, _ptr(xv), _DTYPE[xv.dtype], rows, k, _ptr(bias),
+                                               n if bias is not None else 0, _ptr(tok), int(top_n), _ptr(logits),
+                                               *ptrs, _stream(xv)))
+    return out._replace(logits=logits)
 
 
 # ---------------------------------------------------------------------------------

@@ -1,0 +1,196 @@
+"""GPU parity of linears over 4-bit codes with group scales against a plain product in 64 bits, at the
+edges of the kernels' forms: one row, two, eight and nine (f32 x as row pairs or as planes), sixteen and
+seventeen and prefills; N below a tile, past one, no whole number of tiles, more tiles than two per CU; K
+of one group, inside a unit of 128, one pass, several passes; each group size, scale type, with and
+without zero points.
+
+Bar (f32 outputs): every product of an integer and an f16 is exact in f32; f32 x enters as an f16 hi + lo
+pair that drops at most 2^-22 of it.  What is left is rounding of f32 sums and scalings, 2^-24 each of
+partial sums that stay within a few times the output's own size, some 40 in line: max |error| <= 1e-5 of
+the output's root mean square.  A bf16 output is the f32 result rounded once, bit for bit."""
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+
+F32, BF16, F16 = torch.float32, torch.bfloat16, torch.float16
+
+
+@pytest.fixture(scope="module", autouse=True)
+def dev():
+    import nn_amd
+    assert torch.cuda.is_available(), "GPU tests need a HIP device"
+    nn_amd.init(0)
+    return torch.device("cuda:0")
+
+
+def make(n, k, group, zeros=True, scale=F16, seed=1):
+    """(weight, W in 64 bits)"""
+    import nn_amd
+    g = torch.Generator(device="cuda")
+    g.manual_seed(seed)
+    q = torch.randint(0, 16, (n, k), generator=g, device="cuda", dtype=torch.int32).to(torch.uint8)
+    s = (0.004 + 0.008 * torch.rand(n, k // group, generator=g, device="cuda")).to(scale)
+    s = s * torch.where(torch.rand(n, k // group, generator=g, device="cuda") < 0.1, -1.0, 1.0).to(scale)
+    z = torch.randint(0, 17, (n, k // group), generator=g, device="cuda") if zeros else None
+    w = nn_amd.QuantizedWeight.from_int4_groups(q[:, 0::2] | (q[:, 1::2] << 4), s, z, group)
+    zz = 8.0 if z is None else z.double().repeat_interleave(group, 1)
+    return w, (q.double() - zz) * s.double().repeat_interleave(group, 1)
+
+
+def tokens(m, k, dtype, seed=2):
+    g = torch.Generator(device="cuda")
+    g.manual_seed(seed)
+    return (torch.randn(m, k, generator=g, device="cuda") * torch.exp(torch.randn(k, generator=g, device="cuda"))).to(dtype)
+
+
+def check(y, ref, what=""):
+    assert y.shape == ref.shape and torch.isfinite(y).all()
+    err = (y.double() - ref).abs().max().item() / ref.pow(2).mean().sqrt().item()
+    assert err <= 1e-5, f"{what} max error {err:.2e} of the output's rms"
+
+
+@pytest.mark.parametrize("n,k,group,zeros,scale", [(1, 32, 32, True, F16), (17, 160, 32, False, BF16), (16, 128, 128, True, BF16),
+                                                   (100, 2880, 64, True, F16), (33, 1152, 128, False, F16)])
+def test_dequantize_is_exact(n, k, group, zeros, scale):
+    w, ref = make(n, k, group, zeros, scale)
+    assert w.shape == (n, k) and w.quant_type == 1000
+    assert torch.equal(w.dequantize().double(), ref)  # 5 bits times 11 (8): no rounding
+
+
+SHAPES = [(1, 1, 32, 32), (1, 5, 64, 64), (2, 40, 128, 128), (3, 16, 160, 32), (1, 300, 2880, 64), (8, 33, 1152, 128),
+          (9, 100, 2912, 32), (16, 257, 4096, 128), (1, 8209, 640, 128), (5, 8304, 4096, 64), (12, 8193, 5120, 32),
+          (7, 64, 12288, 128), (16, 48, 8320, 64), (1, 9000, 4224, 128)]
+
+
+@pytest.mark.parametrize("xdt", [F32, BF16])
+@pytest.mark.parametrize("zeros,scale", [(True, F16), (False, F16), (True, BF16)])
+@pytest.mark.parametrize("m,n,k,group", SHAPES)
+def test_rows(m, n, k, group, zeros, scale, xdt):
+    import nn_amd
+    w, ref = make(n, k, group, zeros, scale)
+    x = tokens(m, k, xdt)
+    bias = torch.randn(n, device="cuda")
+    ref = x.double() @ ref.t()
+    check(nn_amd.quantized_linear(x, w), ref)
+    y = nn_amd.quantized_linear(x, w, bias)
+    check(y, ref + bias.double())
+    assert torch.equal(nn_amd.quantized_linear(x, w, bias, out_dtype=BF16), y.to(BF16))
+
+
+PREFILL = [(17, 16, 128, 128), (33, 300, 160, 32), (48, 129, 2880, 64), (64, 257, 1152, 128), (130, 1000, 4096, 128),
+           (203, 512, 2912, 32), (300, 4100, 640, 64), (513, 264, 4224, 128), (1, 512, 1024, 128)]
+
+
+@pytest.mark.parametrize("xdt", [F32, BF16])
+@pytest.mark.parametrize("zeros", [True, False])
+@pytest.mark.parametrize("m,n,k,group", PREFILL)
+def test_prefill(m, n, k, group, zeros, xdt):
+    import nn_amd
+    w, ref = make(n, k, group, zeros, BF16 if n % 2 else F16)
+    x = tokens(m, k, xdt)
+    bias = torch.randn(n, device="cuda")
+    ref = x.double() @ ref.t() + bias.double()
+    y = nn_amd.quantized_linear(x, w, bias)
+    check(y, ref)
+    assert torch.equal(nn_amd.quantized_linear(x, w, bias, out_dtype=BF16), y.to(BF16))
+
+
+def test_leading_dimensions_views_and_empty():
+    import nn_amd
+    w, ref = make(70, 256, 64)
+    x = tokens(12, 512, F32)
+    y = nn_amd.quantized_linear(x[:, :256].view(3, 4, 256), w)  # strided rows
+    check(y, (x[:, :256].double() @ ref.t()).view(3, 4, 70))
+    flat = torch.empty(2 * 256 + 1, device="cuda")
+    v = flat[1:].view(2, 256)  # 4 bytes past an aligned address
+    v.copy_(x[:2, :256])
+    check(nn_amd.quantized_linear(v, w), v.double() @ ref.t())
+    check(nn_amd.quantized_linear(x[:, :256].half(), w), x[:, :256].half().double() @ ref.t())
+    assert nn_amd.quantized_linear(x[:0, :256], w).shape == (0, 70)
+    with pytest.raises(nn_amd.ShapeMismatch):
+        nn_amd.quantized_linear(x, w)
+
+
+@pytest.mark.parametrize("m", [1, 16, 40])
+@pytest.mark.parametrize("xdt", [F32, BF16])
+def test_activation_range(m, xdt):
+    """Rows of very small and very large activations, a row of zeros, and one with zeros but for one value: the
+    power of two of a row and unit keeps each row's precision its own."""
+    import nn_amd
+    w, ref = make(48, 384, 128)
+    x = tokens(m, 384, xdt)
+    x = x * torch.tensor([1e-30, 1.0, 1e30, 0.0] * 10, device="cuda")[:m, None].to(xdt)
+    if m > 4:
+        x[4] = 0
+        x[4, 200] = 3.0
+    y = nn_amd.quantized_linear(x, w)
+    r = x.double() @ ref.t()
+    for t in range(m):
+        rms = r[t].pow(2).mean().sqrt().item()
+        assert (y[t].double() - r[t]).abs().max().item() <= 1e-5 * rms, t
+
+
+@pytest.mark.parametrize("m", [1, 3, 12, 30])
+def test_non_finite_activations_stay_in_their_row(m):
+    import nn_amd
+    w, ref = make(40, 512, 64)
+    for bad in (float("nan"), float("inf"), -float("inf")):
+        for xdt in (F32, BF16):
+            x = tokens(m, 512, xdt)
+            x[m // 2, 77] = bad
+            y = nn_amd.quantized_linear(x, w)
+            assert torch.isnan(y[m // 2]).all()
+            keep = [t for t in range(m) if t != m // 2]
+            if keep:
+                check(y[keep], x[keep].double() @ ref.t())
+
+
+def test_argmax_and_sampling_through_an_int4_head():
+    import nn_amd
+    for n, k, group in ((1, 128, 128), (50, 256, 32), (9001, 512, 64), (32017, 4224, 128)):
+        w, ref = make(n, k, group)
+        x = tokens(1, k, F32)
+        y = nn_amd.quantized_linear(x, w)[0]
+        logits, idx = nn_amd.linear_argmax(x, w)
+        assert torch.equal(logits, y) and idx.item() == int(torch.nonzero(y == y.max())[0])
+        logits, tok = nn_amd.linear_sample(x, w, temperature=1e-6, top_k=1, top_p=None)
+        assert torch.equal(logits, y) and y[tok] == y.max()
+    x[0, 3] = float("nan")
+    with pytest.raises(nn_amd.NonFiniteData):
+        nn_amd.linear_argmax(x, w)
+
+
+@pytest.mark.parametrize("m", [1, 16, 40, 200])
+def test_captured_graph_beside_eager_calls(m):
+    """A captured linear replayed with new inputs, eager calls of other sizes on the stream between the replays."""
+    import nn_amd
+    w, ref = make(500, 1152, 128)
+    w2, _ = make(64, 4096, 64, seed=9)
+    x = tokens(m, 1152, BF16)
+    nn_amd.quantized_linear(x, w)
+    torch.cuda.synchronize()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        y = nn_amd.quantized_linear(x, w)
+    for i in range(4):
+        x.copy_(tokens(m, 1152, BF16, seed=50 + i))
+        nn_amd.quantized_linear(tokens(300, 4096, F32, seed=i), w2)
+        g.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(y, nn_amd.quantized_linear(x, w)), i
+        check(y, x.double() @ ref.t())
+
+
+def test_same_results_every_time_and_on_another_stream():
+    import nn_amd
+    w, _ = make(8300, 4224, 64)
+    for m in (1, 13, 100):
+        x = tokens(m, 4224, F32)
+        y = nn_amd.quantized_linear(x, w)
+        s = torch.cuda.Stream()
+        s.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(s):
+            z = nn_amd.quantized_linear(x, w)
+        torch.cuda.current_stream().wait_stream(s)
+        assert torch.equal(y, z) and torch.equal(y, nn_amd.quantized_linear(x, w))

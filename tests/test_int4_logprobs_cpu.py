@@ -1,0 +1,225 @@
+"""Refusals of the 4-bit group-scaled weights and of the log probabilities that need no GPU, the host
+repack of the 4-bit image against its description, and the plan of a log-probability call."""
+import ctypes
+
+import numpy as np
+import pytest
+import torch
+
+import nn_amd
+from nn_amd import _lib
+
+
+@pytest.fixture(scope="module")
+def lib():
+    return _lib.load()
+
+
+def create(lib, codes, scales, zeros, n, k, group, dtype=1):
+    h = ctypes.c_void_p()
+    ptr = lambda a: None if a is None else a.ctypes.data  # noqa: E731
+    rc = lib.nnq_weight_create_int4(ptr(codes), ptr(scales), dtype, ptr(zeros), n, k, group, ctypes.byref(h))
+    assert not h.value or rc == 0
+    return rc
+
+
+def test_int4_create_refusals(lib):
+    c, s = np.zeros((4, 64), np.uint8), np.ones((4, 1), np.float16)
+    z = np.full((4, 1), 8, np.uint8)
+    assert lib.nnq_weight_create_int4(c.ctypes.data, s.ctypes.data, 1, None, 4, 128, 128, None) == _lib.ERR_INVALID_ARGUMENT
+    assert create(lib, c, s, z, 0, 128, 128) == _lib.ERR_INVALID_ARGUMENT
+    assert create(lib, c, s, z, 4, -128, 128) == _lib.ERR_INVALID_ARGUMENT
+    for group in (0, 16, 48, 256, -32):
+        assert create(lib, c, s, z, 4, 128, group) == _lib.ERR_INVALID_SHAPE, group
+    assert create(lib, c, s, z, 4, 96, 64) == _lib.ERR_INVALID_SHAPE
+    assert "96" in _lib.last_error()
+    assert create(lib, c, s, z, 4, 128, 128, dtype=0) == _lib.ERR_UNSUPPORTED  # f32 scales
+    assert create(lib, None, s, z, 4, 128, 128) == _lib.ERR_INVALID_ARGUMENT
+    assert create(lib, c, None, z, 4, 128, 128) == _lib.ERR_INVALID_ARGUMENT
+    z[2] = 17
+    assert create(lib, c, s, z, 4, 128, 128) == _lib.ERR_INVALID_ARGUMENT
+    assert "zero point 2" in _lib.last_error()
+    for bad in (np.inf, -np.inf, np.nan):
+        s2 = s.copy()
+        s2[3] = bad
+        assert create(lib, c, s2, None, 4, 128, 128) == _lib.ERR_NON_FINITE
+    b = np.array([0x3F80, 0x7F80, 0x3F80, 0x3F80], np.uint16)  # bf16 infinity
+    assert create(lib, c, b, None, 4, 128, 128, dtype=2) == _lib.ERR_NON_FINITE
+    # sizes whose product passes 64 bits are refused before anything is read
+    assert create(lib, c, s, None, 1 << 40, 1 << 30, 128) == _lib.ERR_OUT_OF_MEMORY
+
+
+def test_from_int4_groups_refusals():
+    make = nn_amd.QuantizedWeight.from_int4_groups
+    c, s = torch.zeros(4, 64, dtype=torch.uint8), torch.ones(4, 1, dtype=torch.float16)
+    with pytest.raises(nn_amd.Unsupported):
+        make(c.to(torch.int32), s)
+    with pytest.raises(nn_amd.Unsupported):
+        make(c, s.float())
+    with pytest.raises(nn_amd.Unsupported):
+        make(c.numpy(), s)
+    with pytest.raises(nn_amd.WeightRank):
+        make(c[0], s)
+    for group in (16, 256, 0):
+        with pytest.raises(nn_amd.InvalidShape):
+            make(c, s, group_size=group)
+    with pytest.raises(nn_amd.InvalidShape):
+        make(c[:, :48], s, group_size=64)  # 96 columns
+    with pytest.raises(nn_amd.InvalidShape):
+        make(c[:0], s[:0])
+    with pytest.raises(nn_amd.ShapeMismatch):
+        make(c, s, group_size=64)
+    with pytest.raises(nn_amd.ShapeMismatch):
+        make(c, s, torch.zeros(4, 2, dtype=torch.uint8))
+    with pytest.raises(nn_amd.Unsupported):
+        make(c, s, torch.full((4, 1), 8.0))
+    for z in (-1, 17, 300):
+        with pytest.raises(nn_amd.TensorError):
+            make(c, s, torch.full((4, 1), z, dtype=torch.int64))
+    with pytest.raises(nn_amd.WrongQuantType):
+        nn_amd.QuantizedWeight.from_quantized(np.zeros(64, np.uint8), nn_amd.QuantType.INT4G, (1, 128))
+
+
+def test_int4_gguf_formats_refuse_the_layout(lib):
+    """The block-format entry points do not take the new format's id."""
+    h = ctypes.c_void_p()
+    buf = np.zeros(1024, np.uint8)
+    vp = buf.ctypes.data
+    assert lib.nnq_weight_create(1000, 4, vp, buf.size, 4, 128, ctypes.byref(h)) == _lib.ERR_WRONG_FORMAT
+    assert lib.nnq_mlp_create(1000, 4, vp, vp, buf.size, 1000, 4, vp, buf.size, 128, 128,
+                              ctypes.byref(h)) == _lib.ERR_WRONG_FORMAT
+
+
+class Layout(ctypes.Structure):
+    _fields_ = [("fmt", ctypes.c_int), ("layout", ctypes.c_int), ("n", ctypes.c_int64), ("k", ctypes.c_int64),
+                ("ntile", ctypes.c_int64), ("nblk", ctypes.c_int64), ("qs", ctypes.c_size_t), ("hdr", ctypes.c_size_t),
+                ("aux", ctypes.c_size_t), ("group", ctypes.c_int), ("zeros", ctypes.c_int), ("sbf", ctypes.c_int)]
+
+
+@pytest.mark.parametrize("n,k,group,zeros", [(1, 32, 32, True), (16, 128, 128, False), (17, 160, 32, True),
+                                             (33, 192, 64, False), (5, 2880, 64, True), (40, 384, 128, True)])
+def test_int4_image(lib, n, k, group, zeros):
+    """Every code, scale and zero point at the place the kernels read it, zeros elsewhere."""
+    rng = np.random.default_rng(n * 1000 + k)
+    q = rng.integers(0, 16, (n, k), dtype=np.uint8)
+    codes = np.ascontiguousarray(q[:, 0::2] | (q[:, 1::2] << 4))
+    scales = rng.integers(1, 0x7C00, (n, k // group)).astype(np.uint16)
+    zp = rng.integers(0, 17, (n, k // group), dtype=np.uint8) if zeros else None
+    L, err = Layout(), ctypes.c_char_p()
+    make = lib._ZN3nnq16make_layout_int4EllliiPNS_6LayoutEPPKc
+    make.argtypes = [ctypes.c_int64] * 3 + [ctypes.c_int] * 2 + [ctypes.c_void_p] * 2
+    make.restype = ctypes.c_bool
+    assert make(n, k, group, int(zeros), 0, ctypes.byref(L), ctypes.byref(err))
+    gpu, ub = 128 // group, 1024 + 16 * (128 // group) * (3 if zeros else 2)
+    tiles, units = (n + 15) // 16, (k + 127) // 128
+    assert (L.ntile, L.nblk, L.qs, L.hdr, L.aux) == (tiles, units, tiles * units * ub, 0, 0)
+    img = np.full(L.qs + 64, 0xAB, np.uint8)
+    rep = lib._ZN3nnq11repack_int4EPKhPKtS1_RKNS_6LayoutEllPh
+    rep.argtypes = [ctypes.c_void_p] * 4 + [ctypes.c_int64] * 2 + [ctypes.c_void_p]
+    for t in range(tiles):  # (tile by tile, as the threads of an upload do)
+        rep(codes.ctypes.data, scales.ctypes.data, zp.ctypes.data if zeros else None, ctypes.byref(L), t, t + 1,
+            img.ctypes.data)
+    assert (img[L.qs:] == 0xAB).all()
+    rec = img[:L.qs].reshape(tiles, units, ub)
+    words = rec[:, :, :1024].copy().view(np.uint32).reshape(tiles, units, 4, 16, 4)  # [tile][unit][p][row][j]
+    got = np.zeros((tiles * 16, units * 128), np.uint8)
+    for p in range(4):
+        for j in range(4):
+            for e in range(8):
+                col = 32 * j + 8 * p + e
+                w = (words[:, :, p, :, j] >> (4 * (e // 2) + 16 * (e % 2))) & 15
+                got[:, col::128] = w.transpose(0, 2, 1).reshape(tiles * 16, units)
+    want = np.zeros_like(got)
+    want[:n, :k] = q
+    assert np.array_equal(got, want)
+
+    def per_group(a):
+        g = np.zeros((tiles * 16, units * gpu), a.dtype)
+        g[:n, :k // group] = a
+        return g.reshape(tiles, 16, units, gpu).transpose(0, 2, 1, 3)
+
+    sc = rec[:, :, 1024:1024 + 32 * gpu].copy().view(np.uint16).reshape(tiles, units, 16, gpu)
+    assert np.array_equal(sc, per_group(scales))
+    if zeros:
+        assert np.array_equal(rec[:, :, 1024 + 32 * gpu:].reshape(tiles, units, 16, gpu), per_group(zp))
+
+
+def test_logprob_refusals(lib):
+    f32, i64 = np.zeros(64, np.float32), np.zeros(64, np.int64)
+    p, t = f32.ctypes.data, i64.ctypes.data
+
+    def call(logits=p, dtype=0, m=2, n=8, stride=8, tokens=t, top=0, lp=p, ent=None, ranks=None, tlp=None, tid=None):
+        return lib.nnq_token_logprobs(logits, dtype, m, n, stride, tokens, top, lp, ent, ranks, tlp, tid, None)
+
+    assert call(dtype=3) == _lib.ERR_UNSUPPORTED
+    assert call(m=-1) == _lib.ERR_INVALID_ARGUMENT
+    assert call(n=0) == _lib.ERR_INVALID_SHAPE
+    assert call(n=1 << 31) == _lib.ERR_UNSUPPORTED
+    for top in (-1, 9, 33):
+        assert call(top=top, tlp=p, tid=t) == _lib.ERR_INVALID_SHAPE, top
+    assert call(n=64, stride=64, top=33, tlp=p, tid=t) == _lib.ERR_INVALID_SHAPE
+    assert call(logits=None) == _lib.ERR_INVALID_ARGUMENT
+    assert call(tokens=None) == _lib.ERR_INVALID_ARGUMENT
+    assert call(lp=None) == _lib.ERR_INVALID_ARGUMENT
+    assert call(top=2, tlp=p) == _lib.ERR_INVALID_ARGUMENT
+    assert call(top=2, tid=t) == _lib.ERR_INVALID_ARGUMENT
+    assert call(stride=-8) == _lib.ERR_INVALID_ARGUMENT
+    assert call(logits=p + 2) == _lib.ERR_INVALID_ARGUMENT  # f32 logits at an odd half
+    assert call(tokens=t + 4) == _lib.ERR_INVALID_ARGUMENT
+    assert call(lp=p + 1) == _lib.ERR_INVALID_ARGUMENT
+    assert call(m=0, logits=None, tokens=None, lp=None) == 0  # nothing to do
+    assert lib.nnq_linear_logprobs(None, p, 0, 1, 8, None, 0, t, 0, None, p, None, None, None, None,
+                                   None) == _lib.ERR_NOT_QUANTIZED
+
+
+def test_python_logprob_refusals():
+    with pytest.raises(nn_amd.Unsupported):
+        nn_amd.token_logprobs(torch.zeros(2, 8), torch.zeros(2, dtype=torch.int64))  # host tensor
+    w = nn_amd.QuantizedWeight(ctypes.c_void_p(), nn_amd.QuantType.INT4G, nn_amd.Layout.GROUPS, (16, 256), 0)
+    with pytest.raises(nn_amd.Unsupported):
+        nn_amd.linear_logprobs(torch.zeros(1, 256), w, [0])
+    with pytest.raises(nn_amd.ShapeMismatch):
+        nn_amd.linear_logprobs(torch.zeros(1, 128), w, [0])
+    with pytest.raises(nn_amd.NotQuantized):
+        nn_amd.linear_logprobs(torch.zeros(1, 256), torch.zeros(16, 256), [0])
+    from nn_amd.quantized import _logprob_outputs, _token_ids
+    for top in (-1, 33, 9):
+        with pytest.raises(nn_amd.InvalidShape):
+            _logprob_outputs(2, (2,), 8 if top == 9 else 100, top, False, "cpu")
+    with pytest.raises(nn_amd.ShapeMismatch):
+        _token_ids(torch.zeros(3, dtype=torch.int64), (2,), "cpu")
+    with pytest.raises(nn_amd.Unsupported):
+        _token_ids(torch.zeros(2), (2,), "cpu")
+    for batch in ((), (0,), (2, 3)):
+        rows = int(np.prod(batch, dtype=int))
+        _, out = _logprob_outputs(rows, batch, 8, 4, True, "cpu")
+        assert out.logprobs.shape == out.entropy.shape == out.ranks.shape == batch
+        assert out.top_ids.shape == out.top_logprobs.shape == (*batch, 4)
+
+
+class Plan(ctypes.Structure):
+    _fields_ = [("nseg", ctypes.c_int64), ("rows", ctypes.c_int64), ("slots", ctypes.c_int), ("bytes", ctypes.c_size_t)]
+
+
+@pytest.mark.parametrize("elem", [2, 4])
+@pytest.mark.parametrize("top", [0, 1, 5, 20, 32])
+def test_logprob_plan(lib, top, elem):
+    """The segments cover a row wherever it starts in a 16-byte word; slots hold the alternatives and fit a
+    wave's lanes; rows fit the grid; the scratch stays bounded."""
+    plan = lib._ZN3nnq12logprob_planEllii
+    plan.argtypes = [ctypes.c_int64, ctypes.c_int64, ctypes.c_int, ctypes.c_int]
+    plan.restype = Plan
+    for n in (1, 2045, 2046, 2048, 2049, 8185, 8192, 50257, 151936, 2 ** 31 - 1):
+        for m in (1, 7, 65536, 1 << 33):
+            p = plan(m, n, top, elem)
+            assert p.nseg % 4 == 0 and p.nseg * 2048 >= n + 16 // elem - 1
+            assert top <= p.slots <= 64 and (top == 0) == (p.slots == 0)
+            assert 1 <= p.rows <= min(m, 65535)
+            assert p.bytes == p.rows * p.nseg * (20 + 8 * p.slots)
+            assert p.rows == 1 or p.bytes <= 64 << 20
+    chunk = lib._ZN3nnq15head_chunk_rowsEll
+    chunk.argtypes, chunk.restype = [ctypes.c_int64] * 2, ctypes.c_int64
+    for n in (1, 1000, 151936, 1 << 24):
+        for m in (1, 15, 16, 300, 100000):
+            r = chunk(m, n)
+            assert 1 <= r <= m and (r == m or r % 16 == 0) and (r <= 16 or 4 * n * r <= 160 << 20)
