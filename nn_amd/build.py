@@ -25,7 +25,7 @@ COMMON = ["-O3", "-fPIC", "-std=c++17", "-Wall", "-Wno-unused-function", "-Wno-u
 
 HIP_SOURCES = ["nnq_gemv.hip", "nnq_gemm.hip", "nnq_gemm_ring.hip", "nnq_gemm_wide.hip", "nnq_gemm_wide8.hip",
                "nnq_gemm_wide6.hip", "nnq_gemm_thin.hip", "nnq_gemm_few.hip", "nnq_gemm_blk.hip", "nnq_moe.hip", "nnq_sample.hip",
-               "nnq_int4.hip", "nnq_logprobs.hip"]
+               "nnq_int4.hip", "nnq_int4_gemm.hip", "nnq_logprobs.hip"]
 # per-file device flags: the block-scaled GEMM's MFMAs write their partials to VGPRs (the
 # FMAs that scale them read VGPRs only; with the default accumulator registers every
 # partial costs four extra register reads)
@@ -35,6 +35,7 @@ HIP_SOURCES = ["nnq_gemv.hip", "nnq_gemm.hip", "nnq_gemm_ring.hip", "nnq_gemm_wi
 PRELOAD = ["-mllvm", "-amdgpu-kernarg-preload-count=16"]
 VGPR_MFMA = ["-mllvm", "-amdgpu-mfma-vgpr-form=1"]
 EXTRA_FLAGS = {"nnq_gemm_blk.hip": VGPR_MFMA, "nnq_gemm_wide8.hip": VGPR_MFMA, "nnq_gemm_thin.hip": VGPR_MFMA,
+               "nnq_int4_gemm.hip": VGPR_MFMA,
                "nnq_gemv.hip": PRELOAD,
                "nnq_probe.hip": PRELOAD}
 HOST_SOURCES = ["nnq_abi.cpp", "nnq_plan.cpp", "nnq_repack.cpp", "nnq_host.cpp", "nnq_gguf.cpp"]

@@ -564,9 +564,11 @@ static size_t few_call_scratch(const nnq_weight *w, int64_t m, nnq_dtype x_dtype
     return gemm_few_scratch_bytes(gemm_args(w, nullptr, x_dtype, rows, nullptr, nullptr, NNQ_F32), w->L.fmt);
 }
 
+static size_t int4_scratch_bytes(const nnq_weight *w, int64_t m, nnq_dtype x_dtype);
+
 static size_t linear_scratch_bytes(const nnq_weight *w, int64_t m, nnq_dtype x_dtype, const void *y,
                                    int swiglu_out = 0) {
-    if (w->L.fmt == NNQ_FMT_INT4G) return 0;
+    if (w->L.fmt == NNQ_FMT_INT4G) return int4_scratch_bytes(w, m, x_dtype);
     if (few_batch(w, m, x_dtype)) return few_call_scratch(w, m, x_dtype);
     if (!gemm_batch(w, m, x_dtype)) return 0;
     return gemm_call_scratch(w, m, x_dtype, y, swiglu_out);
@@ -581,7 +583,8 @@ static bool prefill_swiglu(const nnq_weight *w, int64_t m, nnq_dtype x_dtype) {
     return gemm_wide_swiglu(g);
 }
 
-// a validated linear call over 4-bit codes with group scales, in launches of kInt4Rows rows
+// a validated linear call over 4-bit codes with group scales: up to kInt4Rows rows in one launch that
+// reads the weight once, more through the MFMA GEMM
 static Int4Args int4_args(const nnq_weight *w, const void *x, nnq_dtype x_dtype, int64_t m, const float *bias, void *y,
                           nnq_dtype y_dtype) {
     const Layout &L = w->L;
@@ -603,14 +606,29 @@ static Int4Args int4_args(const nnq_weight *w, const void *x, nnq_dtype x_dtype,
     return a;
 }
 
+static size_t int4_scratch_bytes(const nnq_weight *w, int64_t m, nnq_dtype x_dtype) {
+    if (m <= kInt4Rows) return 0;
+    const int64_t mc = int4_chunk_rows(m, w->L.k), tail = m % mc;
+    size_t b = int4_gemm_plan(mc, w->L.n, w->L.k, x_dtype == NNQ_BF16).bytes;
+    if (tail > kInt4Rows) b = std::max(b, int4_gemm_plan(tail, w->L.n, w->L.k, x_dtype == NNQ_BF16).bytes);
+    return b;
+}
+
 static int dispatch_int4(const nnq_weight *w, const void *x, nnq_dtype x_dtype, int64_t m, const float *bias, void *y,
-                         nnq_dtype y_dtype, void *stream) {
+                         nnq_dtype y_dtype, void *stream, void *ext_scratch) {
     const size_t xe = x_dtype == NNQ_BF16 ? 2 : 4, ye = y_dtype == NNQ_BF16 ? 2 : 4;
-    for (int64_t m0 = 0; m0 < m; m0 += kInt4Rows) {
-        int e = launch_int4_rows(int4_args(w, (const uint8_t *)x + (size_t)m0 * w->L.k * xe, x_dtype,
-                                           std::min<int64_t>(kInt4Rows, m - m0), bias,
-                                           (uint8_t *)y + (size_t)m0 * w->L.n * ye, y_dtype),
-                                 stream);
+    const size_t need = int4_scratch_bytes(w, m, x_dtype);
+    Scratch s;
+    void *scr = ext_scratch;
+    if (need && !scr) {
+        HIP_TRY(s.alloc(need, (hipStream_t)stream), "scratch alloc");
+        scr = s.p;
+    }
+    const int64_t mc = int4_chunk_rows(m, w->L.k);
+    for (int64_t m0 = 0; m0 < m; m0 += mc) {
+        const Int4Args a = int4_args(w, (const uint8_t *)x + (size_t)m0 * w->L.k * xe, x_dtype, std::min(mc, m - m0),
+                                     bias, (uint8_t *)y + (size_t)m0 * w->L.n * ye, y_dtype);
+        int e = a.m <= kInt4Rows ? launch_int4_rows(a, stream) : launch_int4_gemm(a, scr, stream);
         if (e) return hip_fail((hipError_t)e, "int4 linear launch");
     }
     return NNQ_OK;
@@ -623,7 +641,7 @@ static int dispatch_linear(const nnq_weight *w, const void *x, nnq_dtype x_dtype
     if (w->L.fmt == NNQ_FMT_INT4G) {
         if (x_swiglu || status || swiglu_out)
             return fail(NNQ_ERR_INVALID_ARGUMENT, "a SwiGLU input or output or a status needs a GGUF block weight");
-        return dispatch_int4(w, x, x_dtype, m, bias, y, y_dtype, stream);
+        return dispatch_int4(w, x, x_dtype, m, bias, y, y_dtype, stream, ext_scratch);
     }
     if (swiglu_out && (w->L.fmt != NNQ_FMT_Q4_K || (m > 2 && !prefill_swiglu(w, m, x_dtype)) || x_swiglu || bias ||
                        w->L.n % 16))

@@ -1,0 +1,77 @@
+// Device helpers shared by the kernels over 4-bit codes with group scales: a unit's scales and zero
+// points, the exact f16 form of the codes, and the f16 parts of activations.
+#pragma once
+
+#include "nnq_device.h"
+#include "nnq_internal.h"
+
+namespace nnq {
+
+typedef _Float16 half2v __attribute__((ext_vector_type(2)));
+
+// row r's GS scales (16 bits each) and zero points (8 bits each) of the unit record at `rec`
+template <int GS, bool Z>
+__device__ __forceinline__ void load_scales(const uint8_t *rec, int r, uint32_t (&s)[(GS + 1) / 2], uint32_t &z) {
+    const uint8_t *sp = rec + 1024 + 2 * GS * r, *zp = rec + 1024 + 32 * GS + GS * r;
+    if constexpr (GS == 1) {
+        s[0] = *reinterpret_cast<const uint16_t *>(sp);
+        if constexpr (Z) z = *zp;
+    } else if constexpr (GS == 2) {
+        s[0] = *reinterpret_cast<const uint32_t *>(sp);
+        if constexpr (Z) z = *reinterpret_cast<const uint16_t *>(zp);
+    } else {
+        const u32x2 v = *reinterpret_cast<const u32x2 *>(sp);
+        s[0] = v[0];
+        s[1] = v[1];
+        if constexpr (Z) z = *reinterpret_cast<const uint32_t *>(zp);
+    }
+}
+
+template <int N>
+__device__ __forceinline__ float group_scale(const uint32_t (&s)[N], int g, int bf16) {
+    const uint32_t h = (s[g >> 1] >> (16 * (g & 1))) & 0xFFFFu;
+    return bf16 ? bf16_to_f32(h) : f16_to_f32(h);
+}
+
+// -(1024 + z) and -(64 + z) as packed f16 (z = 8 without zero points)
+template <bool Z>
+__device__ __forceinline__ void zero_consts(uint32_t zs, int g, uint32_t &c1, uint32_t &c2) {
+    if constexpr (Z) {
+        const uint32_t z = ((zs >> (8 * g)) & 0xFFu) * 0x00010001u;
+        c1 = 0xE400E400u | z;
+        c2 = 0xD400D400u | (z << 4);
+    } else {
+        c1 = 0xE408E408u;
+        c2 = 0xD480D480u;
+    }
+}
+
+__device__ __forceinline__ uint32_t pk_add(uint32_t a, uint32_t b) {
+    return __builtin_bit_cast(uint32_t, __builtin_bit_cast(half2v, a) + __builtin_bit_cast(half2v, b));
+}
+
+// the eight codes of a word -> q - z as f16, in column order
+__device__ __forceinline__ u32x4 codes_f16(uint32_t w, uint32_t c1, uint32_t c2) {
+    const uint32_t v = w >> 8;
+    return u32x4{pk_add((w & 0x000F000Fu) | 0x64006400u, c1), pk_add((w & 0x00F000F0u) | 0x54005400u, c2),
+                 pk_add((v & 0x000F000Fu) | 0x64006400u, c1), pk_add((v & 0x00F000F0u) | 0x54005400u, c2)};
+}
+
+// v * s (s a power of two that brings it into f16's range) as f16, and with LO what that leaves, as f16
+template <bool LO>
+__device__ __forceinline__ void split8(const float (&v)[8], float s, u32x4 &hi, u32x4 &lo) {
+#pragma unroll
+    for (int e = 0; e < 4; e++) {
+        const float p = v[2 * e] * s, q = v[2 * e + 1] * s;
+        const _Float16 hp = (_Float16)p, hq = (_Float16)q;
+        hi[e] = __builtin_bit_cast(uint32_t, half2v{hp, hq});
+        if constexpr (LO) lo[e] = __builtin_bit_cast(uint32_t, half2v{(_Float16)(p - (float)hp), (_Float16)(q - (float)hq)});
+    }
+}
+
+// let `kernel` take `bytes` of dynamic LDS on the current device
+inline hipError_t allow_lds(const void *kernel, size_t bytes) {
+    return bytes <= 65536 ? hipSuccess : hipFuncSetAttribute(kernel, hipFuncAttributeMaxDynamicSharedMemorySize, (int)bytes);
+}
+
+}  // namespace nnq

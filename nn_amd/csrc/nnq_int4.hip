@@ -21,13 +21,12 @@
 #include <algorithm>
 
 #include "nnq_device.h"
+#include "nnq_int4.h"
 #include "nnq_internal.h"
 
 namespace nnq {
 
 namespace {
-
-typedef _Float16 half2v __attribute__((ext_vector_type(2)));
 
 // The raw bytes of one unit of a tile in the lane that holds row lane % 16.
 template <int GS, bool Z>
@@ -40,37 +39,7 @@ struct Unit {
 template <int GS, bool Z>
 __device__ __forceinline__ void load_unit(const uint8_t *rec, int lane, Unit<GS, Z> &u) {
     u.q = ldg128(rec + 16 * lane);
-    const int r = lane & 15;
-    const uint8_t *sp = rec + 1024 + 2 * GS * r, *zp = rec + 1024 + 32 * GS + GS * r;
-    if constexpr (GS == 1) {
-        u.s[0] = *reinterpret_cast<const uint16_t *>(sp);
-        if constexpr (Z) u.z = *zp;
-    } else if constexpr (GS == 2) {
-        u.s[0] = *reinterpret_cast<const uint32_t *>(sp);
-        if constexpr (Z) u.z = *reinterpret_cast<const uint16_t *>(zp);
-    } else {
-        const u32x2 s = *reinterpret_cast<const u32x2 *>(sp);
-        u.s[0] = s[0];
-        u.s[1] = s[1];
-        if constexpr (Z) u.z = *reinterpret_cast<const uint32_t *>(zp);
-    }
-}
-
-template <int GS, bool Z>
-__device__ __forceinline__ float unit_scale(const Unit<GS, Z> &u, int g, int bf16) {
-    const uint32_t h = (u.s[g >> 1] >> (16 * (g & 1))) & 0xFFFFu;
-    return bf16 ? bf16_to_f32(h) : f16_to_f32(h);
-}
-
-__device__ __forceinline__ uint32_t pk_add(uint32_t a, uint32_t b) {
-    return __builtin_bit_cast(uint32_t, __builtin_bit_cast(half2v, a) + __builtin_bit_cast(half2v, b));
-}
-
-// eight codes of one word -> q - z as f16, in column order; c1 = -(1024 + z), c2 = -(64 + z), packed
-__device__ __forceinline__ u32x4 codes_f16(uint32_t w, uint32_t c1, uint32_t c2) {
-    const uint32_t v = w >> 8;
-    return u32x4{pk_add((w & 0x000F000Fu) | 0x64006400u, c1), pk_add((w & 0x00F000F0u) | 0x54005400u, c2),
-                 pk_add((v & 0x000F000Fu) | 0x64006400u, c1), pk_add((v & 0x00F000F0u) | 0x54005400u, c2)};
+    load_scales<GS, Z>(rec, lane & 15, u.s, u.z);
 }
 
 __device__ __forceinline__ void wave_fence() {
@@ -83,10 +52,6 @@ template <int CTRL>
 __device__ __forceinline__ uint32_t umax_row(uint32_t v) {
     const uint32_t o = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, CTRL, 0xF, 0xF, true);
     return v > o ? v : o;
-}
-
-__device__ __forceinline__ uint32_t pack_f16(float a, float b) {
-    return f32_to_f16_bits(a) | (f32_to_f16_bits(b) << 16);
 }
 
 // token rows and A operand planes: bf16 x, 16 rows; f32 x, 8 tokens as row pairs (hi, lo); f32 x, 16
@@ -141,13 +106,7 @@ __device__ __forceinline__ void stage_unit(const Int4Args &a, int64_t u, int lan
             float s, b;
             f16_prescale(__uint_as_float(mx), s, b);
             u32x4 hi, lo;
-#pragma unroll
-            for (int e = 0; e < 4; e++) {
-                const float p = v[2 * e] * s, q = v[2 * e + 1] * s;
-                hi[e] = pack_f16(p, q);
-                if constexpr (XF != XBF16)
-                    lo[e] = pack_f16(p - f16_to_f32(hi[e] & 0xFFFFu), q - f16_to_f32(hi[e] >> 16));
-            }
+            split8<XF != XBF16>(v, s, hi, lo);
             // operand (j, p) of row r at 16-byte slot (4j + p) * 16 + r: c = 4j + p
             u32x4 *slot = reinterpret_cast<u32x4 *>(buf) + c * 16;
             if (t < m) {
@@ -259,12 +218,8 @@ __global__ __launch_bounds__(1024) void int4_rows_kernel(Int4Args a) {
                     float tot[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
                     for (int g = 0; g < GS; g++) {
-                        uint32_t c1 = 0xE408E408u, c2 = 0xD480D480u;  // -(1024 + 8), -(64 + 8)
-                        if constexpr (Z) {
-                            const uint32_t z = ((W[r][j].z >> (8 * g)) & 0xFFu) * 0x00010001u;
-                            c1 = 0xE400E400u | z;
-                            c2 = 0xD400D400u | (z << 4);
-                        }
+                        uint32_t c1, c2;
+                        zero_consts<Z>(W[r][j].z, g, c1, c2);
                         u32x4 B[4 / GS];
 #pragma unroll
                         for (int h = 0; h < 4 / GS; h++) B[h] = codes_f16(W[r][j].q[g * (4 / GS) + h], c1, c2);
@@ -275,7 +230,7 @@ __global__ __launch_bounds__(1024) void int4_rows_kernel(Int4Args a) {
 #pragma unroll
                             for (int h = 0; h < 4 / GS; h++)
                                 acc = mfma16x16x32_f16(A[j][pl][g * (4 / GS) + h], B[h], acc);
-                        const float s = unit_scale<GS, Z>(W[r][j], g, a.scale_bf16);
+                        const float s = group_scale(W[r][j].s, g, a.scale_bf16);
 #pragma unroll
                         for (int i = 0; i < 4; i++) tot[i] = fmaf(s, acc[i], tot[i]);
                     }
@@ -358,16 +313,8 @@ int launch_rows_t(const Int4Args &a, void *stream) {
     const size_t lds = (size_t)waves * (4096 + 64 + 2 * R * 1024);
     if (a.argmax_count) *a.argmax_count = grid;
     auto *kernel = int4_rows_kernel<XF, GS, Z, R, UPW>;
-    static bool big[64] = {false};
-    int dev = 0;
-    hipError_t e = hipGetDevice(&dev);
+    hipError_t e = allow_lds(reinterpret_cast<const void *>(kernel), lds);
     if (e != hipSuccess) return (int)e;
-    if (dev < 0 || dev >= 64 || !big[dev]) {
-        e = hipFuncSetAttribute(reinterpret_cast<const void *>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize,
-                                16 * (4096 + 64 + 2 * R * 1024));
-        if (e != hipSuccess) return (int)e;
-        if (dev >= 0 && dev < 64) big[dev] = true;
-    }
     hipLaunchKernelGGL(kernel, dim3((unsigned)grid), dim3(waves * 64), lds, (hipStream_t)stream, a);
     return (int)hipGetLastError();
 }

@@ -49,6 +49,34 @@ int64_t gemm_chunk_rows(int64_t m, int64_t k) {
     return std::min(m, std::max<int64_t>(1, rows));
 }
 
+// 4-bit prefill: blocks of up to four 32-row tiles, as even as m allows; eight waves (256 columns)
+// where that fills the chip, else four; K split until there is a workgroup per CU, but not below
+// four units a part.
+Int4GemmPlan int4_gemm_plan(int64_t m, int64_t n, int64_t k, int x_bf16) {
+    Int4GemmPlan p{};
+    const int64_t cus = 256, tiles = (m + 31) / 32, units = (k + kInt4Unit - 1) / kInt4Unit;
+    const int64_t rb = (tiles + 3) / 4;
+    p.row_blocks = (int)rb;
+    p.mt = (int)((tiles + rb - 1) / rb);
+    p.waves = rb * ((n + 255) / 256) >= cus * 3 / 4 ? 8 : 4;
+    p.col_blocks = (int)((n + 32 * p.waves - 1) / (32 * p.waves));
+    int64_t ks = 1;
+    while (rb * p.col_blocks * ks * 2 <= cus * 3 / 2 && units / (ks * 2) >= 4) ks *= 2;
+    p.ks = (int)ks;
+    const size_t planes = x_bf16 ? 1 : 2;
+    p.plane = (size_t)tiles * (size_t)units * 8192;
+    p.rowback = p.plane * planes;
+    p.slabs = align256(p.rowback + (size_t)tiles * 32 * 4);
+    p.bytes = p.slabs + (ks > 1 ? (size_t)ks * (size_t)m * (size_t)n * 4 : 0);
+    return p;
+}
+
+// launches of at most 2^30 bytes of staged x and 2^16 rows
+int64_t int4_chunk_rows(int64_t m, int64_t k) {
+    const int64_t rows = ((int64_t)1 << 30) / (4 * (k + kInt4Unit)) / 128 * 128;
+    return std::min(m, std::max<int64_t>(128, std::min<int64_t>(rows, 65536)));
+}
+
 // Rows of 2048-logit segments (one wave each, four to a workgroup; a row that does not start at a
 // 16-byte address begins inside its first segment, by up to 16 / elem - 1 logits).  The candidate
 // slots leave room over the 1.1 to 1.4 top that continuous logits fill.  A launch takes at most
