@@ -272,7 +272,7 @@ int nnq_token_logprobs(const void *logits, nnq_dtype dtype, int64_t m, int64_t n
 
 /* nnq_token_logprobs of logits = x[m, k] @ W^T (+ bias), the linear as nnq_linear with f32
  * output: the scoring of a prompt through the LM head, for any weight.  logits (f32 [m, n],
- * contiguous) may be NULL: then only chunks of rows exist, in the workspace (up to 160 MB). */
+ * contiguous) may be NULL: then only chunks of rows exist, in the workspace (up to 320 MiB). */
 int nnq_linear_logprobs(const nnq_weight *w, const void *x, nnq_dtype x_dtype, int64_t m, int64_t k, const float *bias,
                         int64_t bias_len, const int64_t *tokens, int top_n, float *logits, float *logprobs,
                         float *entropy, int64_t *ranks, float *top_logprobs, int64_t *top_ids, void *stream);

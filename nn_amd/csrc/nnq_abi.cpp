@@ -609,8 +609,8 @@ static Int4Args int4_args(const nnq_weight *w, const void *x, nnq_dtype x_dtype,
 static size_t int4_scratch_bytes(const nnq_weight *w, int64_t m, nnq_dtype x_dtype) {
     if (m <= kInt4Rows) return 0;
     const int64_t mc = int4_chunk_rows(m, w->L.k), tail = m % mc;
-    size_t b = int4_gemm_plan(mc, w->L.n, w->L.k, x_dtype == NNQ_BF16).bytes;
-    if (tail > kInt4Rows) b = std::max(b, int4_gemm_plan(tail, w->L.n, w->L.k, x_dtype == NNQ_BF16).bytes);
+    size_t b = int4_gemm_plan(mc, w->L.n, w->L.k, w->L.group, x_dtype == NNQ_BF16).bytes;
+    if (tail > kInt4Rows) b = std::max(b, int4_gemm_plan(tail, w->L.n, w->L.k, w->L.group, x_dtype == NNQ_BF16).bytes);
     return b;
 }
 

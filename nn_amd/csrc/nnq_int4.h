@@ -50,11 +50,26 @@ __device__ __forceinline__ uint32_t pk_add(uint32_t a, uint32_t b) {
     return __builtin_bit_cast(uint32_t, __builtin_bit_cast(half2v, a) + __builtin_bit_cast(half2v, b));
 }
 
-// the eight codes of a word -> q - z as f16, in column order
-__device__ __forceinline__ u32x4 codes_f16(uint32_t w, uint32_t c1, uint32_t c2) {
-    const uint32_t v = w >> 8;
-    return u32x4{pk_add((w & 0x000F000Fu) | 0x64006400u, c1), pk_add((w & 0x00F000F0u) | 0x54005400u, c2),
-                 pk_add((v & 0x000F000Fu) | 0x64006400u, c1), pk_add((v & 0x00F000F0u) | 0x54005400u, c2)};
+// The masks and exponents of the codes' f16 form: held in registers (one scalar source per
+// instruction, and no literals in three-operand ones), an AND and an OR are one instruction.
+struct CodeMasks {
+    uint32_t lo, hi, e1, e2;
+    __device__ __forceinline__ CodeMasks() {
+        asm("s_mov_b32 %0, 0x000f000f" : "=s"(lo));
+        asm("s_mov_b32 %0, 0x00f000f0" : "=s"(hi));
+        asm("v_mov_b32 %0, 0x64006400" : "=v"(e1));
+        asm("v_mov_b32 %0, 0x54005400" : "=v"(e2));
+    }
+};
+
+// codes 2i and 2i + 1 of a word -> q - z as f16; all eight in column order
+__device__ __forceinline__ uint32_t code_pair(uint32_t w, int i, uint32_t c1, uint32_t c2, const CodeMasks &k) {
+    const uint32_t v = i < 2 ? w : w >> 8;
+    return i & 1 ? pk_add((v & k.hi) | k.e2, c2) : pk_add((v & k.lo) | k.e1, c1);
+}
+__device__ __forceinline__ u32x4 codes_f16(uint32_t w, uint32_t c1, uint32_t c2, const CodeMasks &k) {
+    return u32x4{code_pair(w, 0, c1, c2, k), code_pair(w, 1, c1, c2, k), code_pair(w, 2, c1, c2, k),
+                 code_pair(w, 3, c1, c2, k)};
 }
 
 // v * s (s a power of two that brings it into f16's range) as f16, and with LO what that leaves, as f16

@@ -164,6 +164,7 @@ __global__ __launch_bounds__(1024) void int4_rows_kernel(Int4Args a) {
     const int nblock = (int)((a.ntile + R - 1) / R);
     const int c = lane & 15, p4 = lane >> 4;
 
+    const CodeMasks km;
     u32x4 A[UPW][P][4];
     float back[UPW][4];
     float sum[R][4];
@@ -222,7 +223,7 @@ __global__ __launch_bounds__(1024) void int4_rows_kernel(Int4Args a) {
                         zero_consts<Z>(W[r][j].z, g, c1, c2);
                         u32x4 B[4 / GS];
 #pragma unroll
-                        for (int h = 0; h < 4 / GS; h++) B[h] = codes_f16(W[r][j].q[g * (4 / GS) + h], c1, c2);
+                        for (int h = 0; h < 4 / GS; h++) B[h] = codes_f16(W[r][j].q[g * (4 / GS) + h], c1, c2, km);
                         floatx4 acc = {0.f, 0.f, 0.f, 0.f};
                         // (the lo plane first: added to a finished hi sum its low bits would be cut off)
 #pragma unroll

@@ -24,6 +24,7 @@ namespace nnq {
 
 namespace {
 
+constexpr int W = 4;          // waves of a GEMM workgroup
 constexpr int kPiece = 8192;  // bytes of the A operands of 32 rows and one unit: 8 steps x 64 lanes x 16
 
 __device__ __forceinline__ floatx16 mfma32(u32x4 a, u32x4 b, floatx16 c) {
@@ -31,11 +32,14 @@ __device__ __forceinline__ floatx16 mfma32(u32x4 a, u32x4 b, floatx16 c) {
 }
 
 // Four rows a workgroup (thread % 4): the row's largest |x|, then its 8-column chunks, chunk c of the
-// row at piece c / 16, step (c / 2) % 8, half c % 2.  Chunks past K are zeros.
+// row at piece c / 16, step (c / 2) % 8, half c % 2.  Chunks past K are zeros.  A thread's first kHold
+// chunks stay in registers between the two (all of them up to K = 8192).
+constexpr int kStageThreads = 1024, kHold = 4;
 template <bool XB>
-__global__ __launch_bounds__(512) void int4_stage_kernel(const void *x, int m, int64_t k, int units, uint8_t *xa,
-                                                         int64_t plane, float *rowback) {
-    __shared__ uint32_t red[8][4];
+__global__ __launch_bounds__(kStageThreads) void int4_stage_kernel(const void *x, int m, int64_t k, int units,
+                                                                   uint8_t *xa, int64_t plane, float *rowback) {
+    constexpr int WV = kStageThreads / 64, STEP = kStageThreads / 4;
+    __shared__ uint32_t red[WV][4];
     const int tid = threadIdx.x, lane = tid & 63;
     const int row = (int)blockIdx.x * 4 + (tid & 3), t = min(row, m - 1);
     const int chunks = (int)(k / 8);
@@ -58,30 +62,51 @@ __global__ __launch_bounds__(512) void int4_stage_kernel(const void *x, int m, i
         }
     };
     uint32_t mx = 0;
-    for (int c = tid >> 2; c < chunks; c += 128) {
-        float v[8];
-        load(c, v);
+    auto largest = [&](const float(&v)[8]) {
 #pragma unroll
         for (int e = 0; e < 8; e++) mx = max(mx, __float_as_uint(v[e]) & 0x7FFFFFFFu);
+    };
+    float held[kHold][8];
+#pragma unroll
+    for (int i = 0; i < kHold; i++) {
+        const int c = (tid >> 2) + i * STEP;
+#pragma unroll
+        for (int e = 0; e < 8; e++) held[i][e] = 0.f;
+        if (c < chunks) load(c, held[i]);
+    }
+#pragma unroll
+    for (int i = 0; i < kHold; i++) largest(held[i]);
+    for (int c = (tid >> 2) + kHold * STEP; c < chunks; c += STEP) {
+        float v[8];
+        load(c, v);
+        largest(v);
     }
     for (int o = 4; o < 64; o <<= 1) mx = max(mx, (uint32_t)__shfl_xor((int)mx, o, 64));
     if (lane < 4) red[tid >> 6][lane] = mx;
     __syncthreads();
 #pragma unroll
-    for (int w = 0; w < 8; w++) mx = max(mx, red[w][tid & 3]);
+    for (int w = 0; w < WV; w++) mx = max(mx, red[w][tid & 3]);
     float s, back;
     f16_prescale(__uint_as_float(mx), s, back);
     if (row >= m) return;
     if (tid < 4) rowback[row] = back;
     uint8_t *dst = xa + (int64_t)(row >> 5) * units * kPiece + (row & 31) * 16;
-    for (int c = tid >> 2; c < units * 16; c += 128) {
-        float v[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-        if (c < chunks) load(c, v);
+    auto put = [&](int c, const float(&v)[8]) {
         u32x4 hi, lo;
         split8<!XB>(v, s, hi, lo);
         u32x4 *o = reinterpret_cast<u32x4 *>(dst + (int64_t)(c >> 1) * 1024 + (c & 1) * 512);
         *o = hi;
         if constexpr (!XB) *reinterpret_cast<u32x4 *>(reinterpret_cast<uint8_t *>(o) + plane) = lo;
+    };
+#pragma unroll
+    for (int i = 0; i < kHold; i++) {
+        const int c = (tid >> 2) + i * STEP;
+        if (c < units * 16) put(c, held[i]);
+    }
+    for (int c = (tid >> 2) + kHold * STEP; c < units * 16; c += STEP) {
+        float v[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+        if (c < chunks) load(c, v);
+        put(c, v);
     }
 }
 
@@ -104,7 +129,7 @@ struct Unit32 {
     uint32_t z;
 };
 
-template <int MT, int P, int GS, bool Z, int W>
+template <int MT, int NT, int P, int GS, bool Z>
 __global__ __launch_bounds__(W * 64, 2) void int4_gemm_kernel(Int4GemmArgs a) {
     constexpr int UB = int4_unit_bytes(kInt4Unit / GS, Z);
     constexpr int BUF = MT * P * kPiece;
@@ -122,14 +147,19 @@ __global__ __launch_bounds__(W * 64, 2) void int4_gemm_kernel(Int4GemmArgs a) {
     const int u0 = (int)((int64_t)a.units * kp / a.ks), u1 = (int)((int64_t)a.units * (kp + 1) / a.ks);
 
     const int c32 = lane & 31, h = lane >> 5, r = lane & 15;
-    const int tile0 = (cb * W + wv) * 2;
-    const int tile = min(tile0 + ((lane >> 4) & 1), a.ntile - 1);  // (past the last: not stored)
-    const uint8_t *wp = a.w + (size_t)tile * a.units * UB;
-    auto load_w = [&](int u, Unit32<GS, Z> &o) {
-        const uint8_t *rec = wp + (size_t)u * UB;
-        o.q[0] = *reinterpret_cast<const u32x4 *>(rec + 16 * (16 * h + r));
-        o.q[1] = *reinterpret_cast<const u32x4 *>(rec + 16 * (16 * (2 + h) + r));
-        load_scales<GS, Z>(rec, r, o.s, o.z);
+    const int tile0 = (cb * W + wv) * 2 * NT;
+    const uint8_t *wp[NT];
+#pragma unroll
+    for (int nt = 0; nt < NT; nt++)  // (tiles past the last: not stored)
+        wp[nt] = a.w + (size_t)min(tile0 + 2 * nt + ((lane >> 4) & 1), a.ntile - 1) * a.units * UB;
+    auto load_w = [&](int u, Unit32<GS, Z>(&o)[NT]) {
+#pragma unroll
+        for (int nt = 0; nt < NT; nt++) {
+            const uint8_t *rec = wp[nt] + (size_t)u * UB;
+            o[nt].q[0] = *reinterpret_cast<const u32x4 *>(rec + 16 * (16 * h + r));
+            o[nt].q[1] = *reinterpret_cast<const u32x4 *>(rec + 16 * (16 * (2 + h) + r));
+            load_scales<GS, Z>(rec, r, o[nt].s, o[nt].z);
+        }
     };
     // A pieces: (row block, plane) pairs of a unit, 8 KB each; rows past the last block: the last one
     const int row_pieces = (a.m + 31) / 32;
@@ -147,80 +177,110 @@ __global__ __launch_bounds__(W * 64, 2) void int4_gemm_kernel(Int4GemmArgs a) {
         for (int i = 0; i < NA; i++) *reinterpret_cast<u32x4 *>(lds + buf * BUF + (i * W * 64 + tid) * 16) = ar[i];
     };
 
-    floatx16 tot[MT];
+    // The MFMAs of a step are issued one at a time with the forming of the next step's operands and the
+    // scaling of a finished group's sums between them: a wave that issues MFMAs back to back waits for
+    // the matrix pipe with its own VALU work behind them.  (32 cycles of an MFMA hide six VALU
+    // instructions.)
+    const CodeMasks km;
+    floatx16 tot[MT][NT], part[MT][NT];
 #pragma unroll
     for (int mt = 0; mt < MT; mt++)
 #pragma unroll
-        for (int e = 0; e < 16; e++) tot[mt][e] = 0.f;
-    Unit32<GS, Z> w, wn;
+        for (int nt = 0; nt < NT; nt++)
+#pragma unroll
+            for (int e = 0; e < 16; e++) tot[mt][nt][e] = part[mt][nt][e] = 0.f;
+    float sc[NT];  // the scales of the sums in `part`
+    uint32_t c1[NT], c2[NT];
+    u32x4 af[2][P][MT], bf[2][NT];
+    Unit32<GS, Z> w[NT], wn[NT];
+#pragma unroll
+    for (int nt = 0; nt < NT; nt++) sc[nt] = 0.f;
+    auto read_a = [&](int buf, int s, int q) {
+        af[s & 1][q / MT][q % MT] = *reinterpret_cast<const u32x4 *>(lds + buf * BUF + lane * 16 + q * kPiece + s * 1024);
+    };
+    auto scale_part = [&](int mt, int nt) {
+#pragma unroll
+        for (int e = 0; e < 16; e++) tot[mt][nt][e] = fmaf(sc[nt], part[mt][nt][e], tot[mt][nt][e]);
+        asm volatile("" : "+v"(tot[mt][nt]));  // here: moved on, the sums would keep `part` alive beside its next values
+        __builtin_amdgcn_sched_barrier(0);
+    };
     load_a(u0);
-    load_w(u0, w);
+    load_w(u0, wn);
     store_a(0);
-    __syncthreads();
     for (int u = u0; u < u1; u++) {
         const int buf = (u - u0) & 1;
-        const bool more = u + 1 < u1;
-        if (more) {
+        __syncthreads();
+#pragma unroll
+        for (int nt = 0; nt < NT; nt++) w[nt] = wn[nt];
+        if (u + 1 < u1) {
             load_a(u + 1);
             load_w(u + 1, wn);
         }
-        const uint8_t *ab = lds + buf * BUF + lane * 16;
 #pragma unroll
-        for (int g = 0; g < GS; g++) {
-            uint32_t c1, c2;
-            zero_consts<Z>(w.z, g, c1, c2);
-            floatx16 part[MT];
+        for (int q = 0; q < P * MT; q++) read_a(buf, 0, q);
 #pragma unroll
-            for (int jj = 0; jj < 4 / GS; jj++)
+        for (int nt = 0; nt < NT; nt++) {
+            zero_consts<Z>(w[nt].z, 0, c1[nt], c2[nt]);
+            bf[0][nt] = codes_f16(w[nt].q[0][0], c1[nt], c2[nt], km);
+        }
 #pragma unroll
-                for (int i = 0; i < 2; i++) {
-                    const int j = g * (4 / GS) + jj, step = 2 * j + i;
-                    const u32x4 b = codes_f16(w.q[i][j], c1, c2);
-                    // (the lo plane first: added to a finished hi sum its low bits would be cut off)
+        for (int s = 0; s < 8; s++) {
+            const bool first = s % (8 / GS) == 0, next = s < 7;
+            if (next && (s + 1) % (8 / GS) == 0)
 #pragma unroll
-                    for (int pl = P - 1; pl >= 0; pl--)
+                for (int nt = 0; nt < NT; nt++) zero_consts<Z>(w[nt].z, (s + 1) / (8 / GS), c1[nt], c2[nt]);
+            constexpr int M = P * MT * NT;  // MFMAs of a step
 #pragma unroll
-                        for (int mt = 0; mt < MT; mt++) {
-                            const u32x4 av = *reinterpret_cast<const u32x4 *>(ab + (pl * MT + mt) * kPiece + step * 1024);
-                            floatx16 zero;
+            for (int q = 0; q < M; q++) {
+                // (the lo plane first: added to a finished hi sum its low bits would be cut off)
+                const int pl = P - 1 - q / (MT * NT), mt = q / NT % MT, nt = q % NT;
+                const bool start = first && q < MT * NT;
+                __builtin_amdgcn_sched_barrier(0);
+                if (start) scale_part(mt, nt);
+                floatx16 zero;
 #pragma unroll
-                            for (int e = 0; e < 16; e++) zero[e] = 0.f;
-                            part[mt] = mfma32(av, b, jj == 0 && i == 0 && pl == P - 1 ? zero : part[mt]);
-                        }
+                for (int e = 0; e < 16; e++) zero[e] = 0.f;
+                part[mt][nt] = mfma32(af[s & 1][pl][mt], bf[s & 1][nt], start ? zero : part[mt][nt]);
+                if (next) {
+                    if (q % NT == 0) read_a(buf, s + 1, q / NT);
+#pragma unroll
+                    for (int i = 0; i < 4 * NT; i++)
+                        if (i * M / (4 * NT) == q)
+                            bf[(s + 1) & 1][i / 4][i % 4] =
+                                code_pair(w[i / 4].q[(s + 1) & 1][(s + 1) >> 1], i % 4, c1[i / 4], c2[i / 4], km);
                 }
-            const float s = group_scale(w.s, g, a.scale_bf16);
+            }
+            if (first)
 #pragma unroll
-            for (int mt = 0; mt < MT; mt++)
-#pragma unroll
-                for (int e = 0; e < 16; e++) tot[mt][e] = fmaf(s, part[mt][e], tot[mt][e]);
-            if (GS > 1) __builtin_amdgcn_sched_barrier(0);  // one group's sums at a time: two would spill
+                for (int nt = 0; nt < NT; nt++) sc[nt] = group_scale(w[nt].s, s / (8 / GS), a.scale_bf16);
         }
-        if (more) {
-            store_a(buf ^ 1);  // (read by nobody since the barrier before this unit)
-            w = wn;
-        }
-        __syncthreads();
+        __builtin_amdgcn_sched_barrier(0);
+        if (u + 1 < u1) store_a(buf ^ 1);  // (read by nobody since the barrier before this unit)
     }
 
-    // lane: column c32, rows 8 (e / 4) + 4h + e % 4 of each 32-row tile
-    const int64_t col = (int64_t)tile0 * kTile + c32;
-    if (col >= a.n) return;
+    // lane: column c32 of each 32, rows 8 (e / 4) + 4h + e % 4 of each 32-row tile
     const bool slab = a.ks > 1;
-    const float bias = a.bias && !slab ? a.bias[col] : 0.f;
     float *ys = reinterpret_cast<float *>(a.y) + (slab ? (int64_t)kp * a.m * a.n : 0);
 #pragma unroll
-    for (int mt = 0; mt < MT; mt++)
+    for (int nt = 0; nt < NT; nt++) {
+        const int64_t col = (int64_t)(tile0 + 2 * nt) * kTile + c32;
+        const float bias = a.bias && !slab && col < a.n ? a.bias[col] : 0.f;
 #pragma unroll
-        for (int e = 0; e < 16; e++) {
-            const int row = (rb * MT + mt) * 32 + 8 * (e / 4) + 4 * h + e % 4;
-            if (row < a.m) {
-                const float v = fmaf(tot[mt][e], a.rowback[row], bias);
-                if (!slab && a.y_bf16)
-                    reinterpret_cast<uint16_t *>(a.y)[(int64_t)row * a.n + col] = (uint16_t)f32_to_bf16_bits(v);
-                else
-                    ys[(int64_t)row * a.n + col] = v;
+        for (int mt = 0; mt < MT; mt++) {
+            scale_part(mt, nt);
+#pragma unroll
+            for (int e = 0; e < 16; e++) {
+                const int row = (rb * MT + mt) * 32 + 8 * (e / 4) + 4 * h + e % 4;
+                if (row < a.m && col < a.n) {
+                    const float v = fmaf(tot[mt][nt][e], a.rowback[row], bias);
+                    if (!slab && a.y_bf16)
+                        reinterpret_cast<uint16_t *>(a.y)[(int64_t)row * a.n + col] = (uint16_t)f32_to_bf16_bits(v);
+                    else
+                        ys[(int64_t)row * a.n + col] = v;
+                }
             }
         }
+    }
 }
 
 // y[i] = sum of the ks slabs' [i] in order + bias[i % n]
@@ -237,48 +297,40 @@ __global__ __launch_bounds__(256) void int4_sum_kernel(const float *ys, int ks, 
     }
 }
 
-template <int MT, int P, int GS, bool Z, int W>
+template <int MT, int NT, int P, int GS, bool Z>
 int launch_gemm_t(const Int4GemmArgs &a, void *stream) {
     constexpr size_t lds = 2 * MT * P * kPiece;
-    auto *kernel = int4_gemm_kernel<MT, P, GS, Z, W>;
-    hipError_t e = allow_lds(reinterpret_cast<const void *>(kernel), lds);
-    if (e != hipSuccess) return (int)e;
-    hipLaunchKernelGGL(kernel, dim3((unsigned)(a.row_blocks * a.col_blocks * a.ks)), dim3(W * 64), lds,
-                       (hipStream_t)stream, a);
+    static_assert(lds <= 65536, "LDS of a launch without an attribute");
+    hipLaunchKernelGGL((int4_gemm_kernel<MT, NT, P, GS, Z>), dim3((unsigned)(a.row_blocks * a.col_blocks * a.ks)),
+                       dim3(W * 64), lds, (hipStream_t)stream, a);
     return (int)hipGetLastError();
 }
 
-template <int P, int GS, bool Z, int W>
-int launch_gemm_m(int mt, const Int4GemmArgs &a, void *stream) {
-    switch (mt) {
-    case 1: return launch_gemm_t<1, P, GS, Z, W>(a, stream);
-    case 2: return launch_gemm_t<2, P, GS, Z, W>(a, stream);
-    case 3: return launch_gemm_t<3, P, GS, Z, W>(a, stream);
-    default: return launch_gemm_t<4, P, GS, Z, W>(a, stream);
-    }
-}
-
 template <int P, int GS, bool Z>
-int launch_gemm_w(int waves, int mt, const Int4GemmArgs &a, void *stream) {
-    return waves == 8 ? launch_gemm_m<P, GS, Z, 8>(mt, a, stream) : launch_gemm_m<P, GS, Z, 4>(mt, a, stream);
+int launch_gemm_s(int mt, int nt, const Int4GemmArgs &a, void *stream) {
+    if (mt == 1) return nt == 1 ? launch_gemm_t<1, 1, P, GS, Z>(a, stream) : launch_gemm_t<1, 2, P, GS, Z>(a, stream);
+    if constexpr (P == 1)
+        return nt == 1 ? launch_gemm_t<2, 1, P, GS, Z>(a, stream) : launch_gemm_t<2, 2, P, GS, Z>(a, stream);
+    else
+        return launch_gemm_t<2, 1, P, GS, Z>(a, stream);
 }
 
 template <int P>
-int launch_gemm_g(int group, int zeros, int waves, int mt, const Int4GemmArgs &a, void *stream) {
+int launch_gemm_g(int group, int zeros, int mt, int nt, const Int4GemmArgs &a, void *stream) {
     if (zeros) {
-        if (group == 128) return launch_gemm_w<P, 1, true>(waves, mt, a, stream);
-        if (group == 64) return launch_gemm_w<P, 2, true>(waves, mt, a, stream);
-        return launch_gemm_w<P, 4, true>(waves, mt, a, stream);
+        if (group == 128) return launch_gemm_s<P, 1, true>(mt, nt, a, stream);
+        if (group == 64) return launch_gemm_s<P, 2, true>(mt, nt, a, stream);
+        return launch_gemm_s<P, 4, true>(mt, nt, a, stream);
     }
-    if (group == 128) return launch_gemm_w<P, 1, false>(waves, mt, a, stream);
-    if (group == 64) return launch_gemm_w<P, 2, false>(waves, mt, a, stream);
-    return launch_gemm_w<P, 4, false>(waves, mt, a, stream);
+    if (group == 128) return launch_gemm_s<P, 1, false>(mt, nt, a, stream);
+    if (group == 64) return launch_gemm_s<P, 2, false>(mt, nt, a, stream);
+    return launch_gemm_s<P, 4, false>(mt, nt, a, stream);
 }
 
 }  // namespace
 
 int launch_int4_gemm(const Int4Args &a, void *scratch, void *stream) {
-    const Int4GemmPlan p = int4_gemm_plan(a.m, a.n, a.k, a.x_bf16);
+    const Int4GemmPlan p = int4_gemm_plan(a.m, a.n, a.k, a.group, a.x_bf16);
     if (a.m < 1 || a.m > INT32_MAX / 2 || a.units < 1) return (int)hipErrorInvalidValue;
     uint8_t *base = reinterpret_cast<uint8_t *>(scratch);
     Int4GemmArgs g{};
@@ -301,15 +353,15 @@ int launch_int4_gemm(const Int4Args &a, void *scratch, void *stream) {
     g.n = a.n;
     const dim3 sg((unsigned)((a.m + 3) / 4));
     if (a.x_bf16)
-        hipLaunchKernelGGL((int4_stage_kernel<true>), sg, dim3(512), 0, (hipStream_t)stream, a.x, (int)a.m, a.k,
+        hipLaunchKernelGGL((int4_stage_kernel<true>), sg, dim3(kStageThreads), 0, (hipStream_t)stream, a.x, (int)a.m, a.k,
                            (int)a.units, base, g.plane, rowback);
     else
-        hipLaunchKernelGGL((int4_stage_kernel<false>), sg, dim3(512), 0, (hipStream_t)stream, a.x, (int)a.m, a.k,
+        hipLaunchKernelGGL((int4_stage_kernel<false>), sg, dim3(kStageThreads), 0, (hipStream_t)stream, a.x, (int)a.m, a.k,
                            (int)a.units, base, g.plane, rowback);
     hipError_t e = hipGetLastError();
     if (e != hipSuccess) return (int)e;
-    int rc = a.x_bf16 ? launch_gemm_g<1>(a.group, a.zeros, p.waves, p.mt, g, stream)
-                      : launch_gemm_g<2>(a.group, a.zeros, p.waves, p.mt, g, stream);
+    int rc = a.x_bf16 ? launch_gemm_g<1>(a.group, a.zeros, p.mt, p.nt, g, stream)
+                      : launch_gemm_g<2>(a.group, a.zeros, p.mt, p.nt, g, stream);
     if (rc || p.ks == 1) return rc;
     const int64_t count = a.m * a.n;
     hipLaunchKernelGGL(int4_sum_kernel, dim3((unsigned)std::min<int64_t>((count + 255) / 256, 8192)), dim3(256), 0,

@@ -249,11 +249,11 @@ constexpr int kInt4Rows = 16;  // token rows of one launch_int4_rows
 int launch_int4_rows(const Int4Args &a, void *stream);
 // more rows (nnq_int4_gemm.hip): how m rows run (nnq_plan.cpp), with the scratch's offsets
 struct Int4GemmPlan {
-    int mt, waves, ks;           // 32-row tiles of a workgroup, its waves (32 columns each), K split
+    int mt, nt, ks;              // 32-row tiles of a workgroup, 32-column tiles of its waves, K split
     int row_blocks, col_blocks;  // workgroups along m and n
     size_t plane, rowback, slabs, bytes;
 };
-Int4GemmPlan int4_gemm_plan(int64_t m, int64_t n, int64_t k, int x_bf16);
+Int4GemmPlan int4_gemm_plan(int64_t m, int64_t n, int64_t k, int group, int x_bf16);
 int64_t int4_chunk_rows(int64_t m, int64_t k);  // rows of one launch_int4_gemm
 int launch_int4_gemm(const Int4Args &a, void *scratch, void *stream);
 int launch_int4_dequant(const Layout &L, const uint8_t *w, float *out, void *stream);

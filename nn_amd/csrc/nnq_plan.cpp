@@ -49,19 +49,38 @@ int64_t gemm_chunk_rows(int64_t m, int64_t k) {
     return std::min(m, std::max<int64_t>(1, rows));
 }
 
-// 4-bit prefill: blocks of up to four 32-row tiles, as even as m allows; eight waves (256 columns)
-// where that fills the chip, else four; K split until there is a workgroup per CU, but not below
-// four units a part.
-Int4GemmPlan int4_gemm_plan(int64_t m, int64_t n, int64_t k, int x_bf16) {
+// 4-bit prefill: the workgroup tile (mt x 32 rows, nt x 128 columns) and the K split of the least
+// estimated time.  c workgroups on a CU take c * step + lag per unit of 128 k (fitted on MI355X to
+// 20 to 640 rows of 1024 to 24576 columns, K 1024 to 12288: the choice is within 6% of the best of
+// all tiles and splits there); with K split the slabs are written and read back at 8.5 TB/s (they stay
+// in the last-level cache) by one launch more.  2 x 2 is left out where its registers spill (f32 x,
+// groups of 32: 512 x 12288 x 4096 in 108 us, 82 with 2 x 1).
+Int4GemmPlan int4_gemm_plan(int64_t m, int64_t n, int64_t k, int group, int x_bf16) {
     Int4GemmPlan p{};
     const int64_t cus = 256, tiles = (m + 31) / 32, units = (k + kInt4Unit - 1) / kInt4Unit;
-    const int64_t rb = (tiles + 3) / 4;
-    p.row_blocks = (int)rb;
-    p.mt = (int)((tiles + rb - 1) / rb);
-    p.waves = rb * ((n + 255) / 256) >= cus * 3 / 4 ? 8 : 4;
-    p.col_blocks = (int)((n + 32 * p.waves - 1) / (32 * p.waves));
+    static const double step[2][2][2] = {{{0.50, 0.85}, {0.95, 0}}, {{0.38, 0.70}, {0.62, 1.10}}};
+    static const double lag[2][2][2] = {{{0.20, 0.20}, {0.12, 0}}, {{0.10, 0.21}, {0.12, 0.23}}};
+    const int xb = x_bf16 ? 1 : 0;
+    double best = 1e30;
     int64_t ks = 1;
-    while (rb * p.col_blocks * ks * 2 <= cus * 3 / 2 && units / (ks * 2) >= 4) ks *= 2;
+    for (int mt = 1; mt <= 2; mt++)
+        for (int nt = 1; nt <= 2; nt++) {
+            if (mt == 2 && nt == 2 && (!xb || group == 32)) continue;
+            for (int64_t s = 1; s <= 8 && (s == 1 || units / s >= 2); s++) {
+                const int64_t wg = (tiles + mt - 1) / mt * ((n + 128 * nt - 1) / (128 * nt)) * s;
+                const double c = wg > 4 * cus ? (double)wg / cus : (double)((wg + cus - 1) / cus);
+                double us = (double)((units + s - 1) / s) * (c * step[xb][mt - 1][nt - 1] + lag[xb][mt - 1][nt - 1]);
+                if (s > 1) us += 3.0 + (double)(2 * s) * (double)m * (double)n * 4 / 8.5e6;
+                if (us < best) {
+                    best = us;
+                    p.mt = mt;
+                    p.nt = nt;
+                    ks = s;
+                }
+            }
+        }
+    p.row_blocks = (int)((tiles + p.mt - 1) / p.mt);
+    p.col_blocks = (int)((n + 128 * p.nt - 1) / (128 * p.nt));
     p.ks = (int)ks;
     const size_t planes = x_bf16 ? 1 : 2;
     p.plane = (size_t)tiles * (size_t)units * 8192;
@@ -92,11 +111,13 @@ LogprobPlan logprob_plan(int64_t m, int64_t n, int top, int elem) {
     return p;
 }
 
-// Logits of one chunk: at most 160 MB of f32, which the 256 MB last-level cache holds from the GEMM
-// that writes them to the log probabilities that read them, and whole 16-row MFMA tiles.
+// Chunks of at most 320 MiB of f32 logits (552 rows of 151936), as even as whole 64-row tiles of the
+// GEMMs allow: every chunk reads the weight again, so a short last one costs almost as much as a full
+// one (300 rows of 151936 x 4096 in 4 bits as 272 + 28: 618 us, in one 506).
 int64_t head_chunk_rows(int64_t m, int64_t n) {
-    const int64_t fit = ((int64_t)160 << 20) / (4 * n) / 16 * 16;
-    return std::min(m, std::max<int64_t>(16, fit));
+    const int64_t fit = ((int64_t)320 << 20) / (4 * n), tile = fit >= 64 ? 64 : 16;
+    const int64_t most = std::max<int64_t>(tile, fit / tile * tile), chunks = (m + most - 1) / most;
+    return std::min(m, ((m + chunks - 1) / chunks + tile - 1) / tile * tile);
 }
 
 // ---- dispatch rules ----------------------------------------------------------------

@@ -325,9 +325,9 @@ def test_linear_logprobs(fmt, m, xdt):
 
 
 def test_linear_logprobs_in_chunks():
-    """More rows than one chunk of logits holds (n = 600000: 64 rows), the last chunk shorter; x misaligned."""
+    """More rows than one chunk of logits holds (n = 1200001: 64 rows), the last chunk shorter; x misaligned."""
     import nn_amd
-    n, k, m = 600001, 128, 150
+    n, k, m = 1200001, 128, 150
     w = head("int4", n, k)
     flat = torch.randn(m * k + 1, device="cuda")
     x = flat[1:].view(m, k)

@@ -222,4 +222,5 @@ def test_logprob_plan(lib, top, elem):
     for n in (1, 1000, 151936, 1 << 24):
         for m in (1, 15, 16, 300, 100000):
             r = chunk(m, n)
-            assert 1 <= r <= m and (r == m or r % 16 == 0) and (r <= 16 or 4 * n * r <= 160 << 20)
+            assert 1 <= r <= m and (r == m or r % 16 == 0) and (r <= 16 or 4 * n * r <= 320 << 20)
+            assert r == m or m // r >= 1 and (m + r - 1) // r * r - m < 64 * ((m + r - 1) // r)  # even chunks
