@@ -27,27 +27,35 @@ __device__ __forceinline__ void load_scales(const uint8_t *rec, int r, uint32_t 
     }
 }
 
-template <int N>
-__device__ __forceinline__ float group_scale(const uint32_t (&s)[N], int g, int bf16) {
-    const uint32_t h = (s[g >> 1] >> (16 * (g & 1))) & 0xFFFFu;
-    return bf16 ? bf16_to_f32(h) : f16_to_f32(h);
+// all ones where scales are bf16, zero where they are f16, in a vector register: selecting by a scalar
+// condition would become branches between the MFMAs
+__device__ __forceinline__ uint32_t scale_mask(int bf16) {
+    uint32_t m = bf16 ? 0xFFFFFFFFu : 0u;
+    asm("" : "+v"(m));
+    return m;
 }
-
-// -(1024 + z) and -(64 + z) as packed f16 (z = 8 without zero points)
-template <bool Z>
-__device__ __forceinline__ void zero_consts(uint32_t zs, int g, uint32_t &c1, uint32_t &c2) {
-    if constexpr (Z) {
-        const uint32_t z = ((zs >> (8 * g)) & 0xFFu) * 0x00010001u;
-        c1 = 0xE400E400u | z;
-        c2 = 0xD400D400u | (z << 4);
-    } else {
-        c1 = 0xE408E408u;
-        c2 = 0xD480D480u;
-    }
+template <int N>
+__device__ __forceinline__ float group_scale(const uint32_t (&s)[N], int g, uint32_t mask) {
+    const uint32_t h = s[g >> 1] >> (16 * (g & 1));
+    const uint32_t b = (g & 1) ? s[g >> 1] & 0xFFFF0000u : h << 16, f = __float_as_uint(f16_to_f32(h & 0xFFFFu));
+    return __uint_as_float((b & mask) | (f & ~mask));
 }
 
 __device__ __forceinline__ uint32_t pk_add(uint32_t a, uint32_t b) {
     return __builtin_bit_cast(uint32_t, __builtin_bit_cast(half2v, a) + __builtin_bit_cast(half2v, b));
+}
+
+// -(1024 + z) and -(64 + z) as packed f16 (z = 8 without zero points), for byte g of zs: byte 0xE4 over
+// the zero point is the first, and adding 960 to it the second, exactly
+template <bool Z>
+__device__ __forceinline__ void zero_consts(uint32_t zs, int g, uint32_t &c1, uint32_t &c2) {
+    if constexpr (Z) {
+        c1 = __builtin_amdgcn_perm(0xE4E4E4E4u, zs, 0x04000400u + 0x00010001u * (uint32_t)g);
+        c2 = pk_add(c1, 0x63806380u);
+    } else {
+        c1 = 0xE408E408u;
+        c2 = 0xD480D480u;
+    }
 }
 
 // The masks and exponents of the codes' f16 form: held in registers (one scalar source per

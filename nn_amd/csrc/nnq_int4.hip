@@ -36,10 +36,27 @@ struct Unit {
     uint32_t z;                // GS zero points (8 bits each)
 };
 
+// A tile's records as a buffer: the lane's offset in a vector register, the unit's in a scalar one.
+// (and x: an offset past its end reads zeros)
+__device__ __forceinline__ __amdgpu_buffer_rsrc_t rsrc(const void *p, int64_t bytes) {
+    return __builtin_amdgcn_make_buffer_rsrc(const_cast<void *>(p), 0, (int)min(bytes, (int64_t)0x7FFFFFF0), 0x00020000);
+}
+// (the weight stream non-temporal; lq = 16 lane, and the offsets of the row's scales and zero points)
 template <int GS, bool Z>
-__device__ __forceinline__ void load_unit(const uint8_t *rec, int lane, Unit<GS, Z> &u) {
-    u.q = ldg128(rec + 16 * lane);
-    load_scales<GS, Z>(rec, lane & 15, u.s, u.z);
+__device__ __forceinline__ void load_unit(__amdgpu_buffer_rsrc_t t, int lq, int ls, int lz, int at, Unit<GS, Z> &u) {
+    u.q = __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(t, lq, at, 2));
+    if constexpr (GS == 1) {
+        u.s[0] = __builtin_amdgcn_raw_buffer_load_b16(t, ls, at, 2);
+        if constexpr (Z) u.z = __builtin_amdgcn_raw_buffer_load_b8(t, lz, at, 2);
+    } else if constexpr (GS == 2) {
+        u.s[0] = __builtin_amdgcn_raw_buffer_load_b32(t, ls, at, 2);
+        if constexpr (Z) u.z = __builtin_amdgcn_raw_buffer_load_b16(t, lz, at, 2);
+    } else {
+        const u32x2 s = __builtin_bit_cast(u32x2, __builtin_amdgcn_raw_buffer_load_b64(t, ls, at, 2));
+        u.s[0] = s[0];
+        u.s[1] = s[1];
+        if constexpr (Z) u.z = __builtin_amdgcn_raw_buffer_load_b32(t, lz, at, 2);
+    }
 }
 
 __device__ __forceinline__ void wave_fence() {
@@ -59,86 +76,112 @@ __device__ __forceinline__ uint32_t umax_row(uint32_t v) {
 enum { XBF16 = 0, XPAIR = 1, XPLANES = 2 };
 constexpr int planes(int xf) { return xf == XPLANES ? 2 : 1; }
 
-// x[0..m) of unit u -> A operands of the unit's four MFMAs (per plane) and the rows' powers of two
-// back; `buf` (4 KB) and `bk` (16 floats) are the wave's own.  Lane 16i + c takes columns 8c ..
-// 8c + 7 of row t0 + i.  A unit past K leaves zeros and back = 0.
-template <int XF>
-__device__ __forceinline__ void stage_unit(const Int4Args &a, int64_t u, int lane, uint16_t *buf, float *bk,
-                                           u32x4 (&A)[planes(XF)][4], float (&back)[4]) {
-    const int c = lane & 15, i4 = lane >> 4;
-    const int64_t k0 = u * kInt4Unit + 8 * c;
-    const bool in = k0 < a.k;  // K is a multiple of 32, so a lane's 8 columns are all in or all out
-    const int m = (int)a.m;
-    constexpr int kPass = planes(XF);
+// x[0..m) of the wave's units u0, u0 + waves, .. -> A operands of their MFMAs (per plane) and the rows'
+// power of two back (one for all the units); `buf` (4 KB) and `bk` (16 floats) are the wave's own.
+// Lane 16i + c takes columns 8c .. 8c + 7 of rows i, 4 + i, ..; every row's loads are issued before the
+// first is used.  A unit past K leaves zeros.
+template <int XF, int UPW>
+__device__ __forceinline__ void stage_units(const Int4Args &a, __amdgpu_buffer_rsrc_t rx, int u0, int waves, int lane, uint16_t *buf, float *bk,
+                                            u32x4 (&A)[UPW][planes(XF)][4], float (&back)[4]) {
+    constexpr int IT = XF == XPAIR ? 2 : 4, XR = XF == XBF16 ? 1 : 2;  // rows / 4, 16-byte loads of 8 columns
+    const int c = lane & 15, i4 = lane >> 4, m = (int)a.m;
+    u32x4 raw[IT][UPW][XR];
 #pragma unroll
-    for (int pl = 0; pl < kPass; pl++) {
-        for (int t0 = 0; t0 < m; t0 += 4) {
-            const int t = t0 + i4;
-            float v[8];
+    for (int it = 0; it < IT; it++)
+        if (4 * it < m) {
+            const int t = 4 * it + i4;
 #pragma unroll
-            for (int e = 0; e < 8; e++) v[e] = 0.f;
-            if (in && t < m) {
-                if constexpr (XF == XBF16) {
-                    const u32x4 r = *reinterpret_cast<const u32x4 *>(reinterpret_cast<const uint16_t *>(a.x) + t * a.k + k0);
+            for (int j = 0; j < UPW; j++) {
+                // (K is a multiple of 32, so a lane's 8 columns are all in or all out)
+                const int k0 = (u0 + j * waves) * kInt4Unit + 8 * c;
+                const int at = t < m && k0 < a.k ? (t * (int)a.k + k0) * 2 * XR : 0x7FFFFFF0;
 #pragma unroll
-                    for (int e = 0; e < 4; e++) {
-                        v[2 * e] = __uint_as_float(r[e] << 16);
-                        v[2 * e + 1] = __uint_as_float(r[e] & 0xFFFF0000u);
-                    }
-                } else {
-                    const floatx4 *p = reinterpret_cast<const floatx4 *>(reinterpret_cast<const float *>(a.x) + t * a.k + k0);
-                    const floatx4 r0 = p[0], r1 = p[1];
-#pragma unroll
-                    for (int e = 0; e < 4; e++) {
-                        v[e] = r0[e];
-                        v[4 + e] = r1[e];
-                    }
-                }
+                for (int e = 0; e < XR; e++)
+                    raw[it][j][e] = __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(rx, at, 16 * e, 0));
             }
-            // largest |x| of the row's 128 columns as bits (NaN above infinity above every number)
+        }
+    // the 8 values of a raw group
+    auto values = [&](const u32x4(&r)[XR], float(&v)[8]) {
+        if constexpr (XF == XBF16) {
+#pragma unroll
+            for (int e = 0; e < 4; e++) {
+                v[2 * e] = __uint_as_float(r[0][e] << 16);
+                v[2 * e + 1] = __uint_as_float(r[0][e] & 0xFFFF0000u);
+            }
+        } else {
+#pragma unroll
+            for (int e = 0; e < 8; e++) v[e] = __uint_as_float(r[e / 4][e % 4]);
+        }
+    };
+    float s[IT], b[IT];
+#pragma unroll
+    for (int it = 0; it < IT; it++)
+        if (4 * it < m) {
+            // largest |x| of the row's columns as bits (NaN above infinity above every number)
             uint32_t mx = 0;
 #pragma unroll
-            for (int e = 0; e < 8; e++) mx = max(mx, __float_as_uint(v[e]) & 0x7FFFFFFFu);
+            for (int j = 0; j < UPW; j++) {
+                float v[8];
+                values(raw[it][j], v);
+#pragma unroll
+                for (int e = 0; e < 8; e++) mx = max(mx, __float_as_uint(v[e]) & 0x7FFFFFFFu);
+            }
             mx = umax_row<0xB1>(mx);
             mx = umax_row<0x4E>(mx);
             mx = umax_row<0x141>(mx);
             mx = umax_row<0x140>(mx);
-            float s, b;
-            f16_prescale(__uint_as_float(mx), s, b);
-            u32x4 hi, lo;
-            split8<XF != XBF16>(v, s, hi, lo);
-            // operand (j, p) of row r at 16-byte slot (4j + p) * 16 + r: c = 4j + p
-            u32x4 *slot = reinterpret_cast<u32x4 *>(buf) + c * 16;
-            if (t < m) {
+            f16_prescale(__uint_as_float(mx), s[it], b[it]);
+            const int t = 4 * it + i4;
+            if (c == 0 && t < m) {
                 if constexpr (XF == XPAIR) {
-                    slot[2 * t] = hi;
-                    slot[2 * t + 1] = lo;
-                } else if constexpr (XF == XPLANES) {
-                    slot[t] = pl == 0 ? lo : hi;
+                    bk[2 * t] = b[it];
+                    bk[2 * t + 1] = b[it];
                 } else {
-                    slot[t] = hi;
-                }
-                if (c == 0) {
-                    if constexpr (XF == XPAIR) {
-                        bk[2 * t] = b;
-                        bk[2 * t + 1] = b;
-                    } else {
-                        bk[t] = b;
-                    }
+                    bk[t] = b[it];
                 }
             }
         }
-        wave_fence();
-        // rows past the tokens read what the buffer holds: MFMA rows are independent, theirs are not stored
+    // (the compiler would keep every row's widened values from above instead of widening them again)
 #pragma unroll
-        for (int j = 0; j < 4; j++) A[pl][j] = reinterpret_cast<const u32x4 *>(buf)[(4 * j + i4) * 16 + c];
-        if (pl == kPass - 1) {
-            const floatx4 b4 = *reinterpret_cast<const floatx4 *>(bk + 4 * i4);
+    for (int it = 0; it < IT; it++)
 #pragma unroll
-            for (int e = 0; e < 4; e++) back[e] = b4[e];
+        for (int j = 0; j < UPW; j++)
+#pragma unroll
+            for (int e = 0; e < XR; e++) asm volatile("" : "+v"(raw[it][j][e]));
+    // unit by unit, plane by plane through the buffer: operand (j, p) of row r at 16-byte slot
+    // (4j + p) * 16 + r, with c = 4j + p
+    u32x4 *slot = reinterpret_cast<u32x4 *>(buf) + c * 16;
+#pragma unroll
+    for (int j = 0; j < UPW; j++)
+#pragma unroll
+        for (int pl = 0; pl < planes(XF); pl++) {
+#pragma unroll
+            for (int it = 0; it < IT; it++)
+                if (4 * it < m) {
+                    const int t = 4 * it + i4;
+                    float v[8];
+                    values(raw[it][j], v);
+                    u32x4 hi, lo;
+                    split8<XF != XBF16>(v, s[it], hi, lo);
+                    if (t < m) {
+                        if constexpr (XF == XPAIR) {
+                            slot[2 * t] = hi;
+                            slot[2 * t + 1] = lo;
+                        } else {
+                            slot[t] = XF == XPLANES && pl == 0 ? lo : hi;
+                        }
+                    }
+                }
+            wave_fence();
+            // rows past the tokens read what the buffer holds: MFMA rows are independent, theirs are not stored
+#pragma unroll
+            for (int q = 0; q < 4; q++) A[j][pl][q] = reinterpret_cast<const u32x4 *>(buf)[(4 * q + i4) * 16 + c];
+            wave_fence();
         }
-        wave_fence();
-    }
+    const floatx4 b4 = *reinterpret_cast<const floatx4 *>(bk + 4 * i4);
+#pragma unroll
+    for (int e = 0; e < 4; e++) back[e] = b4[e];
+    wave_fence();
 }
 
 __device__ __forceinline__ uint64_t int4_argmax_key(float v, uint32_t idx) {
@@ -165,58 +208,45 @@ __global__ __launch_bounds__(1024) void int4_rows_kernel(Int4Args a) {
     const int c = lane & 15, p4 = lane >> 4;
 
     const CodeMasks km;
+    const uint32_t sm = scale_mask(a.scale_bf16);
+    const __amdgpu_buffer_rsrc_t rx = rsrc(a.x, a.m * a.k * (XF == XBF16 ? 2 : 4));
     u32x4 A[UPW][P][4];
-    float back[UPW][4];
-    float sum[R][4];
-    Unit<GS, Z> W[R][UPW], N[R][UPW];
+    float back[4];
+    Unit<GS, Z> W[R][UPW];
+    const int lq = 16 * lane, ls = 1024 + 2 * GS * c, lz = 1024 + 32 * GS + GS * c;
     // a tile or a unit that does not exist is read at the last that does: its A operands are zeros,
     // its outputs are not stored
-    auto load = [&](Unit<GS, Z>(&w)[R][UPW], int b, int pass) {
-#pragma unroll
-        for (int r = 0; r < R; r++)
-#pragma unroll
-            for (int j = 0; j < UPW; j++) {
-                const int64_t tile = min((int64_t)b * R + r, a.ntile - 1);
-                const int u = min((pass * UPW + j) * waves + wv, units - 1);
-                load_unit<GS, Z>(a.w + (size_t)(tile * units + u) * UB, lane, w[r][j]);
-            }
+    auto load = [&](int b, int pass, int r, int j) {
+        const int64_t tile = min((int64_t)b * R + r, a.ntile - 1);
+        const __amdgpu_buffer_rsrc_t rs = rsrc(a.w + (size_t)tile * units * UB, (int64_t)units * UB);
+        load_unit<GS, Z>(rs, lq, ls, lz, min((pass * UPW + j) * waves + wv, units - 1) * UB, W[r][j]);
     };
     uint64_t key = 0;
     int b = blockIdx.x, par = 0;
-    if (b < nblock) load(W, b, 0);
+    if (b < nblock)
+#pragma unroll
+        for (int r = 0; r < R; r++)
+#pragma unroll
+            for (int j = 0; j < UPW; j++) load(b, 0, r, j);
     bool first = true;
     for (; b < nblock; b += gridDim.x) {
+        float sum[R][4];
 #pragma unroll
         for (int r = 0; r < R; r++)
 #pragma unroll
             for (int i = 0; i < 4; i++) sum[r][i] = 0.f;
         for (int pass = 0; pass < npass; pass++) {
-            // the next step's loads: the next pass, or the next block's first
+            if (npass > 1 || first) stage_units<XF, UPW>(a, rx, pass * UPW * waves + wv, waves, lane, buf, bk, A, back);
+            first = false;
+            // the next step: the next pass, or the next block's first; a unit's registers are loaded for it
+            // as soon as they have been used
             const bool last = pass + 1 == npass;
-            const int nb = last ? b + (int)gridDim.x : b;
-            if (nb < nblock) load(N, nb, last ? 0 : pass + 1);
-            if (npass > 1 || first) {
+            const int nb = last ? b + (int)gridDim.x : b, np = last ? 0 : pass + 1;
+#pragma unroll
+            for (int r = 0; r < R; r++) {
+                float tot[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
                 for (int j = 0; j < UPW; j++) {
-                    const int u = (pass * UPW + j) * waves + wv;
-                    if (u < units) {
-                        stage_unit<XF>(a, u, lane, buf, bk, A[j], back[j]);
-                    } else {
-#pragma unroll
-                        for (int pl = 0; pl < P; pl++)
-#pragma unroll
-                            for (int q = 0; q < 4; q++) A[j][pl][q] = u32x4{0, 0, 0, 0};
-#pragma unroll
-                        for (int i = 0; i < 4; i++) back[j][i] = 0.f;
-                    }
-                }
-                first = false;
-            }
-#pragma unroll
-            for (int r = 0; r < R; r++)
-#pragma unroll
-                for (int j = 0; j < UPW; j++) {
-                    float tot[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
                     for (int g = 0; g < GS; g++) {
                         uint32_t c1, c2;
@@ -231,17 +261,18 @@ __global__ __launch_bounds__(1024) void int4_rows_kernel(Int4Args a) {
 #pragma unroll
                             for (int h = 0; h < 4 / GS; h++)
                                 acc = mfma16x16x32_f16(A[j][pl][g * (4 / GS) + h], B[h], acc);
-                        const float s = group_scale(W[r][j].s, g, a.scale_bf16);
+                        const float s = group_scale(W[r][j].s, g, sm);
 #pragma unroll
                         for (int i = 0; i < 4; i++) tot[i] = fmaf(s, acc[i], tot[i]);
-                    }
+                        // here: moved behind the loads' branch, the sums would keep every group's `acc`
 #pragma unroll
-                    for (int i = 0; i < 4; i++) sum[r][i] = fmaf(back[j][i], tot[i], sum[r][i]);
+                        for (int i = 0; i < 4; i++) asm volatile("" : "+v"(tot[i]));
+                    }
+                    if (nb < nblock) load(nb, np, r, j);
                 }
 #pragma unroll
-            for (int r = 0; r < R; r++)
-#pragma unroll
-                for (int j = 0; j < UPW; j++) W[r][j] = N[r][j];
+                for (int i = 0; i < 4; i++) sum[r][i] = fmaf(back[i], tot[i], sum[r][i]);
+            }
         }
         // lane 16p + c: rows 4p .. 4p + 3 of output column c, for each tile -> [wave][tile][token][16]
         float *rb = red + par * waves * R * 256;

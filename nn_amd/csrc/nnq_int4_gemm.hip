@@ -182,6 +182,7 @@ __global__ __launch_bounds__(W * 64, 2) void int4_gemm_kernel(Int4GemmArgs a) {
     // the matrix pipe with its own VALU work behind them.  (32 cycles of an MFMA hide six VALU
     // instructions.)
     const CodeMasks km;
+    const uint32_t sm = scale_mask(a.scale_bf16);
     floatx16 tot[MT][NT], part[MT][NT];
 #pragma unroll
     for (int mt = 0; mt < MT; mt++)
@@ -252,7 +253,7 @@ __global__ __launch_bounds__(W * 64, 2) void int4_gemm_kernel(Int4GemmArgs a) {
             }
             if (first)
 #pragma unroll
-                for (int nt = 0; nt < NT; nt++) sc[nt] = group_scale(w[nt].s, s / (8 / GS), a.scale_bf16);
+                for (int nt = 0; nt < NT; nt++) sc[nt] = group_scale(w[nt].s, s / (8 / GS), sm);
         }
         __builtin_amdgcn_sched_barrier(0);
         if (u + 1 < u1) store_a(buf ^ 1);  // (read by nobody since the barrier before this unit)
