@@ -71,6 +71,11 @@ __device__ __forceinline__ uint32_t umax_row(uint32_t v) {
     return v > o ? v : o;
 }
 
+template <int CTRL>
+__device__ __forceinline__ float add_row(float v) {
+    return v + __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(v), CTRL, 0xF, 0xF, true));
+}
+
 // token rows and A operand planes: bf16 x, 16 rows; f32 x, 8 tokens as row pairs (hi, lo); f32 x, 16
 // tokens as two planes (lo, hi)
 enum { XBF16 = 0, XPAIR = 1, XPLANES = 2 };
@@ -214,20 +219,23 @@ __global__ __launch_bounds__(1024) void int4_rows_kernel(Int4Args a) {
     float back[4];
     Unit<GS, Z> W[R][UPW];
     const int lq = 16 * lane, ls = 1024 + 2 * GS * c, lz = 1024 + 32 * GS + GS * c;
-    // a tile or a unit that does not exist is read at the last that does: its A operands are zeros,
-    // its outputs are not stored
-    auto load = [&](int b, int pass, int r, int j) {
-        const int64_t tile = min((int64_t)b * R + r, a.ntile - 1);
-        const __amdgpu_buffer_rsrc_t rs = rsrc(a.w + (size_t)tile * units * UB, (int64_t)units * UB);
-        load_unit<GS, Z>(rs, lq, ls, lz, min((pass * UPW + j) * waves + wv, units - 1) * UB, W[r][j]);
+    // a unit that does not exist is read at the last that does (its A operands are zeros), a tile that does
+    // not exist as a buffer of no bytes
+    auto tile_buffer = [&](int b, int r) {
+        const int64_t tile = (int64_t)b * R + r;
+        return rsrc(a.w + (size_t)min(tile, a.ntile - 1) * units * UB, tile < a.ntile ? (int64_t)units * UB : 0);
+    };
+    auto load = [&](__amdgpu_buffer_rsrc_t t, int pass, int r, int j) {
+        load_unit<GS, Z>(t, lq, ls, lz, min((pass * UPW + j) * waves + wv, units - 1) * UB, W[r][j]);
     };
     uint64_t key = 0;
     int b = blockIdx.x, par = 0;
-    if (b < nblock)
 #pragma unroll
-        for (int r = 0; r < R; r++)
+    for (int r = 0; r < R; r++) {
+        const __amdgpu_buffer_rsrc_t t = tile_buffer(b, r);
 #pragma unroll
-            for (int j = 0; j < UPW; j++) load(b, 0, r, j);
+        for (int j = 0; j < UPW; j++) load(t, 0, r, j);
+    }
     bool first = true;
     for (; b < nblock; b += gridDim.x) {
         float sum[R][4];
@@ -244,6 +252,7 @@ __global__ __launch_bounds__(1024) void int4_rows_kernel(Int4Args a) {
             const int nb = last ? b + (int)gridDim.x : b, np = last ? 0 : pass + 1;
 #pragma unroll
             for (int r = 0; r < R; r++) {
+                const __amdgpu_buffer_rsrc_t t = tile_buffer(nb, r);
                 float tot[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
                 for (int j = 0; j < UPW; j++) {
@@ -264,38 +273,41 @@ __global__ __launch_bounds__(1024) void int4_rows_kernel(Int4Args a) {
                         const float s = group_scale(W[r][j].s, g, sm);
 #pragma unroll
                         for (int i = 0; i < 4; i++) tot[i] = fmaf(s, acc[i], tot[i]);
-                        // here: moved behind the loads' branch, the sums would keep every group's `acc`
+                        // here: moved on, the sums would keep every group's `acc`
 #pragma unroll
                         for (int i = 0; i < 4; i++) asm volatile("" : "+v"(tot[i]));
                     }
-                    if (nb < nblock) load(nb, np, r, j);
+                    load(t, np, r, j);
                 }
 #pragma unroll
                 for (int i = 0; i < 4; i++) sum[r][i] = fmaf(back[i], tot[i], sum[r][i]);
             }
         }
-        // lane 16p + c: rows 4p .. 4p + 3 of output column c, for each tile -> [wave][tile][token][16]
-        float *rb = red + par * waves * R * 256;
+        // lane 16p + c: rows 4p .. 4p + 3 of output column c, for each tile -> [tile][token][column][17 waves]
+        float *rb = red + par * R * 256 * 17;
 #pragma unroll
         for (int r = 0; r < R; r++) {
-            float *o = rb + (wv * R + r) * 256 + c;
+            float *o = rb + (r * 256 + c) * 17 + wv;
             if constexpr (XF == XPAIR) {
-                if (2 * p4 < m) o[(2 * p4) * 16] = sum[r][0] + sum[r][1];
-                if (2 * p4 + 1 < m) o[(2 * p4 + 1) * 16] = sum[r][2] + sum[r][3];
+                if (2 * p4 < m) o[(2 * p4) * 272] = sum[r][0] + sum[r][1];
+                if (2 * p4 + 1 < m) o[(2 * p4 + 1) * 272] = sum[r][2] + sum[r][3];
             } else {
 #pragma unroll
                 for (int i = 0; i < 4; i++)
-                    if (4 * p4 + i < m) o[(4 * p4 + i) * 16] = sum[r][i];
+                    if (4 * p4 + i < m) o[(4 * p4 + i) * 272] = sum[r][i];
             }
         }
         __syncthreads();  // also: every wave is past its reads of the other buffer
-        for (int o = tid; o < R * 256; o += (int)blockDim.x) {
-            const int r = o >> 8, t = (o >> 4) & 15, col = o & 15;
-            if (t >= m) continue;
+        // a wave takes four outputs at a time, a wave's part of each to a lane of 16
+        for (int i = wv; i < R * m * 4; i += waves) {
+            const int r = (i >> 2) >= m, t = (i >> 2) - (r ? m : 0), col = 4 * (i & 3) + p4;
+            float v = c < waves ? rb[((r * 16 + t) * 16 + col) * 17 + c] : 0.f;
+            v = add_row<0xB1>(v);
+            v = add_row<0x4E>(v);
+            v = add_row<0x141>(v);
+            v = add_row<0x140>(v);
             const int64_t row = ((int64_t)b * R + r) * kTile + col;
-            float v = 0.f;
-            for (int w = 0; w < waves; w++) v += rb[(w * R + r) * 256 + t * 16 + col];
-            if (row < a.n) {
+            if (c == 0 && row < a.n) {
                 if (a.bias) v += a.bias[row];
                 if (a.y_bf16)
                     reinterpret_cast<uint16_t *>(a.y)[t * a.n + row] = (uint16_t)f32_to_bf16_bits(v);
@@ -307,7 +319,7 @@ __global__ __launch_bounds__(1024) void int4_rows_kernel(Int4Args a) {
         par ^= 1;
     }
     if (a.argmax_partial) {
-        // m = 1: threads r * 256 + col hold keys (0 elsewhere); one key per workgroup
+        // m = 1: lanes that stored outputs hold keys (0 elsewhere); one key per workgroup
         __syncthreads();
         unsigned long long *kr = reinterpret_cast<unsigned long long *>(red);
         for (int o = 32; o > 0; o >>= 1) {
@@ -342,7 +354,7 @@ int launch_rows_t(const Int4Args &a, void *stream) {
     while (waves > 4 && waves / 2 >= a.units) waves /= 2;
     const int64_t blocks = (a.ntile + R - 1) / R;
     const int64_t grid = std::min<int64_t>(blocks, (int64_t)cus() * (16 / waves));
-    const size_t lds = (size_t)waves * (4096 + 64 + 2 * R * 1024);
+    const size_t lds = (size_t)waves * (4096 + 64) + 2 * R * 256 * 17 * 4;
     if (a.argmax_count) *a.argmax_count = grid;
     auto *kernel = int4_rows_kernel<XF, GS, Z, R, UPW>;
     hipError_t e = allow_lds(reinterpret_cast<const void *>(kernel), lds);
