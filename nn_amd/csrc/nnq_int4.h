@@ -80,6 +80,33 @@ __device__ __forceinline__ u32x4 codes_f16(uint32_t w, uint32_t c1, uint32_t c2,
                  code_pair(w, 3, c1, c2, k)};
 }
 
+typedef unsigned short ushort2v __attribute__((ext_vector_type(2)));
+__device__ __forceinline__ uint32_t pk_max_u16(uint32_t a, uint32_t b) {
+    return __builtin_bit_cast(uint32_t, __builtin_elementwise_max(__builtin_bit_cast(ushort2v, a), __builtin_bit_cast(ushort2v, b)));
+}
+// bf16 pairs as f16 under a power of two, in integers: a bf16 of exponent field e becomes an f16 of field
+// e - E0 with the same 7 mantissa bits, where E0 = max(E - 29, 0) brings the row's largest magnitude
+// (field E) into [2^14, 2^15).  Exact but for values below 2^-29 of that magnitude, which keep an error
+// of at most that; subnormals convert exactly where they count (E0 = 0).  A row with a NaN or infinity
+// (field 255) becomes NaN throughout.
+struct Bf16Scale {
+    uint32_t sub, nan;
+    float back;  // 2^(E0 - 112): f16 value times back = bf16 value
+    __device__ __forceinline__ explicit Bf16Scale(uint32_t largest) {  // bits of the largest magnitude
+        const int e = (int)(largest >> 7), e0 = max(e - 29, 0);
+        sub = (uint32_t)e0 * 0x00800080u;
+        nan = e == 255 ? 0x7E007E00u : 0u;
+        back = __uint_as_float((uint32_t)(e0 + 15) << 23);
+    }
+    __device__ __forceinline__ uint32_t f16(uint32_t x) const {
+        const ushort2v d = __builtin_elementwise_sub_sat(__builtin_bit_cast(ushort2v, x & 0x7FFF7FFFu),
+                                                         __builtin_bit_cast(ushort2v, sub));
+        const ushort2v h = d << (unsigned short)3;
+        return (x & 0x80008000u) | __builtin_bit_cast(uint32_t, h) | nan;
+    }
+    Bf16Scale() = default;
+};
+
 // v * s (s a power of two that brings it into f16's range) as f16, and with LO what that leaves, as f16
 template <bool LO>
 __device__ __forceinline__ void split8(const float (&v)[8], float s, u32x4 &hi, u32x4 &lo) {

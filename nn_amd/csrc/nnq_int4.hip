@@ -9,7 +9,7 @@
 //    B operands of four 16x16x32 f16 MFMAs.  The next step's loads are in flight while the
 //    current one is computed.
 //  * x of a unit is scaled by a power of two per token row (its largest magnitude into
-//    [2^14, 2^15)) to f16 (bf16 x; exact but for values below 2^-31 of that magnitude) or to an
+//    [2^14, 2^15)) to f16 (bf16 x; exact but for values below 2^-29 of that magnitude) or to an
 //    f16 hi + lo pair (f32 x, ~22 bits), and passes through a wave-private LDS buffer into A
 //    operands.  With K in one pass they stay in registers for all the workgroup's tiles.
 //  * A code becomes an exact f16 integer: (w & 0x000F000F) | 0x6400.. is 1024 + q, and
@@ -19,6 +19,7 @@
 //  * Every product is exact in f32; a group's sum is scaled in f32 (one rounding for the scale,
 //    one per addition).  The waves' sums meet in LDS, one barrier per block of tiles.
 #include <algorithm>
+#include <type_traits>
 
 #include "nnq_device.h"
 #include "nnq_int4.h"
@@ -105,48 +106,44 @@ __device__ __forceinline__ void stage_units(const Int4Args &a, __amdgpu_buffer_r
                     raw[it][j][e] = __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(rx, at, 16 * e, 0));
             }
         }
-    // the 8 values of a raw group
-    auto values = [&](const u32x4(&r)[XR], float(&v)[8]) {
-        if constexpr (XF == XBF16) {
-#pragma unroll
-            for (int e = 0; e < 4; e++) {
-                v[2 * e] = __uint_as_float(r[0][e] << 16);
-                v[2 * e + 1] = __uint_as_float(r[0][e] & 0xFFFF0000u);
-            }
-        } else {
-#pragma unroll
-            for (int e = 0; e < 8; e++) v[e] = __uint_as_float(r[e / 4][e % 4]);
-        }
+    struct Scale {
+        float s, back;
     };
-    float s[IT], b[IT];
+    typename std::conditional<XF == XBF16, Bf16Scale, Scale>::type sc[IT];
 #pragma unroll
     for (int it = 0; it < IT; it++)
         if (4 * it < m) {
             // largest |x| of the row's columns as bits (NaN above infinity above every number)
             uint32_t mx = 0;
 #pragma unroll
-            for (int j = 0; j < UPW; j++) {
-                float v[8];
-                values(raw[it][j], v);
+            for (int j = 0; j < UPW; j++)
 #pragma unroll
-                for (int e = 0; e < 8; e++) mx = max(mx, __float_as_uint(v[e]) & 0x7FFFFFFFu);
-            }
+                for (int e = 0; e < 4 * XR; e++) {
+                    if constexpr (XF == XBF16)
+                        mx = pk_max_u16(mx, raw[it][j][0][e] & 0x7FFF7FFFu);
+                    else
+                        mx = max(mx, raw[it][j][e / 4][e % 4] & 0x7FFFFFFFu);
+                }
+            if constexpr (XF == XBF16) mx = max(mx & 0xFFFFu, mx >> 16);
             mx = umax_row<0xB1>(mx);
             mx = umax_row<0x4E>(mx);
             mx = umax_row<0x141>(mx);
             mx = umax_row<0x140>(mx);
-            f16_prescale(__uint_as_float(mx), s[it], b[it]);
+            if constexpr (XF == XBF16)
+                sc[it] = Bf16Scale(mx);
+            else
+                f16_prescale(__uint_as_float(mx), sc[it].s, sc[it].back);
             const int t = 4 * it + i4;
             if (c == 0 && t < m) {
                 if constexpr (XF == XPAIR) {
-                    bk[2 * t] = b[it];
-                    bk[2 * t + 1] = b[it];
+                    bk[2 * t] = sc[it].back;
+                    bk[2 * t + 1] = sc[it].back;
                 } else {
-                    bk[t] = b[it];
+                    bk[t] = sc[it].back;
                 }
             }
         }
-    // (the compiler would keep every row's widened values from above instead of widening them again)
+    // (the compiler would keep every row's masked values from above instead of masking them again)
 #pragma unroll
     for (int it = 0; it < IT; it++)
 #pragma unroll
@@ -164,10 +161,16 @@ __device__ __forceinline__ void stage_units(const Int4Args &a, __amdgpu_buffer_r
             for (int it = 0; it < IT; it++)
                 if (4 * it < m) {
                     const int t = 4 * it + i4;
-                    float v[8];
-                    values(raw[it][j], v);
                     u32x4 hi, lo;
-                    split8<XF != XBF16>(v, s[it], hi, lo);
+                    if constexpr (XF == XBF16) {
+#pragma unroll
+                        for (int e = 0; e < 4; e++) hi[e] = sc[it].f16(raw[it][j][0][e]);
+                    } else {
+                        float v[8];
+#pragma unroll
+                        for (int e = 0; e < 8; e++) v[e] = __uint_as_float(raw[it][j][e / 4][e % 4]);
+                        split8<true>(v, sc[it].s, hi, lo);
+                    }
                     if (t < m) {
                         if constexpr (XF == XPAIR) {
                             slot[2 * t] = hi;
