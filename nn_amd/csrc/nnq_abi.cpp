@@ -606,12 +606,14 @@ static Int4Args int4_args(const nnq_weight *w, const void *x, nnq_dtype x_dtype,
     return a;
 }
 
+static size_t int4_launch_scratch(const nnq_weight *w, int64_t m, nnq_dtype x_dtype) {
+    const int xb = x_dtype == NNQ_BF16;
+    return m <= kInt4Rows ? int4_rows_scratch(m, w->L.n, w->L.k, xb) : int4_gemm_plan(m, w->L.n, w->L.k, w->L.group, xb).bytes;
+}
+
 static size_t int4_scratch_bytes(const nnq_weight *w, int64_t m, nnq_dtype x_dtype) {
-    if (m <= kInt4Rows) return 0;
     const int64_t mc = int4_chunk_rows(m, w->L.k), tail = m % mc;
-    size_t b = int4_gemm_plan(mc, w->L.n, w->L.k, w->L.group, x_dtype == NNQ_BF16).bytes;
-    if (tail > kInt4Rows) b = std::max(b, int4_gemm_plan(tail, w->L.n, w->L.k, w->L.group, x_dtype == NNQ_BF16).bytes);
-    return b;
+    return std::max(int4_launch_scratch(w, mc, x_dtype), tail ? int4_launch_scratch(w, tail, x_dtype) : 0);
 }
 
 static int dispatch_int4(const nnq_weight *w, const void *x, nnq_dtype x_dtype, int64_t m, const float *bias, void *y,
@@ -628,7 +630,7 @@ static int dispatch_int4(const nnq_weight *w, const void *x, nnq_dtype x_dtype, 
     for (int64_t m0 = 0; m0 < m; m0 += mc) {
         const Int4Args a = int4_args(w, (const uint8_t *)x + (size_t)m0 * w->L.k * xe, x_dtype, std::min(mc, m - m0),
                                      bias, (uint8_t *)y + (size_t)m0 * w->L.n * ye, y_dtype);
-        int e = a.m <= kInt4Rows ? launch_int4_rows(a, stream) : launch_int4_gemm(a, scr, stream);
+        int e = a.m <= kInt4Rows ? launch_int4_rows(a, scr, stream) : launch_int4_gemm(a, scr, stream);
         if (e) return hip_fail((hipError_t)e, "int4 linear launch");
     }
     return NNQ_OK;
@@ -792,7 +794,7 @@ static int linear_argmax(const nnq_weight *w, const float *x, int64_t k, const f
         Int4Args a = int4_args(w, x, NNQ_F32, 1, bias, logits, NNQ_F32);
         a.argmax_partial = keys;
         a.argmax_count = &nkeys;
-        e = launch_int4_rows(a, stream);
+        e = launch_int4_rows(a, nullptr, stream);
     } else {
         GemvArgs a{};
         a.qs = w->dev;

@@ -82,67 +82,75 @@ __device__ __forceinline__ float add_row(float v) {
 enum { XBF16 = 0, XPAIR = 1, XPLANES = 2 };
 constexpr int planes(int xf) { return xf == XPLANES ? 2 : 1; }
 
-// x[0..m) of the wave's units u0, u0 + waves, .. -> A operands of their MFMAs (per plane) and the rows'
-// power of two back (one for all the units); `buf` (4 KB) and `bk` (16 floats) are the wave's own.
-// Lane 16i + c takes columns 8c .. 8c + 7 of rows i, 4 + i, ..; every row's loads are issued before the
-// first is used.  A unit past K leaves zeros.
-template <int XF, int UPW>
-__device__ __forceinline__ void stage_units(const Int4Args &a, __amdgpu_buffer_rsrc_t rx, int u0, int waves, int lane, uint16_t *buf, float *bk,
-                                            u32x4 (&A)[UPW][planes(XF)][4], float (&back)[4]) {
-    constexpr int IT = XF == XPAIR ? 2 : 4, XR = XF == XBF16 ? 1 : 2;  // rows / 4, 16-byte loads of 8 columns
+// x of one pass as loaded: lane 16i + c holds columns 8c .. 8c + 7 of rows i, 4 + i, .. (IT of them) of
+// each of the wave's units.
+template <int XF, int IT, int UPW>
+struct XRaw {
+    static constexpr int XR = XF == XBF16 ? 1 : 2;  // 16-byte loads of 8 columns
+    u32x4 r[IT][UPW][XR];
+};
+// (units u0, u0 + waves, ..; rows past m and columns from kend on are zeros.  K is a multiple of 32, so a
+// lane's 8 columns are all in or all out.)
+template <int XF, int IT, int UPW>
+__device__ __forceinline__ void load_x(const Int4Args &a, __amdgpu_buffer_rsrc_t rx, int u0, int waves, int kend, int lane,
+                                       XRaw<XF, IT, UPW> &x) {
+    constexpr int XR = XRaw<XF, IT, UPW>::XR;
     const int c = lane & 15, i4 = lane >> 4, m = (int)a.m;
-    u32x4 raw[IT][UPW][XR];
 #pragma unroll
-    for (int it = 0; it < IT; it++)
-        if (4 * it < m) {
-            const int t = 4 * it + i4;
+    for (int it = 0; it < IT; it++) {
+        const int t = 4 * it + i4;
 #pragma unroll
-            for (int j = 0; j < UPW; j++) {
-                // (K is a multiple of 32, so a lane's 8 columns are all in or all out)
-                const int k0 = (u0 + j * waves) * kInt4Unit + 8 * c;
-                const int at = t < m && k0 < a.k ? (t * (int)a.k + k0) * 2 * XR : 0x7FFFFFF0;
+        for (int j = 0; j < UPW; j++) {
+            const int k0 = (u0 + j * waves) * kInt4Unit + 8 * c;
+            const int at = t < m && k0 < kend ? (t * (int)a.k + k0) * 2 * XR : 0x7FFFFFF0;
 #pragma unroll
-                for (int e = 0; e < XR; e++)
-                    raw[it][j][e] = __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(rx, at, 16 * e, 0));
-            }
+            for (int e = 0; e < XR; e++)
+                x.r[it][j][e] = __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(rx, at, 16 * e, 0));
         }
+    }
+}
+
+// x of one pass -> A operands of its units' MFMAs (per plane) and the rows' power of two back (one for
+// all the units); `buf` (4 KB) and `bk` (16 floats) are the wave's own.  No branches: rows past the
+// tokens are zeros (a branch per row group would spill the operands).
+template <int XF, int IT, int UPW>
+__device__ __forceinline__ void stage_units(int lane, uint16_t *buf, float *bk, XRaw<XF, IT, UPW> &x,
+                                            u32x4 (&A)[UPW][planes(XF)][4], float (&back)[4]) {
+    constexpr int XR = XRaw<XF, IT, UPW>::XR;
+    const int c = lane & 15, i4 = lane >> 4;
+    u32x4(&raw)[IT][UPW][XR] = x.r;
     struct Scale {
         float s, back;
     };
     typename std::conditional<XF == XBF16, Bf16Scale, Scale>::type sc[IT];
 #pragma unroll
-    for (int it = 0; it < IT; it++)
-        if (4 * it < m) {
-            // largest |x| of the row's columns as bits (NaN above infinity above every number)
-            uint32_t mx = 0;
+    for (int it = 0; it < IT; it++) {
+        // largest |x| of the row's columns as bits (NaN above infinity above every number)
+        uint32_t mx = 0;
 #pragma unroll
-            for (int j = 0; j < UPW; j++)
+        for (int j = 0; j < UPW; j++)
 #pragma unroll
-                for (int e = 0; e < 4 * XR; e++) {
-                    if constexpr (XF == XBF16)
-                        mx = pk_max_u16(mx, raw[it][j][0][e] & 0x7FFF7FFFu);
-                    else
-                        mx = max(mx, raw[it][j][e / 4][e % 4] & 0x7FFFFFFFu);
-                }
-            if constexpr (XF == XBF16) mx = max(mx & 0xFFFFu, mx >> 16);
-            mx = umax_row<0xB1>(mx);
-            mx = umax_row<0x4E>(mx);
-            mx = umax_row<0x141>(mx);
-            mx = umax_row<0x140>(mx);
-            if constexpr (XF == XBF16)
-                sc[it] = Bf16Scale(mx);
-            else
-                f16_prescale(__uint_as_float(mx), sc[it].s, sc[it].back);
-            const int t = 4 * it + i4;
-            if (c == 0 && t < m) {
-                if constexpr (XF == XPAIR) {
-                    bk[2 * t] = sc[it].back;
-                    bk[2 * t + 1] = sc[it].back;
-                } else {
-                    bk[t] = sc[it].back;
-                }
+            for (int e = 0; e < 4 * XR; e++) {
+                if constexpr (XF == XBF16)
+                    mx = pk_max_u16(mx, raw[it][j][0][e] & 0x7FFF7FFFu);
+                else
+                    mx = max(mx, raw[it][j][e / 4][e % 4] & 0x7FFFFFFFu);
             }
-        }
+        if constexpr (XF == XBF16) mx = max(mx & 0xFFFFu, mx >> 16);
+        mx = umax_row<0xB1>(mx);
+        mx = umax_row<0x4E>(mx);
+        mx = umax_row<0x141>(mx);
+        mx = umax_row<0x140>(mx);
+        if constexpr (XF == XBF16)
+            sc[it] = Bf16Scale(mx);
+        else
+            f16_prescale(__uint_as_float(mx), sc[it].s, sc[it].back);
+        const int t = 4 * it + i4;  // (the 16 lanes of a row store the same value)
+        if constexpr (XF == XPAIR)
+            *reinterpret_cast<float2 *>(bk + 2 * t) = float2{sc[it].back, sc[it].back};
+        else
+            bk[t] = sc[it].back;
+    }
     // (the compiler would keep every row's masked values from above instead of masking them again)
 #pragma unroll
     for (int it = 0; it < IT; it++)
@@ -158,30 +166,27 @@ __device__ __forceinline__ void stage_units(const Int4Args &a, __amdgpu_buffer_r
 #pragma unroll
         for (int pl = 0; pl < planes(XF); pl++) {
 #pragma unroll
-            for (int it = 0; it < IT; it++)
-                if (4 * it < m) {
-                    const int t = 4 * it + i4;
-                    u32x4 hi, lo;
-                    if constexpr (XF == XBF16) {
+            for (int it = 0; it < IT; it++) {
+                const int t = 4 * it + i4;
+                u32x4 hi, lo;
+                if constexpr (XF == XBF16) {
 #pragma unroll
-                        for (int e = 0; e < 4; e++) hi[e] = sc[it].f16(raw[it][j][0][e]);
-                    } else {
-                        float v[8];
+                    for (int e = 0; e < 4; e++) hi[e] = sc[it].f16(raw[it][j][0][e]);
+                } else {
+                    float v[8];
 #pragma unroll
-                        for (int e = 0; e < 8; e++) v[e] = __uint_as_float(raw[it][j][e / 4][e % 4]);
-                        split8<true>(v, sc[it].s, hi, lo);
-                    }
-                    if (t < m) {
-                        if constexpr (XF == XPAIR) {
-                            slot[2 * t] = hi;
-                            slot[2 * t + 1] = lo;
-                        } else {
-                            slot[t] = XF == XPLANES && pl == 0 ? lo : hi;
-                        }
-                    }
+                    for (int e = 0; e < 8; e++) v[e] = __uint_as_float(raw[it][j][e / 4][e % 4]);
+                    split8<true>(v, sc[it].s, hi, lo);
                 }
+                if constexpr (XF == XPAIR) {
+                    slot[2 * t] = hi;
+                    slot[2 * t + 1] = lo;
+                } else {
+                    slot[t] = XF == XPLANES && pl == 0 ? lo : hi;
+                }
+            }
             wave_fence();
-            // rows past the tokens read what the buffer holds: MFMA rows are independent, theirs are not stored
+            // rows past 4 IT read what the buffer holds: MFMA rows are independent, theirs are not stored
 #pragma unroll
             for (int q = 0; q < 4; q++) A[j][pl][q] = reinterpret_cast<const u32x4 *>(buf)[(4 * q + i4) * 16 + c];
             wave_fence();
@@ -198,8 +203,9 @@ __device__ __forceinline__ uint64_t int4_argmax_key(float v, uint32_t idx) {
     return ((uint64_t)((b & 0x80000000u) ? ~b : (b | 0x80000000u)) << 32) | (0xFFFFFFFFu - idx);
 }
 
-// Blocks b = blockIdx.x, + gridDim.x, ... of R tiles; passes over K of waves * UPW units.
-template <int XF, int GS, bool Z, int R, int UPW>
+// Part kp = blockIdx.x % ks of K, in passes of waves * UPW units, over blocks blockIdx.x / ks, + gridDim.x
+// / ks, ... of R tiles, for up to 4 IT token rows.
+template <int XF, int IT, int GS, bool Z, int R, int UPW>
 __global__ __launch_bounds__(1024) void int4_rows_kernel(Int4Args a) {
     constexpr int P = planes(XF);
     constexpr int UB = int4_unit_bytes(kInt4Unit / GS, Z);
@@ -211,7 +217,10 @@ __global__ __launch_bounds__(1024) void int4_rows_kernel(Int4Args a) {
     float *bk = reinterpret_cast<float *>(lds + waves * 4096 + wv * 64);
     float *red = reinterpret_cast<float *>(lds + waves * (4096 + 64));
     const int m = (int)a.m, units = (int)a.units;
-    const int npass = (units + waves * UPW - 1) / (waves * UPW);
+    const int ks = a.ks, kp = (int)blockIdx.x % ks, step = (int)gridDim.x / ks;
+    const int ub = (int)((int64_t)units * kp / ks), ue = (int)((int64_t)units * (kp + 1) / ks);  // this part's units
+    const int kend = (int)min(a.k, (int64_t)ue * kInt4Unit);
+    const int npass = (ue - ub + waves * UPW - 1) / (waves * UPW);
     const int nblock = (int)((a.ntile + R - 1) / R);
     const int c = lane & 15, p4 = lane >> 4;
 
@@ -229,30 +238,35 @@ __global__ __launch_bounds__(1024) void int4_rows_kernel(Int4Args a) {
         return rsrc(a.w + (size_t)min(tile, a.ntile - 1) * units * UB, tile < a.ntile ? (int64_t)units * UB : 0);
     };
     auto load = [&](__amdgpu_buffer_rsrc_t t, int pass, int r, int j) {
-        load_unit<GS, Z>(t, lq, ls, lz, min((pass * UPW + j) * waves + wv, units - 1) * UB, W[r][j]);
+        load_unit<GS, Z>(t, lq, ls, lz, min(ub + (pass * UPW + j) * waves + wv, ue - 1) * UB, W[r][j]);
     };
     uint64_t key = 0;
-    int b = blockIdx.x, par = 0;
+    int b = (int)blockIdx.x / ks, par = 0;
+    auto x_of = [&](int pass, XRaw<XF, IT, UPW> &x) {
+        load_x<XF, IT, UPW>(a, rx, ub + pass * UPW * waves + wv, waves, kend, lane, x);
+    };
+    // x before the weights: loads return in order, and x comes from L2
+    XRaw<XF, IT, UPW> x;
+    x_of(0, x);
 #pragma unroll
     for (int r = 0; r < R; r++) {
         const __amdgpu_buffer_rsrc_t t = tile_buffer(b, r);
 #pragma unroll
         for (int j = 0; j < UPW; j++) load(t, 0, r, j);
     }
-    bool first = true;
-    for (; b < nblock; b += gridDim.x) {
+    stage_units<XF, IT, UPW>(lane, buf, bk, x, A, back);
+    if (IT == 1 && npass > 1) x_of(1, x);
+    for (; b < nblock; b += step) {
         float sum[R][4];
 #pragma unroll
         for (int r = 0; r < R; r++)
 #pragma unroll
             for (int i = 0; i < 4; i++) sum[r][i] = 0.f;
         for (int pass = 0; pass < npass; pass++) {
-            if (npass > 1 || first) stage_units<XF, UPW>(a, rx, pass * UPW * waves + wv, waves, lane, buf, bk, A, back);
-            first = false;
             // the next step: the next pass, or the next block's first; a unit's registers are loaded for it
             // as soon as they have been used
             const bool last = pass + 1 == npass;
-            const int nb = last ? b + (int)gridDim.x : b, np = last ? 0 : pass + 1;
+            const int nb = last ? b + step : b, np = last ? 0 : pass + 1;
 #pragma unroll
             for (int r = 0; r < R; r++) {
                 const __amdgpu_buffer_rsrc_t t = tile_buffer(nb, r);
@@ -285,6 +299,18 @@ __global__ __launch_bounds__(1024) void int4_rows_kernel(Int4Args a) {
 #pragma unroll
                 for (int i = 0; i < 4; i++) sum[r][i] = fmaf(back[i], tot[i], sum[r][i]);
             }
+            // with K in one pass A stays.  With one row group the x of the pass after next is on its way
+            // while the next is computed; more have no registers for that
+            if (npass > 1 && nb < nblock) {
+                if constexpr (IT > 1) {
+                    XRaw<XF, IT, UPW> xn;
+                    x_of(np, xn);
+                    stage_units<XF, IT, UPW>(lane, buf, bk, xn, A, back);
+                } else {
+                    stage_units<XF, IT, UPW>(lane, buf, bk, x, A, back);
+                    x_of(np + 1 < npass ? np + 1 : 0, x);
+                }
+            }
         }
         // lane 16p + c: rows 4p .. 4p + 3 of output column c, for each tile -> [tile][token][column][17 waves]
         float *rb = red + par * R * 256 * 17;
@@ -311,6 +337,10 @@ __global__ __launch_bounds__(1024) void int4_rows_kernel(Int4Args a) {
             v = add_row<0x140>(v);
             const int64_t row = ((int64_t)b * R + r) * kTile + col;
             if (c == 0 && row < a.n) {
+                if (ks > 1) {
+                    a.slabs[((int64_t)kp * m + t) * a.n + row] = v;
+                    continue;
+                }
                 if (a.bias) v += a.bias[row];
                 if (a.y_bf16)
                     reinterpret_cast<uint16_t *>(a.y)[t * a.n + row] = (uint16_t)f32_to_bf16_bits(v);
@@ -350,39 +380,40 @@ int cus() {
     return n[dev];
 }
 
-template <int XF, int GS, bool Z, int R, int UPW>
+template <int XF, int IT, int GS, bool Z, int R, int UPW>
 int launch_rows_t(const Int4Args &a, void *stream) {
     // a wave for every unit, up to 16; the chip holds 16 / waves workgroups per CU
+    const int64_t part = (a.units + a.ks - 1) / a.ks;
     int waves = 16;
-    while (waves > 4 && waves / 2 >= a.units) waves /= 2;
+    while (waves > 4 && waves / 2 >= part) waves /= 2;
     const int64_t blocks = (a.ntile + R - 1) / R;
-    const int64_t grid = std::min<int64_t>(blocks, (int64_t)cus() * (16 / waves));
+    const int64_t grid = std::min<int64_t>(blocks, std::max<int64_t>(1, (int64_t)cus() * (16 / waves) / a.ks)) * a.ks;
     const size_t lds = (size_t)waves * (4096 + 64) + 2 * R * 256 * 17 * 4;
     if (a.argmax_count) *a.argmax_count = grid;
-    auto *kernel = int4_rows_kernel<XF, GS, Z, R, UPW>;
+    auto *kernel = int4_rows_kernel<XF, IT, GS, Z, R, UPW>;
     hipError_t e = allow_lds(reinterpret_cast<const void *>(kernel), lds);
     if (e != hipSuccess) return (int)e;
     hipLaunchKernelGGL(kernel, dim3((unsigned)grid), dim3(waves * 64), lds, (hipStream_t)stream, a);
     return (int)hipGetLastError();
 }
 
-template <int XF, int GS, bool Z>
+template <int XF, int IT, int GS, bool Z>
 int launch_rows_r(const Int4Args &a, void *stream) {
-    if constexpr (XF == XPLANES) return launch_rows_t<XF, GS, Z, 1, 1>(a, stream);
-    else return a.ntile > 2 * (int64_t)cus() ? launch_rows_t<XF, GS, Z, 2, 2>(a, stream)
-                                             : launch_rows_t<XF, GS, Z, 1, 2>(a, stream);
+    if constexpr (XF == XPLANES) return launch_rows_t<XF, IT, GS, Z, 1, 1>(a, stream);
+    else return a.ntile > 2 * (int64_t)cus() ? launch_rows_t<XF, IT, GS, Z, 2, 2>(a, stream)
+                                             : launch_rows_t<XF, IT, GS, Z, 1, 2>(a, stream);
 }
 
-template <int XF>
+template <int XF, int IT>
 int launch_rows_x(const Int4Args &a, void *stream) {
     if (a.zeros) {
-        if (a.group == 128) return launch_rows_r<XF, 1, true>(a, stream);
-        if (a.group == 64) return launch_rows_r<XF, 2, true>(a, stream);
-        return launch_rows_r<XF, 4, true>(a, stream);
+        if (a.group == 128) return launch_rows_r<XF, IT, 1, true>(a, stream);
+        if (a.group == 64) return launch_rows_r<XF, IT, 2, true>(a, stream);
+        return launch_rows_r<XF, IT, 4, true>(a, stream);
     }
-    if (a.group == 128) return launch_rows_r<XF, 1, false>(a, stream);
-    if (a.group == 64) return launch_rows_r<XF, 2, false>(a, stream);
-    return launch_rows_r<XF, 4, false>(a, stream);
+    if (a.group == 128) return launch_rows_r<XF, IT, 1, false>(a, stream);
+    if (a.group == 64) return launch_rows_r<XF, IT, 2, false>(a, stream);
+    return launch_rows_r<XF, IT, 4, false>(a, stream);
 }
 
 // Bit-exact decode: (q - z) has at most 5 bits and the scale 11, so the product is exact in f32.
@@ -414,11 +445,22 @@ __global__ __launch_bounds__(256) void dequant_int4_kernel(const uint8_t *w, int
 
 }  // namespace
 
-int launch_int4_rows(const Int4Args &a, void *stream) {
-    if (a.m < 1 || a.m > kInt4Rows || a.units < 1 || a.ntile < 1 || (a.argmax_partial && a.m != 1))
+int launch_int4_rows(const Int4Args &g, void *scratch, void *stream) {
+    Int4Args a = g;
+    a.ks = scratch ? int4_rows_split(a.m, a.n, a.k, a.x_bf16) : 1;
+    a.slabs = reinterpret_cast<float *>(scratch);
+    if (a.m < 1 || a.m > kInt4Rows || a.units < 1 || a.ntile < 1 || (a.argmax_partial && (a.m != 1 || a.ks != 1)))
         return (int)hipErrorInvalidValue;
-    if (a.x_bf16) return launch_rows_x<XBF16>(a, stream);
-    return a.m <= 8 ? launch_rows_x<XPAIR>(a, stream) : launch_rows_x<XPLANES>(a, stream);
+    int e;
+    if (a.x_bf16)
+        e = a.m <= 4   ? launch_rows_x<XBF16, 1>(a, stream)
+            : a.m <= 8 ? launch_rows_x<XBF16, 2>(a, stream) : launch_rows_x<XBF16, 4>(a, stream);
+    else if (a.m <= 8)
+        e = a.m <= 4 ? launch_rows_x<XPAIR, 1>(a, stream) : launch_rows_x<XPAIR, 2>(a, stream);
+    else
+        e = launch_rows_x<XPLANES, 4>(a, stream);
+    if (e || a.ks == 1) return e;
+    return launch_int4_sum(a.slabs, a.ks, a.m, a.n, a.bias, a.y, a.y_bf16, stream);
 }
 
 int launch_int4_dequant(const Layout &L, const uint8_t *w, float *out, void *stream) {

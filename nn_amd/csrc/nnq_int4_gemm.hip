@@ -364,9 +364,13 @@ int launch_int4_gemm(const Int4Args &a, void *scratch, void *stream) {
     int rc = a.x_bf16 ? launch_gemm_g<1>(a.group, a.zeros, p.mt, p.nt, g, stream)
                       : launch_gemm_g<2>(a.group, a.zeros, p.mt, p.nt, g, stream);
     if (rc || p.ks == 1) return rc;
-    const int64_t count = a.m * a.n;
+    return launch_int4_sum(slabs, p.ks, a.m, a.n, a.bias, a.y, a.y_bf16, stream);
+}
+
+int launch_int4_sum(const float *slabs, int ks, int64_t m, int64_t n, const float *bias, void *y, int y_bf16, void *stream) {
+    const int64_t count = m * n;
     hipLaunchKernelGGL(int4_sum_kernel, dim3((unsigned)std::min<int64_t>((count + 255) / 256, 8192)), dim3(256), 0,
-                       (hipStream_t)stream, slabs, p.ks, count, a.n, a.bias, a.y, a.y_bf16);
+                       (hipStream_t)stream, slabs, ks, count, n, bias, y, y_bf16);
     return (int)hipGetLastError();
 }
 

@@ -244,9 +244,16 @@ struct Int4Args {
     int64_t ntile, units;
     unsigned long long *argmax_partial;  // optional (m = 1): argmax keys, at most ntile of them
     int64_t *argmax_count;               //   and how many the launch writes
+    int ks;                              // (set by the launch: parts of K, their sums in slabs [ks][m][n])
+    float *slabs;
 };
 constexpr int kInt4Rows = 16;  // token rows of one launch_int4_rows
-int launch_int4_rows(const Int4Args &a, void *stream);
+// scratch: int4_rows_scratch bytes, or null for a launch that does not split K
+int launch_int4_rows(const Int4Args &a, void *scratch, void *stream);
+int int4_rows_split(int64_t m, int64_t n, int64_t k, int x_bf16);
+size_t int4_rows_scratch(int64_t m, int64_t n, int64_t k, int x_bf16);
+// y = the slabs' sum in order (+ bias)
+int launch_int4_sum(const float *slabs, int ks, int64_t m, int64_t n, const float *bias, void *y, int y_bf16, void *stream);
 // more rows (nnq_int4_gemm.hip): how m rows run (nnq_plan.cpp), with the scratch's offsets
 struct Int4GemmPlan {
     int mt, nt, ks;              // 32-row tiles of a workgroup, 32-column tiles of its waves, K split

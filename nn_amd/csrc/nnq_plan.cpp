@@ -49,6 +49,23 @@ int64_t gemm_chunk_rows(int64_t m, int64_t k) {
     return std::min(m, std::max<int64_t>(1, rows));
 }
 
+// Parts of K in a 4-bit call of up to 16 rows.  Sixteen waves hold 32 units of x at a time (16 with f32
+// planes); five rows and more of a longer K split it over workgroups, each of which converts its part of x
+// once for all its tiles and leaves f32 slabs to one launch more (us, split / in passes: 12 bf16 rows of
+// 4096 x 12288 17.4 / 19.8, 8192 x 8192 17.8 / 25.3, 6 f32 rows of 4096 x 12288 16.4 / 18.3).  Up to eight
+// bf16 rows over no more tiles than CUs convert too little for that (5 rows of 4096 x 12288 13.7 / 12.6,
+// 1024 x 8192 10.1 / 8.7; 8192 x 8192 13.6 / 16.8), and up to four rows have the next pass's x in flight.
+int int4_rows_split(int64_t m, int64_t n, int64_t k, int x_bf16) {
+    const int64_t held = (!x_bf16 && m > 8 ? 16 : 32) * kInt4Unit;
+    if (m <= 4 || (x_bf16 && m <= 8 && n <= 256 * kTile)) return 1;
+    return (int)std::min<int64_t>(8, (k + held - 1) / held);
+}
+
+size_t int4_rows_scratch(int64_t m, int64_t n, int64_t k, int x_bf16) {
+    const int ks = int4_rows_split(m, n, k, x_bf16);
+    return ks > 1 ? (size_t)ks * (size_t)m * (size_t)n * 4 : 0;
+}
+
 // 4-bit prefill: the workgroup tile (mt x 32 rows, nt x 128 columns) and the K split of the least
 // estimated time.  c workgroups on a CU take c * step + lag per unit of 128 k (fitted on MI355X to
 // 20 to 640 rows of 1024 to 24576 columns, K 1024 to 12288: the choice is within 6% of the best of
