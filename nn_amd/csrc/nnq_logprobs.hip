@@ -95,12 +95,44 @@ struct LpArgs {
     int64_t *top_id;
 };
 
+// Sum and maximum over the wave's 64 lanes, the same in every lane, without LDS: DPP within the rows
+// of 16, lane swaps between them.  Every lane must be active.
+template <int CTRL>
+__device__ __forceinline__ uint32_t lane_of(uint32_t v) {
+    return (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, CTRL, 0xF, 0xF, true);
+}
+template <class F>
+__device__ __forceinline__ uint32_t across(uint32_t v, F &&f) {
+    v = f(v, lane_of<0xB1>(v));   // lane ^ 1
+    v = f(v, lane_of<0x4E>(v));   // lane ^ 2
+    v = f(v, lane_of<0x141>(v));  // the other quad of 8
+    v = f(v, lane_of<0x140>(v));  // the other half of 16
+    const auto p = __builtin_amdgcn_permlane16_swap(v, v, false, false);
+    v = f(p[0], p[1]);
+    const auto q = __builtin_amdgcn_permlane32_swap(v, v, false, false);
+    return f(q[0], q[1]);
+}
+__device__ __forceinline__ float sum64(float v) {
+    return __uint_as_float(across(__float_as_uint(v), [](uint32_t a, uint32_t b) {
+        return __float_as_uint(__uint_as_float(a) + __uint_as_float(b));
+    }));
+}
+__device__ __forceinline__ float max64(float v) {
+    return __uint_as_float(across(__float_as_uint(v), [](uint32_t a, uint32_t b) {
+        return __float_as_uint(fmaxf(__uint_as_float(a), __uint_as_float(b)));
+    }));
+}
+__device__ __forceinline__ uint32_t sum64u(uint32_t v) {
+    return across(v, [](uint32_t a, uint32_t b) { return a + b; });
+}
+
 // The largest t with at least `want` lanes' or elements' keys >= t, count(t) counting them
 // (non-increasing in t; count(0) >= want).
-template <class F>
+// BITS: only the leading ones are settled (a smaller t).
+template <int BITS, class F>
 __device__ __forceinline__ uint32_t largest_with(int want, F &&count) {
     uint32_t t = 0;
-    for (uint32_t bit = 0x80000000u; bit; bit >>= 1)
+    for (uint32_t bit = 0x80000000u; bit >> (BITS == 32 ? 0 : 32 - BITS); bit >>= 1)
         if (count(t | bit) >= want) t |= bit;
     return t;
 }
@@ -141,7 +173,7 @@ __global__ __launch_bounds__(kSegWaves * 64) void logprob_seg_kernel(LpArgs a) {
     float lm = x[0];
 #pragma unroll
     for (int e = 1; e < kPer; e++) lm = fmaxf(lm, x[e]);
-    const float mx = wave_max(lm);
+    const float mx = max64(lm);
     const float ref = mx == kNegInf ? 0.f : mx;
     float r = 0.f, s = 0.f;
     int cnt = 0;
@@ -154,24 +186,32 @@ __global__ __launch_bounds__(kSegWaves * 64) void logprob_seg_kernel(LpArgs a) {
         r += top ? 0.f : ex;
         s = fmaf(fmaxf(d, -1e30f), ex, s);  // (d = -inf: its e^d is 0)
     }
-    r = wave_sum(r);
-    s = wave_sum(s);
+    r = sum64(r);
+    s = sum64(s);
     const int64_t at = rl * a.nseg + seg;
     if (lane == 0) a.stat[at] = SegStat{mx, r, s, (uint32_t)cnt};
 
     if constexpr (RANK) {
+        // a segment before the token's counts equal logits, one after it does not
+        const int64_t first = seg * kSeg - off;
         uint32_t before = 0;
         if (ask) {
+            if (first > tok) {
 #pragma unroll
-            for (int e = 0; e < kPer; e++) {
-                before += __popcll(__ballot(x[e] > lt));
-                const uint64_t same = __ballot(x[e] == lt);
-                if (same) {  // (slots outside the row are -inf, as a masked token is)
-                    const int64_t i = base + (e / V) * 64 * V + e % V;
-                    before += __popcll(same & __ballot(i >= 0 && i < tok));
+                for (int e = 0; e < kPer; e++) before += x[e] > lt;
+            } else if (first >= 0 && first + kSeg <= tok) {
+#pragma unroll
+                for (int e = 0; e < kPer; e++) before += x[e] >= lt;
+            } else {  // (slots outside the row are -inf, as a masked token is)
+                const int64_t from = -base, to = tok - base;  // places of logits 0 and tok, from the lane's first
+#pragma unroll
+                for (int e = 0; e < kPer; e++) {
+                    const int place = (e / V) * 64 * V + e % V;
+                    before += x[e] > lt || (x[e] == lt && place >= from && place < to);
                 }
             }
         }
+        before = sum64u(before);
         if (lane == 0) a.before[at] = before;
     }
 
@@ -179,14 +219,16 @@ __global__ __launch_bounds__(kSegWaves * 64) void logprob_seg_kernel(LpArgs a) {
         __shared__ uint64_t list[kSegWaves][64];
         const int want = a.top;
         const uint32_t mine = lm == lm ? ord(lm) : 0;  // (no number in the lane)
-        const uint32_t lanes = largest_with(want, [&](uint32_t k) { return __popcll(__ballot(mine >= k)); });
-        float t = unord(max(lanes, kOrdNegInf));  // (-inf is no candidate)
-        int total = 0;
+        // (its leading 16 bits do: a bound at most 2^-7 of its size below lets hardly more candidates in)
+        const uint32_t lanes = largest_with<16>(want, [&](uint32_t k) { return __popcll(__ballot(mine >= k)); });
+        float t = unord(max(lanes, kOrdNegInf + 1));  // (-inf is no candidate)
+        // the lane's candidates as bits, element 0 the highest
+        uint32_t bits = 0;
 #pragma unroll
-        for (int e = 0; e < kPer; e++) total += __popcll(__ballot(x[e] >= t && x[e] > kNegInf));
-        int32_t upto = 0x7FFFFFFF;  // logits equal to t count up to this place of the segment
-        if (total > a.slots) {
-            t = unord(largest_with(want, [&](uint32_t k) {
+        for (int e = 0; e < kPer; e++) bits = bits + bits + (x[e] >= t);
+        const int total = (int)sum64u(__popc(bits));
+        if (total > a.slots) {  // uniform
+            t = unord(largest_with<32>(want, [&](uint32_t k) {
                 const float f = unord(k);
                 int c = 0;
 #pragma unroll
@@ -206,140 +248,165 @@ __global__ __launch_bounds__(kSegWaves * 64) void logprob_seg_kernel(LpArgs a) {
                     c += __popcll(__ballot(x[e] == t && (uint32_t)((e / V) * 64 * V + lane * V + e % V) < (b | bit)));
                 if (c < need) b |= bit;
             }
-            upto = (int32_t)b;
-        }
-        int at_list = 0;
+            const int upto = (int)b;  // logits equal to t count up to this place of the segment
+            bits = 0;
 #pragma unroll
-        for (int e = 0; e < kPer; e++) {
-            const int place = (e / V) * 64 * V + lane * V + e % V;
-            const bool in = x[e] > kNegInf && (x[e] > t || (x[e] == t && place <= upto));
-            const uint64_t b = __ballot(in);
-            if (b) {
-                if (in) {
-                    const int slot = at_list + __builtin_amdgcn_mbcnt_hi((uint32_t)(b >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)b, 0));
-                    if (slot < 64) list[wv][slot] = cand_key(x[e], (uint32_t)(base + (e / V) * 64 * V + e % V));
-                }
-                at_list += __popcll(b);
+            for (int e = 0; e < kPer; e++) {
+                const int place = (e / V) * 64 * V + lane * V + e % V;
+                bits = bits + bits + (x[e] > kNegInf && (x[e] > t || (x[e] == t && place <= upto)));
             }
+        }
+        // a round takes one candidate of every lane that has any
+        int listed = 0;
+        while (__ballot(bits != 0)) {
+            const uint64_t b = __ballot(bits != 0);
+            const int e = bits ? __clz(bits) : 0;
+            float v = x[0];
+#pragma unroll
+            for (int i = 1; i < kPer; i++) v = i == e ? x[i] : v;
+            if (bits) {
+                const int slot = listed + __builtin_amdgcn_mbcnt_hi((uint32_t)(b >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)b, 0));
+                if (slot < 64) list[wv][slot] = cand_key(v, (uint32_t)(base + (e / V) * 64 * V + e % V));
+            }
+            listed += __popcll(b);
+            bits &= ~(0x80000000u >> e);
         }
         __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
         __builtin_amdgcn_wave_barrier();
         __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
-        if (lane < a.slots) a.cand[at * a.slots + lane] = lane < at_list ? list[wv][lane] : 0ull;
+        if (lane < a.slots) a.cand[at * a.slots + lane] = lane < listed ? list[wv][lane] : 0ull;
     }
 }
 
-// sum (or max) over the workgroup of kJoinThreads, the same value in every thread; `tmp` holds
-// one value per wave and is free again after the call
-template <class T, class F>
-__device__ __forceinline__ T join_reduce(T v, T *tmp, F &&f) {
-    for (int o = 32; o > 0; o >>= 1) v = f(v, __shfl_xor(v, o, 64));
-    __syncthreads();
-    if ((threadIdx.x & 63) == 0) tmp[threadIdx.x >> 6] = v;
-    __syncthreads();
-    v = tmp[0];
-#pragma unroll
-    for (int w = 1; w < kJoinThreads / 64; w++) v = f(v, tmp[w]);
-    return v;
-}
-
-template <class T>
+// One workgroup per row.  What it needs is loaded at once (a thread's first segment, its first kHeld
+// keys, the token and its logit), and three barriers separate: the maxima; the sums against the row's
+// maximum, and the bound of the N-th largest key; the list of candidates at or above it.
+constexpr int kHeld = 8;
+template <class T, bool TOP>
 __global__ __launch_bounds__(kJoinThreads) void logprob_join_kernel(LpArgs a) {
-    __shared__ float tf[kJoinThreads / 64];
-    __shared__ uint32_t tu[kJoinThreads / 64];
-    __shared__ uint64_t list[kJoinList];
-    __shared__ uint64_t maxima[kJoinThreads];
-    __shared__ uint32_t listed, bound;
-    const int tid = threadIdx.x, lane = tid & 63;
+    constexpr int NW = kJoinThreads / 64;
+    struct Part {
+        float r, s;
+        uint32_t cnt, before;
+    };
+    __shared__ float wmax[NW];
+    __shared__ Part part[NW];
+    __shared__ uint64_t list[TOP ? kJoinList : 1], maxima[TOP ? kJoinThreads : 1];
+    __shared__ uint32_t listed, bound, counts[NW];
+    const int tid = threadIdx.x, lane = tid & 63, wv = tid >> 6;
     const int64_t rl = blockIdx.x, row = a.row0 + rl;
     const SegStat *st = a.stat + rl * a.nseg;
-    const auto add = [](auto u, auto v) { return u + v; };
-    const auto larger = [](auto u, auto v) { return u > v ? u : v; };
-    float mx = kNegInf;
-    for (int64_t i = tid; i < a.nseg; i += kJoinThreads) mx = fmaxf(mx, st[i].mx);
-    mx = join_reduce(mx, tf, larger);
-    // each segment's sums move by e^(its maximum - the row's); a row without a logit above -inf gives
-    // -inf - -inf = NaN here, and a NaN among the logits came with its segment's sums
-    float r = 0.f, s = 0.f;
-    uint32_t cnt = 0;
-    for (int64_t i = tid; i < a.nseg; i += kJoinThreads) {
-        const SegStat q = st[i];
-        const float d = q.mx - mx;
-        if (d == 0.f) {
-            cnt += q.cnt;
-            r += q.r;
-            s += q.s;
-        } else {
-            const float f = expf(d), z = (float)q.cnt + q.r;
-            r += f * z;
-            s += f * fmaf(fmaxf(d, -1e30f), z, q.s);
-        }
-    }
-    r = join_reduce(r, tf, add);
-    s = join_reduce(s, tf, add);
-    cnt = join_reduce(cnt, tu, add);
-    r += (float)cnt - 1.f;  // (exact up to 2^24 equal maxima)
-    if (mx == kNegInf) r = __uint_as_float(0x7FC00000u);
-    const float lz = log1pf(r);
-    const float nan = __uint_as_float(0x7FC00000u);
-    if (tid == 0) {
-        const int64_t tok = a.tokens[row];
-        const bool ask = tok >= 0 && tok < a.n;
-        const float lt = ask ? widen<T>(reinterpret_cast<const T *>(a.logits)[row * a.stride + tok]) : nan;
-        a.logprob[row] = (lt - mx) - lz;
-        if (a.entropy) a.entropy[row] = lz - s / (1.f + r);
-    }
-    if (a.rank) {
-        uint32_t before = 0;
-        for (int64_t i = tid; i < a.nseg; i += kJoinThreads) before += a.before[rl * a.nseg + i];
-        before = join_reduce(before, tu, add);
-        if (tid == 0) {
-            const float lp = a.logprob[row];  // this thread's own store
-            a.rank[row] = lp == lp ? (int64_t)before : -1;
-        }
-    }
-    if (a.top == 0) return;
-
-    // The top N of the segments' candidates.  As in a segment: the N-th largest of the maxima of 64
-    // parts bounds the N-th largest key's value from below.
     const uint64_t *c = a.cand + rl * a.nseg * a.slots;
-    const int64_t total = a.nseg * a.slots;
-    uint64_t best = 0;
-    for (int64_t i = tid; i < total; i += kJoinThreads) best = larger(best, c[i]);
-    maxima[tid] = best;
+    const int64_t keys = a.nseg * a.slots;
+    const float nan = __uint_as_float(0x7FC00000u);
+    const int64_t tok = a.tokens[row];
+    const bool ask = tok >= 0 && tok < a.n;
+    const float lt = ask ? widen<T>(reinterpret_cast<const T *>(a.logits)[row * a.stride + tok]) : nan;
+    SegStat q{kNegInf, 0.f, 0.f, 0};
+    if (tid < a.nseg) q = st[tid];
+    uint64_t held[kHeld], best = 0;
+    if constexpr (TOP) {
+#pragma unroll
+        for (int i = 0; i < kHeld; i++) held[i] = tid + i * kJoinThreads < keys ? c[tid + i * kJoinThreads] : 0ull;
+#pragma unroll
+        for (int i = 0; i < kHeld; i++) best = max(best, held[i]);
+        for (int64_t i = tid + kHeld * kJoinThreads; i < keys; i += kJoinThreads) best = max(best, c[i]);
+        maxima[tid] = best;
+    }
+    float mx = q.mx;
+    for (int64_t i = tid + kJoinThreads; i < a.nseg; i += kJoinThreads) mx = fmaxf(mx, st[i].mx);
+    mx = max64(mx);
+    if (lane == 0) wmax[wv] = mx;
     if (tid == 0) listed = 0;
     __syncthreads();
-    if (tid < 64) {
+
+    mx = wmax[0];
+#pragma unroll
+    for (int w = 1; w < NW; w++) mx = fmaxf(mx, wmax[w]);
+    // each segment's sums move by e^(its maximum - the row's); a row without a logit above -inf gives
+    // -inf - -inf = NaN here, and a NaN among the logits came with its segment's sums
+    Part t{0.f, 0.f, 0, 0};
+    auto add = [&](const SegStat &g) {
+        const float d = g.mx - mx;
+        if (d == 0.f) {
+            t.cnt += g.cnt;
+            t.r += g.r;
+            t.s += g.s;
+        } else {
+            const float f = expf(d), z = (float)g.cnt + g.r;
+            t.r += f * z;
+            t.s += f * fmaf(fmaxf(d, -1e30f), z, g.s);
+        }
+    };
+    if (tid < a.nseg) add(q);
+    for (int64_t i = tid + kJoinThreads; i < a.nseg; i += kJoinThreads) add(st[i]);
+    if (a.rank)
+        for (int64_t i = tid; i < a.nseg; i += kJoinThreads) t.before += a.before[rl * a.nseg + i];
+    t.r = sum64(t.r);
+    t.s = sum64(t.s);
+    t.cnt = sum64u(t.cnt);
+    t.before = sum64u(t.before);
+    if (lane == 0) part[wv] = t;
+    if (TOP && wv == 0) {
+        // as in a segment: the N-th largest of the maxima of 64 parts
         uint64_t m = maxima[lane];
 #pragma unroll
-        for (int w = 1; w < kJoinThreads / 64; w++) m = larger(m, maxima[64 * w + lane]);
+        for (int w = 1; w < NW; w++) m = max(m, maxima[64 * w + lane]);
         const uint32_t v = (uint32_t)(m >> 32);
-        const uint32_t t = largest_with(a.top, [&](uint32_t k) { return __popcll(__ballot(v >= k)); });
-        if (lane == 0) bound = t;
+        const uint32_t b = largest_with<16>(a.top, [&](uint32_t k) { return __popcll(__ballot(v >= k)); });
+        if (lane == 0) bound = b;
     }
     __syncthreads();
+
+    t = part[0];
+#pragma unroll
+    for (int w = 1; w < NW; w++) {
+        t.r += part[w].r;
+        t.s += part[w].s;
+        t.cnt += part[w].cnt;
+        t.before += part[w].before;
+    }
+    float r = t.r + ((float)t.cnt - 1.f);  // (exact up to 2^24 equal maxima)
+    if (mx == kNegInf) r = nan;
+    const float lz = log1pf(r);
+    if (tid == 0) {
+        const float lp = (lt - mx) - lz;
+        a.logprob[row] = lp;
+        if (a.entropy) a.entropy[row] = lz - t.s / (1.f + r);
+        if (a.rank) a.rank[row] = lp == lp ? (int64_t)t.before : -1;
+    }
+    if constexpr (!TOP) return;
+
     uint64_t low = max((uint64_t)bound << 32, (uint64_t)1);
-    const auto collect = [&]() {
-        for (int64_t i = tid; i < total; i += kJoinThreads) {
-            const uint64_t k = c[i];
-            if (k >= low) {
-                const uint32_t at = atomicAdd(&listed, 1u);
-                if (at < kJoinList) list[at] = k;
-            }
+    auto take = [&](uint64_t k) {
+        if (k >= low) {
+            const uint32_t at = atomicAdd(&listed, 1u);
+            if (at < kJoinList) list[at] = k;
         }
+    };
+    auto collect = [&]() {
+#pragma unroll
+        for (int i = 0; i < kHeld; i++) take(held[i]);
+        for (int64_t i = tid + kHeld * kJoinThreads; i < keys; i += kJoinThreads) take(c[i]);
         __syncthreads();
     };
     collect();
     if (listed > kJoinList) {
         // very many equal values: the exact N-th largest key (keys are unique), bit by bit
-        __syncthreads();
-        uint64_t t = 0;
+        uint64_t least = 0;
         for (uint64_t bit = 1ull << 63; bit; bit >>= 1) {
             uint32_t k = 0;
-            for (int64_t i = tid; i < total; i += kJoinThreads) k += c[i] >= (t | bit);
-            if (join_reduce(k, tu, add) >= (uint32_t)a.top) t |= bit;
+            for (int64_t i = tid; i < keys; i += kJoinThreads) k += c[i] >= (least | bit);
+            k = sum64u(k);
+            __syncthreads();  // (the counts of the last bit have been read)
+            if (lane == 0) counts[wv] = k;
+            __syncthreads();
+            k = 0;
+#pragma unroll
+            for (int w = 0; w < NW; w++) k += counts[w];
+            if (k >= (uint32_t)a.top) least |= bit;
         }
-        low = max(t, (uint64_t)1);
+        low = max(least, (uint64_t)1);
         if (tid == 0) listed = 0;
         __syncthreads();
         collect();
@@ -374,7 +441,10 @@ int launch_lp(const LpArgs &a, int64_t rows, void *stream) {
         hipLaunchKernelGGL((logprob_seg_kernel<T, false, false>), grid, block, 0, (hipStream_t)stream, a);
     hipError_t e = hipGetLastError();
     if (e != hipSuccess) return (int)e;
-    hipLaunchKernelGGL((logprob_join_kernel<T>), dim3((unsigned)rows), dim3(kJoinThreads), 0, (hipStream_t)stream, a);
+    if (a.top)
+        hipLaunchKernelGGL((logprob_join_kernel<T, true>), dim3((unsigned)rows), dim3(kJoinThreads), 0, (hipStream_t)stream, a);
+    else
+        hipLaunchKernelGGL((logprob_join_kernel<T, false>), dim3((unsigned)rows), dim3(kJoinThreads), 0, (hipStream_t)stream, a);
     return (int)hipGetLastError();
 }
 
