@@ -475,17 +475,18 @@ class TokenLogprobs(NamedTuple):
     logits: Optional[torch.Tensor] = None          # f32 [..., n] (linear_logprobs with return_logits)
 
 
-def _logprob_outputs(rows, batch, n, top_n, ranks, device):
+def _logprob_outputs(batch, n, top_n, ranks, device):
     if not 0 <= int(top_n) <= min(32, n):
         raise InvalidShape(f"top_n {top_n} out of range (0 to 32, at most the {n} logits)")
-    lp = torch.empty(2, rows, dtype=torch.float32, device=device)
-    ids = torch.empty(rows * (int(bool(ranks)) + int(top_n)), dtype=torch.int64, device=device)
-    rk = ids[:rows] if ranks else None
-    ti = ids[rows * int(bool(ranks)):] if top_n else None
-    tl = torch.empty(rows * int(top_n), dtype=torch.float32, device=device) if top_n else None
-    ptrs = (_ptr(lp), lp.data_ptr() + 4 * rows, _ptr(rk), _ptr(tl), _ptr(ti))
-    view = lambda t, *more: None if t is None else t.view((*batch, *more))  # noqa: E731
-    return ptrs, TokenLogprobs(view(lp[0]), view(lp[1]), view(rk), view(tl, int(top_n)), view(ti, int(top_n)))
+    top, rk, tl, ti = int(top_n), None, None, None
+    # (a small call is bound by its host side, at 1 to 2 us a tensor: whole allocations, no views)
+    lp, ent = torch.empty((2, *batch), dtype=torch.float32, device=device).unbind(0)
+    if ranks:
+        rk = torch.empty(batch, dtype=torch.int64, device=device)
+    if top:
+        tl = torch.empty((*batch, top), dtype=torch.float32, device=device)
+        ti = torch.empty((*batch, top), dtype=torch.int64, device=device)
+    return (_ptr(lp), _ptr(ent), _ptr(rk), _ptr(tl), _ptr(ti)), TokenLogprobs(lp, ent, rk, tl, ti)
 
 
 def _token_ids(tokens, batch, device):
@@ -495,6 +496,8 @@ def _token_ids(tokens, batch, device):
         raise ShapeMismatch(f"tokens must be {list(batch)}, one per row of logits, got {list(tokens.shape)}")
     if tokens.is_floating_point() or tokens.is_complex() or tokens.dtype == torch.bool:
         raise Unsupported(f"tokens must be integers, got {tokens.dtype}")
+    if tokens.dtype is torch.int64 and tokens.device == device and tokens.is_contiguous():
+        return tokens
     return tokens.to(device=device, dtype=torch.int64).contiguous()
 
 
@@ -523,7 +526,7 @@ def token_logprobs(logits: torch.Tensor, tokens, top_n: int = 0, ranks: bool = F
         v = v.contiguous()
     rows = tok.numel()
     stride = v.stride(0) if v.dim() == 2 else n
-    ptrs, out = _logprob_outputs(rows, batch, n, top_n, ranks, v.device)
+    ptrs, out = _logprob_outputs(batch, n, top_n, ranks, v.device)
     with _on_device(v):
         _check(_lib.load().nnq_token_logprobs(_ptr(v), _DTYPE[v.dtype], rows, n, stride, _ptr(tok), int(top_n), *ptrs,
                                               _stream(v)))
@@ -546,7 +549,7 @@ def linear_logprobs(x: torch.Tensor, weight: QuantizedWeight, tokens, bias: Opti
     batch = xv.shape[:-1]
     tok = _token_ids(tokens, batch, xv.device)
     rows = tok.numel()
-    ptrs, out = _logprob_outputs(rows, batch, n, top_n, ranks, xv.device)
+    ptrs, out = _logprob_outputs(batch, n, top_n, ranks, xv.device)
     logits = xv.new_empty((*batch, n), dtype=torch.float32) if return_logits else None
     with _on_device(xv):
         _check(_lib.load().nnq_linear_logprobs(weight.handle, _ptr(xv), _DTYPE[xv.dtype], rows, k, _ptr(bias),

@@ -185,14 +185,13 @@ def test_python_logprob_refusals():
     from nn_amd.quantized import _logprob_outputs, _token_ids
     for top in (-1, 33, 9):
         with pytest.raises(nn_amd.InvalidShape):
-            _logprob_outputs(2, (2,), 8 if top == 9 else 100, top, False, "cpu")
+            _logprob_outputs((2,), 8 if top == 9 else 100, top, False, "cpu")
     with pytest.raises(nn_amd.ShapeMismatch):
         _token_ids(torch.zeros(3, dtype=torch.int64), (2,), "cpu")
     with pytest.raises(nn_amd.Unsupported):
         _token_ids(torch.zeros(2), (2,), "cpu")
     for batch in ((), (0,), (2, 3)):
-        rows = int(np.prod(batch, dtype=int))
-        _, out = _logprob_outputs(rows, batch, 8, 4, True, "cpu")
+        _, out = _logprob_outputs(batch, 8, 4, True, "cpu")
         assert out.logprobs.shape == out.entropy.shape == out.ranks.shape == batch
         assert out.top_ids.shape == out.top_logprobs.shape == (*batch, 4)
 
