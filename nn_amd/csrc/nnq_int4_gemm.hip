@@ -34,14 +34,18 @@ __device__ __forceinline__ floatx16 mfma32(u32x4 a, u32x4 b, floatx16 c) {
 // Four rows a workgroup (thread % 4): the row's largest |x|, then its 8-column chunks, chunk c of the
 // row at piece c / 16, step (c / 2) % 8, half c % 2.  Chunks past K are zeros.  A thread's first kHold
 // chunks stay in registers between the two (all of them up to K = 8192).
+template <int ROWS>
+__device__ __forceinline__ int stage_row(int b) {
+    return ROWS == 4 ? b * 4 : (b / 16 * 8 + b % 8) * 4 + b / 8 % 2 * 2;
+}
 constexpr int kStageThreads = 1024, kHold = 4;
-template <bool XB>
+template <bool XB, int ROWS>
 __global__ __launch_bounds__(kStageThreads) void int4_stage_kernel(const void *x, int m, int64_t k, int units,
                                                                    uint8_t *xa, int64_t plane, float *rowback) {
-    constexpr int WV = kStageThreads / 64, STEP = kStageThreads / 4;
-    __shared__ uint32_t red[WV][4];
+    constexpr int WV = kStageThreads / 64, STEP = kStageThreads / ROWS;
+    __shared__ uint32_t red[WV][ROWS];
     const int tid = threadIdx.x, lane = tid & 63;
-    const int row = (int)blockIdx.x * 4 + (tid & 3), t = min(row, m - 1);
+    const int row = stage_row<ROWS>((int)blockIdx.x) + tid % ROWS, t = min(row, m - 1);
     const int chunks = (int)(k / 8);
     auto load = [&](int c, float(&v)[8]) {
         if constexpr (XB) {
@@ -69,27 +73,27 @@ __global__ __launch_bounds__(kStageThreads) void int4_stage_kernel(const void *x
     float held[kHold][8];
 #pragma unroll
     for (int i = 0; i < kHold; i++) {
-        const int c = (tid >> 2) + i * STEP;
+        const int c = tid / ROWS + i * STEP;
 #pragma unroll
         for (int e = 0; e < 8; e++) held[i][e] = 0.f;
         if (c < chunks) load(c, held[i]);
     }
 #pragma unroll
     for (int i = 0; i < kHold; i++) largest(held[i]);
-    for (int c = (tid >> 2) + kHold * STEP; c < chunks; c += STEP) {
+    for (int c = tid / ROWS + kHold * STEP; c < chunks; c += STEP) {
         float v[8];
         load(c, v);
         largest(v);
     }
-    for (int o = 4; o < 64; o <<= 1) mx = max(mx, (uint32_t)__shfl_xor((int)mx, o, 64));
-    if (lane < 4) red[tid >> 6][lane] = mx;
+    for (int o = ROWS; o < 64; o <<= 1) mx = max(mx, (uint32_t)__shfl_xor((int)mx, o, 64));
+    if (lane < ROWS) red[tid >> 6][lane] = mx;
     __syncthreads();
 #pragma unroll
-    for (int w = 0; w < WV; w++) mx = max(mx, red[w][tid & 3]);
+    for (int w = 0; w < WV; w++) mx = max(mx, red[w][tid % ROWS]);
     float s, back;
     f16_prescale(__uint_as_float(mx), s, back);
     if (row >= m) return;
-    if (tid < 4) rowback[row] = back;
+    if (tid < ROWS) rowback[row] = back;
     uint8_t *dst = xa + (int64_t)(row >> 5) * units * kPiece + (row & 31) * 16;
     auto put = [&](int c, const float(&v)[8]) {
         u32x4 hi, lo;
@@ -100,10 +104,10 @@ __global__ __launch_bounds__(kStageThreads) void int4_stage_kernel(const void *x
     };
 #pragma unroll
     for (int i = 0; i < kHold; i++) {
-        const int c = (tid >> 2) + i * STEP;
+        const int c = tid / ROWS + i * STEP;
         if (c < units * 16) put(c, held[i]);
     }
-    for (int c = (tid >> 2) + kHold * STEP; c < units * 16; c += STEP) {
+    for (int c = tid / ROWS + kHold * STEP; c < units * 16; c += STEP) {
         float v[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
         if (c < chunks) load(c, v);
         put(c, v);
@@ -259,29 +263,49 @@ __global__ __launch_bounds__(W * 64, 2) void int4_gemm_kernel(Int4GemmArgs a) {
         if (u + 1 < u1) store_a(buf ^ 1);  // (read by nobody since the barrier before this unit)
     }
 
-    // lane: column c32 of each 32, rows 8 (e / 4) + 4h + e % 4 of each 32-row tile
+    // lane: column c32 of each 32, rows 8 i + 4h + e of each 32-row tile.  Everything that is read comes
+    // before the first store: a wait for a load waits for the stores before it, too.
     const bool slab = a.ks > 1;
-    float *ys = reinterpret_cast<float *>(a.y) + (slab ? (int64_t)kp * a.m * a.n : 0);
+    float bias[NT];
 #pragma unroll
     for (int nt = 0; nt < NT; nt++) {
         const int64_t col = (int64_t)(tile0 + 2 * nt) * kTile + c32;
-        const float bias = a.bias && !slab && col < a.n ? a.bias[col] : 0.f;
+        bias[nt] = a.bias && !slab && col < a.n ? a.bias[col] : 0.f;
+    }
 #pragma unroll
-        for (int mt = 0; mt < MT; mt++) {
+    for (int mt = 0; mt < MT; mt++) {
+        floatx4 back[4];  // (whole 32-row tiles are there)
+#pragma unroll
+        for (int i = 0; i < 4; i++)
+            back[i] = *reinterpret_cast<const floatx4 *>(a.rowback + min(rb * MT + mt, row_pieces - 1) * 32 + 4 * h + 8 * i);
+#pragma unroll
+        for (int nt = 0; nt < NT; nt++) {
             scale_part(mt, nt);
 #pragma unroll
-            for (int e = 0; e < 16; e++) {
-                const int row = (rb * MT + mt) * 32 + 8 * (e / 4) + 4 * h + e % 4;
-                if (row < a.m && col < a.n) {
-                    const float v = fmaf(tot[mt][nt][e], a.rowback[row], bias);
-                    if (!slab && a.y_bf16)
-                        reinterpret_cast<uint16_t *>(a.y)[(int64_t)row * a.n + col] = (uint16_t)f32_to_bf16_bits(v);
-                    else
-                        ys[(int64_t)row * a.n + col] = v;
+            for (int e = 0; e < 16; e++) tot[mt][nt][e] = fmaf(tot[mt][nt][e], back[e / 4][e % 4], bias[nt]);
+        }
+    }
+    auto store = [&](auto *y, auto &&as) {
+#pragma unroll
+        for (int mt = 0; mt < MT; mt++) {
+            const int row0 = (rb * MT + mt) * 32 + 4 * h;
+#pragma unroll
+            for (int nt = 0; nt < NT; nt++) {
+                const int64_t col = (int64_t)(tile0 + 2 * nt) * kTile + c32;
+                if (col >= a.n) continue;
+                auto *p = y + (int64_t)row0 * a.n + col;
+#pragma unroll
+                for (int e = 0; e < 16; e++) {
+                    if (row0 + 8 * (e / 4) + e % 4 < a.m) *p = as(tot[mt][nt][e]);
+                    p += e % 4 == 3 ? 5 * a.n : a.n;
                 }
             }
         }
-    }
+    };
+    if (!slab && a.y_bf16)
+        store(reinterpret_cast<uint16_t *>(a.y), [](float v) { return (uint16_t)f32_to_bf16_bits(v); });
+    else
+        store(reinterpret_cast<float *>(a.y) + (slab ? (int64_t)kp * a.m * a.n : 0), [](float v) { return v; });
 }
 
 // y[i] = sum of the ks slabs' [i] in order + bias[i % n]
@@ -328,6 +352,17 @@ int launch_gemm_g(int group, int zeros, int mt, int nt, const Int4GemmArgs &a, v
     return launch_gemm_s<P, 4, false>(mt, nt, a, stream);
 }
 
+template <int ROWS>
+void launch_stage(const Int4Args &a, uint8_t *xa, int64_t plane, float *rowback, void *stream) {
+    const dim3 grid((unsigned)(ROWS == 4 ? (a.m + 3) / 4 : (a.m + 31) / 32 * 16)), block(kStageThreads);
+    if (a.x_bf16)
+        hipLaunchKernelGGL((int4_stage_kernel<true, ROWS>), grid, block, 0, (hipStream_t)stream, a.x, (int)a.m, a.k,
+                           (int)a.units, xa, plane, rowback);
+    else
+        hipLaunchKernelGGL((int4_stage_kernel<false, ROWS>), grid, block, 0, (hipStream_t)stream, a.x, (int)a.m, a.k,
+                           (int)a.units, xa, plane, rowback);
+}
+
 }  // namespace
 
 int launch_int4_gemm(const Int4Args &a, void *scratch, void *stream) {
@@ -352,13 +387,8 @@ int launch_int4_gemm(const Int4Args &a, void *scratch, void *stream) {
     g.row_blocks = p.row_blocks;
     g.col_blocks = p.col_blocks;
     g.n = a.n;
-    const dim3 sg((unsigned)((a.m + 3) / 4));
-    if (a.x_bf16)
-        hipLaunchKernelGGL((int4_stage_kernel<true>), sg, dim3(kStageThreads), 0, (hipStream_t)stream, a.x, (int)a.m, a.k,
-                           (int)a.units, base, g.plane, rowback);
-    else
-        hipLaunchKernelGGL((int4_stage_kernel<false>), sg, dim3(kStageThreads), 0, (hipStream_t)stream, a.x, (int)a.m, a.k,
-                           (int)a.units, base, g.plane, rowback);
+    if (a.m > 512) launch_stage<4>(a, base, g.plane, rowback, stream);
+    else launch_stage<2>(a, base, g.plane, rowback, stream);
     hipError_t e = hipGetLastError();
     if (e != hipSuccess) return (int)e;
     int rc = a.x_bf16 ? launch_gemm_g<1>(a.group, a.zeros, p.mt, p.nt, g, stream)
