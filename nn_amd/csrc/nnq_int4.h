@@ -9,22 +9,37 @@ namespace nnq {
 
 typedef _Float16 half2v __attribute__((ext_vector_type(2)));
 
-// row r's GS scales (16 bits each) and zero points (8 bits each) of the unit record at `rec`
-template <int GS, bool Z>
-__device__ __forceinline__ void load_scales(const uint8_t *rec, int r, uint32_t (&s)[(GS + 1) / 2], uint32_t &z) {
-    const uint8_t *sp = rec + 1024 + 2 * GS * r, *zp = rec + 1024 + 32 * GS + GS * r;
+// A buffer: a lane's offset in a vector register, the uniform one in a scalar one.  (An offset of the
+// lane past its end reads zeros.)
+__device__ __forceinline__ __amdgpu_buffer_rsrc_t rsrc(const void *p, int64_t bytes) {
+    return __builtin_amdgcn_make_buffer_rsrc(const_cast<void *>(p), 0, (int)min(bytes, (int64_t)0x7FFFFFF0), 0x00020000);
+}
+// 16 bytes a lane from a buffer straight into LDS: the wave's 64 pieces land one after another at `lds`.
+// (The host pass has no such builtin and would drop the kernels' launch stubs.)
+__device__ __forceinline__ void copy16_lds(__amdgpu_buffer_rsrc_t t, uint8_t *lds, int voff, int soff) {
+#if defined(__HIP_DEVICE_COMPILE__)
+    __builtin_amdgcn_raw_ptr_buffer_load_lds(t, (__attribute__((address_space(3))) void *)lds, 16, voff, soff, 0, 0);
+#endif
+}
+// a row's GS scales (16 bits each) at ls and zero points (8 bits each) at lz of the unit record at `at`;
+// AUX: the cache policy (2: non-temporal).  WORD: the zero points' whole aligned word (widening a byte of
+// it would wait for it in the next round of a loop that loads ahead).
+template <int GS, bool Z, int AUX, bool WORD>
+__device__ __forceinline__ void load_scales(__amdgpu_buffer_rsrc_t t, int ls, int lz, int at, uint32_t (&s)[(GS + 1) / 2],
+                                            uint32_t &z) {
     if constexpr (GS == 1) {
-        s[0] = *reinterpret_cast<const uint16_t *>(sp);
-        if constexpr (Z) z = *zp;
+        s[0] = __builtin_amdgcn_raw_buffer_load_b16(t, ls, at, AUX);
+        if constexpr (Z && !WORD) z = __builtin_amdgcn_raw_buffer_load_b8(t, lz, at, AUX);
     } else if constexpr (GS == 2) {
-        s[0] = *reinterpret_cast<const uint32_t *>(sp);
-        if constexpr (Z) z = *reinterpret_cast<const uint16_t *>(zp);
+        s[0] = __builtin_amdgcn_raw_buffer_load_b32(t, ls, at, AUX);
+        if constexpr (Z && !WORD) z = __builtin_amdgcn_raw_buffer_load_b16(t, lz, at, AUX);
     } else {
-        const u32x2 v = *reinterpret_cast<const u32x2 *>(sp);
+        const u32x2 v = __builtin_bit_cast(u32x2, __builtin_amdgcn_raw_buffer_load_b64(t, ls, at, AUX));
         s[0] = v[0];
         s[1] = v[1];
-        if constexpr (Z) z = *reinterpret_cast<const uint32_t *>(zp);
+        if constexpr (Z && !WORD) z = __builtin_amdgcn_raw_buffer_load_b32(t, lz, at, AUX);
     }
+    if constexpr (Z && WORD) z = __builtin_amdgcn_raw_buffer_load_b32(t, lz & ~3, at, AUX);
 }
 
 // all ones where scales are bf16, zero where they are f16, in a vector register: selecting by a scalar
@@ -46,11 +61,12 @@ __device__ __forceinline__ uint32_t pk_add(uint32_t a, uint32_t b) {
 }
 
 // -(1024 + z) and -(64 + z) as packed f16 (z = 8 without zero points), for byte g of zs: byte 0xE4 over
-// the zero point is the first, and adding 960 to it the second, exactly
+// the zero point is the first, and adding 960 to it the second, exactly.  `sel` selects byte 0.
+constexpr uint32_t kZeroSel = 0x04000400u;
 template <bool Z>
-__device__ __forceinline__ void zero_consts(uint32_t zs, int g, uint32_t &c1, uint32_t &c2) {
+__device__ __forceinline__ void zero_consts(uint32_t zs, int g, uint32_t &c1, uint32_t &c2, uint32_t sel = kZeroSel) {
     if constexpr (Z) {
-        c1 = __builtin_amdgcn_perm(0xE4E4E4E4u, zs, 0x04000400u + 0x00010001u * (uint32_t)g);
+        c1 = __builtin_amdgcn_perm(0xE4E4E4E4u, zs, sel + 0x00010001u * (uint32_t)g);
         c2 = pk_add(c1, 0x63806380u);
     } else {
         c1 = 0xE408E408u;

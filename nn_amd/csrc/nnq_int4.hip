@@ -37,27 +37,11 @@ struct Unit {
     uint32_t z;                // GS zero points (8 bits each)
 };
 
-// A tile's records as a buffer: the lane's offset in a vector register, the unit's in a scalar one.
-// (and x: an offset past its end reads zeros)
-__device__ __forceinline__ __amdgpu_buffer_rsrc_t rsrc(const void *p, int64_t bytes) {
-    return __builtin_amdgcn_make_buffer_rsrc(const_cast<void *>(p), 0, (int)min(bytes, (int64_t)0x7FFFFFF0), 0x00020000);
-}
 // (the weight stream non-temporal; lq = 16 lane, and the offsets of the row's scales and zero points)
 template <int GS, bool Z>
 __device__ __forceinline__ void load_unit(__amdgpu_buffer_rsrc_t t, int lq, int ls, int lz, int at, Unit<GS, Z> &u) {
     u.q = __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(t, lq, at, 2));
-    if constexpr (GS == 1) {
-        u.s[0] = __builtin_amdgcn_raw_buffer_load_b16(t, ls, at, 2);
-        if constexpr (Z) u.z = __builtin_amdgcn_raw_buffer_load_b8(t, lz, at, 2);
-    } else if constexpr (GS == 2) {
-        u.s[0] = __builtin_amdgcn_raw_buffer_load_b32(t, ls, at, 2);
-        if constexpr (Z) u.z = __builtin_amdgcn_raw_buffer_load_b16(t, lz, at, 2);
-    } else {
-        const u32x2 s = __builtin_bit_cast(u32x2, __builtin_amdgcn_raw_buffer_load_b64(t, ls, at, 2));
-        u.s[0] = s[0];
-        u.s[1] = s[1];
-        if constexpr (Z) u.z = __builtin_amdgcn_raw_buffer_load_b32(t, lz, at, 2);
-    }
+    load_scales<GS, Z, 2, false>(t, ls, lz, at, u.s, u.z);
 }
 
 __device__ __forceinline__ void wave_fence() {

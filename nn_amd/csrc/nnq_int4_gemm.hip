@@ -15,6 +15,7 @@
 //    group, beside 8 (group 128), 4 or 2 MFMAs of 32 cycles.
 //  * With too few workgroups K is split: f32 slabs, added in order by int4_sum_kernel.
 #include <algorithm>
+#include <type_traits>
 
 #include "nnq_device.h"
 #include "nnq_int4.h"
@@ -152,41 +153,43 @@ __global__ __launch_bounds__(W * 64, 2) void int4_gemm_kernel(Int4GemmArgs a) {
 
     const int c32 = lane & 31, h = lane >> 5, r = lane & 15;
     const int tile0 = (cb * W + wv) * 2 * NT;
-    const uint8_t *wp[NT];
+    // (buffers: one register of a lane's offset for all loads of a kind instead of a pair for each)
+    __amdgpu_buffer_rsrc_t wb[NT];
+    int pair[NT];  // from the first tile of a pair to the second; tiles past the last: not stored
 #pragma unroll
-    for (int nt = 0; nt < NT; nt++)  // (tiles past the last: not stored)
-        wp[nt] = a.w + (size_t)min(tile0 + 2 * nt + ((lane >> 4) & 1), a.ntile - 1) * a.units * UB;
+    for (int nt = 0; nt < NT; nt++) {
+        const int t = min(tile0 + 2 * nt, a.ntile - 1);
+        wb[nt] = rsrc(a.w + (size_t)t * a.units * UB, (int64_t)min(2, a.ntile - t) * a.units * UB);
+        pair[nt] = (lane & 16) && t + 1 < a.ntile ? a.units * UB : 0;
+    }
     auto load_w = [&](int u, Unit32<GS, Z>(&o)[NT]) {
 #pragma unroll
         for (int nt = 0; nt < NT; nt++) {
-            const uint8_t *rec = wp[nt] + (size_t)u * UB;
-            o[nt].q[0] = *reinterpret_cast<const u32x4 *>(rec + 16 * (16 * h + r));
-            o[nt].q[1] = *reinterpret_cast<const u32x4 *>(rec + 16 * (16 * (2 + h) + r));
-            load_scales<GS, Z>(rec, r, o[nt].s, o[nt].z);
+            const int lq = pair[nt] + 16 * (16 * h + r), ls = pair[nt] + 1024 + 2 * GS * r;
+            const int lz = pair[nt] + 1024 + 32 * GS + GS * r;
+            o[nt].q[0] = __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(wb[nt], lq, u * UB, 0));
+            o[nt].q[1] = __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(wb[nt], lq + 512, u * UB, 0));
+            load_scales<GS, Z, 0, true>(wb[nt], ls, lz, u * UB, o[nt].s, o[nt].z);
         }
     };
     // A pieces: (row block, plane) pairs of a unit, 8 KB each; rows past the last block: the last one
     const int row_pieces = (a.m + 31) / 32;
-    u32x4 ar[NA];
-    auto load_a = [&](int u) {
+    const __amdgpu_buffer_rsrc_t xb = rsrc(a.xa, P * a.plane);
+    auto copy_a = [&](int u, int buf) {
 #pragma unroll
         for (int i = 0; i < NA; i++) {
-            const int p = (i * W * 64 + tid) / 512, off = (i * W * 64 + tid) % 512;
-            const int pc = min(rb * MT + p % MT, row_pieces - 1);
-            ar[i] = *reinterpret_cast<const u32x4 *>(a.xa + (p / MT) * a.plane + ((int64_t)pc * a.units + u) * kPiece + off * 16);
+            const int p = i / 2, pc = min(rb * MT + p % MT, row_pieces - 1);
+            const int at = (p / MT) * (int)a.plane + (pc * a.units + u) * kPiece + i % 2 * 4096;
+            copy16_lds(xb, lds + buf * BUF + (i * W + wv) * 1024, tid * 16, at);
         }
     };
-    auto store_a = [&](int buf) {
-#pragma unroll
-        for (int i = 0; i < NA; i++) *reinterpret_cast<u32x4 *>(lds + buf * BUF + (i * W * 64 + tid) * 16) = ar[i];
-    };
-
+    static_assert(W * 64 * 16 * 2 == kPiece, "two loads of the workgroup a piece");
     // The MFMAs of a step are issued one at a time with the forming of the next step's operands and the
     // scaling of a finished group's sums between them: a wave that issues MFMAs back to back waits for
     // the matrix pipe with its own VALU work behind them.  (32 cycles of an MFMA hide six VALU
     // instructions.)
     const CodeMasks km;
-    const uint32_t sm = scale_mask(a.scale_bf16);
+    const uint32_t sm = scale_mask(a.scale_bf16), zsel = kZeroSel + 0x00010001u * (uint32_t)(GS * r & 3);
     floatx16 tot[MT][NT], part[MT][NT];
 #pragma unroll
     for (int mt = 0; mt < MT; mt++)
@@ -197,11 +200,16 @@ __global__ __launch_bounds__(W * 64, 2) void int4_gemm_kernel(Int4GemmArgs a) {
     float sc[NT];  // the scales of the sums in `part`
     uint32_t c1[NT], c2[NT];
     u32x4 af[2][P][MT], bf[2][NT];
-    Unit32<GS, Z> w[NT], wn[NT];
+    Unit32<GS, Z> w2[2][NT];  // this unit's weights and the next one's, in turn (copied, they would be waited for at once)
 #pragma unroll
     for (int nt = 0; nt < NT; nt++) sc[nt] = 0.f;
     auto read_a = [&](int buf, int s, int q) {
         af[s & 1][q / MT][q % MT] = *reinterpret_cast<const u32x4 *>(lds + buf * BUF + lane * 16 + q * kPiece + s * 1024);
+    };
+    auto arrive = [&]() {
+        __builtin_amdgcn_s_waitcnt(0x0070);  // vmcnt(0) lgkmcnt(0)
+        __builtin_amdgcn_s_barrier();
+        __builtin_amdgcn_sched_barrier(0);
     };
     auto scale_part = [&](int mt, int nt) {
 #pragma unroll
@@ -209,31 +217,41 @@ __global__ __launch_bounds__(W * 64, 2) void int4_gemm_kernel(Int4GemmArgs a) {
         asm volatile("" : "+v"(tot[mt][nt]));  // here: moved on, the sums would keep `part` alive beside its next values
         __builtin_amdgcn_sched_barrier(0);
     };
-    load_a(u0);
-    load_w(u0, wn);
-    store_a(0);
-    for (int u = u0; u < u1; u++) {
-        const int buf = (u - u0) & 1;
-        __syncthreads();
-#pragma unroll
-        for (int nt = 0; nt < NT; nt++) w[nt] = wn[nt];
-        if (u + 1 < u1) {
-            load_a(u + 1);
-            load_w(u + 1, wn);
-        }
+    // A unit's last step already reads and forms the next unit's first, so that no MFMA waits at a unit's
+    // edge.  The barrier before it is the unit's only one: this unit's A pieces have been read (the loads of
+    // step 7's operands are waited for there) and the copies of the next one, issued a unit earlier, have
+    // landed, as have the weights; copies and loads of the unit after that start behind it.  Past the last
+    // unit the last one is loaded again.
+    auto begin = [&](auto parity) {
+        constexpr int buf = decltype(parity)::value;
+        copy_a(u0, buf);
+        load_w(u0, w2[buf]);
+        copy_a(min(u0 + 1, u1 - 1), buf ^ 1);
+        load_w(min(u0 + 1, u1 - 1), w2[buf ^ 1]);
+        arrive();
 #pragma unroll
         for (int q = 0; q < P * MT; q++) read_a(buf, 0, q);
 #pragma unroll
         for (int nt = 0; nt < NT; nt++) {
-            zero_consts<Z>(w[nt].z, 0, c1[nt], c2[nt]);
-            bf[0][nt] = codes_f16(w[nt].q[0][0], c1[nt], c2[nt], km);
+            zero_consts<Z>(w2[buf][nt].z, 0, c1[nt], c2[nt], zsel);
+            bf[0][nt] = codes_f16(w2[buf][nt].q[0][0], c1[nt], c2[nt], km);
         }
+    };
+    auto unit = [&](auto parity, int ahead) {
+        constexpr int buf = decltype(parity)::value;
 #pragma unroll
         for (int s = 0; s < 8; s++) {
-            const bool first = s % (8 / GS) == 0, next = s < 7;
-            if (next && (s + 1) % (8 / GS) == 0)
+            const Unit32<GS, Z>(&w)[NT] = w2[s == 7 ? buf ^ 1 : buf];  // of the operands to form
+            const bool first = s % (8 / GS) == 0;
+            const int sn = (s + 1) % 8;
+            if (s == 7) {
+                arrive();
+                copy_a(ahead, buf);
+                load_w(ahead, w2[buf]);
+            }
+            if (sn % (8 / GS) == 0)
 #pragma unroll
-                for (int nt = 0; nt < NT; nt++) zero_consts<Z>(w[nt].z, (s + 1) / (8 / GS), c1[nt], c2[nt]);
+                for (int nt = 0; nt < NT; nt++) zero_consts<Z>(w[nt].z, sn / (8 / GS), c1[nt], c2[nt], zsel);
             constexpr int M = P * MT * NT;  // MFMAs of a step
 #pragma unroll
             for (int q = 0; q < M; q++) {
@@ -246,21 +264,30 @@ __global__ __launch_bounds__(W * 64, 2) void int4_gemm_kernel(Int4GemmArgs a) {
 #pragma unroll
                 for (int e = 0; e < 16; e++) zero[e] = 0.f;
                 part[mt][nt] = mfma32(af[s & 1][pl][mt], bf[s & 1][nt], start ? zero : part[mt][nt]);
-                if (next) {
-                    if (q % NT == 0) read_a(buf, s + 1, q / NT);
+                if (q % NT == 0) read_a(s == 7 ? buf ^ 1 : buf, sn, q / NT);
 #pragma unroll
-                    for (int i = 0; i < 4 * NT; i++)
-                        if (i * M / (4 * NT) == q)
-                            bf[(s + 1) & 1][i / 4][i % 4] =
-                                code_pair(w[i / 4].q[(s + 1) & 1][(s + 1) >> 1], i % 4, c1[i / 4], c2[i / 4], km);
-                }
+                for (int j = 0; j < 4 * NT; j++)
+                    if (j * M / (4 * NT) == q)
+                        bf[sn & 1][j / 4][j % 4] = code_pair(w[j / 4].q[sn & 1][sn >> 1], j % 4, c1[j / 4], c2[j / 4], km);
             }
             if (first)
 #pragma unroll
-                for (int nt = 0; nt < NT; nt++) sc[nt] = group_scale(w[nt].s, s / (8 / GS), sm);
+                for (int nt = 0; nt < NT; nt++) sc[nt] = group_scale(w2[buf][nt].s, s / (8 / GS), sm);
         }
-        __builtin_amdgcn_sched_barrier(0);
-        if (u + 1 < u1) store_a(buf ^ 1);  // (read by nobody since the barrier before this unit)
+    };
+    const std::integral_constant<int, 0> even;
+    const std::integral_constant<int, 1> odd;
+    int u = u0;
+    if ((u1 - u0) & 1) {
+        begin(odd);
+        unit(odd, min(u0 + 2, u1 - 1));
+        u++;
+    } else {
+        begin(even);
+    }
+    for (; u < u1; u += 2) {
+        unit(even, min(u + 2, u1 - 1));
+        unit(odd, min(u + 3, u1 - 1));
     }
 
     // lane: column c32 of each 32, rows 8 i + 4h + e of each 32-row tile.  Everything that is read comes
@@ -334,7 +361,7 @@ int launch_gemm_t(const Int4GemmArgs &a, void *stream) {
 template <int P, int GS, bool Z>
 int launch_gemm_s(int mt, int nt, const Int4GemmArgs &a, void *stream) {
     if (mt == 1) return nt == 1 ? launch_gemm_t<1, 1, P, GS, Z>(a, stream) : launch_gemm_t<1, 2, P, GS, Z>(a, stream);
-    if constexpr (P == 1)
+    if constexpr (P == 1 && GS != 4)
         return nt == 1 ? launch_gemm_t<2, 1, P, GS, Z>(a, stream) : launch_gemm_t<2, 2, P, GS, Z>(a, stream);
     else
         return launch_gemm_t<2, 1, P, GS, Z>(a, stream);
