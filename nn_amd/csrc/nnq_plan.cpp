@@ -68,15 +68,15 @@ size_t int4_rows_scratch(int64_t m, int64_t n, int64_t k, int x_bf16) {
 
 // 4-bit prefill: the workgroup tile (mt x 32 rows, nt x 128 columns) and the K split of the least
 // estimated time.  c workgroups on a CU take c * step + lag per unit of 128 k (fitted on MI355X to
-// 20 to 640 rows of 1024 to 24576 columns, K 1024 to 12288: the choice is within 6% of the best of
-// all tiles and splits there); with K split the slabs are written and read back at 8.5 TB/s (they stay
-// in the last-level cache) by one launch more.  2 x 2 is left out where its registers spill (f32 x,
-// groups of 32: 512 x 12288 x 4096 in 108 us, 82 with 2 x 1).
+// 20 to 1024 rows of 1024 to 40960 columns, K 1024 to 12288: the choice is within 6% of the best of
+// all tiles and splits there, 10% where a call takes under 20 us); with K split the slabs are written
+// and read back at 5.6 TB/s by one launch more.  2 x 2 is left out where its registers spill (f32 x,
+// groups of 32).
 Int4GemmPlan int4_gemm_plan(int64_t m, int64_t n, int64_t k, int group, int x_bf16) {
     Int4GemmPlan p{};
     const int64_t cus = 256, tiles = (m + 31) / 32, units = (k + kInt4Unit - 1) / kInt4Unit;
-    static const double step[2][2][2] = {{{0.50, 0.85}, {0.95, 0}}, {{0.38, 0.70}, {0.62, 1.10}}};
-    static const double lag[2][2][2] = {{{0.20, 0.20}, {0.12, 0}}, {{0.10, 0.21}, {0.12, 0.23}}};
+    static const double step[2][2][2] = {{{0.42, 0.74}, {0.80, 0}}, {{0.255, 0.47}, {0.41, 0.76}}};
+    static const double lag[2][2][2] = {{{0.08, 0.01}, {0.00, 0}}, {{0.15, 0.09}, {0.05, 0.14}}};
     const int xb = x_bf16 ? 1 : 0;
     double best = 1e30;
     int64_t ks = 1;
@@ -87,7 +87,7 @@ Int4GemmPlan int4_gemm_plan(int64_t m, int64_t n, int64_t k, int group, int x_bf
                 const int64_t wg = (tiles + mt - 1) / mt * ((n + 128 * nt - 1) / (128 * nt)) * s;
                 const double c = wg > 4 * cus ? (double)wg / cus : (double)((wg + cus - 1) / cus);
                 double us = (double)((units + s - 1) / s) * (c * step[xb][mt - 1][nt - 1] + lag[xb][mt - 1][nt - 1]);
-                if (s > 1) us += 3.0 + (double)(2 * s) * (double)m * (double)n * 4 / 8.5e6;
+                if (s > 1) us += 1.5 + (double)(2 * s) * (double)m * (double)n * 4 / 5.6e6;
                 if (us < best) {
                     best = us;
                     p.mt = mt;

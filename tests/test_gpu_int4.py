@@ -44,9 +44,16 @@ def tokens(m, k, dtype, seed=2):
     return (torch.randn(m, k, generator=g, device="cuda") * torch.exp(torch.randn(k, generator=g, device="cuda"))).to(dtype)
 
 
-def check(y, ref, what=""):
+def check(y, ref, what="", bias=None):
+    """``bias`` was added to ``ref``'s product: it may cancel the product (one output: to any extent), whose
+    rounding errors are of its own size and stay, and the addition rounds once, 2^-24 of at most the two's
+    sum.  So the size that counts is then the root mean square of the product and of the bias together."""
     assert y.shape == ref.shape and torch.isfinite(y).all()
-    err = (y.double() - ref).abs().max().item() / ref.pow(2).mean().sqrt().item()
+    size = ref.pow(2).mean()
+    if bias is not None:
+        b = bias.double()
+        size = (ref - b).pow(2).mean() + b.pow(2).mean()
+    err = (y.double() - ref).abs().max().item() / size.sqrt().item()
     assert err <= 1e-5, f"{what} max error {err:.2e} of the output's rms"
 
 
@@ -74,7 +81,7 @@ def test_rows(m, n, k, group, zeros, scale, xdt):
     ref = x.double() @ ref.t()
     check(nn_amd.quantized_linear(x, w), ref)
     y = nn_amd.quantized_linear(x, w, bias)
-    check(y, ref + bias.double())
+    check(y, ref + bias.double(), bias=bias)
     assert torch.equal(nn_amd.quantized_linear(x, w, bias, out_dtype=BF16), y.to(BF16))
 
 
