@@ -431,6 +431,8 @@ int nnq_weight_create_int4(const uint8_t *codes, const void *scales, nnq_dtype s
     if (!codes || !scales) return fail(NNQ_ERR_INVALID_ARGUMENT, "codes or scales is null");
     size_t bytes = 0;
     if (!array_bytes(n + kTile, k + kInt4Unit, 1, &bytes) || bytes > (size_t)INT64_MAX) return size_fail();
+    // (the kernels address 128 rows of x and a tile's records with 32-bit offsets)
+    if (k > kInt4MaxK) return fail(NNQ_ERR_UNSUPPORTED, "in_features %lld (at most 2^20 in 4-bit groups)", (long long)k);
     const uint16_t *sc = reinterpret_cast<const uint16_t *>(scales);
     const uint16_t ex = scale_dtype == NNQ_BF16 ? 0x7F80 : 0x7C00;
     const int64_t groups = n * (k / group);

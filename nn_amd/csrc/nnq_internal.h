@@ -54,6 +54,7 @@ struct Layout {
 bool make_layout(int fmt, int layout, int64_t n, int64_t k, Layout *out, const char **err);
 bool make_layout_int4(int64_t n, int64_t k, int64_t group, int zeros, int scale_bf16, Layout *out, const char **err);
 constexpr int kInt4Unit = 128;  // k of one unit
+constexpr int64_t kInt4MaxK = (int64_t)1 << 20;
 constexpr int int4_unit_bytes(int group, int zeros) { return 1024 + kTile * (kInt4Unit / group) * (zeros ? 3 : 2); }
 
 // Host repack: source block bytes (format/layout as given) -> device image (Layout::total bytes).

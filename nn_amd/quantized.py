@@ -253,7 +253,7 @@ class QuantizedWeight:
         codes: uint8 [out_features, in_features / 2], two to a byte with the even column in the
         low half; scales: float16 or bfloat16 [out_features, in_features / group_size]; zeros:
         integers from 0 to 16 of the same shape, or None for 8 throughout; group_size 32, 64 or
-        128.  The tensors may be on the host or a device and are copied."""
+        128, in_features at most 2^20.  The tensors may be on the host or a device and are copied."""
         for t, what in ((codes, "codes"), (scales, "scales")):
             if not isinstance(t, torch.Tensor):
                 raise Unsupported(f"{what} must be a tensor")
@@ -270,6 +270,8 @@ class QuantizedWeight:
             raise ShapeMismatch(f"scales must be [{n}, {k // group}], got {list(scales.shape)}")
         z = None
         if zeros is not None:
+            if not isinstance(zeros, torch.Tensor):
+                raise Unsupported("zeros must be a tensor")
             if tuple(zeros.shape) != (n, k // group):
                 raise ShapeMismatch(f"zeros must be [{n}, {k // group}], got {list(zeros.shape)}")
             if zeros.is_floating_point() or zeros.is_complex() or zeros.dtype == torch.bool:

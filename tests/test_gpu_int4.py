@@ -8,6 +8,8 @@ Bar (f32 outputs): every product of an integer and an f16 is exact in f32; f32 x
 pair that drops at most 2^-22 of it.  What is left is rounding of f32 sums and scalings, 2^-24 each of
 partial sums that stay within a few times the output's own size, some 40 in line: max |error| <= 1e-5 of
 the output's root mean square.  A bf16 output is the f32 result rounded once, bit for bit."""
+import ctypes
+
 import pytest
 import torch
 
@@ -166,6 +168,64 @@ def test_argmax_and_sampling_through_an_int4_head():
     x[0, 3] = float("nan")
     with pytest.raises(nn_amd.NonFiniteData):
         nn_amd.linear_argmax(x, w)
+
+
+@pytest.mark.parametrize("m", [5, 9, 16])
+@pytest.mark.parametrize("xdt", [F32, BF16])
+def test_rows_over_a_split_k(m, xdt):
+    """K split over workgroups: a row of NaN stays a row of NaN, the others and a replayed graph are right."""
+    import nn_amd
+    w, ref = make(4500, 9600, 64)  # 75 units: parts of unequal length
+    x = tokens(m, 9600, xdt)
+    x[m // 2, 9599] = float("nan")
+    keep = [t for t in range(m) if t != m // 2]
+    nn_amd.quantized_linear(x, w)
+    torch.cuda.synchronize()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        y = nn_amd.quantized_linear(x, w)
+    for i in range(3):
+        x[keep] = tokens(m, 9600, xdt, seed=20 + i)[keep]
+        eager = nn_amd.quantized_linear(x, w)
+        g.replay()
+        torch.cuda.synchronize()
+        assert torch.isnan(y[m // 2]).all() and torch.equal(y[keep], eager[keep])
+        check(y[keep], x[keep].double() @ ref.t())
+
+
+def test_rows_in_several_launches():
+    """More rows than one launch stages: the rows on both sides of the edge, the first and the last."""
+    import nn_amd
+    w, ref = make(24, 32768, 128)
+    x = tokens(8200, 32768, BF16)
+    y = nn_amd.quantized_linear(x, w)
+    rows = list(range(0, 8200, 411)) + list(range(8050, 8080)) + [8199]
+    check(y[rows], x[rows].double() @ ref.t())
+
+
+def test_outputs_past_32_bits():
+    import nn_amd
+    w, ref = make(17000, 128, 64)
+    x = tokens(66000, 128, BF16)
+    y = nn_amd.quantized_linear(x, w)  # 4.5 GB
+    rows = [0, 31999, 65535, 65536, 65999] + list(range(63150, 63180))  # 63161 x 17000 x 4 bytes is 2^32
+    check(y[rows], x[rows].double() @ ref.t())
+
+
+def test_sampling_without_allocation_through_an_int4_head():
+    from nn_amd import _lib
+    w, _ = make(9001, 4224, 64)
+    x = tokens(1, 4224, F32)[0].contiguous()
+    for top_k, top_p, seed in ((20, 0.9, 3), (50, 1.0, 8)):
+        cfg = _lib.Sampling(0.7, top_k, 1, top_p, 1.0, 0.0, seed)
+        out = []
+        for name in ("nnq_linear_sample", "nnq_linear_sample_noalloc"):
+            logits, tok = torch.empty(9001, device="cuda"), torch.full((1,), -1, dtype=torch.int32, device="cuda")
+            rc = getattr(_lib.load(), name)(w.handle, x.data_ptr(), 4224, None, 0, logits.data_ptr(), None, 0,
+                                            ctypes.byref(cfg), tok.data_ptr(), torch.cuda.current_stream().cuda_stream)
+            assert rc == 0, _lib.last_error()
+            out.append((logits, int(tok)))
+        assert torch.equal(out[0][0], out[1][0]) and out[0][1] == out[1][1] >= 0
 
 
 @pytest.mark.parametrize("m", [1, 16, 40, 200])

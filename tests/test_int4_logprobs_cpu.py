@@ -45,11 +45,14 @@ def test_int4_create_refusals(lib):
         assert create(lib, c, s2, None, 4, 128, 128) == _lib.ERR_NON_FINITE
     b = np.array([0x3F80, 0x7F80, 0x3F80, 0x3F80], np.uint16)  # bf16 infinity
     assert create(lib, c, b, None, 4, 128, 128, dtype=2) == _lib.ERR_NON_FINITE
+    assert create(lib, c, s, None, 4, 1 << 21, 128) == _lib.ERR_UNSUPPORTED  # (nothing is read)
     # sizes whose product passes 64 bits are refused before anything is read
     assert create(lib, c, s, None, 1 << 40, 1 << 30, 128) == _lib.ERR_OUT_OF_MEMORY
 
 
 def test_from_int4_groups_refusals():
+    with pytest.raises(nn_amd.Unsupported):
+        nn_amd.QuantizedWeight.from_int4_groups(torch.zeros(4, 64, dtype=torch.uint8), torch.ones(4, 1).half(), [[8]] * 4)
     make = nn_amd.QuantizedWeight.from_int4_groups
     c, s = torch.zeros(4, 64, dtype=torch.uint8), torch.ones(4, 1, dtype=torch.float16)
     with pytest.raises(nn_amd.Unsupported):
@@ -78,6 +81,42 @@ def test_from_int4_groups_refusals():
             make(c, s, torch.full((4, 1), z, dtype=torch.int64))
     with pytest.raises(nn_amd.WrongQuantType):
         nn_amd.QuantizedWeight.from_quantized(np.zeros(64, np.uint8), nn_amd.QuantType.INT4G, (1, 128))
+
+
+class GemmPlan(ctypes.Structure):
+    _fields_ = [(f, ctypes.c_int) for f in ("mt", "nt", "ks", "row_blocks", "col_blocks")] + \
+               [(f, ctypes.c_size_t) for f in ("plane", "rowback", "slabs", "bytes")]
+
+
+@pytest.mark.parametrize("xb", [0, 1])
+@pytest.mark.parametrize("group", [32, 64, 128])
+def test_int4_plans(lib, xb, group):
+    """Every shape has a tile that is built, workgroups that cover it, parts of K that none is empty of and
+    scratch regions that hold what the launches write."""
+    plan, split = lib._ZN3nnq14int4_gemm_planElllii, lib._ZN3nnq15int4_rows_splitEllli
+    rows_scratch, chunk = lib._ZN3nnq17int4_rows_scratchEllli, lib._ZN3nnq15int4_chunk_rowsEll
+    i64 = ctypes.c_int64
+    plan.argtypes, plan.restype = [i64, i64, i64, ctypes.c_int, ctypes.c_int], GemmPlan
+    split.argtypes, split.restype = [i64, i64, i64, ctypes.c_int], ctypes.c_int
+    rows_scratch.argtypes, rows_scratch.restype = [i64, i64, i64, ctypes.c_int], ctypes.c_size_t
+    chunk.argtypes, chunk.restype = [i64, i64], i64
+    for n in (1, 16, 100, 4096, 12288, 151936):
+        for k in (group, 128, 320 * group // 32, 4096, 12288, 1 << 20):
+            units = (k + 127) // 128
+            for m in (1, 4, 5, 8, 9, 16):
+                ks = split(m, n, k, xb)
+                assert 1 <= ks <= min(8, units) and (m > 4 or ks == 1)  # (one row: no scratch)
+                assert rows_scratch(m, n, k, xb) == (ks * m * n * 4 if ks > 1 else 0)
+            for m in (1, 17, 32, 33, 203, 640, 5000, 65536):
+                r = chunk(m, k)
+                assert 1 <= r <= m and (r == m or r % 128 == 0)
+                p = plan(r, n, k, group, xb)
+                assert p.mt in (1, 2) and p.nt in (1, 2) and not (p.mt == p.nt == 2 and (not xb or group == 32))
+                assert 1 <= p.ks <= max(1, units // 2) and p.row_blocks * p.mt * 32 >= r and p.col_blocks * p.nt * 128 >= n
+                planes, tiles = 1 if xb else 2, (r + 31) // 32
+                assert p.plane == tiles * units * 8192 and planes * p.plane < 2 ** 31  # 32-bit offsets
+                assert p.rowback == planes * p.plane and p.slabs >= p.rowback + tiles * 128 and p.slabs % 256 == 0
+                assert p.bytes >= p.slabs + (p.ks * r * n * 4 if p.ks > 1 else 0)
 
 
 def test_int4_gguf_formats_refuse_the_layout(lib):
