@@ -158,6 +158,13 @@ int nnq_weight_create(nnq_format fmt, nnq_layout layout, const uint8_t *bytes, s
 int nnq_weight_create_int4(const uint8_t *codes, const void *scales, nnq_dtype scale_dtype, const uint8_t *zeros,
                            int64_t n, int64_t k, int64_t group, nnq_weight **out);
 
+/* nnq_weight_create_int4 of arrays in the current device's memory (codes 4-byte aligned),
+ * read in order on `stream` and repacked by the device: for checkpoints that are loaded
+ * there.  Returns when the weight is there (it synchronizes the stream; not for a stream
+ * that is being captured). */
+int nnq_weight_create_int4_device(const uint8_t *codes, const void *scales, nnq_dtype scale_dtype, const uint8_t *zeros,
+                                  int64_t n, int64_t k, int64_t group, nnq_weight **out, void *stream);
+
 int nnq_weight_destroy(nnq_weight *w);
 
 /* Shape / format queries (QuantizedStorage::shape / quant_type, quantized.rs:142-152). */

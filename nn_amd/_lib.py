@@ -81,6 +81,8 @@ SIGNATURES = {
     "nnq_gguf_weight_create": (c_int, [c_void_p, ctypes.c_char_p, c_int, c_int, ctypes.POINTER(c_void_p)]),
     "nnq_weight_create_int4": (c_int, [c_void_p, c_void_p, c_int, c_void_p, c_i64, c_i64, c_i64,
                                        ctypes.POINTER(c_void_p)]),
+    "nnq_weight_create_int4_device": (c_int, [c_void_p, c_void_p, c_int, c_void_p, c_i64, c_i64, c_i64,
+                                              ctypes.POINTER(c_void_p), c_void_p]),
     "nnq_token_logprobs": (c_int, [c_void_p, c_int, c_i64, c_i64, c_i64, c_void_p, c_int, c_void_p, c_void_p, c_void_p,
                                    c_void_p, c_void_p, c_void_p]),
     "nnq_linear_logprobs": (c_int, [c_void_p, c_void_p, c_int, c_i64, c_i64, c_void_p, c_i64, c_void_p, c_int, c_void_p,

@@ -10,6 +10,7 @@
 #include <cstring>
 #include <memory>
 #include <mutex>
+#include <new>
 #include <string>
 #include <thread>
 #include <vector>
@@ -417,29 +418,46 @@ int nnq_weight_create(nnq_format fmt, nnq_layout layout, const uint8_t *bytes, s
     return NNQ_OK;
 }
 
-int nnq_weight_create_int4(const uint8_t *codes, const void *scales, nnq_dtype scale_dtype, const uint8_t *zeros,
-                           int64_t n, int64_t k, int64_t group, nnq_weight **out) {
+}  // extern "C"
+
+// what nnq_weight_create_int4 and its device form refuse, and the layout
+static int check_int4(const uint8_t *codes, const void *scales, nnq_dtype scale_dtype, const uint8_t *zeros, int64_t n,
+                      int64_t k, int64_t group, nnq_weight **out, Layout *L) {
     if (!out) return fail(NNQ_ERR_INVALID_ARGUMENT, "out is null");
     *out = nullptr;
     if (n <= 0 || k <= 0) return fail(NNQ_ERR_INVALID_ARGUMENT, "weight shape [%lld, %lld]", (long long)n, (long long)k);
     if (scale_dtype != NNQ_F16 && scale_dtype != NNQ_BF16)
         return fail(NNQ_ERR_UNSUPPORTED, "scale dtype %d (f16 or bf16)", (int)scale_dtype);
-    Layout L;
     const char *err = nullptr;
-    if (!make_layout_int4(n, k, group, zeros != nullptr, scale_dtype == NNQ_BF16, &L, &err))
+    if (!make_layout_int4(n, k, group, zeros != nullptr, scale_dtype == NNQ_BF16, L, &err))
         return fail(NNQ_ERR_INVALID_SHAPE, "%s (in_features %lld, group %lld)", err, (long long)k, (long long)group);
     if (!codes || !scales) return fail(NNQ_ERR_INVALID_ARGUMENT, "codes or scales is null");
     size_t bytes = 0;
     if (!array_bytes(n + kTile, k + kInt4Unit, 1, &bytes) || bytes > (size_t)INT64_MAX) return size_fail();
     // (the kernels address 128 rows of x and a tile's records with 32-bit offsets)
     if (k > kInt4MaxK) return fail(NNQ_ERR_UNSUPPORTED, "in_features %lld (at most 2^20 in 4-bit groups)", (long long)k);
+    return NNQ_OK;
+}
+
+static int bad_int4_scale(int64_t i) { return fail(NNQ_ERR_NON_FINITE, "scale %lld is not finite", (long long)i); }
+static int bad_int4_zero(int64_t i) {
+    return fail(NNQ_ERR_INVALID_ARGUMENT, "zero point %lld is over 16", (long long)i);
+}
+
+extern "C" {
+
+int nnq_weight_create_int4(const uint8_t *codes, const void *scales, nnq_dtype scale_dtype, const uint8_t *zeros,
+                           int64_t n, int64_t k, int64_t group, nnq_weight **out) {
+    Layout L;
+    const int rc = check_int4(codes, scales, scale_dtype, zeros, n, k, group, out, &L);
+    if (rc) return rc;
     const uint16_t *sc = reinterpret_cast<const uint16_t *>(scales);
     const uint16_t ex = scale_dtype == NNQ_BF16 ? 0x7F80 : 0x7C00;
     const int64_t groups = n * (k / group);
     for (int64_t i = 0; i < groups; i++)
-        if ((sc[i] & ex) == ex) return fail(NNQ_ERR_NON_FINITE, "scale %lld is not finite", (long long)i);
+        if ((sc[i] & ex) == ex) return bad_int4_scale(i);
     for (int64_t i = 0; zeros && i < groups; i++)
-        if (zeros[i] > 16) return fail(NNQ_ERR_INVALID_ARGUMENT, "zero point %lld is %d (0 to 16)", (long long)i, zeros[i]);
+        if (zeros[i] > 16) return bad_int4_zero(i);
     std::vector<uint8_t> host;
     nnq_weight *w = nullptr;
     try {
@@ -457,6 +475,39 @@ int nnq_weight_create_int4(const uint8_t *codes, const void *scales, nnq_dtype s
         if (w->dev) hipFree(w->dev);
         delete w;
         return hip_fail(e, "weight upload");
+    }
+    *out = w;
+    return NNQ_OK;
+}
+
+int nnq_weight_create_int4_device(const uint8_t *codes, const void *scales, nnq_dtype scale_dtype, const uint8_t *zeros,
+                                  int64_t n, int64_t k, int64_t group, nnq_weight **out, void *stream) {
+    Layout L;
+    const int rc = check_int4(codes, scales, scale_dtype, zeros, n, k, group, out, &L);
+    if (rc) return rc;
+    if (((uintptr_t)codes & 3) || ((uintptr_t)scales & 1))
+        return fail(NNQ_ERR_INVALID_ARGUMENT, "codes must be 4-byte and scales 2-byte aligned");
+    const hipStream_t st = (hipStream_t)stream;
+    nnq_weight *w = new (std::nothrow) nnq_weight;
+    if (!w) return fail(NNQ_ERR_OUT_OF_MEMORY, "weight handle");
+    w->L = L;
+    hipGetDevice(&w->device);
+    unsigned long long bad[2] = {0, 0};
+    // (the two indices behind the image)
+    const size_t at = (L.total() + 15) / 16 * 16;
+    hipError_t e = hipMalloc(&w->dev, at + sizeof bad);
+    if (e == hipSuccess) e = hipMemsetAsync(w->dev + at, 0xFF, sizeof bad, st);
+    if (e == hipSuccess)
+        e = (hipError_t)launch_int4_repack(L, codes, reinterpret_cast<const uint16_t *>(scales), zeros, w->dev,
+                                           reinterpret_cast<unsigned long long *>(w->dev + at), stream);
+    if (e == hipSuccess) e = hipMemcpyAsync(bad, w->dev + at, sizeof bad, hipMemcpyDeviceToHost, st);
+    if (e == hipSuccess) e = hipStreamSynchronize(st);
+    const bool ok = e == hipSuccess && bad[0] == ~0ull && bad[1] == ~0ull;
+    if (!ok) {
+        if (w->dev) hipFree(w->dev);
+        delete w;
+        if (e != hipSuccess) return hip_fail(e, "weight repack");
+        return bad[0] != ~0ull ? bad_int4_scale((int64_t)bad[0]) : bad_int4_zero((int64_t)bad[1]);
     }
     *out = w;
     return NNQ_OK;

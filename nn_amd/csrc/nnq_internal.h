@@ -264,6 +264,8 @@ struct Int4GemmPlan {
 Int4GemmPlan int4_gemm_plan(int64_t m, int64_t n, int64_t k, int group, int x_bf16);
 int64_t int4_chunk_rows(int64_t m, int64_t k);  // rows of one launch_int4_gemm
 int launch_int4_gemm(const Int4Args &a, void *scratch, void *stream);
+int launch_int4_repack(const Layout &L, const uint8_t *codes, const uint16_t *scales, const uint8_t *zeros, uint8_t *w,
+                       unsigned long long *bad, void *stream);
 int launch_int4_dequant(const Layout &L, const uint8_t *w, float *out, void *stream);
 
 // ---- log probabilities (nnq_logprobs.hip) -------------------------------------------

@@ -67,6 +67,34 @@ def test_dequantize_is_exact(n, k, group, zeros, scale):
     assert torch.equal(w.dequantize().double(), ref)  # 5 bits times 11 (8): no rounding
 
 
+@pytest.mark.parametrize("zeros", [True, False])
+@pytest.mark.parametrize("n,k,group", [(1, 32, 32), (17, 160, 32), (16, 128, 128), (100, 2880, 64), (333, 1152, 128), (8209, 4224, 32)])
+def test_image_made_on_the_device(n, k, group, zeros):
+    """The same weight from host arrays, device arrays and an odd view of them."""
+    import nn_amd
+    g = torch.Generator()
+    g.manual_seed(n)
+    flat = torch.randint(0, 256, (n * k // 2 + 1,), generator=g, dtype=torch.int32).to(torch.uint8)
+    c = flat[1:].view(n, k // 2)
+    s = (0.01 * torch.randn(n, k // group, generator=g)).half()
+    z = torch.randint(0, 17, (n, k // group), generator=g) if zeros else None
+    make = lambda *t: nn_amd.QuantizedWeight.from_int4_groups(*t, group)  # noqa: E731
+    host, x = make(c, s, z), tokens(20, k, BF16)
+    ref, y = host.dequantize(), nn_amd.quantized_linear(x, host)
+    cz = None if z is None else z.cuda()
+    for w in (make(c.cuda(), s.cuda(), cz), make(flat.cuda()[1:].view(n, k // 2), s, z), make(c, s.cuda(), cz)):
+        assert torch.equal(w.dequantize(), ref) and torch.equal(nn_amd.quantized_linear(x, w), y)
+    bad = s.clone()
+    bad[n // 2, -1] = float("inf")
+    with pytest.raises(nn_amd.NonFiniteData, match=str((n // 2 + 1) * (k // group) - 1)):
+        make(c.cuda(), bad, z)
+    if zeros:
+        bad = z.to(torch.uint8)
+        bad[-1, 0] = 17
+        with pytest.raises(nn_amd.TensorError, match="zero point"):
+            make(c.cuda(), s, bad)
+
+
 SHAPES = [(1, 1, 32, 32), (1, 5, 64, 64), (2, 40, 128, 128), (3, 16, 160, 32), (1, 300, 2880, 64), (8, 33, 1152, 128),
           (9, 100, 2912, 32), (16, 257, 4096, 128), (1, 8209, 640, 128), (5, 8304, 4096, 64), (12, 8193, 5120, 32),
           (7, 64, 12288, 128), (16, 48, 8320, 64), (1, 9000, 4224, 128)]

@@ -50,6 +50,20 @@ def test_int4_create_refusals(lib):
     assert create(lib, c, s, None, 1 << 40, 1 << 30, 128) == _lib.ERR_OUT_OF_MEMORY
 
 
+def test_int4_device_create_refusals(lib):
+    """What the device form refuses before it touches memory."""
+    f, h = lib.nnq_weight_create_int4_device, ctypes.c_void_p()
+    ok = [4096, 8192, 1, 12288, 4, 128, 128]
+    for i, v, code in ((0, None, _lib.ERR_INVALID_ARGUMENT), (1, None, _lib.ERR_INVALID_ARGUMENT), (0, 4098, _lib.ERR_INVALID_ARGUMENT),
+                       (1, 8193, _lib.ERR_INVALID_ARGUMENT), (2, 0, _lib.ERR_UNSUPPORTED), (4, 0, _lib.ERR_INVALID_ARGUMENT),
+                       (5, 96, _lib.ERR_INVALID_SHAPE), (5, 1 << 21, _lib.ERR_UNSUPPORTED), (6, 16, _lib.ERR_INVALID_SHAPE),
+                       (4, 1 << 60, _lib.ERR_OUT_OF_MEMORY)):
+        args = list(ok)
+        args[i] = v
+        assert f(*args, ctypes.byref(h), None) == code, (i, v)
+    assert f(*ok, None, None) == _lib.ERR_INVALID_ARGUMENT and not h.value
+
+
 def test_from_int4_groups_refusals():
     with pytest.raises(nn_amd.Unsupported):
         nn_amd.QuantizedWeight.from_int4_groups(torch.zeros(4, 64, dtype=torch.uint8), torch.ones(4, 1).half(), [[8]] * 4)
