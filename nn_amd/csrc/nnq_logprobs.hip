@@ -195,7 +195,7 @@ __global__ __launch_bounds__(kSegWaves * 64) void logprob_seg_kernel(LpArgs a) {
         // a segment before the token's counts equal logits, one after it does not
         const int64_t first = seg * kSeg - off;
         uint32_t before = 0;
-        if (ask) {
+        if (ask && lt <= mx) {  // (a likely token: few segments reach its logit)
             if (first > tok) {
 #pragma unroll
                 for (int e = 0; e < kPer; e++) before += x[e] > lt;
