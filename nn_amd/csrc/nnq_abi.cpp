@@ -636,7 +636,7 @@ static bool prefill_swiglu(const nnq_weight *w, int64_t m, nnq_dtype x_dtype) {
     return gemm_wide_swiglu(g);
 }
 
-// a validated linear call over 4-bit codes with group scales: up to kInt4Rows rows in one launch that
+// a validated linear call over 4-bit codes with group scales: few rows in one launch that
 // reads the weight once, more through the MFMA GEMM
 static Int4Args int4_args(const nnq_weight *w, const void *x, nnq_dtype x_dtype, int64_t m, const float *bias, void *y,
                           nnq_dtype y_dtype) {
@@ -661,7 +661,7 @@ static Int4Args int4_args(const nnq_weight *w, const void *x, nnq_dtype x_dtype,
 
 static size_t int4_launch_scratch(const nnq_weight *w, int64_t m, nnq_dtype x_dtype) {
     const int xb = x_dtype == NNQ_BF16;
-    return m <= kInt4Rows ? int4_rows_scratch(m, w->L.n, w->L.k, xb) : int4_gemm_plan(m, w->L.n, w->L.k, w->L.group, xb).bytes;
+    return int4_takes_rows(m, w->L.n, w->L.k, xb) ? int4_rows_scratch(m, w->L.n, w->L.k, xb) : int4_gemm_plan(m, w->L.n, w->L.k, w->L.group, xb).bytes;
 }
 
 static size_t int4_scratch_bytes(const nnq_weight *w, int64_t m, nnq_dtype x_dtype) {
@@ -683,7 +683,7 @@ static int dispatch_int4(const nnq_weight *w, const void *x, nnq_dtype x_dtype, 
     for (int64_t m0 = 0; m0 < m; m0 += mc) {
         const Int4Args a = int4_args(w, (const uint8_t *)x + (size_t)m0 * w->L.k * xe, x_dtype, std::min(mc, m - m0),
                                      bias, (uint8_t *)y + (size_t)m0 * w->L.n * ye, y_dtype);
-        int e = a.m <= kInt4Rows ? launch_int4_rows(a, scr, stream) : launch_int4_gemm(a, scr, stream);
+        int e = int4_takes_rows(a.m, a.n, a.k, a.x_bf16) ? launch_int4_rows(a, scr, stream) : launch_int4_gemm(a, scr, stream);
         if (e) return hip_fail((hipError_t)e, "int4 linear launch");
     }
     return NNQ_OK;

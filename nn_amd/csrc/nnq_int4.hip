@@ -191,7 +191,7 @@ __device__ __forceinline__ uint64_t int4_argmax_key(float v, uint32_t idx) {
 // / ks, ... of R tiles, for up to 4 IT token rows.
 template <int XF, int IT, int GS, bool Z, int R, int UPW>
 __global__ __launch_bounds__(1024) void int4_rows_kernel(Int4Args a) {
-    constexpr int P = planes(XF);
+    constexpr int P = planes(XF), TOK = 4 * IT;  // tokens
     constexpr int UB = int4_unit_bytes(kInt4Unit / GS, Z);
     const int tid = threadIdx.x, lane = tid & 63;
     const int wv = __builtin_amdgcn_readfirstlane(tid >> 6), waves = (int)(blockDim.x >> 6);
@@ -297,10 +297,10 @@ __global__ __launch_bounds__(1024) void int4_rows_kernel(Int4Args a) {
             }
         }
         // lane 16p + c: rows 4p .. 4p + 3 of output column c, for each tile -> [tile][token][column][17 waves]
-        float *rb = red + par * R * 256 * 17;
+        float *rb = red + par * R * TOK * 272;
 #pragma unroll
         for (int r = 0; r < R; r++) {
-            float *o = rb + (r * 256 + c) * 17 + wv;
+            float *o = rb + (r * TOK * 16 + c) * 17 + wv;
             if constexpr (XF == XPAIR) {
                 if (2 * p4 < m) o[(2 * p4) * 272] = sum[r][0] + sum[r][1];
                 if (2 * p4 + 1 < m) o[(2 * p4 + 1) * 272] = sum[r][2] + sum[r][3];
@@ -313,8 +313,12 @@ __global__ __launch_bounds__(1024) void int4_rows_kernel(Int4Args a) {
         __syncthreads();  // also: every wave is past its reads of the other buffer
         // a wave takes four outputs at a time, a wave's part of each to a lane of 16
         for (int i = wv; i < R * m * 4; i += waves) {
-            const int r = (i >> 2) >= m, t = (i >> 2) - (r ? m : 0), col = 4 * (i & 3) + p4;
-            float v = c < waves ? rb[((r * 16 + t) * 16 + col) * 17 + c] : 0.f;
+            int r = 0, t = i >> 2;
+#pragma unroll
+            for (int q = 1; q < R; q++)
+                if (t >= m) r++, t -= m;
+            const int col = 4 * (i & 3) + p4;
+            float v = c < waves ? rb[((r * TOK + t) * 16 + col) * 17 + c] : 0.f;
             v = add_row<0xB1>(v);
             v = add_row<0x4E>(v);
             v = add_row<0x141>(v);
@@ -364,15 +368,20 @@ int cus() {
     return n[dev];
 }
 
-template <int XF, int IT, int GS, bool Z, int R, int UPW>
-int launch_rows_t(const Int4Args &a, void *stream) {
-    // a wave for every unit, up to 16; the chip holds 16 / waves workgroups per CU
+// a wave for every unit of a part of K, 4 to 16
+int rows_waves(const Int4Args &a) {
     const int64_t part = (a.units + a.ks - 1) / a.ks;
     int waves = 16;
     while (waves > 4 && waves / 2 >= part) waves /= 2;
+    return waves;
+}
+
+template <int XF, int IT, int GS, bool Z, int R, int UPW>
+int launch_rows_t(const Int4Args &a, void *stream) {
+    const int waves = rows_waves(a);  // the chip holds 16 / waves workgroups per CU
     const int64_t blocks = (a.ntile + R - 1) / R;
     const int64_t grid = std::min<int64_t>(blocks, std::max<int64_t>(1, (int64_t)cus() * (16 / waves) / a.ks)) * a.ks;
-    const size_t lds = (size_t)waves * (4096 + 64) + 2 * R * 256 * 17 * 4;
+    const size_t lds = (size_t)waves * (4096 + 64) + 2 * R * 4 * IT * 272 * 4;
     if (a.argmax_count) *a.argmax_count = grid;
     auto *kernel = int4_rows_kernel<XF, IT, GS, Z, R, UPW>;
     hipError_t e = allow_lds(reinterpret_cast<const void *>(kernel), lds);
@@ -383,9 +392,17 @@ int launch_rows_t(const Int4Args &a, void *stream) {
 
 template <int XF, int IT, int GS, bool Z>
 int launch_rows_r(const Int4Args &a, void *stream) {
-    if constexpr (XF == XPLANES) return launch_rows_t<XF, IT, GS, Z, 1, 1>(a, stream);
-    else return a.ntile > 2 * (int64_t)cus() ? launch_rows_t<XF, IT, GS, Z, 2, 2>(a, stream)
-                                             : launch_rows_t<XF, IT, GS, Z, 1, 2>(a, stream);
+    if constexpr (XF == XPLANES) {
+        return launch_rows_t<XF, IT, GS, Z, 1, 1>(a, stream);
+    } else {
+        // Two tiles at a time where every workgroup has more than two; up to 16 units a wave has one, not a
+        // second that does not exist (us, R = 2: 1 x 2048 -> 151936 34 with one unit a wave, 56 with two,
+        // 1024 -> 151936 20 and 30; R = 1: 2048 -> 4096 4.6 and 5.1; 8 x 2048 -> 12288 9.1 and 12.0).
+        const bool two = a.ntile > 2 * (int64_t)cus() * (16 / rows_waves(a));
+        if ((a.units + a.ks - 1) / a.ks <= 16)
+            return two ? launch_rows_t<XF, IT, GS, Z, 2, 1>(a, stream) : launch_rows_t<XF, IT, GS, Z, 1, 1>(a, stream);
+        return two ? launch_rows_t<XF, IT, GS, Z, 2, 2>(a, stream) : launch_rows_t<XF, IT, GS, Z, 1, 2>(a, stream);
+    }
 }
 
 template <int XF, int IT>

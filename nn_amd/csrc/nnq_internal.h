@@ -248,7 +248,8 @@ struct Int4Args {
     int ks;                              // (set by the launch: parts of K, their sums in slabs [ks][m][n])
     float *slabs;
 };
-constexpr int kInt4Rows = 16;  // token rows of one launch_int4_rows
+constexpr int kInt4Rows = 16;  // the most token rows of one launch_int4_rows
+bool int4_takes_rows(int64_t m, int64_t n, int64_t k, int x_bf16);  // or launch_int4_gemm
 // scratch: int4_rows_scratch bytes, or null for a launch that does not split K
 int launch_int4_rows(const Int4Args &a, void *scratch, void *stream);
 int int4_rows_split(int64_t m, int64_t n, int64_t k, int x_bf16);

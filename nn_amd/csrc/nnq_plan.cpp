@@ -66,6 +66,23 @@ size_t int4_rows_scratch(int64_t m, int64_t n, int64_t k, int x_bf16) {
     return ks > 1 ? (size_t)ks * (size_t)m * (size_t)n * 4 : 0;
 }
 
+// Whether a 4-bit call of up to 16 rows takes the kernel for rows: always up to four; above, the shorter of
+// two estimates (us, U units of 128 k, T 16-row tiles per CU), fitted on MI355X to 22 weights of 1024 to
+// 151936 rows and K 512 to 12288 at 5 to 16 token rows.  The rows kernel's grows with the token rows, each of
+// which it sums over its waves and stores apart (8 bf16 rows of 151936 x 1024 40 us, GEMM 25; x 4096 72 and
+// 77; 16 f32 rows of 24576 x 4096 33 and 25, of 4096 x 4096 12 and 13.6).  The mean choice takes 1% more
+// than the better one, the worst 22% (2 us).
+bool int4_takes_rows(int64_t m, int64_t n, int64_t k, int x_bf16) {
+    if (m <= 4 || m > kInt4Rows) return m <= 4;
+    static const double rows[2][2][5] = {{{3.3, 0.085, 0.033, 0.083, 0.14}, {5.1, 0.051, 0.084, 0.062, 0.0}},
+                                         {{3.0, 0.05, 0.037, 0.07, 0.2}, {2.5, 0.11, 0.007, 0.105, 0.7}}};
+    static const double gemm[2][3] = {{9.1, 0.05, 0.069}, {8.6, 0.044, 0.057}};
+    const double units = (double)((k + kInt4Unit - 1) / kInt4Unit);
+    const double tiles = std::max(1.0, (double)((n + kTile - 1) / kTile) / 256);
+    const double *r = rows[x_bf16 ? 1 : 0][m > 8], *g = gemm[x_bf16 ? 1 : 0];
+    return r[0] + r[1] * units + tiles * (r[2] * units + r[3] * (double)m + r[4]) <= g[0] + g[1] * units + g[2] * tiles * units;
+}
+
 // 4-bit prefill: the workgroup tile (mt x 32 rows, nt x 128 columns) and the K split of the least
 // estimated time.  c workgroups on a CU take c * step + lag per unit of 128 k (fitted on MI355X to
 // 20 to 1024 rows of 1024 to 40960 columns, K 1024 to 12288: the choice is within 6% of the best of

@@ -115,6 +115,25 @@ def test_rows(m, n, k, group, zeros, scale, xdt):
     assert torch.equal(nn_amd.quantized_linear(x, w, bias, out_dtype=BF16), y.to(BF16))
 
 
+# up to 16 units of K: one a wave, with one tile at a time or two, in workgroups of 16, 8 and 4 waves
+SHORT_K = [(1, 8304, 2048, 64), (4, 8193, 1984, 32), (3, 17000, 1024, 128), (2, 33025, 512, 128), (1, 40000, 96, 32),
+           (7, 9000, 1920, 64), (8, 300, 2048, 128), (13, 8300, 2048, 128), (16, 500, 1152, 128), (5, 16500, 640, 128)]
+
+
+@pytest.mark.parametrize("xdt", [F32, BF16])
+@pytest.mark.parametrize("zeros", [True, False])
+@pytest.mark.parametrize("m,n,k,group", SHORT_K)
+def test_rows_of_a_short_k(m, n, k, group, zeros, xdt):
+    import nn_amd
+    w, ref = make(n, k, group, zeros)
+    x = tokens(m, k, xdt)
+    y = nn_amd.quantized_linear(x, w)
+    check(y, x.double() @ ref.t())
+    if m == 1 and xdt is F32:
+        logits, idx = nn_amd.linear_argmax(x, w)
+        assert torch.equal(logits, y[0]) and idx.item() == int(torch.nonzero(y[0] == y.max())[0])
+
+
 PREFILL = [(17, 16, 128, 128), (33, 300, 160, 32), (48, 129, 2880, 64), (64, 257, 1152, 128), (130, 1000, 4096, 128),
            (203, 512, 2912, 32), (300, 4100, 640, 64), (513, 264, 4224, 128), (1, 512, 1024, 128)]
 

@@ -109,7 +109,9 @@ def test_int4_plans(lib, xb, group):
     scratch regions that hold what the launches write."""
     plan, split = lib._ZN3nnq14int4_gemm_planElllii, lib._ZN3nnq15int4_rows_splitEllli
     rows_scratch, chunk = lib._ZN3nnq17int4_rows_scratchEllli, lib._ZN3nnq15int4_chunk_rowsEll
+    takes = lib._ZN3nnq15int4_takes_rowsEllli
     i64 = ctypes.c_int64
+    takes.argtypes, takes.restype = [i64, i64, i64, ctypes.c_int], ctypes.c_bool
     plan.argtypes, plan.restype = [i64, i64, i64, ctypes.c_int, ctypes.c_int], GemmPlan
     split.argtypes, split.restype = [i64, i64, i64, ctypes.c_int], ctypes.c_int
     rows_scratch.argtypes, rows_scratch.restype = [i64, i64, i64, ctypes.c_int], ctypes.c_size_t
@@ -117,6 +119,7 @@ def test_int4_plans(lib, xb, group):
     for n in (1, 16, 100, 4096, 12288, 151936):
         for k in (group, 128, 320 * group // 32, 4096, 12288, 1 << 20):
             units = (k + 127) // 128
+            assert all(takes(m, n, k, xb) for m in (1, 4)) and not takes(17, n, k, xb)
             for m in (1, 4, 5, 8, 9, 16):
                 ks = split(m, n, k, xb)
                 assert 1 <= ks <= min(8, units) and (m > 4 or ks == 1)  # (one row: no scratch)
@@ -131,6 +134,16 @@ def test_int4_plans(lib, xb, group):
                 assert p.plane == tiles * units * 8192 and planes * p.plane < 2 ** 31  # 32-bit offsets
                 assert p.rowback == planes * p.plane and p.slabs >= p.rowback + tiles * 128 and p.slabs % 256 == 0
                 assert p.bytes >= p.slabs + (p.ks * r * n * 4 if p.ks > 1 else 0)
+
+
+def test_int4_few_rows_or_gemm(lib):
+    """The rule's two sides, as measured (8 bf16 rows: 72 us against 77, 40 against 25; 16 f32 rows: 12
+    against 13.6, 33 against 25)."""
+    takes = lib._ZN3nnq15int4_takes_rowsEllli
+    takes.argtypes, takes.restype = [ctypes.c_int64] * 3 + [ctypes.c_int], ctypes.c_bool
+    for m, n, k, xb, rows in ((8, 151936, 4096, 1, 1), (8, 151936, 1024, 1, 0), (16, 4096, 4096, 0, 1),
+                              (12, 4096, 12288, 1, 1), (16, 65536, 512, 1, 0), (5, 5751, 2880, 0, 1), (16, 24576, 4096, 0, 0)):
+        assert takes(m, n, k, xb) == bool(rows), (m, n, k, xb)
 
 
 def test_int4_gguf_formats_refuse_the_layout(lib):
