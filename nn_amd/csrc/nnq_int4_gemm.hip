@@ -6,14 +6,20 @@
 // an operand: scale * (q - z) has up to 16 significant bits.
 //  * int4_stage_kernel writes x once as f16 of x * 2^s_row (f32 x: a hi and a lo plane) in the order
 //    of the MFMA's A operands, per 32 rows and unit of 128 k one 8 KB piece, and 2^-s_row per row.
-//  * int4_gemm_kernel: a workgroup of W waves takes MT * 32 rows and W * 32 columns.  The A pieces of
-//    a unit go through two LDS buffers, one barrier per unit; a wave's weights go from memory straight
-//    into its registers and become the B operands of its own 32 columns, each used for MT MFMAs, so
-//    no operand is dequantized twice in a workgroup and none passes through LDS.
+//  * int4_gemm_kernel: a workgroup of four waves takes MT * 32 rows and NT * 128 columns.  The A
+//    pieces of a unit are copied straight to one of two LDS buffers, a unit ahead, with one barrier
+//    per unit; a wave's weights go from memory into its registers, a unit ahead too, and become the B
+//    operands of its own NT * 32 columns, each used for MT MFMAs, so no operand is dequantized twice
+//    in a workgroup and none passes through LDS.  (An A operand read from LDS feeds NT MFMAs: with NT
+//    = 1 the reads take as long as the MFMAs.)
 //  * A group's MFMAs start from zero (results in VGPRs, the build's VGPR-form option for this file)
 //    and are added to the totals times the scale of the lane's column: 16 FMAs per 32 x 32 tile and
 //    group, beside 8 (group 128), 4 or 2 MFMAs of 32 cycles.
 //  * With too few workgroups K is split: f32 slabs, added in order by int4_sum_kernel.
+// Measured (MI355X, bf16 x, groups of 128): 512 x 4096 -> 12288 54 us + 6 of staging, 0.95 PFLOP/s;
+// 300 x 4096 -> 151936 360 to 410 us, 1.04 to 0.91 PFLOP/s, the clock lower the longer it runs (the
+// library's f16 product of 8192^3: 1.06 to 1.3).  The MFMAs alone, with nothing beside them, take
+// 78 us of 512 x 4096 -> 24576 (1.3 PFLOP/s), all of the kernel 108.
 #include <algorithm>
 #include <type_traits>
 
@@ -32,9 +38,12 @@ __device__ __forceinline__ floatx16 mfma32(u32x4 a, u32x4 b, floatx16 c) {
     return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(half8, a), __builtin_bit_cast(half8, b), c, 0, 0, 0);
 }
 
-// Four rows a workgroup (thread % 4): the row's largest |x|, then its 8-column chunks, chunk c of the
+// ROWS rows a workgroup (thread % ROWS): the row's largest |x|, then its 8-column chunks, chunk c of the
 // row at piece c / 16, step (c / 2) % 8, half c % 2.  Chunks past K are zeros.  A thread's first kHold
-// chunks stay in registers between the two (all of them up to K = 8192).
+// chunks stay in registers between the two (all of them up to K = 8192, two rows: 16384).  Four adjacent
+// rows write 64 bytes together; two fill the chip from half as many rows, and the two halves of four go to
+// one XCD, whose L2 joins them (us, two / four: 203 f32 rows of 12288 8.8 / 14.0, 512 bf16 rows of 4096
+// 5.4 / 5.5, 2048 10.2 / 9.4).
 template <int ROWS>
 __device__ __forceinline__ int stage_row(int b) {
     return ROWS == 4 ? b * 4 : (b / 16 * 8 + b % 8) * 4 + b / 8 % 2 * 2;

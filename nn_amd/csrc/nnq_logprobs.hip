@@ -7,8 +7,9 @@
 // Keeping the maximum's own 1 out of R holds the log probability of a nearly certain token, and
 // the entropy of such a row, to a relative 2^-23 where 1 + R would round R away.
 //
-// Bound: one read of the logits (HBM, or the cache that a GEMM left them in), with some fourteen
-// VALU instructions and an exponential per logit beside it.  Two launches:
+// Bound: one read of the logits (HBM, or the cache that a GEMM left them in), with some twelve VALU
+// instructions and an exponential per logit beside it, twenty with rank and alternatives.  Two
+// launches:
 //   logprob_seg_kernel   one wave per 2048 logits of a row, all of them in registers: the segment's
 //                        maximum, then (count of the maximum, R, S) against it, how many logits
 //                        come before the token, and the candidates of the top N.
@@ -19,6 +20,10 @@
 // the 2048 reach it (N = 20).  Where more do than there are slots (many equal logits, or a row's
 // largest in few lanes) the exact N-th value, and among its equals the lowest indices, are
 // found the same way over all 2048.
+// Measured (MI355X, f32 logits of 151936): 512 rows 51.5 + 4.7 us (6.0 TB/s, the streaming read's rate
+// is 7.0); 301 rows with rank and 5 alternatives 35.5 + 4.7 us (5.2 TB/s; the VALU is busy 80% of it);
+// one row with 20 alternatives 6.0 + 5.4 us, both latency, and 19 us from Python (five tensors and two
+// launches).  48 bf16 rows of 50257 7.4 + 4.6 us.
 #include <algorithm>
 
 #include "nnq_device.h"
