@@ -187,6 +187,60 @@ def test_activation_range(m, xdt):
         assert (y[t].double() - r[t]).abs().max().item() <= 1e-5 * rms, t
 
 
+@pytest.mark.parametrize("m", [1, 6, 12, 40])
+def test_smallest_and_largest_scales(m):
+    """f16 scales below the smallest normal one and at the largest, each the only ones of a weight."""
+    import nn_amd
+    for value in (2.0 ** -24, 3 * 2.0 ** -20, 65504.0):
+        q = torch.randint(0, 256, (50, 192), dtype=torch.int32).to(torch.uint8)
+        s = torch.full((50, 6), value, dtype=F16)
+        w = nn_amd.QuantizedWeight.from_int4_groups(q.cuda(), s, None, 64)
+        codes = torch.stack([q & 15, q >> 4], 2).view(50, 384).double().cuda() - 8
+        assert torch.equal(w.dequantize().double(), codes * value)
+        for xdt in (F32, BF16):
+            x = tokens(m, 384, xdt)
+            check(nn_amd.quantized_linear(x, w), x.double() @ (codes * value).t(), value)
+
+
+@pytest.mark.parametrize("m", [1, 6, 12, 40])
+def test_activations_below_the_smallest_normal(m):
+    """f32 x of multiples of 2^-140 (subnormal: nine bits are left), scales that bring the result back up."""
+    import nn_amd
+    g = torch.Generator(device="cuda")
+    g.manual_seed(5)
+    q = torch.randint(0, 256, (40, 128), generator=g, device="cuda", dtype=torch.int32).to(torch.uint8)
+    w = nn_amd.QuantizedWeight.from_int4_groups(q, torch.full((40, 2), 65504.0, dtype=F16), None, 128)
+    codes = torch.stack([q & 15, q >> 4], 2).view(40, 256).double() - 8
+    x = torch.randint(-400, 401, (m, 256), generator=g, device="cuda").float() * 2.0 ** -140
+    assert x.abs().max() < torch.finfo(F32).tiny and x.abs().max() > 0
+    check(nn_amd.quantized_linear(x, w), x.double() @ (codes * 65504.0).t())
+
+
+def test_threads_on_their_own_streams_and_on_one():
+    """Calls of two host threads, each on a stream of its own, then both on one."""
+    import threading
+    import nn_amd
+    w, _ = make(4500, 9600, 64)
+    xs = [tokens(m, 9600, F32, seed=m) for m in (7, 40)]
+    want = [nn_amd.quantized_linear(x, w) for x in xs]
+    torch.cuda.synchronize()
+    one = torch.cuda.Stream()
+    for streams in ([torch.cuda.Stream(), torch.cuda.Stream()], [one, one]):
+        bad = []
+
+        def loop(i):
+            with torch.cuda.stream(streams[i]):
+                for _ in range(30):
+                    if not torch.equal(nn_amd.quantized_linear(xs[i], w), want[i]):
+                        bad.append(i)
+
+        threads = [threading.Thread(target=loop, args=(i,)) for i in range(2)]
+        [t.start() for t in threads]
+        [t.join() for t in threads]
+        torch.cuda.synchronize()
+        assert not bad
+
+
 @pytest.mark.parametrize("m", [1, 3, 12, 30])
 def test_non_finite_activations_stay_in_their_row(m):
     import nn_amd
