@@ -17,9 +17,9 @@
 //                        and added in a fixed order, and the N largest candidates by rank.
 // Candidates of a segment: the N-th largest of the 64 lanes' maxima is a lower bound of the N-th
 // largest logit (N <= 32), found with ballots over its bits; on continuous logits about 1.2 N of
-// the 2048 reach it (N = 20).  Where more do than there are slots (many equal logits, or a row's
-// largest in few lanes) the exact N-th value, and among its equals the lowest indices, are
-// found the same way over all 2048.
+// the 2048 reach it (N = 20).  Of more than there are slots the largest are kept; of more than 64 (many
+// equal logits, or a row's largest in few lanes) the exact N-th value, and among its equals the lowest
+// indices, are found the same way over all 2048.
 // Measured (MI355X, f32 logits of 151936): 512 rows 51.5 + 4.7 us (6.0 TB/s, the streaming read's rate
 // is 7.0); 301 rows with rank and 5 alternatives 35.5 + 4.7 us (5.2 TB/s; the VALU is busy 80% of it);
 // one row with 20 alternatives 6.0 + 5.4 us, both latency, and 19 us from Python (five tensors and two
@@ -224,41 +224,54 @@ __global__ __launch_bounds__(kSegWaves * 64) void logprob_seg_kernel(LpArgs a) {
         __shared__ uint64_t list[kSegWaves][64];
         const int want = a.top;
         const uint32_t mine = lm == lm ? ord(lm) : 0;  // (no number in the lane)
-        // (its leading 16 bits do: a bound at most 2^-7 of its size below lets hardly more candidates in)
-        const uint32_t lanes = largest_with<16>(want, [&](uint32_t k) { return __popcll(__ballot(mine >= k)); });
+        // (its leading 24 bits do: a bound 2^-15 of its size below lets hardly more candidates in, also for
+        // logits far from 0; with 16 bits 301 x 151936 logits around 300 took 114 us, 43 with 24)
+        const uint32_t lanes = largest_with<24>(want, [&](uint32_t k) { return __popcll(__ballot(mine >= k)); });
         float t = unord(max(lanes, kOrdNegInf + 1));  // (-inf is no candidate)
         // the lane's candidates as bits, element 0 the highest
         uint32_t bits = 0;
 #pragma unroll
         for (int e = 0; e < kPer; e++) bits = bits + bits + (x[e] >= t);
         const int total = (int)sum64u(__popc(bits));
-        if (total > a.slots) {  // uniform
-            t = unord(largest_with<32>(want, [&](uint32_t k) {
-                const float f = unord(k);
+        if (total > 64) {  // uniform
+            // The exact N-th largest: the lanes' bound in all its bits where fewer logits lie above it (many
+            // logits equal to it), else searched over the 2048.
+            auto above = [&]() {
                 int c = 0;
 #pragma unroll
-                for (int e = 0; e < kPer; e++) c += __popcll(__ballot(x[e] >= f && x[e] > kNegInf));
+                for (int e = 0; e < kPer; e++) c += __popcll(__ballot(x[e] > t));
                 return c;
-            }));
-            int more = 0;
+            };
+            t = unord(max(largest_with<32>(want, [&](uint32_t k) { return __popcll(__ballot(mine >= k)); }), kOrdNegInf + 1));
+            int more = above();
+            if (more >= want) {
+                t = unord(largest_with<32>(want, [&](uint32_t k) {
+                    const float f = unord(k);
+                    int c = 0;
 #pragma unroll
-            for (int e = 0; e < kPer; e++) more += __popcll(__ballot(x[e] > t));
-            // the lowest `need` of the logits equal to t: the largest bound with fewer, plus one
-            const int need = want - more;
-            uint32_t b = 0;
-            for (uint32_t bit = kSeg / 2; bit; bit >>= 1) {
-                int c = 0;
-#pragma unroll
-                for (int e = 0; e < kPer; e++)
-                    c += __popcll(__ballot(x[e] == t && (uint32_t)((e / V) * 64 * V + lane * V + e % V) < (b | bit)));
-                if (c < need) b |= bit;
+                    for (int e = 0; e < kPer; e++) c += __popcll(__ballot(x[e] >= f));
+                    return c;
+                }));
+                more = above();
             }
-            const int upto = (int)b;  // logits equal to t count up to this place of the segment
+            // of the logits equal to it the first want - more in index order
+            uint32_t before = more;
             bits = 0;
 #pragma unroll
-            for (int e = 0; e < kPer; e++) {
-                const int place = (e / V) * 64 * V + lane * V + e % V;
-                bits = bits + bits + (x[e] > kNegInf && (x[e] > t || (x[e] == t && place <= upto)));
+            for (int v = 0; v < kPer / V; v++) {
+                uint32_t at_lane = before;
+#pragma unroll
+                for (int e = 0; e < V; e++) {
+                    const uint64_t b = __ballot(x[v * V + e] == t);
+                    at_lane = __builtin_amdgcn_mbcnt_hi((uint32_t)(b >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)b, at_lane));
+                    before += __popcll(b);
+                }
+#pragma unroll
+                for (int e = 0; e < V; e++) {
+                    const bool eq = x[v * V + e] == t;
+                    bits = bits + bits + (x[v * V + e] > t || (eq && at_lane < (uint32_t)want));
+                    at_lane += eq;
+                }
             }
         }
         // a round takes one candidate of every lane that has any
@@ -279,7 +292,14 @@ __global__ __launch_bounds__(kSegWaves * 64) void logprob_seg_kernel(LpArgs a) {
         __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
         __builtin_amdgcn_wave_barrier();
         __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
-        if (lane < a.slots) a.cand[at * a.slots + lane] = lane < listed ? list[wv][lane] : 0ull;
+        const uint64_t key = lane < listed ? list[wv][lane] : 0ull;
+        int place = lane;
+        if (listed > a.slots) {  // uniform: the largest `slots` of up to 64
+            place = 0;
+            for (int j = 0; j < listed; j++) place += list[wv][j] > key;
+            if (lane >= listed) place = a.slots;
+        }
+        if (place < a.slots) a.cand[at * a.slots + place] = key;
     }
 }
 
@@ -358,7 +378,7 @@ __global__ __launch_bounds__(kJoinThreads) void logprob_join_kernel(LpArgs a) {
 #pragma unroll
         for (int w = 1; w < NW; w++) m = max(m, maxima[64 * w + lane]);
         const uint32_t v = (uint32_t)(m >> 32);
-        const uint32_t b = largest_with<16>(a.top, [&](uint32_t k) { return __popcll(__ballot(v >= k)); });
+        const uint32_t b = largest_with<24>(a.top, [&](uint32_t k) { return __popcll(__ballot(v >= k)); });
         if (lane == 0) bound = b;
     }
     __syncthreads();

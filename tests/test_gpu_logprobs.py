@@ -124,6 +124,38 @@ def test_ties(top, dtype):
     check(nn_amd.token_logprobs(x, t, top_n=top, ranks=True), plain(x, t, top), top)
 
 
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("top", [1, 5, 20, 32])
+def test_candidates_around_the_slots(dtype, top):
+    """From fewer than a segment's slots to more than a wave's lanes reach the bound, all equal or not: copies of
+    the largest value, logits far from 0, masks of the type's lowest value, the largest in one run of the row."""
+    import nn_amd
+    n = 5000
+    rows = []
+    g = torch.Generator(device="cuda")
+    g.manual_seed(top)
+    base = torch.randn(n, generator=g, device="cuda")
+    for k in (3, 9, 30, 40, 63, 64, 65, 200):
+        r = base.clone()
+        r[torch.randperm(2040, generator=g, device="cuda")[:k]] = 6.0  # in the first segment
+        rows.append(r)
+    rows += [base + 300.0, base * 1e-3 + 3000.0, base * 1e-30]
+    low = torch.full((n,), torch.finfo(dtype).min, device="cuda")
+    few = torch.randperm(n, generator=g, device="cuda")
+    for k in (0, 1, top - 1, top, 90):
+        r = low.clone()
+        r[few[:k]] = base[few[:k]]
+        rows.append(r)
+    r = base.clone()
+    r[1000:1100] = 10.0 - torch.arange(100, device="cuda") / 16  # lanes of 4 or 8 hold all of the largest
+    rows.append(r)
+    rows.append(-torch.arange(n, device="cuda") / 32.0)
+    x = torch.stack(rows).to(dtype)
+    t = torch.randint(0, n, (len(rows),), generator=g, device="cuda")
+    check(nn_amd.token_logprobs(x, t, top_n=top, ranks=True), plain(x, t, top), top)
+    check(nn_amd.token_logprobs(x[:, 1:], t.clamp(max=n - 2), top_n=top, ranks=True), plain(x[:, 1:], t.clamp(max=n - 2), top), top)
+
+
 def test_many_equal_logits_over_many_segments():
     """Every segment offers as many candidates as it may, all equal: more than the join's list holds."""
     import nn_amd
