@@ -5,7 +5,9 @@
 //   rank_t = #{l_i > l_t} + #{l_i = l_t, i < t},  and the N largest l_i (lowest index first among
 //   equals) with their log probabilities.
 // Keeping the maximum's own 1 out of R holds the log probability of a nearly certain token, and
-// the entropy of such a row, to a relative 2^-23 where 1 + R would round R away.
+// the entropy of such a row, to a few 2^-24 relative to themselves where 1 + R would round R away: each term
+// has its d's rounding, 2^-24 |d|, and 2^-22, and the sums theirs.  (Down to d = -87; below, e^d is taken
+// for 0.)
 //
 // Bound: one read of the logits (HBM, or the cache that a GEMM left them in), with some twelve VALU
 // instructions and an exponential per logit beside it, twenty with rank and alternatives.  Two
@@ -131,6 +133,17 @@ __device__ __forceinline__ uint32_t sum64u(uint32_t v) {
     return across(v, [](uint32_t a, uint32_t b) { return a + b; });
 }
 
+// e^d for d from -1e30 to 0, to a relative 2^-22 (below d = -87.3, where it would be subnormal, it may be 0).
+// 2^p alone, with p = d log2(e) rounded, would be off by up to 2^-18 at d = -80: half a step of p, and the
+// constant's own rounding, which moves every term the same way.  The factor that is missing is e^(d - p log(2)),
+// 1 + a number below 2^-17; three FMAs beside the product and the exponential (301 rows with rank and
+// alternatives: 41.1 -> 41.4 us the whole call, 512 without 55.4 -> 55.8).
+__device__ __forceinline__ float exp_of(float d) {
+    const float p = d * 1.44269504088896340736f, e = __builtin_amdgcn_exp2f(p);
+    // log(2) in two parts: 0x1.62e43p-1 and what is left of it
+    return fmaf(e, fmaf(p, 1.9046542e-9f, fmaf(p, -0x1.62e43p-1f, d)), e);
+}
+
 // The largest t with at least `want` lanes' or elements' keys >= t, count(t) counting them
 // (non-increasing in t; count(0) >= want).
 // BITS: only the leading ones are settled (a smaller t).
@@ -184,12 +197,12 @@ __global__ __launch_bounds__(kSegWaves * 64) void logprob_seg_kernel(LpArgs a) {
     int cnt = 0;
 #pragma unroll
     for (int e = 0; e < kPer; e++) {
-        const float d = x[e] - ref;
-        const float ex = __builtin_amdgcn_exp2f(d * 1.44269504088896340736f);
+        const float d = __builtin_elementwise_maximum(x[e] - ref, -1e30f);  // (-inf: its e^d is 0; NaN stays)
+        const float ex = exp_of(d);
         const bool top = d == 0.f;
         cnt += __popcll(__ballot(top));
         r += top ? 0.f : ex;
-        s = fmaf(fmaxf(d, -1e30f), ex, s);  // (d = -inf: its e^d is 0)
+        s = fmaf(d, ex, s);
     }
     r = sum64(r);
     s = sum64(s);

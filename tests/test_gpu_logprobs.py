@@ -231,6 +231,23 @@ def test_nearly_certain_tokens():
     near(r.entropy, ref["entropy"], 0.0, 1e-5)
 
 
+@pytest.mark.parametrize("dtype", [F32, BF16, F16])
+def test_one_term_beside_the_largest(dtype):
+    """Two logits an exact distance d apart, d = -1 to -86: R is the one term e^d, and log1p(R) and the entropy are
+    as good as that and log1p.  Bar: e^d to 2^-22 (the hardware's 2^p to a unit in the last place, 2^-23, one
+    rounding of the correction, 2^-24, its terms left out below that), log1p to 2 units, 2^-22; the entropy's
+    other part -d R / (1 + R) has e^d's 2^-22 and four roundings of at most 2^-24, its last addition one more.
+    So 9 x 2^-24 relative for both."""
+    import nn_amd
+    d = torch.arange(1, 87, device="cuda")
+    x = torch.stack([torch.zeros_like(d), -d], 1).to(dtype)
+    t = torch.zeros(86, dtype=torch.int64, device="cuda")
+    r = nn_amd.token_logprobs(x, t)
+    ref = plain(x, t, 1)
+    near(r.logprobs, ref["logprobs"], 0.0, 9 * 2 ** -24)
+    near(r.entropy, ref["entropy"], 0.0, 9 * 2 ** -24)
+
+
 def test_tokens_outside_the_vocabulary():
     import nn_amd
     x, _ = draw(5, 3000, F32, seed=8)
