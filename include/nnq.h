@@ -151,7 +151,8 @@ int nnq_weight_create(nnq_format fmt, nnq_layout layout, const uint8_t *bytes, s
  * half; scales [n, k / group], NNQ_F16 or NNQ_BF16 bits; zeros [n, k / group], one byte
  * each from 0 to 16, or NULL for 8 throughout (symmetric codes).  group is 32, 64 or 128 and
  * k a multiple of it (NNQ_ERR_INVALID_SHAPE), at most 2^20 (NNQ_ERR_UNSUPPORTED); a zero
- * point over 16 is NNQ_ERR_INVALID_ARGUMENT, a scale that is not finite NNQ_ERR_NON_FINITE.  Columns are in
+ * point over 16 is NNQ_ERR_INVALID_ARGUMENT, a scale that is not finite NNQ_ERR_NON_FINITE, one of 2^88 and
+ * more in magnitude NNQ_ERR_UNSUPPORTED (the sums' range would not hold it).  Columns are in
  * order (an activation-ordered checkpoint is sorted, and its input permuted, by the caller).
  * The weight works in every call that takes an nnq_weight.  No counterpart in the
  * reference, whose 4-bit weights are Q4_K blocks. */

@@ -440,6 +440,9 @@ static int check_int4(const uint8_t *codes, const void *scales, nnq_dtype scale_
 }
 
 static int bad_int4_scale(int64_t i) { return fail(NNQ_ERR_NON_FINITE, "scale %lld is not finite", (long long)i); }
+static int large_int4_scale(int64_t i) {
+    return fail(NNQ_ERR_UNSUPPORTED, "scale %lld is 2^88 or more in magnitude", (long long)i);
+}
 static int bad_int4_zero(int64_t i) {
     return fail(NNQ_ERR_INVALID_ARGUMENT, "zero point %lld is over 16", (long long)i);
 }
@@ -456,6 +459,8 @@ int nnq_weight_create_int4(const uint8_t *codes, const void *scales, nnq_dtype s
     const int64_t groups = n * (k / group);
     for (int64_t i = 0; i < groups; i++)
         if ((sc[i] & ex) == ex) return bad_int4_scale(i);
+    for (int64_t i = 0; scale_dtype == NNQ_BF16 && i < groups; i++)
+        if ((sc[i] & ex) >= kInt4ScaleLimit) return large_int4_scale(i);
     for (int64_t i = 0; zeros && i < groups; i++)
         if (zeros[i] > 16) return bad_int4_zero(i);
     std::vector<uint8_t> host;
@@ -492,8 +497,8 @@ int nnq_weight_create_int4_device(const uint8_t *codes, const void *scales, nnq_
     if (!w) return fail(NNQ_ERR_OUT_OF_MEMORY, "weight handle");
     w->L = L;
     hipGetDevice(&w->device);
-    unsigned long long bad[2] = {0, 0};
-    // (the two indices behind the image)
+    unsigned long long bad[3] = {0, 0, 0};
+    // (the three indices behind the image)
     const size_t at = (L.total() + 15) / 16 * 16;
     hipError_t e = hipMalloc(&w->dev, at + sizeof bad);
     if (e == hipSuccess) e = hipMemsetAsync(w->dev + at, 0xFF, sizeof bad, st);
@@ -502,12 +507,13 @@ int nnq_weight_create_int4_device(const uint8_t *codes, const void *scales, nnq_
                                            reinterpret_cast<unsigned long long *>(w->dev + at), stream);
     if (e == hipSuccess) e = hipMemcpyAsync(bad, w->dev + at, sizeof bad, hipMemcpyDeviceToHost, st);
     if (e == hipSuccess) e = hipStreamSynchronize(st);
-    const bool ok = e == hipSuccess && bad[0] == ~0ull && bad[1] == ~0ull;
+    const bool ok = e == hipSuccess && bad[0] == ~0ull && bad[1] == ~0ull && bad[2] == ~0ull;
     if (!ok) {
         if (w->dev) hipFree(w->dev);
         delete w;
         if (e != hipSuccess) return hip_fail(e, "weight repack");
-        return bad[0] != ~0ull ? bad_int4_scale((int64_t)bad[0]) : bad_int4_zero((int64_t)bad[1]);
+        return bad[0] != ~0ull   ? bad_int4_scale((int64_t)bad[0])
+               : bad[2] != ~0ull ? large_int4_scale((int64_t)bad[2]) : bad_int4_zero((int64_t)bad[1]);
     }
     *out = w;
     return NNQ_OK;

@@ -451,9 +451,9 @@ __global__ __launch_bounds__(256) void dequant_int4_kernel(const uint8_t *w, int
 }
 
 // The image of codes, scales and zero points that are on the device already; one wave per (tile, unit),
-// lane 16p + r the 16 bytes of row r (rows and columns past the end: zeros).  bad[0] and bad[1] (start: all
-// ones): the lowest index of a scale that is not finite and of a zero point above 16.  Bound by HBM: it
-// reads and writes the weight once (151936 x 4096: under 0.34 ms, the whole call).
+// lane 16p + r the 16 bytes of row r (rows and columns past the end: zeros).  bad[0], bad[1] and bad[2] (start:
+// all ones): the lowest index of a scale that is not finite, of a zero point above 16 and of a bf16 scale that
+// is too large.  Bound by HBM: it reads and writes the weight once (151936 x 4096: under 0.34 ms, the whole call).
 __global__ __launch_bounds__(256) void int4_repack_kernel(const uint8_t *codes, const uint16_t *scales,
                                                           const uint8_t *zeros, int64_t n, int64_t k, int64_t units,
                                                           int64_t jobs, int group, int scale_bf16, uint8_t *w,
@@ -480,6 +480,7 @@ __global__ __launch_bounds__(256) void int4_repack_kernel(const uint8_t *codes, 
         const bool in = srow < n && g < ngroup;
         const uint32_t s = in ? scales[at] : 0u, ex = scale_bf16 ? 0x7F80u : 0x7C00u;
         if ((s & ex) == ex) atomicMin(bad, (unsigned long long)at);
+        else if (scale_bf16 && (s & ex) >= kInt4ScaleLimit) atomicMin(bad + 2, (unsigned long long)at);
         reinterpret_cast<uint16_t *>(rec + 1024)[lane] = (uint16_t)s;
         if (zeros) {
             const uint32_t z = in ? zeros[at] : 0u;

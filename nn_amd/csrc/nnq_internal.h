@@ -55,6 +55,10 @@ bool make_layout(int fmt, int layout, int64_t n, int64_t k, Layout *out, const c
 bool make_layout_int4(int64_t n, int64_t k, int64_t group, int zeros, int scale_bf16, Layout *out, const char **err);
 constexpr int kInt4Unit = 128;  // k of one unit
 constexpr int64_t kInt4MaxK = (int64_t)1 << 20;
+// Exponent bits of the smallest bf16 scale that is refused, 2^88.  The kernels sum scale * (code - zero) * x with
+// x raised to below 2^15 and bring the sum down at the end: below it no sum of 2^20 columns of at most 16 passes
+// 2^88 * 2^39.
+constexpr uint16_t kInt4ScaleLimit = (127 + 88) << 7;
 constexpr int int4_unit_bytes(int group, int zeros) { return 1024 + kTile * (kInt4Unit / group) * (zeros ? 3 : 2); }
 
 // Host repack: source block bytes (format/layout as given) -> device image (Layout::total bytes).

@@ -251,7 +251,7 @@ class QuantizedWeight:
         4-bit checkpoints outside GGUF (no counterpart in the reference).
 
         codes: uint8 [out_features, in_features / 2], two to a byte with the even column in the
-        low half; scales: float16 or bfloat16 [out_features, in_features / group_size]; zeros:
+        low half; scales: float16 or bfloat16 [out_features, in_features / group_size], below 2^88; zeros:
         integers from 0 to 16 of the same shape, or None for 8 throughout; group_size 32, 64 or
         128, in_features at most 2^20.  The tensors are copied; with codes on a device the device lays them
         out (151936 x 4096 in 0.4 ms, from host arrays in 100)."""

@@ -203,6 +203,29 @@ def test_smallest_and_largest_scales(m):
 
 
 @pytest.mark.parametrize("m", [1, 6, 12, 40])
+def test_smallest_and_largest_bf16_scales(m):
+    """The smallest subnormal one, the smallest normal one and the largest that is taken, each the only ones of a
+    weight; and the smallest that is refused, from host and device arrays.  (x brings the results to where f32 is
+    normal.)"""
+    import nn_amd
+    q = torch.randint(0, 256, (50, 192), generator=torch.Generator().manual_seed(m), dtype=torch.int32).to(torch.uint8)
+    codes = torch.stack([q & 15, q >> 4], 2).view(50, 384).double().cuda() - 8
+    for value, size in ((2.0 ** -133, 2.0 ** 40), (2.0 ** -126, 2.0 ** 40), (255 * 2.0 ** 80, 1.0), (255 * 2.0 ** 80, 2.0 ** -30)):
+        s = torch.full((50, 6), value, dtype=BF16)
+        assert s[0, 0].double().item() == value
+        w = nn_amd.QuantizedWeight.from_int4_groups(q.cuda(), s, None, 64)
+        assert torch.equal(w.dequantize().double(), codes * value)
+        for xdt in (F32, BF16):
+            x = tokens(m, 384, xdt) * size
+            check(nn_amd.quantized_linear(x, w), x.double() @ (codes * value).t(), value)
+    for bad in (2.0 ** 88, -2.0 ** 110):
+        s[7, 3] = bad
+        for c in (q, q.cuda()):
+            with pytest.raises(nn_amd.Unsupported, match="scale 45 "):
+                nn_amd.QuantizedWeight.from_int4_groups(c, s, None, 64)
+
+
+@pytest.mark.parametrize("m", [1, 6, 12, 40])
 def test_activations_below_the_smallest_normal(m):
     """f32 x of multiples of 2^-140 (subnormal: nine bits are left), scales that bring the result back up."""
     import nn_amd

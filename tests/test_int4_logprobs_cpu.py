@@ -50,6 +50,18 @@ def test_int4_create_refusals(lib):
     assert create(lib, c, s, None, 1 << 40, 1 << 30, 128) == _lib.ERR_OUT_OF_MEMORY
 
 
+def test_int4_scales_out_of_range(lib):
+    """bf16 scales of 2^88 and more in magnitude; the largest below it passes (and the call goes on to the device)."""
+    c = np.zeros((4, 64), np.uint8)
+    for bits, refused in ((0x6B80, True), (0xEB80, True), (0x7F7F, True), (0xFF7F, True), (0x6B7F, False), (0xEB7F, False),
+                          (0x0001, False)):
+        s = np.array([0x3F80, 0x3F80, bits, 0x3F80], np.uint16)
+        assert (create(lib, c, s, None, 4, 128, 128, dtype=2) == _lib.ERR_UNSUPPORTED) == refused, hex(bits)
+        assert not refused or "scale 2 " in _lib.last_error()
+    s = np.array([0x7BFF, 0x7BFF, 0xFBFF, 0x7BFF], np.uint16)  # f16 65504: the same bits would be too large in bf16
+    assert create(lib, c, s, None, 4, 128, 128, dtype=1) != _lib.ERR_UNSUPPORTED
+
+
 def test_int4_device_create_refusals(lib):
     """What the device form refuses before it touches memory."""
     f, h = lib.nnq_weight_create_int4_device, ctypes.c_void_p()
