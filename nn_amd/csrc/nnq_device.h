@@ -57,7 +57,7 @@ __device__ __forceinline__ void f16_prescale(float amax, float &s, float &back) 
     s = __uint_as_float((uint32_t)(127 + se) << 23);
     back = __uint_as_float((uint32_t)(127 - se) << 23);
     if (amax == 0.0f) s = back = 1.0f;
-    if (!(amax <= 3.0e38f)) s = back = __uint_as_float(0x7FC00000u);
+    if (!(amax <= 3.402823466e38f)) s = back = __uint_as_float(0x7FC00000u);
 }
 
 // DPP quad permutations: the value of lane (l ^ 1) / (l ^ 2) within each group of 4.

@@ -323,7 +323,7 @@ namespace nnq {
 // Power of two s with amax * s in [2^14, 2^15) (1 for amax = 0, NaN for a non-finite
 // amax), exponent clamped to +-126: the device f16_prescale.
 static float prescale_pow2(float amax) {
-    if (!(amax <= 3.0e38f)) return std::nanf("");
+    if (!(amax <= 3.402823466e38f)) return std::nanf("");
     if (amax == 0.0f) return 1.0f;
     uint32_t u;
     std::memcpy(&u, &amax, 4);

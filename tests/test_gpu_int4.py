@@ -226,6 +226,27 @@ def test_smallest_and_largest_bf16_scales(m):
 
 
 @pytest.mark.parametrize("m", [1, 6, 12, 40])
+@pytest.mark.parametrize("xdt", [F32, BF16])
+def test_largest_finite_activations(m, xdt):
+    """Activations up to the type's largest value are numbers, not infinities: rows of 3.1e38 to 3.38e38 beside
+    ordinary ones, scales that keep the results in f32's range."""
+    import nn_amd
+    g = torch.Generator(device="cuda")
+    g.manual_seed(m)
+    q = torch.randint(0, 256, (50, 192), generator=g, device="cuda", dtype=torch.int32).to(torch.uint8)
+    codes = torch.stack([q & 15, q >> 4], 2).view(50, 384).double() - 8
+    w = nn_amd.QuantizedWeight.from_int4_groups(q, torch.full((50, 3), 2.0 ** -24, dtype=F16), None, 128)
+    x = tokens(m, 384, xdt)
+    big = 3.1e38 + 0.28e38 * torch.rand(384, generator=g, device="cuda")
+    x[0] = big.to(xdt) * torch.where(torch.rand(384, generator=g, device="cuda") < 0.5, -1.0, 1.0).to(xdt)
+    x[m // 2, 100] = torch.finfo(xdt).max
+    assert torch.isfinite(x).all()
+    y, ref = nn_amd.quantized_linear(x, w), x.double() @ (codes * 2.0 ** -24).t()
+    for t in range(m):
+        check(y[t], ref[t], t)
+
+
+@pytest.mark.parametrize("m", [1, 6, 12, 40])
 def test_activations_below_the_smallest_normal(m):
     """f32 x of multiples of 2^-140 (subnormal: nine bits are left), scales that bring the result back up."""
     import nn_amd
