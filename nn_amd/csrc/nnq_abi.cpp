@@ -12,6 +12,7 @@
 #include <mutex>
 #include <new>
 #include <string>
+#include <system_error>
 #include <thread>
 #include <vector>
 
@@ -293,13 +294,23 @@ void parallel_for(int64_t n, F &&fn) {
         fn(0, n);
         return;
     }
-    std::vector<std::thread> th;
-    int64_t per = (n + nt - 1) / nt;
-    for (int64_t t = 0; t < nt; t++) {
-        int64_t lo = t * per, hi = std::min(n, lo + per);
-        if (lo < hi) th.emplace_back([&fn, lo, hi] { fn(lo, hi); });
+    struct Joined {
+        std::vector<std::thread> th;
+        ~Joined() {
+            for (auto &x : th) x.join();
+        }
+    } t;
+    t.th.reserve((size_t)nt);
+    const int64_t per = (n + nt - 1) / nt;
+    int64_t lo = 0;
+    try {
+        for (; lo < n; lo += per) {
+            const int64_t hi = std::min(n, lo + per);
+            t.th.emplace_back([&fn, lo, hi] { fn(lo, hi); });
+        }
+    } catch (const std::system_error &) {
+        fn(lo, n);  // no more threads: what is left runs here
     }
-    for (auto &x : th) x.join();
 }
 
 }  // namespace
@@ -469,7 +480,7 @@ int nnq_weight_create_int4(const uint8_t *codes, const void *scales, nnq_dtype s
         host.resize(L.total());
         parallel_for(L.ntile, [&](int64_t lo, int64_t hi) { repack_int4(codes, sc, zeros, L, lo, hi, host.data()); });
         w = new nnq_weight;
-    } catch (const std::exception &ex) {  // no memory, no thread
+    } catch (const std::exception &ex) {  // no memory
         return fail(NNQ_ERR_OUT_OF_MEMORY, "weight repack: %s", ex.what());
     }
     w->L = L;

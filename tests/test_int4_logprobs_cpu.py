@@ -1,6 +1,9 @@
 """Refusals of the 4-bit group-scaled weights and of the log probabilities that need no GPU, the host
 repack of the 4-bit image against its description, and the plan of a log-probability call."""
 import ctypes
+import resource
+import subprocess
+import sys
 
 import numpy as np
 import pytest
@@ -60,6 +63,32 @@ def test_int4_scales_out_of_range(lib):
         assert not refused or "scale 2 " in _lib.last_error()
     s = np.array([0x7BFF, 0x7BFF, 0xFBFF, 0x7BFF], np.uint16)  # f16 65504: the same bits would be too large in bf16
     assert create(lib, c, s, None, 4, 128, 128, dtype=1) != _lib.ERR_UNSUPPORTED
+
+
+def test_int4_create_where_threads_cannot_start():
+    """The host repack starts a thread per CPU.  Where only the first few start (stacks of 4 GiB in an address
+    space that has room for two more), the call does the rest itself; a running thread must not be dropped,
+    which would end the process."""
+    child = '''
+import ctypes, resource, sys
+lib = ctypes.CDLL(sys.argv[1])
+n, k = 32768, 32
+codes, scales = (ctypes.c_uint8 * (n * k // 2))(), (ctypes.c_uint16 * n)(*[0x3C00] * n)
+i64, h = ctypes.c_int64, ctypes.c_void_p()
+used = int(open("/proc/self/statm").read().split()[0]) * resource.getpagesize()
+resource.setrlimit(resource.RLIMIT_AS, (used + (10 << 30),) * 2)
+rc = lib.nnq_weight_create_int4(codes, scales, 1, None, i64(n), i64(k), i64(32), ctypes.byref(h))
+print("returned", rc)
+'''
+
+    def limits():
+        resource.setrlimit(resource.RLIMIT_STACK, (4 << 30, resource.getrlimit(resource.RLIMIT_STACK)[1]))
+
+    r = subprocess.run([sys.executable, "-c", child, _lib.LIB_PATH], preexec_fn=limits, capture_output=True, text=True,
+                       timeout=60)
+    assert r.returncode == 0 and "returned" in r.stdout, (r.returncode, r.stderr[-500:])
+    # (the device's refusal where there is none, but not the repack's)
+    assert int(r.stdout.split()[-1]) != _lib.ERR_OUT_OF_MEMORY
 
 
 def test_int4_device_create_refusals(lib):
