@@ -501,6 +501,8 @@ def _logprob_outputs(batch, n, top_n, ranks, device):
 def _token_ids(tokens, batch, device):
     if not isinstance(tokens, torch.Tensor):
         tokens = torch.as_tensor(tokens)
+        if tokens.numel() == 0:
+            tokens = tokens.long()  # (an empty list has no type of its own)
     if tuple(tokens.shape) != tuple(batch):
         raise ShapeMismatch(f"tokens must be {list(batch)}, one per row of logits, got {list(tokens.shape)}")
     if tokens.is_floating_point() or tokens.is_complex() or tokens.dtype == torch.bool:

@@ -291,6 +291,14 @@ def test_views(dtype):
         nn_amd.token_logprobs(x, t[:-1])
 
 
+def test_no_rows():
+    import nn_amd
+    x, _ = draw(2, 5003, F32, seed=2)
+    for r in (nn_amd.token_logprobs(x[:0], [], top_n=4, ranks=True),
+              nn_amd.linear_logprobs(torch.zeros(0, 512, device="cuda"), head("int4", 5003, 512), [], top_n=4, ranks=True)):
+        assert r.logprobs.shape == r.entropy.shape == r.ranks.shape == (0,) and r.top_ids.shape == (0, 4)
+
+
 def test_more_rows_than_one_launch_takes():
     """70000 rows: two launches; and few long rows whose candidates pass one launch's scratch."""
     import nn_amd

@@ -303,6 +303,20 @@ def test_python_logprob_refusals():
         assert out.top_ids.shape == out.top_logprobs.shape == (*batch, 4)
 
 
+def test_no_tokens_from_a_list():
+    """An empty batch is nothing to do, also where its tokens come as a list; an empty float tensor is a mistake."""
+    from nn_amd.quantized import _token_ids
+    for tokens, batch in (([], (0,)), ((), (0,)), ([[], []], (2, 0)), (np.zeros((0,), np.int32), (0,))):
+        t = _token_ids(tokens, batch, torch.device("cpu"))
+        assert t.dtype is torch.int64 and tuple(t.shape) == batch
+    with pytest.raises(nn_amd.ShapeMismatch):
+        _token_ids([], (1,), torch.device("cpu"))
+    with pytest.raises(nn_amd.Unsupported):
+        _token_ids(torch.zeros(0), (0,), torch.device("cpu"))
+    with pytest.raises(nn_amd.Unsupported):
+        _token_ids([0.5], (1,), torch.device("cpu"))
+
+
 class Plan(ctypes.Structure):
     _fields_ = [("nseg", ctypes.c_int64), ("rows", ctypes.c_int64), ("slots", ctypes.c_int), ("bytes", ctypes.c_size_t)]
 
