@@ -116,14 +116,21 @@ class QuantType(enum.IntEnum):
     MXFP4 = 39
     INT4G = 1000  # 4-bit codes with group scales (QuantizedWeight.from_int4_groups); no GGUF type
 
+    def _blocks(self):
+        if self == QuantType.INT4G:
+            raise WrongQuantType("INT4G weights have no blocks: codes, scales and zero points are arrays of their own")
+
     def block_size(self) -> int:
+        self._blocks()
         return 32 if self in (QuantType.Q8_0, QuantType.MXFP4) else 256
 
     def block_bytes(self) -> int:
+        self._blocks()
         return {QuantType.Q8_0: 34, QuantType.Q4_K: 144, QuantType.Q6_K: 210, QuantType.MXFP4: 17}[self]
 
     def expected_bytes(self, num_elements: int) -> Optional[int]:
         """QuantType::expected_bytes (quantized.rs:79-89)."""
+        self._blocks()
         if num_elements == 0:
             return 0
         if num_elements % self.block_size():

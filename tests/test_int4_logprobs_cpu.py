@@ -138,6 +138,16 @@ def test_from_int4_groups_refusals():
         nn_amd.QuantizedWeight.from_quantized(np.zeros(64, np.uint8), nn_amd.QuantType.INT4G, (1, 128))
 
 
+def test_int4g_has_no_blocks():
+    q = nn_amd.QuantType.INT4G
+    for call in (q.block_size, q.block_bytes, lambda: q.expected_bytes(256), lambda: q.expected_bytes(0),
+                 lambda: q.expected_bytes(100)):
+        with pytest.raises(nn_amd.WrongQuantType):
+            call()
+    assert [t.block_size() for t in nn_amd.QuantType if t != q] == [32, 256, 256, 32]
+    assert [t.expected_bytes(512) for t in nn_amd.QuantType if t != q] == [544, 288, 420, 272]
+
+
 class GemmPlan(ctypes.Structure):
     _fields_ = [(f, ctypes.c_int) for f in ("mt", "nt", "ks", "row_blocks", "col_blocks")] + \
                [(f, ctypes.c_size_t) for f in ("plane", "rowback", "slabs", "bytes")]
