@@ -399,6 +399,32 @@ def test_linear_logprobs_in_chunks():
         near(r.top_logprobs[i:i + 1], ref["top_logprobs"], 1e-5 + tol, 2 ** -23)
 
 
+def test_every_output_of_several_chunks():
+    """Rows in three chunks, the logits asked for or kept in the workspace: each of the five outputs is, bit for
+    bit, what token_logprobs gives for those logits in one call, and the definition's in rows of every chunk."""
+    import nn_amd
+    n, k, m = 1200001, 128, 150
+    w = head("int4", n, k)
+    g = torch.Generator(device="cuda")
+    g.manual_seed(4)
+    x = torch.randn(m, k, generator=g, device="cuda")
+    t = torch.randint(0, n, (m,), generator=g, device="cuda")
+    bias = torch.randn(n, generator=g, device="cuda")
+    kept = nn_amd.linear_logprobs(x, w, t, bias, top_n=3, ranks=True, return_logits=True)
+    inner = nn_amd.linear_logprobs(x, w, t, bias, top_n=3, ranks=True)
+    whole = nn_amd.token_logprobs(kept.logits, t, top_n=3, ranks=True)
+    assert kept.logits.shape == (m, n) and inner.logits is None
+    for name, a, b, c in zip(whole._fields, whole[:5], kept[:5], inner[:5]):
+        assert torch.equal(a, b) and torch.equal(a, c), name
+    rows = torch.tensor([0, 63, 64, 127, 128, 149], device="cuda")
+    some = type(kept)(*(v[rows] for v in kept[:5]))
+    check(some, plain(kept.logits[rows], t[rows], 3), 3)
+    # (the logits are the linear's: one row takes another kernel than many, sums in another order)
+    for i in (0, 64, 149):
+        y = nn_amd.quantized_linear(x[i:i + 1], w, bias)
+        assert (y[0] - kept.logits[i]).abs().max() <= 2e-5 * y.abs().max()
+
+
 def test_scoring_loop_as_a_server_runs_it():
     """A prompt scored, then tokens sampled one at a time with their log probabilities, nothing returning to the
     host in between; the last step captured in a graph and replayed."""
