@@ -14,7 +14,6 @@ no CPU fallback: without the library or a GPU these functions raise.
 """
 from __future__ import annotations
 
-import contextlib
 import ctypes
 import enum
 from typing import NamedTuple, Optional, Sequence
@@ -176,6 +175,22 @@ def _stream(t: torch.Tensor):
     return _raw_stream(t.device.index)
 
 
+_current_device = getattr(torch._C, "_cuda_getDevice", torch.cuda.current_device)
+
+
+def _launch(t: torch.Tensor, fn, *args):
+    """``fn(*args, stream)`` on the current stream of the device of `t`, with that device current: the raw handle
+    of a default stream is 0, which means the current device's."""
+    index = t.device.index
+    if index == _current_device():
+        rc = fn(*args, _stream(t) if _raw_stream is None else _raw_stream(index))
+    else:
+        with torch.cuda.device(index):
+            rc = fn(*args, _stream(t))
+    if rc != _lib.OK:
+        _check(rc)
+
+
 def _ptr(t: Optional[torch.Tensor]):
     return t.data_ptr() if t is not None else None
 
@@ -324,7 +339,7 @@ class QuantizedWeight:
     def dequantize(self) -> torch.Tensor:
         """Bit-exact f32 decode on the device (QuantizedStorage::dequantize)."""
         out = torch.empty(self.shape, dtype=torch.float32, device=f"cuda:{self.device}")
-        _check(_lib.load().nnq_dequant(self._h, _ptr(out), _stream(out)))
+        _launch(out, _lib.load().nnq_dequant, self._h, _ptr(out))
         return out
 
 
@@ -359,8 +374,8 @@ def quantized_linear(input: torch.Tensor, weight: QuantizedWeight, bias: Optiona
     out_dtype = out_dtype or torch.float32
     y = x.new_empty((*x.shape[:-1], n), dtype=out_dtype)
     m = x.numel() // k
-    _check(_lib.load().nnq_linear(weight.handle, _ptr(x), _DTYPE[x.dtype], m, k, _ptr(bias),
-                                  n if bias is not None else 0, _ptr(y), _DTYPE[out_dtype], _stream(x)))
+    _launch(x, _lib.load().nnq_linear, weight.handle, _ptr(x), _DTYPE[x.dtype], m, k, _ptr(bias),
+            n if bias is not None else 0, _ptr(y), _DTYPE[out_dtype])
     return y
 
 
@@ -391,7 +406,7 @@ def argmax(logits: torch.Tensor) -> torch.Tensor:
     v = _device_input(logits, "logits").float().contiguous()
     idx = torch.empty(1, dtype=torch.int32, device=v.device)
     st = torch.empty(1, dtype=torch.int32, device=v.device)  # written by the call
-    _check(_lib.load().nnq_argmax_f32(_ptr(v), v.numel(), _ptr(idx), _ptr(st), _stream(v)))
+    _launch(v, _lib.load().nnq_argmax_f32, _ptr(v), v.numel(), _ptr(idx), _ptr(st))
     if int(st.item()) != 0:
         raise NonFiniteData("argmax/argmin input contains NaN")
     return idx.view(torch.int32)[0].to(torch.int64)
@@ -411,8 +426,8 @@ def linear_argmax(x: torch.Tensor, weight: QuantizedWeight, bias: Optional[torch
     logits = xv.new_empty(n)
     idx = xv.new_empty((), dtype=torch.int64)
     st = xv.new_empty(1, dtype=torch.int32) if check else None  # written by the call
-    _check(_lib.load().nnq_linear_argmax_i64(weight.handle, _ptr(xv), k, _ptr(bias), n if bias is not None else 0,
-                                             _ptr(logits), _ptr(idx), _ptr(st), _stream(xv)))
+    _launch(xv, _lib.load().nnq_linear_argmax_i64, weight.handle, _ptr(xv), k, _ptr(bias),
+            n if bias is not None else 0, _ptr(logits), _ptr(idx), _ptr(st))
     if check and int(st.item()) != 0:
         raise NonFiniteData("argmax input contains NaN")
     return logits, idx
@@ -450,8 +465,7 @@ def sample_token(logits: torch.Tensor, temperature: float = 0.7, top_k: Optional
     past, n_past = _past(past_tokens, v.device)
     tok = torch.empty(1, dtype=torch.int32, device=v.device)
     cfg = _sampling(temperature, top_k, top_p, repetition_penalty, frequency_penalty, seed)
-    _check(_lib.load().nnq_sample_token(_ptr(v), v.numel(), _ptr(past), n_past, ctypes.byref(cfg), _ptr(tok),
-                                        _stream(v)))
+    _launch(v, _lib.load().nnq_sample_token, _ptr(v), v.numel(), _ptr(past), n_past, ctypes.byref(cfg), _ptr(tok))
     return tok.view(torch.int32)[0].to(torch.int64)
 
 
@@ -471,8 +485,8 @@ def linear_sample(x: torch.Tensor, weight: QuantizedWeight, bias: Optional[torch
     past, n_past = _past(past_tokens, xv.device)
     tok = torch.empty(1, dtype=torch.int32, device=xv.device)
     cfg = _sampling(temperature, top_k, top_p, repetition_penalty, frequency_penalty, seed)
-    _check(_lib.load().nnq_linear_sample(weight.handle, _ptr(xv), k, _ptr(bias), n if bias is not None else 0,
-                                         _ptr(logits), _ptr(past), n_past, ctypes.byref(cfg), _ptr(tok), _stream(xv)))
+    _launch(xv, _lib.load().nnq_linear_sample, weight.handle, _ptr(xv), k, _ptr(bias), n if bias is not None else 0,
+            _ptr(logits), _ptr(past), n_past, ctypes.byref(cfg), _ptr(tok))
     return logits, tok.view(torch.int32)[0].to(torch.int64)
 
 
@@ -519,11 +533,6 @@ def _token_ids(tokens, batch, device):
     return tokens.to(device=device, dtype=torch.int64).contiguous()
 
 
-def _on_device(t: torch.Tensor):
-    """Make the device of `t` current for a launch (nothing to do on the current one)."""
-    return contextlib.nullcontext() if t.device.index == torch.cuda.current_device() else torch.cuda.device(t.device)
-
-
 def token_logprobs(logits: torch.Tensor, tokens, top_n: int = 0, ranks: bool = False) -> TokenLogprobs:
     """For each row of device logits [..., n] (f32, bf16 or f16; rows may be strided) and its token:
     the token's log probability, the entropy of the distribution, with ``ranks`` the token's place
@@ -545,9 +554,8 @@ def token_logprobs(logits: torch.Tensor, tokens, top_n: int = 0, ranks: bool = F
     rows = tok.numel()
     stride = v.stride(0) if v.dim() == 2 else n
     ptrs, out = _logprob_outputs(batch, n, top_n, ranks, v.device)
-    with _on_device(v):
-        _check(_lib.load().nnq_token_logprobs(_ptr(v), _DTYPE[v.dtype], rows, n, stride, _ptr(tok), int(top_n), *ptrs,
-                                              _stream(v)))
+    _launch(v, _lib.load().nnq_token_logprobs, _ptr(v), _DTYPE[v.dtype], rows, n, stride, _ptr(tok), int(top_n),
+            *ptrs)
     return out
 
 
@@ -569,10 +577,8 @@ def linear_logprobs(x: torch.Tensor, weight: QuantizedWeight, tokens, bias: Opti
     rows = tok.numel()
     ptrs, out = _logprob_outputs(batch, n, top_n, ranks, xv.device)
     logits = xv.new_empty((*batch, n), dtype=torch.float32) if return_logits else None
-    with _on_device(xv):
-        _check(_lib.load().nnq_linear_logprobs(weight.handle, _ptr(xv), _DTYPE[xv.dtype], rows, k, _ptr(bias),
-                                               n if bias is not None else 0, _ptr(tok), int(top_n), _ptr(logits),
-                                               *ptrs, _stream(xv)))
+    _launch(xv, _lib.load().nnq_linear_logprobs, weight.handle, _ptr(xv), _DTYPE[xv.dtype], rows, k, _ptr(bias),
+            n if bias is not None else 0, _ptr(tok), int(top_n), _ptr(logits), *ptrs)
     return out._replace(logits=logits)
 
 
@@ -625,8 +631,8 @@ class QuantizedMLP:
         od = out_dtype if out_dtype is not None else torch.float32
         y = xx.new_empty((m, self.hidden), dtype=od)
         st = xx.new_empty(1, dtype=torch.int32) if check else None  # written by the call (m > 0)
-        _check(_lib.load().nnq_mlp_forward(self._h, _ptr(xx), _DTYPE[xx.dtype], m, self.hidden, _ptr(y), _DTYPE[od],
-                                           _ptr(st), _stream(xx)))
+        _launch(xx, _lib.load().nnq_mlp_forward, self._h, _ptr(xx), _DTYPE[xx.dtype], m, self.hidden, _ptr(y),
+                _DTYPE[od], _ptr(st))
         if check and m > 0 and int(st.item()) != 0:
             raise NonFiniteData("Qwen3MLP output contains NaN or Inf")
         return y.reshape(*x.shape[:-1], self.hidden)
@@ -733,8 +739,7 @@ class QuantizedMoE:
             raise Unsupported("this MoE was created without a router")
         xx = self._input(x)
         lg = torch.empty((xx.shape[0], self.num_experts), dtype=torch.float32, device=xx.device)
-        _check(_lib.load().nnq_router_logits(self._router, _ptr(xx), _DTYPE[xx.dtype], xx.shape[0], _ptr(lg),
-                                             _stream(xx)))
+        _launch(xx, _lib.load().nnq_router_logits, self._router, _ptr(xx), _DTYPE[xx.dtype], xx.shape[0], _ptr(lg))
         return lg
 
     def block_forward(self, x: torch.Tensor, top_k: int = 4, swiglu_limit: float = 7.0,
@@ -752,9 +757,8 @@ class QuantizedMoE:
         ti = xx.new_empty((T, top_k), dtype=torch.int32) if return_routing else None
         tw = xx.new_empty((T, top_k), dtype=torch.float32) if return_routing else None
         st = xx.new_empty(1, dtype=torch.int32) if check else None  # written by the call (T > 0)
-        _check(_lib.load().nnq_moe_block_forward(self._h, self._router, _ptr(xx), _DTYPE[xx.dtype], T, int(top_k),
-                                                 float(swiglu_limit), _ptr(y), _ptr(ti), _ptr(tw), _ptr(st),
-                                                 _stream(xx)))
+        _launch(xx, _lib.load().nnq_moe_block_forward, self._h, self._router, _ptr(xx), _DTYPE[xx.dtype], T,
+                int(top_k), float(swiglu_limit), _ptr(y), _ptr(ti), _ptr(tw), _ptr(st))
         if check and T > 0 and int(st.item()) != 0:
             raise NonFiniteData("QuantizedMoeBlock output contains NaN or Inf")
         if return_routing:
@@ -774,8 +778,8 @@ class QuantizedMoE:
         y = xx.new_empty((T, self.hidden), dtype=torch.float32)
         ti = xx.new_empty((T, top_k), dtype=torch.int32) if return_routing else None
         tw = xx.new_empty((T, top_k), dtype=torch.float32) if return_routing else None
-        _check(_lib.load().nnq_moe_forward(self._h, _ptr(xx), _DTYPE[xx.dtype], T, _ptr(lg), int(top_k),
-                                           float(swiglu_limit), _ptr(y), _ptr(ti), _ptr(tw), _stream(xx)))
+        _launch(xx, _lib.load().nnq_moe_forward, self._h, _ptr(xx), _DTYPE[xx.dtype], T, _ptr(lg), int(top_k),
+                float(swiglu_limit), _ptr(y), _ptr(ti), _ptr(tw))
         if return_routing:
             return y, ti, tw
         return y
@@ -785,7 +789,7 @@ class QuantizedMoE:
     def dequant_expert(self, e: int):
         gu = torch.empty((self.hidden, 2 * self.inter), dtype=torch.float32, device=f"cuda:{self.device}")
         dn = torch.empty((self.inter, self.hidden), dtype=torch.float32, device=f"cuda:{self.device}")
-        _check(_lib.load().nnq_moe_dequant_expert(self._h, int(e), _ptr(gu), _ptr(dn), _stream(gu)))
+        _launch(gu, _lib.load().nnq_moe_dequant_expert, self._h, int(e), _ptr(gu), _ptr(dn))
         return gu, dn
 
 
@@ -855,7 +859,7 @@ def dequantize_mxfp4_ocp(blocks, n: int, device: int = 0) -> torch.Tensor:
     if b.numel() < ((int(n) + 31) // 32) * 17:
         raise DataLengthMismatch(f"{b.numel()} bytes hold fewer than {n} values")
     out = torch.empty(int(n), dtype=torch.float32, device=b.device)
-    _check(_lib.load().nnq_dequant_mxfp4_ocp(_ptr(b), int(n), _ptr(out), _stream(out)))
+    _launch(out, _lib.load().nnq_dequant_mxfp4_ocp, _ptr(b), int(n), _ptr(out))
     return out
 
 

@@ -327,6 +327,56 @@ def test_no_tokens_from_a_list():
         _token_ids([0.5], (1,), torch.device("cpu"))
 
 
+class OnOther(torch.Tensor):
+    """A host tensor that says it is on the second device."""
+    is_cuda = property(lambda self: True)
+    device = property(lambda self: torch.device("cuda", 1))
+
+
+def test_launches_are_made_on_the_device_of_their_tensors(monkeypatch):
+    """The raw handle of a default stream is 0 and means the current device's: every call that takes a 4-bit weight
+    or its logits makes its tensors' device current for the launch, and puts the caller's back."""
+    from nn_amd import quantized
+    now, calls = [0], []
+
+    class Switch:
+        def __init__(self, device):
+            self.to = torch.device(device).index
+
+        def __enter__(self):
+            self.back, now[0] = now[0], self.to
+
+        def __exit__(self, *exc):
+            now[0] = self.back
+
+    class Lib:
+        def __getattr__(self, name):
+            return lambda *args: calls.append((name, now[0])) or 0
+
+    empty = torch.empty
+    monkeypatch.setattr(quantized._lib, "load", lambda: Lib())
+    monkeypatch.setattr(quantized, "_current_device", lambda: now[0], raising=False)
+    monkeypatch.setattr(torch.cuda, "current_device", lambda: now[0])
+    monkeypatch.setattr(quantized, "_raw_stream", lambda index: 0)
+    monkeypatch.setattr(torch.cuda, "device", Switch)
+    monkeypatch.setattr(torch, "empty", lambda *a, device=None, **kw: empty(*a, **kw).as_subclass(OnOther))
+    w = nn_amd.QuantizedWeight(ctypes.c_void_p(), nn_amd.QuantType.INT4G, nn_amd.Layout.GROUPS, (16, 256), 1)
+    x = torch.zeros(2, 256).as_subclass(OnOther)
+    logits, t = torch.zeros(16).as_subclass(OnOther), torch.zeros(2, dtype=torch.int64).as_subclass(OnOther)
+    for call, name in ((lambda: nn_amd.quantized_linear(x, w), "nnq_linear"),
+                       (lambda: nn_amd.linear_argmax(x[0], w, check=False), "nnq_linear_argmax_i64"),
+                       (lambda: nn_amd.linear_sample(x[0], w), "nnq_linear_sample"),
+                       (lambda: nn_amd.sample_token(logits), "nnq_sample_token"),
+                       (lambda: nn_amd.token_logprobs(x, t, top_n=2), "nnq_token_logprobs"),
+                       (lambda: nn_amd.linear_logprobs(x, w, t), "nnq_linear_logprobs"),
+                       (w.dequantize, "nnq_dequant")):
+        for current in (0, 1):
+            calls.clear()
+            now[0] = current
+            call()
+            assert calls == [(name, 1)] and now[0] == current
+
+
 class Plan(ctypes.Structure):
     _fields_ = [("nseg", ctypes.c_int64), ("rows", ctypes.c_int64), ("slots", ctypes.c_int), ("bytes", ctypes.c_size_t)]
 
