@@ -9,8 +9,8 @@
 // has its d's rounding, 2^-24 |d|, and 2^-22, and the sums theirs.  (Down to d = -87; below, e^d is taken
 // for 0.)
 //
-// Bound: one read of the logits (HBM, or the cache that a GEMM left them in), with some twelve VALU
-// instructions and an exponential per logit beside it, twenty with rank and alternatives.  Two
+// Bound: one read of the logits (HBM, or the cache that a GEMM left them in), with some fifteen VALU
+// instructions and an exponential per logit beside it, twenty-three with rank and alternatives.  Two
 // launches:
 //   logprob_seg_kernel   one wave per 2048 logits of a row, all of them in registers: the segment's
 //                        maximum, then (count of the maximum, R, S) against it, how many logits
@@ -22,10 +22,10 @@
 // the 2048 reach it (N = 20).  Of more than there are slots the largest are kept; of more than 64 (many
 // equal logits, or a row's largest in few lanes) the exact N-th value, and among its equals the lowest
 // indices, are found the same way over all 2048.
-// Measured (MI355X, f32 logits of 151936): 512 rows 51.5 + 4.7 us (6.0 TB/s, the streaming read's rate
-// is 7.0); 301 rows with rank and 5 alternatives 35.5 + 4.7 us (5.2 TB/s; the VALU is busy 80% of it);
-// one row with 20 alternatives 6.0 + 5.4 us, both latency, and 19 us from Python (five tensors and two
-// launches).  48 bf16 rows of 50257 7.4 + 4.6 us.
+// Measured (MI355X, f32 logits of 151936): 512 rows 53.5 + 5.0 us (5.8 TB/s, the streaming read's rate
+// is 7.0); 301 rows with rank and 5 alternatives 36.4 + 4.7 us (5.0 TB/s; the VALU is busy 90% of it);
+// one row with 20 alternatives 6.2 + 5.1 us, both latency, and 19 us from Python (five tensors and two
+// launches).  48 bf16 rows of 50257 7.8 + 4.8 us.
 #include <algorithm>
 
 #include "nnq_device.h"
@@ -137,7 +137,7 @@ __device__ __forceinline__ uint32_t sum64u(uint32_t v) {
 // 2^p alone, with p = d log2(e) rounded, would be off by up to 2^-18 at d = -80: half a step of p, and the
 // constant's own rounding, which moves every term the same way.  The factor that is missing is e^(d - p log(2)),
 // 1 + a number below 2^-17; three FMAs beside the product and the exponential (301 rows with rank and
-// alternatives: 41.1 -> 41.4 us the whole call, 512 without 55.4 -> 55.8).
+// alternatives: 41.3 -> 41.5 us the whole call, 512 without 55.5 -> 56.5).
 __device__ __forceinline__ float exp_of(float d) {
     const float p = d * 1.44269504088896340736f, e = __builtin_amdgcn_exp2f(p);
     // log(2) in two parts: 0x1.62e43p-1 and what is left of it
@@ -194,14 +194,14 @@ __global__ __launch_bounds__(kSegWaves * 64) void logprob_seg_kernel(LpArgs a) {
     const float mx = max64(lm);
     const float ref = mx == kNegInf ? 0.f : mx;
     float r = 0.f, s = 0.f;
-    int cnt = 0;
+    int cnt = kSeg;
 #pragma unroll
     for (int e = 0; e < kPer; e++) {
         const float d = __builtin_elementwise_maximum(x[e] - ref, -1e30f);  // (-inf: its e^d is 0; NaN stays)
         const float ex = exp_of(d);
-        const bool top = d == 0.f;
-        cnt += __popcll(__ballot(top));
-        r += top ? 0.f : ex;
+        const bool below = d != 0.f;  // (or NaN)
+        cnt -= __popcll(__ballot(below));
+        r += below ? ex : 0.f;
         s = fmaf(d, ex, s);
     }
     r = sum64(r);
