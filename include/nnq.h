@@ -154,8 +154,9 @@ int nnq_weight_create(nnq_format fmt, nnq_layout layout, const uint8_t *bytes, s
  * point over 16 is NNQ_ERR_INVALID_ARGUMENT, a scale that is not finite NNQ_ERR_NON_FINITE, one of 2^88 and
  * more in magnitude NNQ_ERR_UNSUPPORTED (the sums' range would not hold it).  Columns are in
  * order (an activation-ordered checkpoint is sorted, and its input permuted, by the caller).
- * The weight works in every call that takes an nnq_weight.  No counterpart in the
- * reference, whose 4-bit weights are Q4_K blocks. */
+ * The weight works in every call that takes an nnq_weight.  In a linear over it a row of x
+ * that holds NaN or an infinity gives a row of NaN, other rows are not touched.  No
+ * counterpart in the reference, whose 4-bit weights are Q4_K blocks. */
 int nnq_weight_create_int4(const uint8_t *codes, const void *scales, nnq_dtype scale_dtype, const uint8_t *zeros,
                            int64_t n, int64_t k, int64_t group, nnq_weight **out);
 
@@ -270,7 +271,7 @@ int nnq_linear_sample_noalloc(const nnq_weight *w, const float *x, int64_t k, co
  * A logit of -inf (a masked token) has probability 0 and is never among the alternatives;
  * places that no token fills get id -1 and log probability -inf.  A row that holds NaN or
  * +inf, or nothing above -inf, has NaN for every log probability and the entropy, as
- * log_softmax gives.  A token outside [0, n) (padding) has log probability NaN; where that
+ * log_softmax gives (its ids mean nothing).  A token outside [0, n) (padding) has log probability NaN; where that
  * is NaN the rank is -1.  Rows may overlap or repeat (row_stride 0).  m = 0 is a no-op.
  * Stands beside nnq_sample_token; no counterpart in the reference, which returns tokens
  * only. */
@@ -280,7 +281,8 @@ int nnq_token_logprobs(const void *logits, nnq_dtype dtype, int64_t m, int64_t n
 
 /* nnq_token_logprobs of logits = x[m, k] @ W^T (+ bias), the linear as nnq_linear with f32
  * output: the scoring of a prompt through the LM head, for any weight.  logits (f32 [m, n],
- * contiguous) may be NULL: then only chunks of rows exist, in the workspace (up to 320 MiB). */
+ * contiguous) may be NULL: then only chunks of rows exist, in the workspace (up to 320 MiB, or
+ * 16 rows where those are more). */
 int nnq_linear_logprobs(const nnq_weight *w, const void *x, nnq_dtype x_dtype, int64_t m, int64_t k, const float *bias,
                         int64_t bias_len, const int64_t *tokens, int top_n, float *logits, float *logprobs,
                         float *entropy, int64_t *ranks, float *top_logprobs, int64_t *top_ids, void *stream);

@@ -20,10 +20,11 @@
 //    one per addition).  The waves' sums meet in LDS, one barrier per block of tiles.
 //  * Five rows and more of a long K split it over workgroups (int4_rows_split), and from some size on
 //    the GEMM's two launches are shorter (int4_takes_rows).
-// Measured (MI355X, on the device): 1 x 4096 -> 4096 5.2 us (8.7 MB), -> 24576 11.0 us (4.8 TB/s), ->
-// 151936 52 us (6.2 TB/s, the streaming read's rate is 7.0); 5 f32 rows of 2880 -> 5751 9.3 us; 12 bf16
-// rows of 12288 -> 4096 16.3 us with the sum: reading and converting x in every workgroup (25 MB from
-// L2) before its first tile, and the second launch.
+// Measured (MI355X, in a graph, over copies of the weight that together pass the 256 MB Infinity Cache; in
+// parentheses one weight again and again): 1 x 4096 -> 4096 5.6 us (5.5; 8.7 MB, an empty launch is 1.8), ->
+// 24576 12.5 us (11.1), 4.2 TB/s, -> 151936 52 us (326 MB, 6.2 TB/s; the streaming read's rate is 7.0); 5
+// f32 rows of 2880 -> 5751 9.6 us (9.2); 12 bf16 rows of 12288 -> 4096 16.5 us (16.1) with the sum: reading
+// and converting x in every workgroup (25 MB from L2) before its first tile, and the second launch.
 #include <algorithm>
 #include <type_traits>
 

@@ -275,7 +275,9 @@ class QuantizedWeight:
         codes: uint8 [out_features, in_features / 2], two to a byte with the even column in the
         low half; scales: float16 or bfloat16 [out_features, in_features / group_size], below 2^88; zeros:
         integers from 0 to 16 of the same shape, or None for 8 throughout; group_size 32, 64 or
-        128, in_features at most 2^20.  The tensors are copied; with codes on a device the device lays them
+        128, in_features at most 2^20.  Checkpoints that hold codes packed otherwise (several rows or columns
+        to a 32-bit word) are unpacked to this order by the caller.  The tensors are copied; with codes on a
+        device the device lays them
         out (151936 x 4096 in 0.4 ms, from host arrays in 100)."""
         for t, what in ((codes, "codes"), (scales, "scales")):
             if not isinstance(t, torch.Tensor):
@@ -509,7 +511,8 @@ def _logprob_outputs(batch, n, top_n, ranks, device):
     if not 0 <= int(top_n) <= min(32, n):
         raise InvalidShape(f"top_n {top_n} out of range (0 to 32, at most the {n} logits)")
     top, rk, tl, ti = int(top_n), None, None, None
-    # (a small call is bound by its host side, at 1 to 2 us a tensor: whole allocations, no views)
+    # (a small call is bound by its host side, at 1 to 2 us a tensor: log probabilities and entropies are the two
+    # halves of one allocation, the rest whole ones without views)
     lp, ent = torch.empty((2, *batch), dtype=torch.float32, device=device).unbind(0)
     if ranks:
         rk = torch.empty(batch, dtype=torch.int64, device=device)
