@@ -83,13 +83,16 @@ typedef enum nnq_format {
  *  NNQ_LAYOUT_OCP     nn-core Mxfp4Block (crates/nn-core/src/layers/quantized/mxfp4.rs:70-84,177-244):
  *                     17-byte blocks [shared_exp][16 packed] along the flattened order, the LOW nibble =
  *                     even element, scale 2^(shared_exp - 127) with byte 0 -> 2^-127.
- *  NNQ_LAYOUT_GROUPS  NNQ_FMT_INT4G: codes, scales and zero points in arrays of their own. */
+ *  NNQ_LAYOUT_GROUPS  NNQ_FMT_INT4G: codes, scales and zero points in arrays of their own.
+ *  NNQ_LAYOUT_ROWS    NNQ_FMT_MXFP4 linear weights: codes and scales of W[n, k] in arrays of their own,
+ *                     blocks of 32 along k. */
 typedef enum nnq_layout {
     NNQ_LAYOUT_GGUF = 0,
     NNQ_LAYOUT_NN_GGUF = 1,
     NNQ_LAYOUT_GPTOSS = 2,
     NNQ_LAYOUT_OCP = 3,
-    NNQ_LAYOUT_GROUPS = 4
+    NNQ_LAYOUT_GROUPS = 4,
+    NNQ_LAYOUT_ROWS = 5
 } nnq_layout;
 
 typedef enum nnq_dtype {
@@ -167,6 +170,21 @@ int nnq_weight_create_int4(const uint8_t *codes, const void *scales, nnq_dtype s
 int nnq_weight_create_int4_device(const uint8_t *codes, const void *scales, nnq_dtype scale_dtype, const uint8_t *zeros,
                                   int64_t n, int64_t k, int64_t group, nnq_weight **out, void *stream);
 
+/* Upload W[n, k] in MXFP4 with blocks of 32 along k:
+ *   W[r][j] = e2m1(code[r][j]) * 2^(scale[r][j / 32] - 127),
+ * e2m1 the values 0, 0.5, 1, 1.5, 2, 3, 4, 6 (codes 0 to 7) and their negatives (8 to 15).  Host arrays, row-major:
+ * codes [n, k / 2], two to a byte with the even column in the low half; scales [n, k / 32], the biased exponents.  k is
+ * a multiple of 32 (NNQ_ERR_INVALID_SHAPE), at most 2^20 (NNQ_ERR_UNSUPPORTED); a scale byte over 252, whose values
+ * would not all be finite, is NNQ_ERR_NON_FINITE.  The weight works in every call that takes an nnq_weight, x as it is
+ * there: bf16 x in bf16 products, f32 x as three bf16 parts that sum to it.  A row of f32 x that holds an infinity
+ * gives a row of NaN.  Stands beside the MXFP4 experts (nnq_moe_create), whose blocks run along the output. */
+int nnq_weight_create_mxfp4(const uint8_t *codes, const uint8_t *scales, int64_t n, int64_t k, nnq_weight **out);
+
+/* nnq_weight_create_mxfp4 of arrays in the current device's memory, read in order on `stream` and laid out by the
+ * device.  Returns when the weight is there (it synchronizes the stream; not for a stream that is being captured). */
+int nnq_weight_create_mxfp4_device(const uint8_t *codes, const uint8_t *scales, int64_t n, int64_t k, nnq_weight **out,
+                                   void *stream);
+
 int nnq_weight_destroy(nnq_weight *w);
 
 /* Shape / format queries (QuantizedStorage::shape / quant_type, quantized.rs:142-152). */
@@ -192,6 +210,39 @@ int nnq_dequant(const nnq_weight *w, float *out, void *stream);
  * and QLinear::forward (crates/nn-core/src/layers/quantized/linear.rs:366-400). */
 int nnq_linear(const nnq_weight *w, const void *x, nnq_dtype x_dtype, int64_t m, int64_t k, const float *bias,
                int64_t bias_len, void *y, nnq_dtype y_dtype, void *stream);
+
+/* ---- MXFP4 rows: quantization and products of 4-bit operands ----------------------- */
+
+/* How a block of 32 values gets its scale 2^s (s from -127 to 125), m its largest magnitude:
+ *  NNQ_MX_CEIL   the smallest with m <= 6 * 2^s (as nnq_quantize_mxfp4_ocp);
+ *  NNQ_MX_FLOOR  2^(floor(log2 m) - 2): up to 8 * 2^s, and what is over 6 * 2^s becomes that.
+ * A block of zeros has s = -127. */
+typedef enum nnq_mx_rule {
+    NNQ_MX_CEIL = 0,
+    NNQ_MX_FLOOR = 1
+} nnq_mx_rule;
+
+/* Quantize rows of x (row r at element r * row_stride, k values, a multiple of 32; NNQ_F32 or NNQ_BF16) on the device:
+ * codes [rows, k / 2] (4-byte aligned) and scales [rows, k / 32] as nnq_weight_create_mxfp4 reads them.  Each value goes
+ * to the nearest code, halves to the even one (nnq_quantize_mxfp4_ocp: to the smaller magnitude), magnitudes beyond
+ * 6 * 2^125 to that.  A block that holds NaN or an infinity has scale byte 255 (NaN) and codes 0.  rows = 0 is a no-op. */
+int nnq_mxfp4_quantize(const void *x, nnq_dtype x_dtype, int64_t rows, int64_t k, int64_t row_stride, nnq_mx_rule rule,
+                       uint8_t *codes, uint8_t *scales, void *stream);
+
+/* The values that rows of codes and scales stand for: out [rows, k], 16-byte aligned, NNQ_F32 or NNQ_BF16 (exact in both).
+ * A block with scale byte 255 is NaN. */
+int nnq_mxfp4_dequantize(const uint8_t *codes, const uint8_t *scales, int64_t rows, int64_t k, void *out,
+                         nnq_dtype out_dtype, void *stream);
+
+/* y[m, n] = q(x)[m, k] @ W^T (+ bias[n]) for an NNQ_FMT_MXFP4 weight, q the quantization above: products of 4-bit
+ * operands, f32 sums.  Arguments and errors as nnq_linear; another weight is NNQ_ERR_WRONG_FORMAT.  A row of x that
+ * holds NaN or an infinity gives a row of NaN. */
+int nnq_mxfp4_linear(const nnq_weight *w, const void *x, nnq_dtype x_dtype, int64_t m, int64_t k, nnq_mx_rule rule,
+                     const float *bias, int64_t bias_len, void *y, nnq_dtype y_dtype, void *stream);
+
+/* The same with x quantized already: codes [m, k / 2] (16-byte aligned) and scales [m, k / 32] on the device. */
+int nnq_mxfp4_linear_codes(const nnq_weight *w, const uint8_t *codes, const uint8_t *scales, int64_t m, int64_t k,
+                           const float *bias, int64_t bias_len, void *y, nnq_dtype y_dtype, void *stream);
 
 /* First index of the maximum of logits[n] (strict `>`), written as u32 to
  * `idx` (device).  NaN input -> *status_dev = NNQ_ERR_NON_FINITE (device int,
@@ -286,6 +337,36 @@ int nnq_token_logprobs(const void *logits, nnq_dtype dtype, int64_t m, int64_t n
 int nnq_linear_logprobs(const nnq_weight *w, const void *x, nnq_dtype x_dtype, int64_t m, int64_t k, const float *bias,
                         int64_t bias_len, const int64_t *tokens, int top_n, float *logits, float *logprobs,
                         float *entropy, int64_t *ranks, float *top_logprobs, int64_t *top_ids, void *stream);
+
+/* ---- beam search --------------------------------------------------------------------- */
+
+/* One step of a beam search.  Item b's beam j has the score scores[b][j] (f32, a sum of log probabilities) and the
+ * logits at element b * batch_stride + j * beam_stride (n of them; NNQ_F32, NNQ_BF16 or NNQ_F16).  Its continuation by
+ * token t is worth scores[b][j] + log(softmax(row)[t]); of all the item's continuations the `keep` largest go to
+ *   out_scores [batch, keep] f32, parents [batch, keep] (the beam j) and tokens [batch, keep], device i64,
+ * in descending order, equal ones by beam, then token.  Values are compared before they are rounded to f32: the sum over
+ * a row in f32 (its exponentials to 2^-22), the rest in 64 bits.
+ * finished [batch, beams] (device bytes, may be NULL): a beam that is not 0 there has one continuation, by end_token
+ * (any non-negative token) with its score unchanged; its logits are not read.  A beam whose score is not finite has none
+ * (-inf: unused beams, as all but one at the first step), nor has one whose row holds NaN or +inf or nothing above
+ * -inf; a logit of -inf is no continuation.  Places that are left get parent and token -1 and score -inf.
+ * beams from 1 to 32, keep from 1 to 32 (NNQ_ERR_INVALID_SHAPE).  batch = 0 is a no-op.  Outputs must not overlap the
+ * inputs.  Stands beside nnq_sample_token; no counterpart in the reference, which decodes single sequences. */
+int nnq_beam_select(const void *logits, nnq_dtype dtype, int64_t batch, int64_t beams, int64_t n, int64_t batch_stride,
+                    int64_t beam_stride, const float *scores, const uint8_t *finished, int64_t end_token, int64_t keep,
+                    float *out_scores, int64_t *parents, int64_t *tokens, void *stream);
+
+/* The states that follow: for each of n_states device tensors, in place,
+ *   state[b * beams + j] = state[b * beams + parents[b][j]]  (all reads before the writes),
+ * parents [batch, beams] device i64.  A slot whose parent is itself, or outside [0, beams) (as a place that
+ * nnq_beam_select left), stays as it is.  states: host array of the tensors' addresses, all of one geometry: the slot
+ * dimension has stride slot_stride, the other ndim (up to 8) sizes[] and strides[], all in elements of elem_bytes; e.g.
+ * the used part of a cache.  Bytes between the elements are neither read nor written.  Elements of one tensor that
+ * overlap are NNQ_ERR_INVALID_ARGUMENT (tensors that overlap one another are the caller's to avoid), more than four
+ * dimensions that do not follow one another NNQ_ERR_UNSUPPORTED.  beams from 1 to 32.  Only slots that move are
+ * read and written. */
+int nnq_beam_reorder(void *const *states, int64_t n_states, int64_t batch, int64_t beams, int64_t slot_stride, int ndim,
+                     const int64_t *sizes, const int64_t *strides, int64_t elem_bytes, const int64_t *parents, void *stream);
 
 /* ---- Qwen3 SwiGLU MLP ----------------------------------------------------------- */
 

@@ -6,10 +6,10 @@ MXFP4 mixture-of-experts layer (GPT-OSS and nn-core OCP MXFP4 layouts); ``nn_amd
 operator surface in Python.
 """
 from .quantized import (  # noqa: F401
-    BiasMismatch, DataLengthMismatch, InvalidShape, Layout, NonFiniteData, NotQuantized, QuantizedMatmulError,
+    BeamSelection, BiasMismatch, DataLengthMismatch, InvalidShape, Layout, Mxfp4Rows, NonFiniteData, NotQuantized, QuantizedMatmulError,
     QuantizedMLP, QuantizedMoE, QuantizedWeight, QuantType, RankMismatch, ShapeMismatch, TensorError, TokenLogprobs,
     Unsupported, WeightRank,
-    WrongQuantType, argmax, dequantize_mxfp4_ocp, device_count, init, linear_argmax, linear_logprobs, linear_sample,
-    sample_token, token_logprobs,
+    WrongQuantType, argmax, beam_reorder, beam_select, dequantize_mxfp4_ocp, device_count, init, linear_argmax, linear_logprobs, linear_sample,
+    mxfp4_linear, quantize_mxfp4_rows, sample_token, token_logprobs,
     quantize_mxfp4, quantize_mxfp4_ocp, quantize_q4_k, quantize_q6_k, quantize_q8_0, quantized_linear, quantized_matmul_q4_k, quantized_matmul_q6_k, quantized_matmul_q8_0,
     synth_normal)

@@ -87,6 +87,18 @@ SIGNATURES = {
                                    c_void_p, c_void_p, c_void_p]),
     "nnq_linear_logprobs": (c_int, [c_void_p, c_void_p, c_int, c_i64, c_i64, c_void_p, c_i64, c_void_p, c_int, c_void_p,
                                     c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p]),
+    "nnq_weight_create_mxfp4": (c_int, [c_void_p, c_void_p, c_i64, c_i64, ctypes.POINTER(c_void_p)]),
+    "nnq_weight_create_mxfp4_device": (c_int, [c_void_p, c_void_p, c_i64, c_i64, ctypes.POINTER(c_void_p), c_void_p]),
+    "nnq_mxfp4_quantize": (c_int, [c_void_p, c_int, c_i64, c_i64, c_i64, c_int, c_void_p, c_void_p, c_void_p]),
+    "nnq_mxfp4_dequantize": (c_int, [c_void_p, c_void_p, c_i64, c_i64, c_void_p, c_int, c_void_p]),
+    "nnq_mxfp4_linear": (c_int, [c_void_p, c_void_p, c_int, c_i64, c_i64, c_int, c_void_p, c_i64, c_void_p, c_int,
+                                 c_void_p]),
+    "nnq_mxfp4_linear_codes": (c_int, [c_void_p, c_void_p, c_void_p, c_i64, c_i64, c_void_p, c_i64, c_void_p, c_int,
+                                       c_void_p]),
+    "nnq_beam_select": (c_int, [c_void_p, c_int, c_i64, c_i64, c_i64, c_i64, c_i64, c_void_p, c_void_p, c_i64, c_i64,
+                                c_void_p, c_void_p, c_void_p, c_void_p]),
+    "nnq_beam_reorder": (c_int, [c_void_p, c_i64, c_i64, c_i64, c_i64, c_int, c_void_p, c_void_p, c_i64, c_void_p,
+                                 c_void_p]),
     "nnq_quantize_q4_k": (c_int, [c_void_p, c_sz, c_void_p]),
     "nnq_quantize_mxfp4": (c_int, [c_void_p, c_sz, c_void_p, c_void_p]),
     "nnq_quantize_q8_0": (c_int, [c_void_p, c_sz, c_void_p]),

@@ -25,7 +25,7 @@ COMMON = ["-O3", "-fPIC", "-std=c++17", "-Wall", "-Wno-unused-function", "-Wno-u
 
 HIP_SOURCES = ["nnq_gemv.hip", "nnq_gemm.hip", "nnq_gemm_ring.hip", "nnq_gemm_wide.hip", "nnq_gemm_wide8.hip",
                "nnq_gemm_wide6.hip", "nnq_gemm_thin.hip", "nnq_gemm_few.hip", "nnq_gemm_blk.hip", "nnq_moe.hip", "nnq_sample.hip",
-               "nnq_int4.hip", "nnq_int4_gemm.hip", "nnq_logprobs.hip"]
+               "nnq_int4.hip", "nnq_int4_gemm.hip", "nnq_logprobs.hip", "nnq_mxfp4.hip", "nnq_mxfp4_gemm.hip", "nnq_beam.hip"]
 # per-file device flags: the block-scaled GEMM's MFMAs write their partials to VGPRs (the
 # FMAs that scale them read VGPRs only; with the default accumulator registers every
 # partial costs four extra register reads)

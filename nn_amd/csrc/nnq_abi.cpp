@@ -530,6 +530,68 @@ int nnq_weight_create_int4_device(const uint8_t *codes, const void *scales, nnq_
     return NNQ_OK;
 }
 
+}  // extern "C"
+
+static int check_mxfp4(const uint8_t *codes, const uint8_t *scales, int64_t n, int64_t k, nnq_weight **out, Layout *L) {
+    if (!out) return fail(NNQ_ERR_INVALID_ARGUMENT, "out is null");
+    *out = nullptr;
+    if (n <= 0 || k <= 0) return fail(NNQ_ERR_INVALID_ARGUMENT, "weight shape [%lld, %lld]", (long long)n, (long long)k);
+    size_t bytes = 0;
+    if (!array_bytes(n, k, 1, &bytes) || bytes > (size_t)1 << 60) return size_fail();
+    const char *err = nullptr;
+    if (!make_layout_mxfp4(n, k, L, &err)) return fail(NNQ_ERR_INVALID_SHAPE, "%s, got %lld", err, (long long)k);
+    // (the kernels address a tile's records and the rows of x with 32-bit offsets)
+    if (k > kMxMaxK) return fail(NNQ_ERR_UNSUPPORTED, "in_features %lld (at most 2^20 in MXFP4 rows)", (long long)k);
+    if (!codes || !scales) return fail(NNQ_ERR_INVALID_ARGUMENT, "codes or scales is null");
+    return NNQ_OK;
+}
+
+extern "C" {
+
+int nnq_weight_create_mxfp4_device(const uint8_t *codes, const uint8_t *scales, int64_t n, int64_t k, nnq_weight **out,
+                                   void *stream) {
+    Layout L;
+    const int rc = check_mxfp4(codes, scales, n, k, out, &L);
+    if (rc) return rc;
+    const hipStream_t st = (hipStream_t)stream;
+    nnq_weight *w = new (std::nothrow) nnq_weight;
+    if (!w) return fail(NNQ_ERR_OUT_OF_MEMORY, "weight handle");
+    w->L = L;
+    hipGetDevice(&w->device);
+    unsigned long long bad = 0;
+    const size_t at = (L.total() + 15) / 16 * 16;  // (the index behind the image)
+    hipError_t e = hipMalloc(&w->dev, at + sizeof bad);
+    if (e == hipSuccess) e = hipMemsetAsync(w->dev + at, 0xFF, sizeof bad, st);
+    if (e == hipSuccess)
+        e = (hipError_t)launch_mx_repack(codes, scales, n, k, w->dev, reinterpret_cast<unsigned long long *>(w->dev + at), stream);
+    if (e == hipSuccess) e = hipMemcpyAsync(&bad, w->dev + at, sizeof bad, hipMemcpyDeviceToHost, st);
+    if (e == hipSuccess) e = hipStreamSynchronize(st);
+    if (e != hipSuccess || bad != ~0ull) {
+        if (w->dev) hipFree(w->dev);
+        delete w;
+        if (e != hipSuccess) return hip_fail(e, "weight repack");
+        return fail(NNQ_ERR_NON_FINITE, "scale byte %lld is over %d", (long long)bad, kMxScaleMax);
+    }
+    *out = w;
+    return NNQ_OK;
+}
+
+int nnq_weight_create_mxfp4(const uint8_t *codes, const uint8_t *scales, int64_t n, int64_t k, nnq_weight **out) {
+    Layout L;
+    int rc = check_mxfp4(codes, scales, n, k, out, &L);
+    if (rc) return rc;
+    const size_t cb = (size_t)n * (size_t)k / 2, sb = (size_t)n * (size_t)k / 32, at = align256(cb);
+    for (size_t i = 0; i < sb; i++)
+        if (scales[i] > kMxScaleMax) return fail(NNQ_ERR_NON_FINITE, "scale byte %zu is over %d", i, kMxScaleMax);
+    uint8_t *tmp = nullptr;
+    hipError_t e = hipMalloc(&tmp, at + sb);
+    if (e == hipSuccess) e = hipMemcpy(tmp, codes, cb, hipMemcpyHostToDevice);
+    if (e == hipSuccess) e = hipMemcpy(tmp + at, scales, sb, hipMemcpyHostToDevice);
+    rc = e == hipSuccess ? nnq_weight_create_mxfp4_device(tmp, tmp + at, n, k, out, nullptr) : hip_fail(e, "weight upload");
+    if (tmp) hipFree(tmp);
+    return rc;
+}
+
 int nnq_weight_destroy(nnq_weight *w) {
     if (!w) return NNQ_OK;
     if (w->dev) hipFree(w->dev);
@@ -550,8 +612,9 @@ int nnq_weight_info(const nnq_weight *w, int *fmt, int *layout, int64_t *n, int6
 int nnq_dequant(const nnq_weight *w, float *out, void *stream) {
     if (!w) return fail(NNQ_ERR_NOT_QUANTIZED, "weight handle is null");
     if (!out) return fail(NNQ_ERR_INVALID_ARGUMENT, "out is null");
-    int e = w->L.fmt == NNQ_FMT_INT4G
-                ? launch_int4_dequant(w->L, w->dev, out, stream)
+    int e = w->L.fmt == NNQ_FMT_INT4G ? launch_int4_dequant(w->L, w->dev, out, stream)
+            : w->L.fmt == NNQ_FMT_MXFP4
+                ? launch_mx_dequant_image(w->L, w->dev, out, stream)
                 : launch_dequant(w->L.fmt, w->dev, w->dev + w->L.qs_bytes, w->L.n, w->L.k, w->L.ntile, w->L.nblk, out,
                                  stream);
     if (e) return hip_fail((hipError_t)e, "dequant launch");
@@ -639,6 +702,7 @@ static size_t int4_scratch_bytes(const nnq_weight *w, int64_t m, nnq_dtype x_dty
 static size_t linear_scratch_bytes(const nnq_weight *w, int64_t m, nnq_dtype x_dtype, const void *y,
                                    int swiglu_out = 0) {
     if (w->L.fmt == NNQ_FMT_INT4G) return int4_scratch_bytes(w, m, x_dtype);
+    if (w->L.fmt == NNQ_FMT_MXFP4) return mx_linear_scratch(m, w->L.n, w->L.k, x_dtype == NNQ_BF16 ? kMxBf16 : kMxF32);
     if (few_batch(w, m, x_dtype)) return few_call_scratch(w, m, x_dtype);
     if (!gemm_batch(w, m, x_dtype)) return 0;
     return gemm_call_scratch(w, m, x_dtype, y, swiglu_out);
@@ -706,6 +770,46 @@ static int dispatch_int4(const nnq_weight *w, const void *x, nnq_dtype x_dtype, 
     return NNQ_OK;
 }
 
+// a validated linear call over an MXFP4 weight, x of any kind (xs: its scales where it is codes)
+static MxArgs mx_args(const nnq_weight *w, const void *x, const uint8_t *xs, int x_kind, int floor_rule, int64_t m,
+                      const float *bias, void *y, nnq_dtype y_dtype) {
+    MxArgs a{};
+    a.w = w->dev;
+    a.x = x;
+    a.xs = xs;
+    a.x_kind = x_kind;
+    a.floor_rule = floor_rule;
+    a.bias = bias;
+    a.y = y;
+    a.y_bf16 = y_dtype == NNQ_BF16;
+    a.n = w->L.n;
+    a.k = w->L.k;
+    a.m = m;
+    a.ntile = w->L.ntile;
+    a.units = w->L.nblk;
+    return a;
+}
+
+static int dispatch_mx(const nnq_weight *w, const void *x, const uint8_t *xs, int x_kind, int floor_rule, int64_t m,
+                       const float *bias, void *y, nnq_dtype y_dtype, void *stream, void *ext_scratch) {
+    const int64_t n = w->L.n, k = w->L.k, mc = mx_chunk_rows(m, k);
+    const size_t ye = y_dtype == NNQ_BF16 ? 2 : 4, need = mx_linear_scratch(m, n, k, x_kind);
+    const size_t xrow = x_kind == kMxCodes ? (size_t)k / 2 : (size_t)k * (x_kind == kMxBf16 || x_kind == kMxQuantBf16 ? 2 : 4);
+    Scratch s;
+    void *scr = ext_scratch;
+    if (need && !scr) {
+        HIP_TRY(s.alloc(need, (hipStream_t)stream), "scratch alloc");
+        scr = s.p;
+    }
+    for (int64_t m0 = 0; m0 < m; m0 += mc) {
+        const MxArgs a = mx_args(w, (const uint8_t *)x + (size_t)m0 * xrow, xs ? xs + (size_t)m0 * (k / 32) : nullptr, x_kind,
+                                 floor_rule, std::min(mc, m - m0), bias, (uint8_t *)y + (size_t)m0 * n * ye, y_dtype);
+        int e = mx_takes_rows(a.m, n, k, x_kind) ? launch_mx_rows(a, scr, stream) : launch_mx_gemm(a, scr, stream);
+        if (e) return hip_fail((hipError_t)e, "mxfp4 linear launch");
+    }
+    return NNQ_OK;
+}
+
 static int dispatch_linear(const nnq_weight *w, const void *x, nnq_dtype x_dtype, int64_t m, const float *bias,
                            void *y, nnq_dtype y_dtype, void *stream, int x_swiglu = 0, int32_t *status = nullptr,
                            int status_mode = 0, void *ext_scratch = nullptr, int swiglu_out = 0) {
@@ -714,6 +818,11 @@ static int dispatch_linear(const nnq_weight *w, const void *x, nnq_dtype x_dtype
         if (x_swiglu || status || swiglu_out)
             return fail(NNQ_ERR_INVALID_ARGUMENT, "a SwiGLU input or output or a status needs a GGUF block weight");
         return dispatch_int4(w, x, x_dtype, m, bias, y, y_dtype, stream, ext_scratch);
+    }
+    if (w->L.fmt == NNQ_FMT_MXFP4) {
+        if (x_swiglu || status || swiglu_out)
+            return fail(NNQ_ERR_INVALID_ARGUMENT, "a SwiGLU input or output or a status needs a GGUF block weight");
+        return dispatch_mx(w, x, nullptr, x_dtype == NNQ_BF16 ? kMxBf16 : kMxF32, 0, m, bias, y, y_dtype, stream, ext_scratch);
     }
     if (swiglu_out && (w->L.fmt != NNQ_FMT_Q4_K || (m > 2 && !prefill_swiglu(w, m, x_dtype)) || x_swiglu || bias ||
                        w->L.n % 16))
@@ -822,6 +931,150 @@ int nnq_linear(const nnq_weight *w, const void *x, nnq_dtype x_dtype, int64_t m,
     return NNQ_OK;
 }
 
+// ---- MXFP4 rows ------------------------------------------------------------------------
+
+static int check_mx_rows(int64_t rows, int64_t k) {
+    if (rows < 0) return fail(NNQ_ERR_INVALID_ARGUMENT, "rows = %lld", (long long)rows);
+    if (k <= 0 || k % 32) return fail(NNQ_ERR_INVALID_SHAPE, "rows of %lld values (a positive multiple of 32)", (long long)k);
+    size_t bytes = 0;
+    if (!array_bytes(rows, k, 4, &bytes) || bytes > (size_t)1 << 48) return size_fail();
+    return NNQ_OK;
+}
+
+static int check_mx_rule(nnq_mx_rule rule) {
+    if (rule != NNQ_MX_CEIL && rule != NNQ_MX_FLOOR) return fail(NNQ_ERR_INVALID_ARGUMENT, "scale rule %d", (int)rule);
+    return NNQ_OK;
+}
+
+int nnq_mxfp4_quantize(const void *x, nnq_dtype x_dtype, int64_t rows, int64_t k, int64_t row_stride, nnq_mx_rule rule,
+                       uint8_t *codes, uint8_t *scales, void *stream) {
+    int rc = check_mx_rows(rows, k);
+    if (rc || (rc = check_mx_rule(rule))) return rc;
+    if (x_dtype != NNQ_F32 && x_dtype != NNQ_BF16) return fail(NNQ_ERR_UNSUPPORTED, "input dtype %d (f32 or bf16)", (int)x_dtype);
+    if (row_stride < 0) return fail(NNQ_ERR_INVALID_ARGUMENT, "row stride %lld", (long long)row_stride);
+    if (rows == 0) return NNQ_OK;
+    if (!x || !codes || !scales) return fail(NNQ_ERR_INVALID_ARGUMENT, "null pointer");
+    if ((uintptr_t)x % (x_dtype == NNQ_F32 ? 4 : 2) || (uintptr_t)codes % 4)
+        return fail(NNQ_ERR_INVALID_ARGUMENT, "x must be aligned to its type and codes to 4 bytes");
+    int e = launch_mx_quantize(x, x_dtype == NNQ_BF16, rows, k, rows == 1 ? k : row_stride, rule == NNQ_MX_FLOOR, codes, scales, stream);
+    if (e) return hip_fail((hipError_t)e, "mxfp4 quantize launch");
+    return NNQ_OK;
+}
+
+int nnq_mxfp4_dequantize(const uint8_t *codes, const uint8_t *scales, int64_t rows, int64_t k, void *out,
+                         nnq_dtype out_dtype, void *stream) {
+    int rc = check_mx_rows(rows, k);
+    if (rc) return rc;
+    if (out_dtype != NNQ_F32 && out_dtype != NNQ_BF16) return fail(NNQ_ERR_UNSUPPORTED, "output dtype %d (f32 or bf16)", (int)out_dtype);
+    if (rows == 0) return NNQ_OK;
+    if (!codes || !scales || !out) return fail(NNQ_ERR_INVALID_ARGUMENT, "null pointer");
+    if ((uintptr_t)codes % 4 || (uintptr_t)out % 16) return fail(NNQ_ERR_INVALID_ARGUMENT, "codes must be 4-byte and out 16-byte aligned");
+    int e = launch_mx_dequantize(codes, scales, rows * k, out, out_dtype == NNQ_BF16, stream);
+    if (e) return hip_fail((hipError_t)e, "mxfp4 dequantize launch");
+    return NNQ_OK;
+}
+
+}  // extern "C"
+
+static int check_mx_weight(const nnq_weight *w) {
+    if (!w) return fail(NNQ_ERR_NOT_QUANTIZED, "weight tensor is not quantized (null handle)");
+    if (w->L.fmt != NNQ_FMT_MXFP4) return fail(NNQ_ERR_WRONG_FORMAT, "a product of 4-bit operands needs an MXFP4 weight, got format %d", w->L.fmt);
+    return NNQ_OK;
+}
+
+extern "C" {
+
+int nnq_mxfp4_linear(const nnq_weight *w, const void *x, nnq_dtype x_dtype, int64_t m, int64_t k, nnq_mx_rule rule,
+                     const float *bias, int64_t bias_len, void *y, nnq_dtype y_dtype, void *stream) {
+    int rc = check_mx_weight(w);
+    if (rc || (rc = check_linear(w, x, x_dtype, m, k, bias, bias_len, y, y_dtype)) || (rc = check_mx_rule(rule))) return rc;
+    if (m == 0) return NNQ_OK;
+    if (misaligned_out(y)) return fail(NNQ_ERR_INVALID_ARGUMENT, "y must be 4-byte aligned");
+    const int kind = x_dtype == NNQ_BF16 ? kMxQuantBf16 : kMxQuantF32, fl = rule == NNQ_MX_FLOOR;
+    if (!misaligned_in(x)) return dispatch_mx(w, x, nullptr, kind, fl, m, bias, y, y_dtype, stream, nullptr);
+    // workspace: [staged x][the linear's scratch]
+    size_t xbytes = 0, off[2], total = 0;
+    if (!array_bytes(m, k, x_dtype == NNQ_BF16 ? 2 : 4, &xbytes)) return size_fail();
+    const size_t sizes[2] = {xbytes, mx_linear_scratch(m, w->L.n, k, kind)};
+    if (!plan_regions(sizes, 2, off, &total)) return size_fail();
+    Scratch s;
+    HIP_TRY(s.alloc(total, (hipStream_t)stream), "scratch alloc");
+    uint8_t *base = reinterpret_cast<uint8_t *>(s.p);
+    HIP_TRY(hipMemcpyAsync(base, x, xbytes, hipMemcpyDeviceToDevice, (hipStream_t)stream), "stage x");
+    return dispatch_mx(w, base, nullptr, kind, fl, m, bias, y, y_dtype, stream, sizes[1] ? base + off[1] : nullptr);
+}
+
+int nnq_mxfp4_linear_codes(const nnq_weight *w, const uint8_t *codes, const uint8_t *scales, int64_t m, int64_t k,
+                           const float *bias, int64_t bias_len, void *y, nnq_dtype y_dtype, void *stream) {
+    int rc = check_mx_weight(w);
+    if (rc || (rc = check_linear(w, codes, NNQ_BF16, m, k, bias, bias_len, y, y_dtype))) return rc;
+    if (m == 0) return NNQ_OK;
+    if (!scales) return fail(NNQ_ERR_INVALID_ARGUMENT, "scales is null");
+    if (misaligned_out(y) || misaligned_in(codes)) return fail(NNQ_ERR_INVALID_ARGUMENT, "codes must be 16-byte and y 4-byte aligned");
+    return dispatch_mx(w, codes, scales, kMxCodes, 0, m, bias, y, y_dtype, stream, nullptr);
+}
+
+// ---- beam search -------------------------------------------------------------------------
+
+int nnq_beam_select(const void *logits, nnq_dtype dtype, int64_t batch, int64_t beams, int64_t n, int64_t batch_stride,
+                    int64_t beam_stride, const float *scores, const uint8_t *finished, int64_t end_token, int64_t keep,
+                    float *out_scores, int64_t *parents, int64_t *tokens, void *stream) {
+    if (dtype != NNQ_F32 && dtype != NNQ_BF16 && dtype != NNQ_F16)
+        return fail(NNQ_ERR_UNSUPPORTED, "logits dtype %d (f32, bf16 or f16)", (int)dtype);
+    if (batch < 0) return fail(NNQ_ERR_INVALID_ARGUMENT, "batch = %lld", (long long)batch);
+    if (beams < 1 || beams > kBeams) return fail(NNQ_ERR_INVALID_SHAPE, "%lld beams (1 to %d)", (long long)beams, kBeams);
+    if (keep < 1 || keep > kBeamKeep) return fail(NNQ_ERR_INVALID_SHAPE, "keep %lld (1 to %d)", (long long)keep, kBeamKeep);
+    if (n <= 0) return fail(NNQ_ERR_INVALID_SHAPE, "beam selection over a zero-length dimension");
+    if (n > kLogprobMaxVocab) return fail(NNQ_ERR_UNSUPPORTED, "%lld logits in a row (at most 2^31 - 1)", (long long)n);
+    if (batch == 0) return NNQ_OK;
+    if (!logits || !scores || !out_scores || !parents || !tokens) return fail(NNQ_ERR_INVALID_ARGUMENT, "null pointer");
+    if (batch_stride < 0 || beam_stride < 0) return fail(NNQ_ERR_INVALID_ARGUMENT, "negative stride");
+    if (finished && end_token < 0) return fail(NNQ_ERR_INVALID_ARGUMENT, "end token %lld", (long long)end_token);
+    if ((uintptr_t)logits % (dtype == NNQ_F32 ? 4 : 2)) return fail(NNQ_ERR_INVALID_ARGUMENT, "logits are not aligned to their type");
+    if (((uintptr_t)parents | (uintptr_t)tokens) & 7 || ((uintptr_t)scores | (uintptr_t)out_scores) & 3)
+        return fail(NNQ_ERR_INVALID_ARGUMENT, "parents and tokens must be 8-byte, scores 4-byte aligned");
+    Scratch s;
+    HIP_TRY(s.alloc(beam_plan(batch, (int)beams, n, (int)keep).bytes, (hipStream_t)stream), "scratch alloc");
+    int e = launch_beam_select(BeamArgs{logits, (int)dtype, batch, n, batch_stride, beam_stride, (int)beams, (int)keep, scores,
+                                        finished, end_token, out_scores, parents, tokens},
+                               s.p, stream);
+    if (e) return hip_fail((hipError_t)e, "beam selection launch");
+    return NNQ_OK;
+}
+
+int nnq_beam_reorder(void *const *states, int64_t n_states, int64_t batch, int64_t beams, int64_t slot_stride, int ndim,
+                     const int64_t *sizes, const int64_t *strides, int64_t elem_bytes, const int64_t *parents, void *stream) {
+    if (n_states < 0 || batch < 0) return fail(NNQ_ERR_INVALID_ARGUMENT, "%lld states, batch %lld", (long long)n_states, (long long)batch);
+    if (beams < 1 || beams > kBeams) return fail(NNQ_ERR_INVALID_SHAPE, "%lld beams (1 to %d)", (long long)beams, kBeams);
+    if (ndim < 0 || ndim > 8 || elem_bytes < 1 || elem_bytes > 16 || slot_stride < 0 || (ndim && (!sizes || !strides)))
+        return fail(NNQ_ERR_INVALID_ARGUMENT, "%d dimensions of %lld-byte elements", ndim, (long long)elem_bytes);
+    if (batch > INT64_MAX / kBeams || slot_stride > (int64_t)1 << 56) return size_fail();
+    for (int i = 0; i < ndim; i++)
+        if (strides[i] > (int64_t)1 << 56) return size_fail();
+    if (n_states == 0 || batch == 0 || beams == 1) return NNQ_OK;
+    if (!states || !parents) return fail(NNQ_ERR_INVALID_ARGUMENT, "null pointer");
+    if ((uintptr_t)parents & 7) return fail(NNQ_ERR_INVALID_ARGUMENT, "parents must be 8-byte aligned");
+    uintptr_t bits = 0;
+    for (int64_t i = 0; i < n_states; i++) {
+        if (!states[i]) return fail(NNQ_ERR_INVALID_ARGUMENT, "state %lld is null", (long long)i);
+        bits |= (uintptr_t)states[i];
+    }
+    ReorderArgs a{};
+    a.parents = parents;
+    a.batch = batch;
+    a.beams = (int)beams;
+    const char *err = reorder_geometry(batch * beams, slot_stride, ndim, sizes, strides, elem_bytes, bits, &a);
+    if (err) return fail(a.dims < 0 ? NNQ_ERR_UNSUPPORTED : NNQ_ERR_INVALID_ARGUMENT, "state tensors have %s", err);
+    if (a.pieces == 0) return NNQ_OK;
+    for (int64_t i = 0; i < n_states; i += kReorderTensors) {
+        const int count = (int)std::min<int64_t>(kReorderTensors, n_states - i);
+        for (int j = 0; j < count; j++) a.state[j] = reinterpret_cast<uint8_t *>(states[i + j]);
+        int e = launch_beam_reorder(a, count, stream);
+        if (e) return hip_fail((hipError_t)e, "beam reorder launch");
+    }
+    return NNQ_OK;
+}
+
 int nnq_argmax_f32(const float *logits, int64_t n, uint32_t *idx, int32_t *status_dev, void *stream) {
     if (!logits || !idx) return fail(NNQ_ERR_INVALID_ARGUMENT, "null pointer");
     if (n <= 0) return fail(NNQ_ERR_INVALID_SHAPE, "argmax over a zero-length dimension");
@@ -865,6 +1118,11 @@ static int linear_argmax(const nnq_weight *w, const float *x, int64_t k, const f
         a.argmax_partial = keys;
         a.argmax_count = &nkeys;
         e = launch_int4_rows(a, nullptr, stream);
+    } else if (L.fmt == NNQ_FMT_MXFP4) {
+        MxArgs a = mx_args(w, x, nullptr, kMxF32, 0, 1, bias, logits, NNQ_F32);
+        a.argmax_partial = keys;
+        a.argmax_count = &nkeys;
+        e = launch_mx_rows(a, nullptr, stream);
     } else {
         GemvArgs a{};
         a.qs = w->dev;

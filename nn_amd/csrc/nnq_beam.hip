@@ -1,0 +1,371 @@
+// Beam search on gfx950: the choice of continuations, and the states that follow it.
+//
+// nnq_beam_select: item b's beam j with score s_j offers token t the value
+//   v = s_j + l_t - log sum_i e^(l_i),
+// and the `keep` largest of an item's values are wanted.  Within a beam v has the order of l, so the keep largest
+// logits of every beam hold them.  Two launches:
+//   beam_seg_kernel   one wave per 2048 logits of a beam: the maximum, the sum of e^(l - maximum) over the other
+//                     elements, and the candidates (nnq_logits.h).  Beams that offer nothing by themselves (ended
+//                     ones, scores of -inf) are not read.
+//   beam_join_kernel  one workgroup per item: log sum e^l of each beam from its segments, in 64 bits and in a fixed
+//                     order, and the largest values of the beams' candidates, compared in 64 bits.
+// A row's segments begin at its multiples of 2048 wherever it lies, so that equal rows have equal sums and their
+// continuations tie exactly.
+#include <algorithm>
+
+#include "nnq_device.h"
+#include "nnq_internal.h"
+#include "nnq_logits.h"
+
+namespace nnq {
+
+namespace {
+
+constexpr int kBeamWaves = 4;
+constexpr int kBeamThreads = 1024;
+constexpr int kBeamList = 1024;  // candidates that the join ranks in LDS
+
+struct BeamStat {
+    float mx, r;   // a segment's maximum, the sum of e^(l - mx) over its elements below it
+    uint32_t cnt;  // elements equal to it
+    uint32_t pad;
+};
+
+struct BeamDev {
+    BeamArgs a;
+    int64_t item0, nseg;  // the launch's first item
+    int slots;
+    BeamStat *stat;       // [items][beams][nseg]
+    uint64_t *cand;       // [items][beams][nseg][slots]
+};
+
+__device__ __forceinline__ bool beam_ended(const BeamArgs &a, int64_t row) { return a.finished && a.finished[row]; }
+__device__ __forceinline__ bool finite_score(float s) { return (__float_as_uint(s) & 0x7F800000u) != 0x7F800000u; }
+
+// 16 bytes at the element's own alignment
+typedef u32x4 u32x4_by2 __attribute__((aligned(2)));
+typedef u32x4 u32x4_by4 __attribute__((aligned(4)));
+template <class T>
+__device__ __forceinline__ u32x4 load16(const T *p) {
+    if constexpr (sizeof(T) == 4) return *reinterpret_cast<const u32x4_by4 *>(p);
+    else return *reinterpret_cast<const u32x4_by2 *>(p);
+}
+
+template <class T>
+__global__ __launch_bounds__(kBeamWaves * 64) void beam_seg_kernel(BeamDev g) {
+    constexpr int V = 16 / (int)sizeof(T);  // logits of one 16-byte load
+    const BeamArgs &a = g.a;
+    const int lane = threadIdx.x & 63;
+    const int wv = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
+    const int64_t rl = blockIdx.y, item = g.item0 + rl / a.beams, beam = rl % a.beams;
+    const int64_t seg = (int64_t)blockIdx.x * kBeamWaves + wv;
+    if (!finite_score(a.scores[item * a.beams + beam]) || beam_ended(a, item * a.beams + beam)) return;
+    const T *p = reinterpret_cast<const T *>(a.logits) + item * a.batch_stride + beam * a.beam_stride;
+    const int64_t base = seg * kSeg + (int64_t)lane * V;  // logit of element 0
+    float x[kPer];
+#pragma unroll
+    for (int v = 0; v < kPer / V; v++) {
+        const int64_t i = base + v * 64 * V;
+        if (i + V <= a.n) {
+            widen16<T>(load16(p + i), x + v * V);
+        } else {
+#pragma unroll
+            for (int e = 0; e < V; e++) x[v * V + e] = i + e < a.n ? widen<T>(p[i + e]) : kNegInf;
+        }
+    }
+    // (fmaxf passes over NaN; a NaN reaches the sum through its difference)
+    float lm = x[0];
+#pragma unroll
+    for (int e = 1; e < kPer; e++) lm = fmaxf(lm, x[e]);
+    const float mx = max64(lm);
+    const float ref = mx == kNegInf ? 0.f : mx;
+    float r = 0.f;
+    int cnt = kSeg;
+#pragma unroll
+    for (int e = 0; e < kPer; e++) {
+        const float d = __builtin_elementwise_maximum(x[e] - ref, -1e30f);  // (-inf: its e^d is 0; NaN stays)
+        const float ex = exp_of(d);
+        const bool below = d != 0.f;  // (or NaN)
+        cnt -= __popcll(__ballot(below));
+        r += below ? ex : 0.f;
+    }
+    r = sum64(r);
+    const int64_t at = rl * g.nseg + seg;
+    if (lane == 0) g.stat[at] = BeamStat{mx, r, (uint32_t)cnt, 0};
+    __shared__ uint64_t list[kBeamWaves][64];
+    segment_candidates<V>(x, lm, base, a.keep, g.slots, lane, list[wv], g.cand + at * g.slots);
+}
+
+// larger values have larger ones (v is a number)
+__device__ __forceinline__ uint64_t ord64(double v) {
+    const uint64_t u = (uint64_t)__double_as_longlong(v + 0.0);
+    return u >> 63 ? ~u : u | 0x8000000000000000ull;
+}
+__device__ __forceinline__ double unord64(uint64_t o) {
+    return __longlong_as_double((long long)(o >> 63 ? o & 0x7FFFFFFFFFFFFFFFull : ~o));
+}
+
+// a candidate: its value's order (0: none), its beam and its key (logit, then index)
+struct Cand {
+    uint64_t v, key;
+    int beam;
+};
+__device__ __forceinline__ bool ahead(const Cand &x, const Cand &y) {
+    return x.v > y.v || (x.v == y.v && (x.beam < y.beam || (x.beam == y.beam && x.key > y.key)));
+}
+__device__ __forceinline__ Cand shfl_cand(const Cand &c, int o) {
+    return Cand{(uint64_t)__shfl_xor((unsigned long long)c.v, o, 64), (uint64_t)__shfl_xor((unsigned long long)c.key, o, 64),
+                __shfl_xor(c.beam, o, 64)};
+}
+
+__global__ __launch_bounds__(kBeamThreads) void beam_join_kernel(BeamDev g) {
+    constexpr int NW = kBeamThreads / 64;
+    __shared__ double off[kBeams];   // score - log sum e^(l - maximum) (NaN: the beam offers nothing from its logits)
+    __shared__ float top[kBeams];    // the maximum (taken off a logit before anything is added: both may be far from 0)
+    __shared__ uint64_t ended[kBeams];  // the order of an ended beam's score (0: not ended)
+    __shared__ uint64_t maxima[kBeamThreads], bound;
+    __shared__ Cand list[kBeamList], part[NW];
+    __shared__ uint32_t listed;
+    const BeamArgs &a = g.a;
+    const int tid = threadIdx.x, lane = tid & 63, wv = tid >> 6;
+    const int64_t item = g.item0 + blockIdx.x;
+    const BeamStat *stat = g.stat + (int64_t)blockIdx.x * a.beams * g.nseg;
+    const uint64_t *cand = g.cand + (int64_t)blockIdx.x * a.beams * g.nseg * g.slots;
+    const int64_t keys = g.nseg * g.slots;
+    const double nan = __longlong_as_double(0x7FF8000000000000ll);
+    if (tid == 0) listed = 0;
+    for (int b = wv; b < a.beams; b += NW) {
+        const float score = a.scores[item * a.beams + b];
+        float mx = kNegInf;
+        const bool fin = finite_score(score), end = beam_ended(a, item * a.beams + b);
+        double o = nan;
+        if (fin && !end) {
+            const BeamStat *st = stat + b * g.nseg;
+            for (int64_t i = lane; i < g.nseg; i += 64) mx = fmaxf(mx, st[i].mx);
+            mx = max64(mx);
+            double r = 0.0, cnt = 0.0;  // everything but the elements equal to the maximum, and their number
+            for (int64_t i = lane; i < g.nseg; i += 64) {
+                const BeamStat q = st[i];
+                if (q.mx == mx) {
+                    cnt += (double)q.cnt;
+                    r += (double)q.r;
+                } else {
+                    const double f = exp((double)q.mx - (double)mx);
+                    r += f * ((double)q.cnt + (double)q.r);
+                }
+            }
+            for (int s = 32; s > 0; s >>= 1) {
+                r += __shfl_xor(r, s, 64);
+                cnt += __shfl_xor(cnt, s, 64);
+            }
+            // (a row without a logit above -inf: mx = -inf)
+            o = mx == kNegInf ? nan : (double)score - log1p(r + (cnt - 1.0));
+        }
+        if (lane == 0) {
+            off[b] = o;
+            top[b] = mx;
+            ended[b] = fin && end ? ord64((double)score) : 0;
+        }
+    }
+    __syncthreads();
+
+    auto value = [&](double o, float mx, uint64_t key) -> uint64_t {
+        return key ? ord64(o + ((double)unord((uint32_t)(key >> 32)) - (double)mx)) : 0;
+    };
+    auto each = [&](auto &&f) {  // the thread's candidates
+        for (int b = 0; b < a.beams; b++) {
+            const double o = off[b];
+            const float mx = top[b];
+            if (ended[b]) {
+                if (tid == b) f(Cand{ended[b], 1, b});
+            } else if (o == o) {
+                for (int64_t i = tid; i < keys; i += kBeamThreads) {
+                    const uint64_t k = cand[b * keys + i];
+                    f(Cand{value(o, mx, k), k, b});
+                }
+            }
+        }
+    };
+    uint64_t best = 0;
+    each([&](const Cand &c) { best = max(best, c.v); });
+    maxima[tid] = best;
+    __syncthreads();
+    if (wv == 0) {
+        // the keep-th largest of the maxima of 64 parts is a lower bound of the keep-th largest value (its leading 32 bits)
+        uint64_t m = maxima[lane];
+#pragma unroll
+        for (int w = 1; w < NW; w++) m = max(m, maxima[64 * w + lane]);
+        const uint32_t v = (uint32_t)(m >> 32);
+        const uint32_t b = largest_with<32>(a.keep, [&](uint32_t k) { return __popcll(__ballot(v >= k)); });
+        if (lane == 0) bound = max((uint64_t)b << 32, (uint64_t)1);
+    }
+    __syncthreads();
+    const uint64_t low = bound;
+    each([&](const Cand &c) {
+        if (c.v >= low) {
+            const uint32_t at = atomicAdd(&listed, 1u);
+            if (at < kBeamList) list[at] = c;
+        }
+    });
+    __syncthreads();
+    auto put = [&](int place, const Cand &c) {
+        const int64_t at = item * a.keep + place;
+        a.out_scores[at] = c.v ? (float)unord64(c.v) : kNegInf;
+        a.parents[at] = c.v ? c.beam : -1;
+        a.tokens[at] = !c.v ? -1 : ended[c.beam] ? a.end_token : (int64_t)(0xFFFFFFFFu - (uint32_t)c.key);
+    };
+    const int got = (int)min(listed, (uint32_t)kBeamList);
+    if (listed <= kBeamList) {
+        for (int i = tid; i < got; i += kBeamThreads) {
+            const Cand c = list[i];
+            int place = 0;
+            for (int j = 0; j < got; j++) place += ahead(list[j], c);
+            if (place < a.keep) put(place, c);
+        }
+        if (tid >= got && tid < a.keep) put(tid, Cand{0, 0, 0});
+        return;
+    }
+    // very many equal values: one place after another, the first of what is behind the last one
+    Cand last{~0ull, ~0ull, -1};
+    for (int place = 0; place < a.keep; place++) {
+        Cand c{0, 0, kBeams};
+        each([&](const Cand &x) {
+            if (x.v && ahead(last, x) && ahead(x, c)) c = x;
+        });
+        for (int s = 32; s > 0; s >>= 1) {
+            const Cand o = shfl_cand(c, s);
+            if (ahead(o, c)) c = o;
+        }
+        if (lane == 0) part[wv] = c;
+        __syncthreads();
+        c = part[0];
+        for (int w = 1; w < NW; w++)
+            if (ahead(part[w], c)) c = part[w];
+        if (tid == 0) put(place, c);
+        last = c;
+        __syncthreads();  // (part is written again)
+        if (!c.v) last = Cand{0, 0, kBeams};
+    }
+}
+
+template <class T>
+int launch_select(const BeamDev &g, int64_t items, void *stream) {
+    hipLaunchKernelGGL(beam_seg_kernel<T>, dim3((unsigned)(g.nseg / kBeamWaves), (unsigned)(items * g.a.beams)), dim3(kBeamWaves * 64), 0,
+                       (hipStream_t)stream, g);
+    hipError_t e = hipGetLastError();
+    if (e != hipSuccess) return (int)e;
+    hipLaunchKernelGGL(beam_join_kernel, dim3((unsigned)items), dim3(kBeamThreads), 0, (hipStream_t)stream, g);
+    return (int)hipGetLastError();
+}
+
+// ---- states -----------------------------------------------------------------------------
+// Bound: the bytes of the slots that move, written once, and of their parents, read once.  A thread takes one piece (up
+// to 16 bytes) of all slots of an item: it reads the pieces of the parents of all slots that move before it writes any,
+// so that the copy is in place whatever the parents are, and a parent of several slots comes from HBM once.
+template <int N>
+struct Bytes {
+    typedef uint8_t type;
+};
+template <>
+struct Bytes<2> {
+    typedef uint16_t type;
+};
+template <>
+struct Bytes<4> {
+    typedef uint32_t type;
+};
+template <>
+struct Bytes<8> {
+    typedef u32x2 type;
+};
+template <>
+struct Bytes<16> {
+    typedef u32x4 type;
+};
+
+template <int VEC, int MOST>
+__global__ __launch_bounds__(256) void beam_reorder_kernel(ReorderArgs a) {
+    typedef typename Bytes<VEC>::type T;
+    __shared__ int from[MOST];
+    __shared__ int moves;
+    const int tid = threadIdx.x;
+    if (tid == 0) moves = 0;
+    __syncthreads();
+    for (int64_t item = blockIdx.y; item < a.batch; item += gridDim.y) {
+        if (tid < a.beams) {
+            const int64_t p = a.parents[item * a.beams + tid];
+            const bool move = p >= 0 && p < a.beams && p != tid;
+            from[tid] = move ? (int)p : -1;
+            if (move) moves = 1;
+        }
+        __syncthreads();
+        if (moves) {
+            int f[MOST];
+#pragma unroll
+            for (int j = 0; j < MOST; j++) f[j] = j < a.beams ? __builtin_amdgcn_readfirstlane(from[j]) : -1;
+            for (int64_t i = (int64_t)blockIdx.x * 256 + tid; i < a.pieces; i += (int64_t)gridDim.x * 256) {
+                uint8_t *p = a.state[blockIdx.z] + item * a.beams * a.slot_stride;
+                int64_t left = i;
+#pragma unroll
+                for (int d = kReorderDims - 1; d >= 0; d--) {
+                    if (a.size[d] == 1) continue;
+                    const int64_t q = left / a.size[d];
+                    p += (left - q * a.size[d]) * a.stride[d];
+                    left = q;
+                }
+                T v[MOST];
+#pragma unroll
+                for (int j = 0; j < MOST; j++)
+                    if (f[j] >= 0) v[j] = *reinterpret_cast<const T *>(p + f[j] * a.slot_stride);
+#pragma unroll
+                for (int j = 0; j < MOST; j++)
+                    if (f[j] >= 0) *reinterpret_cast<T *>(p + j * a.slot_stride) = v[j];
+            }
+        }
+        __syncthreads();
+        if (tid == 0) moves = 0;
+        __syncthreads();
+    }
+}
+
+template <int VEC>
+int launch_reorder(const ReorderArgs &a, int tensors, void *stream) {
+    const dim3 grid((unsigned)std::min<int64_t>((a.pieces + 255) / 256, 65536), (unsigned)std::min<int64_t>(a.batch, 65535), (unsigned)tensors);
+    if (a.beams <= 4) hipLaunchKernelGGL((beam_reorder_kernel<VEC, 4>), grid, dim3(256), 0, (hipStream_t)stream, a);
+    else if (a.beams <= 8) hipLaunchKernelGGL((beam_reorder_kernel<VEC, 8>), grid, dim3(256), 0, (hipStream_t)stream, a);
+    else hipLaunchKernelGGL((beam_reorder_kernel<VEC, 32>), grid, dim3(256), 0, (hipStream_t)stream, a);
+    return (int)hipGetLastError();
+}
+
+}  // namespace
+
+int launch_beam_select(const BeamArgs &a, void *scratch, void *stream) {
+    const BeamPlan p = beam_plan(a.batch, a.beams, a.n, a.keep);
+    BeamDev g{};
+    g.a = a;
+    g.nseg = p.nseg;
+    g.slots = p.slots;
+    g.cand = reinterpret_cast<uint64_t *>(scratch);
+    g.stat = reinterpret_cast<BeamStat *>(g.cand + (size_t)p.items * a.beams * p.nseg * p.slots);
+    for (int64_t i = 0; i < a.batch; i += p.items) {
+        g.item0 = i;
+        const int64_t items = std::min(p.items, a.batch - i);
+        const int e = a.dtype == NNQ_F32 ? launch_select<float>(g, items, stream)
+                      : a.dtype == NNQ_BF16 ? launch_select<Bf16>(g, items, stream) : launch_select<F16>(g, items, stream);
+        if (e) return e;
+    }
+    return 0;
+}
+
+int launch_beam_reorder(const ReorderArgs &a, int tensors, void *stream) {
+    if (tensors < 1 || tensors > kReorderTensors || a.beams < 1 || a.beams > kBeams) return (int)hipErrorInvalidValue;
+    switch (a.vec) {
+    case 16: return launch_reorder<16>(a, tensors, stream);
+    case 8: return launch_reorder<8>(a, tensors, stream);
+    case 4: return launch_reorder<4>(a, tensors, stream);
+    case 2: return launch_reorder<2>(a, tensors, stream);
+    default: return launch_reorder<1>(a, tensors, stream);
+    }
+}
+
+}  // namespace nnq

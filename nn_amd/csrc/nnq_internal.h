@@ -273,6 +273,96 @@ int launch_int4_repack(const Layout &L, const uint8_t *codes, const uint16_t *sc
                        unsigned long long *bad, void *stream);
 int launch_int4_dequant(const Layout &L, const uint8_t *w, float *out, void *stream);
 
+// ---- MXFP4 rows (nnq_mxfp4.hip, nnq_mxfp4_gemm.hip) ---------------------------------
+constexpr int kMxUnit = 128;      // k of one unit
+constexpr int kMxRecord = 1088;   // bytes of a record: 16 rows of a unit, codes and scales
+constexpr int kMxScaleMax = 252;  // the largest scale byte of a weight: 6 * 2^125 is finite in f32
+constexpr int64_t kMxMaxK = (int64_t)1 << 20;
+constexpr int kMxRows = 16;       // the most token rows of one launch_mx_rows
+inline int64_t mx_units(int64_t k) { return (k + kMxUnit - 1) / kMxUnit; }
+inline int64_t mx_tiles(int64_t rows) { return (rows + kTile - 1) / kTile; }
+bool make_layout_mxfp4(int64_t n, int64_t k, Layout *out, const char **err);
+// x of a linear: as it is, to be quantized, or codes with their scales
+enum MxInput { kMxBf16, kMxF32, kMxQuantBf16, kMxQuantF32, kMxCodes };
+struct MxArgs {
+    const uint8_t *w;   // the image
+    const void *x;      // [m, k], 16-byte aligned; kMxCodes: codes [m, k / 2]
+    const uint8_t *xs;  // kMxCodes: scales [m, k / 32]
+    const float *bias;  // [n] or null
+    void *y;            // [m, n] f32 or bf16
+    int x_kind, y_bf16;
+    int floor_rule;     // the quantization's (mx_scale_byte)
+    int64_t n, k, m;
+    int64_t ntile, units;
+    unsigned long long *argmax_partial;  // optional (m = 1): argmax keys, at most ntile of them
+    int64_t *argmax_count;               //   and how many the launch writes
+    int ks;                              // (set by the launch: parts of K, their sums in slabs [ks][m][n])
+    float *slabs;
+};
+// how m rows run (nnq_plan.cpp), with the scratch's offsets
+struct MxRowsPlan {
+    int ks, planes;  // planes: f32 x goes through its bf16 planes in the scratch
+    size_t slabs, bytes;
+};
+MxRowsPlan mx_rows_plan(int64_t m, int64_t n, int64_t k, int x_kind);
+struct MxGemmPlan {
+    int mt, nt, ks;              // 32-row tiles of a workgroup, 32-column tiles of its waves, K split
+    int row_blocks, col_blocks;  // workgroups along m and n
+    size_t slabs, bytes;         // (x's planes or records come first)
+};
+MxGemmPlan mx_gemm_plan(int64_t m, int64_t n, int64_t k, int x_kind);
+bool mx_takes_rows(int64_t m, int64_t n, int64_t k, int x_kind);  // or launch_mx_gemm
+int64_t mx_chunk_rows(int64_t m, int64_t k);
+size_t mx_linear_scratch(int64_t m, int64_t n, int64_t k, int x_kind);  // of a call in chunks
+int launch_mx_rows(const MxArgs &a, void *scratch, void *stream);
+int launch_mx_gemm(const MxArgs &a, void *scratch, void *stream);
+int launch_mx_quantize(const void *x, int x_bf16, int64_t rows, int64_t k, int64_t row_stride, int floor_rule,
+                       uint8_t *codes, uint8_t *scales, void *stream);
+int launch_mx_dequantize(const uint8_t *codes, const uint8_t *scales, int64_t count, void *out, int out_bf16, void *stream);
+int launch_mx_quantize_image(const void *x, int x_bf16, int64_t m, int64_t k, int floor_rule, uint8_t *image, void *stream);
+int launch_mx_repack(const uint8_t *codes, const uint8_t *scales, int64_t n, int64_t k, uint8_t *image,
+                     unsigned long long *bad, void *stream);
+int launch_mx_dequant_image(const Layout &L, const uint8_t *image, float *out, void *stream);
+int launch_mx_split(const float *x, int64_t count, uint16_t *planes, void *stream);
+
+// ---- beam search (nnq_beam.hip) --------------------------------------------------------
+constexpr int kBeams = 32;     // the most beams of a batch item
+constexpr int kBeamKeep = 32;  // and candidates kept
+struct BeamArgs {
+    const void *logits;       // beam j of item b at element b * batch_stride + j * beam_stride, n of them
+    int dtype;                // nnq_dtype
+    int64_t batch, n, batch_stride, beam_stride;
+    int beams, keep;
+    const float *scores;      // [batch][beams]
+    const uint8_t *finished;  // [batch][beams] or null
+    int64_t end_token;
+    float *out_scores;        // [batch][keep]
+    int64_t *parents, *tokens;
+};
+// items of a launch, segments of a row, candidate slots of a segment, scratch bytes (nnq_plan.cpp)
+struct BeamPlan {
+    int64_t items, nseg;
+    int slots;
+    size_t bytes;
+};
+BeamPlan beam_plan(int64_t batch, int beams, int64_t n, int keep);
+int launch_beam_select(const BeamArgs &a, void *scratch, void *stream);
+
+constexpr int kReorderDims = 4, kReorderTensors = 32;
+// one geometry: `pieces` of `vec` bytes for each slot, at sum of (index of dim d) * stride[d]; innermost dim last
+struct ReorderArgs {
+    uint8_t *state[kReorderTensors];
+    const int64_t *parents;  // [batch][beams]
+    int64_t batch, slot_stride;
+    int beams, vec, dims;
+    int64_t size[kReorderDims], stride[kReorderDims];  // (strides in bytes; unused dims: size 1)
+    int64_t pieces;
+};
+// the geometry of a state tensor (nnq_plan.cpp): null, or why it is refused
+const char *reorder_geometry(int64_t slots, int64_t slot_stride, int ndim, const int64_t *sizes, const int64_t *strides,
+                             int64_t elem, uintptr_t address_bits, ReorderArgs *out);
+int launch_beam_reorder(const ReorderArgs &a, int tensors, void *stream);
+
 // ---- log probabilities (nnq_logprobs.hip) -------------------------------------------
 struct LogprobArgs {
     const void *logits;     // row r at element r * stride, n of them

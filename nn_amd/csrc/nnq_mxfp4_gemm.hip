@@ -1,0 +1,328 @@
+// Linears over MXFP4 rows on gfx950 for more than sixteen token rows (nnq_mxfp4.hip has the formula and the image).
+//  * mx_gemm16_kernel: x in bf16 (f32 x: three bf16 planes that sum to it), 32x32x16 bf16 MFMAs.  A code times its
+//    scale is exact in bf16, one conversion for two of them, so nothing is scaled afterwards.
+//  * mx_gemm4_kernel: x quantized to MXFP4, 32x32x64 block-scaled MFMAs on the codes and scales as they are.
+// A workgroup of four waves takes MT * 32 rows and NT * 128 columns.  The A pieces of a unit (128 k) are copied
+// straight to one of two LDS buffers, a unit ahead, with one barrier a unit; a wave's weights go from memory into its
+// registers, a unit ahead too.  With too few workgroups K is split: f32 slabs, added in order.
+#include <algorithm>
+#include <type_traits>
+
+#include "nnq_device.h"
+#include "nnq_internal.h"
+#include "nnq_mxfp4.h"
+
+namespace nnq {
+
+namespace {
+
+constexpr int W = 4;          // waves of a workgroup
+constexpr int kPiece = 8192;  // bf16 bytes of 32 rows and one unit
+
+__device__ __forceinline__ floatx16 mfma32_bf16(u32x4 a, u32x4 b, floatx16 c) {
+    return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
+}
+__device__ __forceinline__ floatx16 mfma32_mx(u32x4 a, uint32_t sa, u32x4 b, uint32_t sb, floatx16 c) {
+#if defined(__HIP_DEVICE_COMPILE__)
+    const i32x8 av = {(int)a[0], (int)a[1], (int)a[2], (int)a[3], 0, 0, 0, 0}, bv = {(int)b[0], (int)b[1], (int)b[2], (int)b[3], 0, 0, 0, 0};
+    return __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(av, bv, c, 4, 4, 0, (int)sa, 0, (int)sb);
+#else
+    return c;
+#endif
+}
+
+struct MxGemmArgs {
+    const uint8_t *w, *x;  // x: bf16 planes [P][m][k], or the records of the quantized rows
+    const float *bias;
+    void *y;               // [m][n], or with ks > 1 f32 slabs [ks][m][n] without the bias
+    int y_bf16;
+    int m, units, ntile, ks;
+    int row_blocks, col_blocks;
+    int64_t n, k;
+};
+
+// where a workgroup works: workgroup ids go round the 8 XCDs, each takes a contiguous run, the row blocks of a column
+// block (which share its weights) one after another
+struct MxPlace {
+    int rb, cb, kp, u0, u1;
+    __device__ __forceinline__ explicit MxPlace(const MxGemmArgs &a) {
+        const int total = a.row_blocks * a.col_blocks * a.ks, bid = (int)blockIdx.x;
+        const int per = total / 8, extra = total % 8, xcd = bid % 8, at = bid / 8;
+        const int t = xcd * per + min(xcd, extra) + at;
+        rb = t % a.row_blocks;
+        cb = t / a.row_blocks % a.col_blocks;
+        kp = t / (a.row_blocks * a.col_blocks);
+        u0 = (int)((int64_t)a.units * kp / a.ks);
+        u1 = (int)((int64_t)a.units * (kp + 1) / a.ks);
+    }
+};
+
+// A wave's weights of a unit, NT * 32 columns: lane 32h + 16b + r holds row r of tile b, its blocks h and 2 + h.
+template <int NT>
+struct MxB {
+    u32x4 q[NT][2];
+    uint32_t s[NT][2];
+};
+template <int NT>
+struct MxBLoad {
+    __amdgpu_buffer_rsrc_t buf[NT];
+    int off[NT];  // the lane's; tiles past the last are read as the last (not stored)
+    __device__ __forceinline__ MxBLoad(const MxGemmArgs &a, int tile0, int lane) {
+#pragma unroll
+        for (int nt = 0; nt < NT; nt++) {
+            const int t = min(tile0 + 2 * nt, a.ntile - 1), bytes = a.units * kMxRecord;
+            buf[nt] = rsrc(a.w + (size_t)t * bytes, (int64_t)min(2, a.ntile - t) * bytes);
+            off[nt] = (lane & 16) && t + 1 < a.ntile ? bytes : 0;
+        }
+    }
+    __device__ __forceinline__ void load(int u, int lane, MxB<NT> &o) const {
+        const int slot = 16 * (lane >> 5) + (lane & 15);
+#pragma unroll
+        for (int nt = 0; nt < NT; nt++)
+#pragma unroll
+            for (int i = 0; i < 2; i++) {
+                o.q[nt][i] = __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(buf[nt], off[nt] + 16 * slot + 512 * i, u * kMxRecord, 0));
+                o.s[nt][i] = __builtin_amdgcn_raw_buffer_load_b8(buf[nt], off[nt] + 1024 + slot + 32 * i, u * kMxRecord, 0);
+            }
+    }
+};
+
+__device__ __forceinline__ void arrive() {
+    __builtin_amdgcn_s_waitcnt(0x0070);  // vmcnt(0) lgkmcnt(0)
+    __builtin_amdgcn_s_barrier();
+    __builtin_amdgcn_sched_barrier(0);
+}
+
+// lane: column lane % 32 of each 32, rows 8 i + 4h + e of each 32-row tile.  The bias is read before the first store:
+// a wait for a load waits for the stores before it, too.
+template <int MT, int NT>
+__device__ __forceinline__ void mx_store(const MxGemmArgs &a, const MxPlace &at, int tile0, int lane, floatx16 (&acc)[MT][NT]) {
+    const bool slab = a.ks > 1;
+    const int h = lane >> 5;
+    float bias[NT];
+#pragma unroll
+    for (int nt = 0; nt < NT; nt++) {
+        const int64_t col = (int64_t)(tile0 + 2 * nt) * kTile + (lane & 31);
+        bias[nt] = a.bias && !slab && col < a.n ? a.bias[col] : 0.f;
+    }
+    auto store = [&](auto *y, auto &&as) {
+#pragma unroll
+        for (int mt = 0; mt < MT; mt++) {
+            const int row0 = (at.rb * MT + mt) * 32 + 4 * h;
+#pragma unroll
+            for (int nt = 0; nt < NT; nt++) {
+                const int64_t col = (int64_t)(tile0 + 2 * nt) * kTile + (lane & 31);
+                if (col >= a.n) continue;
+                auto *p = y + (int64_t)row0 * a.n + col;
+#pragma unroll
+                for (int e = 0; e < 16; e++) {
+                    if (row0 + 8 * (e / 4) + e % 4 < a.m) *p = as(acc[mt][nt][e] + bias[nt]);
+                    p += e % 4 == 3 ? 5 * a.n : a.n;
+                }
+            }
+        }
+    };
+    if (!slab && a.y_bf16)
+        store(reinterpret_cast<uint16_t *>(a.y), [](float v) { return (uint16_t)f32_to_bf16_bits(v); });
+    else
+        store(reinterpret_cast<float *>(a.y) + (slab ? (int64_t)at.kp * a.m * a.n : 0), [](float v) { return v; });
+}
+
+template <int MT, int NT>
+__device__ __forceinline__ void mx_clear(floatx16 (&acc)[MT][NT]) {
+#pragma unroll
+    for (int mt = 0; mt < MT; mt++)
+#pragma unroll
+        for (int nt = 0; nt < NT; nt++)
+#pragma unroll
+            for (int e = 0; e < 16; e++) acc[mt][nt][e] = 0.f;
+}
+
+// LDS of an A piece: row r's 16-byte chunk c (columns 8c .. 8c + 7 of the unit) at r * 256 + (c ^ r % 16) * 16: a copy
+// moves whole 256-byte rows, and the 16 lanes that read one chunk of 16 rows together find it in 16 different
+// places of the banks.
+template <int MT, int NT, int P>
+__global__ __launch_bounds__(W * 64, 2) void mx_gemm16_kernel(MxGemmArgs a) {
+    constexpr int BUF = MT * P * kPiece, NA = BUF / (W * 1024);  // copies of a wave and unit
+    extern __shared__ __attribute__((aligned(16))) uint8_t lds[];
+    const int tid = threadIdx.x, lane = tid & 63;
+    const int wv = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const MxPlace at(a);
+    const int tile0 = (at.cb * W + wv) * 2 * NT;
+    const MxBLoad<NT> bl(a, tile0, lane);
+    // Copy i of a wave: rows 4 (i W + wv) .. + 3 of the pieces [plane][row tile][32 rows].  Rows past m belong to the
+    // next plane or lie past the buffer (zeros); they are not stored.
+    const int k = (int)a.k;
+    const int64_t plane = (int64_t)a.m * k * 2;
+    const __amdgpu_buffer_rsrc_t xb = rsrc(a.x, P * plane);
+    const int l16 = lane >> 4, swz = ((lane & 15) ^ ((4 * wv + l16) & 15)) * 8;  // (W = 4: row % 16 is the same for every i)
+    auto copy_a = [&](int u, int buf) {
+        const bool in = u * kMxUnit + swz < k;
+#pragma unroll
+        for (int i = 0; i < NA; i++) {
+            const int row = 4 * (i * W + wv), pl = row / (MT * 32);
+            const int off = ((at.rb * MT * 32 + row % (MT * 32) + l16) * k + swz) * 2;
+            copy16_lds(xb, lds + buf * BUF + (i * W + wv) * 1024, in ? off : 0x7FFFFFF0, pl * (int)plane + u * kMxUnit * 2);
+        }
+    };
+    const int c32 = lane & 31, h = lane >> 5;
+    floatx16 acc[MT][NT];
+    mx_clear(acc);
+    MxB<NT> b[2];
+    copy_a(at.u0, 0);
+    bl.load(at.u0, lane, b[0]);
+    auto unit = [&](auto parity, int u) {
+        constexpr int buf = decltype(parity)::value;
+        arrive();
+        const int next = min(u + 1, at.u1 - 1);
+        copy_a(next, buf ^ 1);
+        bl.load(next, lane, b[buf ^ 1]);
+#pragma unroll
+        for (int s = 0; s < 8; s++) {
+            // step s: word s / 2 of blocks 2 (s % 2) + h
+            const int chunk = (2 * (s & 1) + h) * 4 + (s >> 1);
+            u32x4 af[P][MT], bf[NT];
+#pragma unroll
+            for (int p = 0; p < P; p++)
+#pragma unroll
+                for (int mt = 0; mt < MT; mt++)
+                    af[p][mt] = *reinterpret_cast<const u32x4 *>(lds + buf * BUF + (p * MT + mt) * kPiece + c32 * 256 + ((chunk ^ (c32 & 15)) << 4));
+#pragma unroll
+            for (int nt = 0; nt < NT; nt++) bf[nt] = mx_codes_bf16(b[buf].q[nt][s & 1][s >> 1], mx_scale(b[buf].s[nt][s & 1]));
+            // (the lo plane first: added to a finished hi sum its low bits would be cut off)
+#pragma unroll
+            for (int p = P - 1; p >= 0; p--)
+#pragma unroll
+                for (int mt = 0; mt < MT; mt++)
+#pragma unroll
+                    for (int nt = 0; nt < NT; nt++) acc[mt][nt] = mfma32_bf16(af[p][mt], bf[nt], acc[mt][nt]);
+        }
+    };
+    int u = at.u0;
+    for (; u + 1 < at.u1; u += 2) {
+        unit(std::integral_constant<int, 0>(), u);
+        unit(std::integral_constant<int, 1>(), u + 1);
+    }
+    if (u < at.u1) unit(std::integral_constant<int, 0>(), u);
+    mx_store(a, at, tile0, lane, acc);
+}
+
+template <int MT, int NT>
+__global__ __launch_bounds__(W * 64, 2) void mx_gemm4_kernel(MxGemmArgs a) {
+    constexpr int REC = 2 * MT;                   // records (16-row tiles) of a unit
+    constexpr int SC = (REC + 3) / 4 * 256;       // their scales: a copy holds four records'
+    constexpr int BUF = REC * 1024 + SC;
+    extern __shared__ __attribute__((aligned(16))) uint8_t lds[];
+    const int tid = threadIdx.x, lane = tid & 63;
+    const int wv = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const MxPlace at(a);
+    const int tile0 = (at.cb * W + wv) * 2 * NT;
+    const MxBLoad<NT> bl(a, tile0, lane);
+    const int mtiles = (a.m + 15) / 16, bytes = a.units * kMxRecord;
+    const __amdgpu_buffer_rsrc_t xb = rsrc(a.x, (int64_t)mtiles * bytes);
+    // (row tiles past the last: the last one again, not stored)
+    auto copy_a = [&](int u, int buf) {
+#pragma unroll
+        for (int i = 0; i < (REC + W - 1) / W; i++) {
+            const int rec = i * W + wv;
+            if (rec < REC)
+                copy16_lds(xb, lds + buf * BUF + rec * 1024, 16 * lane, min(at.rb * REC + rec, mtiles - 1) * bytes + u * kMxRecord);
+        }
+        if (wv < SC / 256) {
+            const int rec = min(at.rb * REC + min(4 * wv + (lane >> 4), REC - 1), mtiles - 1);
+#if defined(__HIP_DEVICE_COMPILE__)
+            __builtin_amdgcn_raw_ptr_buffer_load_lds(xb, (__attribute__((address_space(3))) void *)(lds + buf * BUF + REC * 1024 + wv * 256), 4,
+                                                     rec * bytes + 1024 + 4 * (lane & 15), u * kMxRecord, 0, 0);
+#endif
+        }
+    };
+    const int b16 = (lane >> 4) & 1, slot = 16 * (lane >> 5) + (lane & 15);
+    floatx16 acc[MT][NT];
+    mx_clear(acc);
+    MxB<NT> b[2];
+    copy_a(at.u0, 0);
+    bl.load(at.u0, lane, b[0]);
+    auto unit = [&](auto parity, int u) {
+        constexpr int buf = decltype(parity)::value;
+        arrive();
+        const int next = min(u + 1, at.u1 - 1);
+        copy_a(next, buf ^ 1);
+        bl.load(next, lane, b[buf ^ 1]);
+#pragma unroll
+        for (int i = 0; i < 2; i++) {
+            u32x4 af[MT];
+            uint32_t as[MT];
+#pragma unroll
+            for (int mt = 0; mt < MT; mt++) {
+                af[mt] = *reinterpret_cast<const u32x4 *>(lds + buf * BUF + (2 * mt + b16) * 1024 + 512 * i + 16 * slot);
+                as[mt] = lds[buf * BUF + REC * 1024 + (2 * mt + b16) * 64 + 32 * i + slot];
+            }
+#pragma unroll
+            for (int mt = 0; mt < MT; mt++)
+#pragma unroll
+                for (int nt = 0; nt < NT; nt++) acc[mt][nt] = mfma32_mx(af[mt], as[mt], b[buf].q[nt][i], b[buf].s[nt][i], acc[mt][nt]);
+        }
+    };
+    int u = at.u0;
+    for (; u + 1 < at.u1; u += 2) {
+        unit(std::integral_constant<int, 0>(), u);
+        unit(std::integral_constant<int, 1>(), u + 1);
+    }
+    if (u < at.u1) unit(std::integral_constant<int, 0>(), u);
+    mx_store(a, at, tile0, lane, acc);
+}
+
+template <int MT, int NT, int P>
+int launch16(const MxGemmArgs &a, void *stream) {
+    constexpr size_t lds = 2 * MT * P * kPiece;
+    auto *kernel = mx_gemm16_kernel<MT, NT, P>;
+    hipError_t e = allow_lds(reinterpret_cast<const void *>(kernel), lds);
+    if (e != hipSuccess) return (int)e;
+    hipLaunchKernelGGL(kernel, dim3((unsigned)(a.row_blocks * a.col_blocks * a.ks)), dim3(W * 64), lds, (hipStream_t)stream, a);
+    return (int)hipGetLastError();
+}
+template <int MT, int NT>
+int launch4(const MxGemmArgs &a, void *stream) {
+    constexpr size_t lds = 2 * (2 * MT * 1024 + (2 * MT + 3) / 4 * 256);
+    hipLaunchKernelGGL((mx_gemm4_kernel<MT, NT>), dim3((unsigned)(a.row_blocks * a.col_blocks * a.ks)), dim3(W * 64), lds,
+                       (hipStream_t)stream, a);
+    return (int)hipGetLastError();
+}
+
+}  // namespace
+
+int launch_mx_gemm(const MxArgs &a, void *scratch, void *stream) {
+    const MxGemmPlan p = mx_gemm_plan(a.m, a.n, a.k, a.x_kind);
+    if (a.m < 1 || a.m > INT32_MAX / 2 || a.units < 1 || (p.bytes && !scratch)) return (int)hipErrorInvalidValue;
+    uint8_t *base = reinterpret_cast<uint8_t *>(scratch);
+    float *slabs = reinterpret_cast<float *>(base + p.slabs);
+    MxGemmArgs g{};
+    g.w = a.w;
+    g.x = reinterpret_cast<const uint8_t *>(a.x);
+    g.bias = a.bias;
+    g.y = p.ks > 1 ? (void *)slabs : a.y;
+    g.y_bf16 = a.y_bf16;
+    g.m = (int)a.m;
+    g.units = (int)a.units;
+    g.ntile = (int)a.ntile;
+    g.ks = p.ks;
+    g.row_blocks = p.row_blocks;
+    g.col_blocks = p.col_blocks;
+    g.n = a.n;
+    g.k = a.k;
+    int e = 0;
+    if (a.x_kind != kMxBf16) {
+        if (a.x_kind == kMxF32) e = launch_mx_split(reinterpret_cast<const float *>(a.x), a.m * a.k, reinterpret_cast<uint16_t *>(base), stream);
+        else if (a.x_kind == kMxCodes) e = launch_mx_repack(reinterpret_cast<const uint8_t *>(a.x), a.xs, a.m, a.k, base, nullptr, stream);
+        else e = launch_mx_quantize_image(a.x, a.x_kind == kMxQuantBf16, a.m, a.k, a.floor_rule, base, stream);
+        if (e) return e;
+        g.x = base;
+    }
+    if (a.x_kind == kMxBf16) e = p.mt == 1 ? launch16<1, 2, 1>(g, stream) : launch16<2, 2, 1>(g, stream);
+    else if (a.x_kind == kMxF32) e = launch16<1, 2, 3>(g, stream);
+    else e = p.mt == 1 ? launch4<1, 2>(g, stream) : p.mt == 2 ? launch4<2, 2>(g, stream) : launch4<4, 2>(g, stream);
+    if (e || p.ks == 1) return e;
+    return launch_int4_sum(slabs, p.ks, a.m, a.n, a.bias, a.y, a.y_bf16, stream);
+}
+
+}  // namespace nnq

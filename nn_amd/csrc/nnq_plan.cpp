@@ -130,6 +130,114 @@ int64_t int4_chunk_rows(int64_t m, int64_t k) {
     return std::min(m, std::max<int64_t>(128, std::min<int64_t>(rows, 65536)));
 }
 
+// ---- MXFP4 rows ----
+
+bool mx_takes_rows(int64_t m, int64_t n, int64_t k, int x_kind) { return m <= kMxRows; }
+
+// f32 x of up to five rows is split into its bf16 planes by the kernel that uses it, of more by one launch before it
+MxRowsPlan mx_rows_plan(int64_t m, int64_t n, int64_t k, int x_kind) {
+    MxRowsPlan p{};
+    p.ks = 1;
+    p.planes = x_kind == kMxF32 && m > 5;
+    p.slabs = p.planes ? align256((size_t)m * (size_t)k * 6) : 0;
+    p.bytes = p.slabs + (p.ks > 1 ? (size_t)p.ks * (size_t)m * (size_t)n * 4 : 0);
+    return p;
+}
+
+MxGemmPlan mx_gemm_plan(int64_t m, int64_t n, int64_t k, int x_kind) {
+    MxGemmPlan p{};
+    const bool four = x_kind >= kMxQuantBf16;
+    const int64_t tiles = (m + 31) / 32;
+    p.nt = 2;
+    p.mt = x_kind == kMxF32 ? 1 : tiles == 1 ? 1 : four && tiles > 2 ? 4 : 2;
+    p.ks = 1;
+    p.row_blocks = (int)((tiles + p.mt - 1) / p.mt);
+    p.col_blocks = (int)((n + 128 * p.nt - 1) / (128 * p.nt));
+    const size_t x = four ? (size_t)(mx_tiles(m) * mx_units(k)) * kMxRecord : x_kind == kMxF32 ? (size_t)m * (size_t)k * 6 : 0;
+    p.slabs = align256(x);
+    p.bytes = p.slabs + (p.ks > 1 ? (size_t)p.ks * (size_t)m * (size_t)n * 4 : 0);
+    return p;
+}
+
+// launches whose x the kernels reach with 32-bit offsets (three bf16 planes: 6 bytes a value), whole 128-row tiles
+int64_t mx_chunk_rows(int64_t m, int64_t k) {
+    const int64_t rows = ((int64_t)1 << 30) / (6 * (k + kMxUnit)) / 128 * 128;
+    return std::min(m, std::max<int64_t>(128, std::min<int64_t>(rows, 65536)));
+}
+
+size_t mx_linear_scratch(int64_t m, int64_t n, int64_t k, int x_kind) {
+    const int64_t mc = mx_chunk_rows(m, k), tail = m % mc;
+    auto launch = [&](int64_t r) { return mx_takes_rows(r, n, k, x_kind) ? mx_rows_plan(r, n, k, x_kind).bytes : mx_gemm_plan(r, n, k, x_kind).bytes; };
+    return std::max(launch(mc), tail ? launch(tail) : 0);
+}
+
+// ---- beam search ----
+
+// Segments of 2048 logits, four waves to a workgroup; a launch's rows fit its grid and its scratch stays near 64 MiB.
+BeamPlan beam_plan(int64_t batch, int beams, int64_t n, int keep) {
+    BeamPlan p{};
+    p.nseg = ((n + 2047) / 2048 + 3) / 4 * 4;
+    p.slots = std::min(64, (keep + keep / 2 + 6 + 3) / 4 * 4);
+    const int64_t per = beams * p.nseg * (16 + 8 * (int64_t)p.slots);
+    p.items = std::max<int64_t>(1, std::min({batch, ((int64_t)64 << 20) / per, (int64_t)65535 / beams}));
+    p.bytes = (size_t)(p.items * per);
+    return p;
+}
+
+const char *reorder_geometry(int64_t slots, int64_t slot_stride, int ndim, const int64_t *sizes, const int64_t *strides,
+                             int64_t elem, uintptr_t address_bits, ReorderArgs *out) {
+    struct Dim {
+        int64_t size, stride;
+    };
+    Dim d[16], all[17];
+    int n = 0;
+    out->pieces = 0;
+    out->dims = 0;
+    for (int i = 0; i < ndim; i++) {
+        if (sizes[i] < 0 || strides[i] < 0) return "negative size or stride";
+        if (sizes[i] == 0) return nullptr;  // (no pieces)
+        if (sizes[i] > 1) d[n++] = Dim{sizes[i], strides[i] * elem};
+    }
+    std::sort(d, d + n, [](const Dim &a, const Dim &b) { return a.stride > b.stride; });
+    // elements that lie apart: each stride covers what the smaller ones span
+    for (int i = 0; i < n; i++) all[i] = d[i];
+    all[n] = Dim{slots, slot_stride * elem};
+    std::sort(all, all + n + 1, [](const Dim &a, const Dim &b) { return a.stride < b.stride; });
+    int64_t span = elem;
+    for (int i = 0; i <= n; i++) {
+        if (all[i].size <= 1) continue;
+        if (all[i].stride < span) return "elements that overlap";
+        if (__builtin_mul_overflow(all[i].stride, all[i].size - 1, &all[i].size) || __builtin_add_overflow(span, all[i].size, &span))
+            return "a span beyond 2^63 bytes";
+    }
+    // dims that follow one another are one
+    Dim c[17];
+    int m = 0;
+    c[m++] = Dim{elem, 1};  // bytes of an element, innermost
+    for (int i = n - 1; i >= 0; i--) {
+        if (d[i].stride == c[m - 1].size * c[m - 1].stride) c[m - 1].size *= d[i].size;
+        else c[m++] = d[i];
+    }
+    if (m > kReorderDims) out->dims = -1;
+    if (m > kReorderDims) return "more than 4 dimensions that do not follow one another";
+    uintptr_t bits = address_bits | (uintptr_t)c[0].size | (uintptr_t)(slots > 1 ? slot_stride * elem : 0);
+    for (int i = 1; i < m; i++) bits |= (uintptr_t)c[i].stride;
+    out->vec = bits & 1 ? 1 : bits & 2 ? 2 : bits & 4 ? 4 : bits & 8 ? 8 : 16;
+    out->slot_stride = slot_stride * elem;
+    out->dims = m;
+    out->pieces = 1;
+    for (int i = 0; i < kReorderDims; i++) {
+        out->size[i] = 1;
+        out->stride[i] = 0;
+    }
+    for (int i = 0; i < m; i++) {  // innermost last
+        out->size[kReorderDims - 1 - i] = i ? c[i].size : c[0].size / out->vec;
+        out->stride[kReorderDims - 1 - i] = i ? c[i].stride : out->vec;
+        out->pieces *= out->size[kReorderDims - 1 - i];
+    }
+    return nullptr;
+}
+
 // Rows of 2048-logit segments (one wave each, four to a workgroup; a row that does not start at a
 // 16-byte address begins inside its first segment, by up to 16 / elem - 1 logits).  The candidate
 // slots leave room over the 1.1 to 1.4 top that continuous logits fill.  A launch takes at most

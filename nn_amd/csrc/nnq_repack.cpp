@@ -89,6 +89,22 @@ bool make_layout_int4(int64_t n, int64_t k, int64_t group, int zeros, int scale_
     return true;
 }
 
+bool make_layout_mxfp4(int64_t n, int64_t k, Layout *L, const char **err) {
+    *L = Layout{};
+    if (k % 32) {
+        *err = "in_features must be a multiple of 32";
+        return false;
+    }
+    L->fmt = NNQ_FMT_MXFP4;
+    L->layout = NNQ_LAYOUT_ROWS;
+    L->n = n;
+    L->k = k;
+    L->ntile = mx_tiles(n);
+    L->nblk = mx_units(k);
+    L->qs_bytes = (size_t)L->ntile * L->nblk * kMxRecord;
+    return true;
+}
+
 // A pair of columns (2i, 2i + 1) of a lane's 8 sits at bits 4i and 16 + 4i, so that masking a
 // word, or the word shifted right by 8, with 0x000F000F or 0x00F000F0 leaves one pair as the
 // low mantissa bits of two f16.  Columns past k and rows past n have codes, scales and zero

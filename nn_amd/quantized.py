@@ -143,6 +143,7 @@ class Layout(enum.IntEnum):
     GPTOSS = 2     # GPT-OSS Mxfp4Tensor
     OCP = 3        # nn-core Mxfp4Block / Mxfp4Tensor (17-byte blocks, low nibble first)
     GROUPS = 4     # INT4G: codes, scales and zero points in arrays of their own
+    ROWS = 5       # MXFP4 linear weights: codes and scales of [n, k], blocks along k
 
 
 _DTYPE = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}
@@ -320,6 +321,31 @@ class QuantizedWeight:
                 _check(_lib.load().nnq_weight_create_int4(*args))
         return cls(h, QuantType.INT4G, Layout.GROUPS, (n, k), device)
 
+    @classmethod
+    def from_mxfp4_rows(cls, codes: torch.Tensor, scales: torch.Tensor, device: int = 0) -> "QuantizedWeight":
+        """W[r, j] = e2m1(code[r, j]) * 2^(scale[r, j // 32] - 127): MXFP4 with blocks along in_features, the form
+        of ``quantize_mxfp4_rows`` and of checkpoints (the MXFP4 experts' blocks run along the output).
+
+        codes: uint8 [out_features, in_features / 2], two to a byte with the even column in the low half; scales:
+        uint8 [out_features, in_features / 32], up to 252; in_features at most 2^20.  The tensors are copied.
+        ``quantized_linear`` and the calls beside it keep x in full precision, ``mxfp4_linear`` quantizes it."""
+        codes, scales = _mxfp4_rows(codes, scales)
+        if codes.dim() != 2:
+            raise WeightRank(f"codes must be 2-D [out_features, in_features / 2], got rank {codes.dim()}")
+        n, k = codes.shape[0], 2 * codes.shape[1]
+        if n == 0 or k == 0:
+            raise InvalidShape(f"weight [{n}, {k}]")
+        where = torch.device("cuda", device) if codes.is_cuda else torch.device("cpu")
+        c, s = (t.detach().to(where).contiguous() for t in (codes, scales))
+        init(device)
+        with torch.cuda.device(device):
+            h = ctypes.c_void_p()
+            if codes.is_cuda:
+                _check(_lib.load().nnq_weight_create_mxfp4_device(_ptr(c), _ptr(s), n, k, ctypes.byref(h), _stream(c)))
+            else:
+                _check(_lib.load().nnq_weight_create_mxfp4(_ptr(c), _ptr(s), n, k, ctypes.byref(h)))
+        return cls(h, QuantType.MXFP4, Layout.ROWS, (n, k), device)
+
     def __del__(self):
         h = getattr(self, "_h", None)
         if h is not None and h.value:
@@ -378,6 +404,122 @@ def quantized_linear(input: torch.Tensor, weight: QuantizedWeight, bias: Optiona
     m = x.numel() // k
     _launch(x, _lib.load().nnq_linear, weight.handle, _ptr(x), _DTYPE[x.dtype], m, k, _ptr(bias),
             n if bias is not None else 0, _ptr(y), _DTYPE[out_dtype])
+    return y
+
+
+# ---------------------------------------------------------------------------------
+# MXFP4 rows
+# ---------------------------------------------------------------------------------
+
+_SCALE_RULES = {"ceil": 0, "floor": 1}
+
+
+def _mxfp4_rows(codes, scales):
+    for t, what in ((codes, "codes"), (scales, "scales")):
+        if not isinstance(t, torch.Tensor):
+            raise Unsupported(f"{what} must be a tensor")
+        if t.dtype != torch.uint8:
+            raise Unsupported(f"{what} must be uint8, got {t.dtype}")
+    if codes.dim() < 1 or codes.shape[-1] % 16:
+        raise InvalidShape(f"codes {list(codes.shape)} are not whole blocks of 32 (16 bytes) along the last dimension")
+    if tuple(scales.shape) != (*codes.shape[:-1], codes.shape[-1] // 16):
+        raise ShapeMismatch(f"scales must be {[*codes.shape[:-1], codes.shape[-1] // 16]}, got {list(scales.shape)}")
+    return codes, scales
+
+
+def _scale_rule(rule) -> int:
+    if rule not in _SCALE_RULES:
+        raise TensorError(f"scale rule {rule!r} (\"ceil\" or \"floor\")")
+    return _SCALE_RULES[rule]
+
+
+class Mxfp4Rows(NamedTuple):
+    """Device rows in MXFP4 (``quantize_mxfp4_rows``): value j of a row is e2m1(code j) * 2^(scale[j // 32] - 127)."""
+    codes: torch.Tensor   # uint8 [..., k / 2], two to a byte with the even column in the low half
+    scales: torch.Tensor  # uint8 [..., k / 32]; 255: the block is NaN
+
+    def dequantize(self, dtype: torch.dtype = torch.float32) -> torch.Tensor:
+        """The values, exact in f32 and in bf16."""
+        codes, scales = _mxfp4_rows(self.codes, self.scales)
+        _device_input(codes, "codes")
+        _device_input(scales, "scales", codes.device.index)
+        if dtype not in (torch.float32, torch.bfloat16):
+            raise Unsupported(f"output dtype {dtype} (float32 or bfloat16)")
+        out = torch.empty((*codes.shape[:-1], 2 * codes.shape[-1]), dtype=dtype, device=codes.device)
+        if out.numel():
+            c, s = _aligned(codes.contiguous(), 4), scales.contiguous()
+            k = out.shape[-1]
+            _launch(out, _lib.load().nnq_mxfp4_dequantize, _ptr(c), _ptr(s), out.numel() // k, k, _ptr(out), _DTYPE[dtype])
+        return out
+
+
+def _aligned(t: torch.Tensor, by: int) -> torch.Tensor:
+    return t.clone() if t.data_ptr() % by else t
+
+
+def quantize_mxfp4_rows(x: torch.Tensor, scale_rule: str = "ceil") -> Mxfp4Rows:
+    """Device x [..., k] (f32, bf16, others widened to f32; k a multiple of 32) to MXFP4 with blocks of 32 along k.
+
+    The scale 2^s of a block whose largest magnitude is m: with "ceil" the smallest with m <= 6 * 2^s (as
+    ``quantize_mxfp4_ocp``), with "floor" 2^(floor(log2 m) - 2), where values over 6 * 2^s become that.  Codes are the
+    nearest, halves to even.  A block with NaN or an infinity becomes NaN (scale 255).  No host synchronisation."""
+    rule = _scale_rule(scale_rule)
+    _device_input(x, "x")
+    if x.dim() < 1 or x.shape[-1] == 0 or x.shape[-1] % 32:
+        raise InvalidShape(f"x {list(x.shape)}: the last dimension must be a positive multiple of 32")
+    if x.dtype not in (torch.float32, torch.bfloat16):
+        x = x.float()
+    k = x.shape[-1]
+    v = x if x.dim() <= 2 else x.reshape(-1, k)
+    if v.stride(-1) != 1:
+        v = v.contiguous()
+    codes = torch.empty((*x.shape[:-1], k // 2), dtype=torch.uint8, device=x.device)
+    scales = torch.empty((*x.shape[:-1], k // 32), dtype=torch.uint8, device=x.device)
+    _launch(v, _lib.load().nnq_mxfp4_quantize, _ptr(v), _DTYPE[v.dtype], x.numel() // k, k, v.stride(0) if v.dim() == 2 else k,
+            rule, _ptr(codes), _ptr(scales))
+    return Mxfp4Rows(codes, scales)
+
+
+def mxfp4_linear(input, weight: QuantizedWeight, bias: Optional[torch.Tensor] = None,
+                 out_dtype: Optional[torch.dtype] = None, scale_rule: str = "ceil") -> torch.Tensor:
+    """``y = q(input) @ weight^T + bias`` for a weight of ``QuantizedWeight.from_mxfp4_rows``, q the quantization of
+    ``quantize_mxfp4_rows``: both operands of the product in 4 bits, sums in f32.  ``input``: [..., in_features] (f32,
+    bf16, others widened to f32), or ``Mxfp4Rows`` quantized before.  Output dtype as ``quantized_linear``.  A row with
+    NaN or an infinity gives a row of NaN."""
+    if not isinstance(weight, QuantizedWeight):
+        raise NotQuantized("mxfp4_linear: weight is not quantized")
+    if weight.quant_type != QuantType.MXFP4:
+        raise WrongQuantType(f"mxfp4_linear needs an MXFP4 weight, got {weight.quant_type.name}")
+    rule = _scale_rule(scale_rule)
+    n, k = weight.shape
+    rows = isinstance(input, Mxfp4Rows)
+    if rows:
+        codes, scales = _mxfp4_rows(*input)
+        if codes.dim() < 2:
+            raise RankMismatch(f"expected rank >= 2, got {codes.dim()}")
+        if 2 * codes.shape[-1] != k:
+            raise ShapeMismatch(f"quantized matmul shape mismatch: input last dim {2 * codes.shape[-1]} != weight in_features {k}")
+        x = _aligned(_device_input(codes, "codes", weight.device).contiguous(), 16)
+        scales = _device_input(scales, "scales", weight.device).contiguous()
+        m = x.numel() // (k // 2)
+    else:
+        x = _validate_input(input, k, weight.device)
+        m = x.numel() // k
+    if bias is not None:
+        if bias.dim() != 1 or bias.shape[0] != n:
+            raise BiasMismatch(f"bias shape mismatch: expected [{n}], got {list(bias.shape)}")
+        bias = _side_input(bias, x)
+    out_dtype = out_dtype or torch.float32
+    if out_dtype not in (torch.float32, torch.bfloat16):
+        raise Unsupported(f"output dtype {out_dtype} (float32 or bfloat16)")
+    y = x.new_empty((*x.shape[:-1], n), dtype=out_dtype)
+    nb = n if bias is not None else 0
+    if rows:
+        _launch(x, _lib.load().nnq_mxfp4_linear_codes, weight.handle, _ptr(x), _ptr(scales), m, k, _ptr(bias), nb, _ptr(y),
+                _DTYPE[out_dtype])
+    else:
+        _launch(x, _lib.load().nnq_mxfp4_linear, weight.handle, _ptr(x), _DTYPE[x.dtype], m, k, rule, _ptr(bias), nb, _ptr(y),
+                _DTYPE[out_dtype])
     return y
 
 
@@ -583,6 +725,105 @@ def linear_logprobs(x: torch.Tensor, weight: QuantizedWeight, tokens, bias: Opti
     _launch(xv, _lib.load().nnq_linear_logprobs, weight.handle, _ptr(xv), _DTYPE[xv.dtype], rows, k, _ptr(bias),
             n if bias is not None else 0, _ptr(tok), int(top_n), _ptr(logits), *ptrs)
     return out._replace(logits=logits)
+
+
+# ---------------------------------------------------------------------------------
+# beam search
+# ---------------------------------------------------------------------------------
+
+
+class BeamSelection(NamedTuple):
+    """The continuations that a beam search keeps (see ``beam_select``)."""
+    scores: torch.Tensor   # f32 [..., keep], descending
+    parents: torch.Tensor  # int64 [..., keep]: the beam that is continued; -1: none
+    tokens: torch.Tensor   # int64 [..., keep]
+
+
+def beam_select(logits: torch.Tensor, scores: torch.Tensor, keep: Optional[int] = None,
+                finished: Optional[torch.Tensor] = None, end_token: int = 0) -> BeamSelection:
+    """One step of a beam search: of all continuations of each item's beams the ``keep`` (up to 32; default: as many as
+    beams) with the largest scores[..., j] + log_softmax(logits[..., j, :])[token], in descending order, equal ones by
+    beam, then token.  No host synchronisation.
+
+    logits: device [..., beams, n] (f32, bf16 or f16; beams up to 32; beams and items may be strided); scores [..., beams]
+    in f32, sums of log probabilities (at the first step 0 for one beam and -inf for the rest).  finished: bool [...,
+    beams]: such a beam has one continuation, by ``end_token``, with its score unchanged.  A beam whose score is not
+    finite offers nothing, nor does one whose logits hold NaN or +inf; a logit of -inf is no continuation.  Places that
+    are left have parent and token -1 and score -inf."""
+    _device_input(logits, "logits")
+    if logits.dim() < 2 or logits.shape[-1] == 0:
+        raise InvalidShape(f"logits must be [..., beams, n], got {list(logits.shape)}")
+    if logits.dtype not in _DTYPE:
+        logits = logits.float()
+    batch, beams, n = logits.shape[:-2], logits.shape[-2], logits.shape[-1]
+    if not isinstance(scores, torch.Tensor) or scores.shape != logits.shape[:-1]:
+        raise ShapeMismatch(f"scores must be a tensor {[*batch, beams]}, one per row of logits")
+    if scores.is_complex():
+        raise Unsupported(f"scores must be real, got {scores.dtype}")
+    keep = beams if keep is None else int(keep)
+    if not 1 <= beams <= 32 or not 1 <= keep <= 32:
+        raise InvalidShape(f"{beams} beams, keep {keep} (1 to 32 each)")
+    s = _side_input(scores, logits)
+    f = None
+    if finished is not None:
+        if not isinstance(finished, torch.Tensor) or finished.shape != scores.shape or finished.dtype is not torch.bool:
+            raise ShapeMismatch(f"finished must be a bool tensor {[*batch, beams]}")
+        if int(end_token) < 0:
+            raise TensorError(f"end token {end_token}")
+        f = finished.to(logits.device).contiguous()
+    v = logits if logits.dim() in (2, 3) else logits.reshape(-1, beams, n)
+    if v.stride(-1) != 1 and n > 1:
+        v = v.contiguous()
+    items = v.shape[0] if v.dim() == 3 else 1
+    out = torch.empty((*batch, keep), dtype=torch.float32, device=v.device)
+    parents, tokens = torch.empty((2, *batch, keep), dtype=torch.int64, device=v.device).unbind(0)
+    _launch(v, _lib.load().nnq_beam_select, _ptr(v), _DTYPE[v.dtype], items, beams, n, v.stride(0) if v.dim() == 3 else 0,
+            v.stride(-2), _ptr(s), _ptr(f), int(end_token), keep, _ptr(out), _ptr(parents), _ptr(tokens))
+    return BeamSelection(out, parents, tokens)
+
+
+def beam_reorder(states, parents: torch.Tensor, dim: int = 0) -> None:
+    """The states that follow a step: slot b * beams + j along ``dim`` of each state becomes a copy of slot
+    b * beams + parents[b, j], in place, whatever the parents are (all reads come before the writes).
+
+    states: a device tensor or several on one device, of any dtypes, which must not overlap; strided ones are written where
+    they lie, so ``cache[..., :used, :]`` moves the used part only.  parents: integers [batch, beams] or [beams] (beams
+    up to 32) on that device; a slot whose parent is itself, or outside [0, beams) as the -1 of ``beam_select``, stays as it
+    is, and only slots that move are read and written.  No host synchronisation."""
+    states = [states] if isinstance(states, torch.Tensor) else list(states)
+    if not isinstance(parents, torch.Tensor) or parents.dim() not in (1, 2):
+        raise ShapeMismatch("parents must be a tensor [batch, beams] or [beams]")
+    if parents.is_floating_point() or parents.is_complex() or parents.dtype == torch.bool:
+        raise Unsupported(f"parents must be integers, got {parents.dtype}")
+    _device_input(parents, "parents")
+    beams = parents.shape[-1]
+    batch = parents.shape[0] if parents.dim() == 2 else 1
+    if not 1 <= beams <= 32:
+        raise InvalidShape(f"{beams} beams (1 to 32)")
+    alike = {}
+    for t in states:
+        _device_input(t, "state")
+        if t.device != parents.device:
+            raise Unsupported(f"state is on {t.device}, parents on {parents.device}")
+        if not -t.dim() <= dim < t.dim():
+            raise RankMismatch(f"a state of rank {t.dim()} has no dimension {dim}")
+        d = dim % t.dim()
+        if t.shape[d] != batch * beams:
+            raise ShapeMismatch(f"state {list(t.shape)} must have {batch} x {beams} slots along dimension {d}")
+        if t.numel():
+            alike.setdefault((t.shape, t.stride(), t.element_size(), d), []).append(t.data_ptr())
+    for ptrs in alike.values():
+        if len(set(ptrs)) != len(ptrs):
+            raise TensorError("a state is given twice")
+    p = parents if parents.dtype is torch.int64 else parents.long()
+    p = p.contiguous()
+    for (shape, stride, elem, d), ptrs in alike.items():
+        sizes, strides = [*shape[:d], *shape[d + 1:]], [*stride[:d], *stride[d + 1:]]
+        if len(sizes) > 8:
+            raise Unsupported(f"a state of rank {len(shape)} (at most 9)")
+        i64s = ctypes.c_int64 * len(sizes)
+        _launch(p, _lib.load().nnq_beam_reorder, (ctypes.c_void_p * len(ptrs))(*ptrs), len(ptrs), batch, beams, stride[d], len(sizes),
+                i64s(*sizes), i64s(*strides), elem, _ptr(p))
 
 
 # ---------------------------------------------------------------------------------
