@@ -275,11 +275,12 @@ int launch_int4_dequant(const Layout &L, const uint8_t *w, float *out, void *str
 
 // ---- MXFP4 rows (nnq_mxfp4.hip, nnq_mxfp4_gemm.hip) ---------------------------------
 constexpr int kMxUnit = 128;      // k of one unit
-constexpr int kMxRecord = 1088;   // bytes of a record: 16 rows of a unit, codes and scales
+constexpr int kMxPair = 2176;     // bytes of a record: 16 rows of two units, codes (2 x 1024) and scales (128)
 constexpr int kMxScaleMax = 252;  // the largest scale byte of a weight: 6 * 2^125 is finite in f32
 constexpr int64_t kMxMaxK = (int64_t)1 << 20;
 constexpr int kMxRows = 16;       // the most token rows of one launch_mx_rows
 inline int64_t mx_units(int64_t k) { return (k + kMxUnit - 1) / kMxUnit; }
+inline int64_t mx_pairs(int64_t k) { return (k + 2 * kMxUnit - 1) / (2 * kMxUnit); }
 inline int64_t mx_tiles(int64_t rows) { return (rows + kTile - 1) / kTile; }
 bool make_layout_mxfp4(int64_t n, int64_t k, Layout *out, const char **err);
 // x of a linear: as it is, to be quantized, or codes with their scales

@@ -3,10 +3,12 @@
 // weights, and the linears of one to sixteen token rows:
 //   y[t][r] = sum_k W[r][k] x[t][k] (+ bias[r]),  x as it is (bf16 products) or quantized to MXFP4 too.
 //
-// Image: 16-row tiles, per (tile, unit of 128 columns) one record of 1088 bytes: lane 16p + r's 16 bytes are block p
-// (columns 32p .. 32p + 31 of the unit) of row r in column order, then 64 scale bytes in the same order.  One 16-byte
-// load a lane is the operand of one 16x16x128 block-scaled MFMA, with the scales as they are, and, block by block
-// turned into bf16, of four 16x16x32 bf16 MFMAs (their k order is that of the lanes, the same for both sides).
+// Image: 16-row tiles, per (tile, pair of units of 128 columns) one record of 2176 bytes: for each unit lane 16p + r's 16
+// bytes, block p (columns 32p .. 32p + 31) of row r in column order; then 32 words of scales, word 16h + r's byte
+// 2 (unit) + i that of block 2i + h of row r.  One 16-byte load a lane is the operand of one 16x16x128 block-scaled MFMA, of
+// a 32x32x64 one (blocks 2i and 2i + 1 of 32 rows; the byte of its scales' word selected by the instruction), and,
+// block by block turned into bf16, of four 16x16x32 bf16 MFMAs (their k order is that of the lanes, the same for both
+// sides).  The unit that fills up the last pair holds zeros.
 #include <algorithm>
 #include <type_traits>
 
@@ -65,6 +67,12 @@ __global__ __launch_bounds__(256) void mx_quantize_kernel(const uint8_t *x, int6
     }
 }
 
+// where lane 16p + r of job (tile, unit; an even number of units a tile) finds its block's codes and scale
+__device__ __forceinline__ int64_t mx_codes_at(int64_t job, int lane) { return (job >> 1) * kMxPair + (job & 1) * 1024 + 16 * lane; }
+__device__ __forceinline__ int64_t mx_scale_at(int64_t job, int lane) {
+    return (job >> 1) * kMxPair + 2048 + 4 * (16 * ((lane >> 4) & 1) + (lane & 15)) + 2 * (job & 1) + (lane >> 5);
+}
+
 // x rows (whole units) to the records of the image, for a product of 4-bit operands: lane 16p + r quantizes block p
 // of row r, as a lane of the kernels below does.
 template <bool BF16>
@@ -85,9 +93,8 @@ __global__ __launch_bounds__(256) void mx_quantize_image_kernel(const uint8_t *x
     }
     uint32_t byte;
     const u32x4 q = mx_quantize_block<BF16>(v, floor_rule, byte);
-    uint8_t *rec = image + job * kMxRecord;
-    *reinterpret_cast<u32x4 *>(rec + 16 * lane) = q;
-    rec[1024 + lane] = (uint8_t)byte;
+    *reinterpret_cast<u32x4 *>(image + mx_codes_at(job, lane)) = q;
+    image[mx_scale_at(job, lane)] = (uint8_t)byte;
 }
 
 // The image of codes and scales that are on the device; one wave per (tile, unit).  Rows and columns past the end:
@@ -106,9 +113,8 @@ __global__ __launch_bounds__(256) void mx_repack_kernel(const uint8_t *codes, co
         s = scales[at];
         if (bad && s > kMxScaleMax) atomicMin(bad, (unsigned long long)at);
     }
-    uint8_t *rec = image + job * kMxRecord;
-    *reinterpret_cast<u32x4 *>(rec + 16 * lane) = q;
-    rec[1024 + lane] = (uint8_t)s;
+    *reinterpret_cast<u32x4 *>(image + mx_codes_at(job, lane)) = q;
+    image[mx_scale_at(job, lane)] = (uint8_t)s;
 }
 
 // rows of codes -> values (f32 or bf16), eight of them a thread; exact but for f32 subnormals below bf16's 2^-133,
@@ -143,9 +149,8 @@ __global__ __launch_bounds__(256) void mx_dequant_image_kernel(const uint8_t *im
     const int lane = threadIdx.x & 63;
     const int64_t row = job / units * kTile + (lane & 15), k0 = job % units * kMxUnit + 32 * (lane >> 4);
     if (row >= n || k0 >= k) return;
-    const uint8_t *rec = image + job * kMxRecord;
-    const u32x4 q = ldg128(rec + 16 * lane);
-    const float s = mx_scale(rec[1024 + lane]);
+    const u32x4 q = ldg128(image + mx_codes_at(job, lane));
+    const float s = mx_scale(image[mx_scale_at(job, lane)]);
 #pragma unroll
     for (int j = 0; j < 4; j++) {
         const u32x4 b = mx_codes_bf16(q[j], s);
@@ -289,16 +294,18 @@ __global__ __launch_bounds__(1024) void mx_rows_kernel(MxArgs a) {
     XOp<XF> x[UPW];
     u32x4 wq[R][UPW];
     uint32_t ws[R][UPW];
+    const int64_t tile_bytes = (int64_t)((units + 1) / 2) * kMxPair;
+    const int ls = 2048 + 4 * (16 * (p4 & 1) + c) + (p4 >> 1);
     // a unit that does not exist is read at the last that does (its x is zeros), a tile that does not exist as a
     // buffer of no bytes
     auto tile_buffer = [&](int b, int r) {
         const int64_t tile = (int64_t)b * R + r;
-        return rsrc(a.w + (size_t)min(tile, a.ntile - 1) * units * kMxRecord, tile < a.ntile ? (int64_t)units * kMxRecord : 0);
+        return rsrc(a.w + min(tile, a.ntile - 1) * tile_bytes, tile < a.ntile ? tile_bytes : 0);
     };
     auto load_w = [&](__amdgpu_buffer_rsrc_t t, int pass, int r, int j) {
-        const int at = min(ub + (pass * UPW + j) * waves + wv, ue - 1) * kMxRecord;
-        wq[r][j] = __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(t, 16 * lane, at, 2));
-        ws[r][j] = __builtin_amdgcn_raw_buffer_load_b8(t, 1024 + lane, at, 2);
+        const int u = min(ub + (pass * UPW + j) * waves + wv, ue - 1), at = (u >> 1) * kMxPair;
+        wq[r][j] = __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(t, 16 * lane, at + (u & 1) * 1024, 2));
+        ws[r][j] = __builtin_amdgcn_raw_buffer_load_b8(t, ls, at + 2 * (u & 1), 2);
     };
     auto load_x = [&](int pass) {
 #pragma unroll
@@ -472,7 +479,7 @@ int launch_mx_dequantize(const uint8_t *codes, const uint8_t *scales, int64_t co
 }
 
 int launch_mx_quantize_image(const void *x, int x_bf16, int64_t m, int64_t k, int floor_rule, uint8_t *image, void *stream) {
-    const int64_t units = mx_units(k), jobs = mx_tiles(m) * units;
+    const int64_t units = 2 * mx_pairs(k), jobs = mx_tiles(m) * units;
     if ((jobs + 3) / 4 > INT32_MAX) return (int)hipErrorInvalidValue;
     const uint8_t *p = reinterpret_cast<const uint8_t *>(x);
     if (x_bf16)
@@ -484,15 +491,15 @@ int launch_mx_quantize_image(const void *x, int x_bf16, int64_t m, int64_t k, in
 
 int launch_mx_repack(const uint8_t *codes, const uint8_t *scales, int64_t n, int64_t k, uint8_t *image,
                      unsigned long long *bad, void *stream) {
-    const int64_t units = mx_units(k), jobs = mx_tiles(n) * units;
+    const int64_t units = 2 * mx_pairs(k), jobs = mx_tiles(n) * units;
     if ((jobs + 3) / 4 > INT32_MAX) return (int)hipErrorInvalidValue;
     hipLaunchKernelGGL(mx_repack_kernel, dim3(wave_jobs(jobs)), dim3(256), 0, (hipStream_t)stream, codes, scales, n, k, units, jobs, image, bad);
     return (int)hipGetLastError();
 }
 
 int launch_mx_dequant_image(const Layout &L, const uint8_t *image, float *out, void *stream) {
-    const int64_t jobs = L.ntile * L.nblk;
-    hipLaunchKernelGGL(mx_dequant_image_kernel, dim3(wave_jobs(jobs)), dim3(256), 0, (hipStream_t)stream, image, L.n, L.k, L.nblk, jobs, out);
+    const int64_t units = 2 * mx_pairs(L.k), jobs = L.ntile * units;
+    hipLaunchKernelGGL(mx_dequant_image_kernel, dim3(wave_jobs(jobs)), dim3(256), 0, (hipStream_t)stream, image, L.n, L.k, units, jobs, out);
     return (int)hipGetLastError();
 }
 

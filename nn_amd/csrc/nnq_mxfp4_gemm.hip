@@ -22,12 +22,22 @@ constexpr int kPiece = 8192;  // bf16 bytes of 32 rows and one unit
 __device__ __forceinline__ floatx16 mfma32_bf16(u32x4 a, u32x4 b, floatx16 c) {
     return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
 }
+template <int BYTE>
 __device__ __forceinline__ floatx16 mfma32_mx(u32x4 a, uint32_t sa, u32x4 b, uint32_t sb, floatx16 c) {
 #if defined(__HIP_DEVICE_COMPILE__)
     const i32x8 av = {(int)a[0], (int)a[1], (int)a[2], (int)a[3], 0, 0, 0, 0}, bv = {(int)b[0], (int)b[1], (int)b[2], (int)b[3], 0, 0, 0, 0};
-    return __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(av, bv, c, 4, 4, 0, (int)sa, 0, (int)sb);
+    return __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(av, bv, c, 4, 4, BYTE, (int)sa, BYTE, (int)sb);
 #else
     return c;
+#endif
+}
+
+// bytes of a stage's A in LDS: 2 mt tiles' codes and the four waves' copies of scales
+constexpr int mx_gemm4_stage(int mt) { return 2 * mt * 2048 + 1024; }
+// 4 bytes a lane from a buffer straight into LDS
+__device__ __forceinline__ void copy4_lds(__amdgpu_buffer_rsrc_t t, uint8_t *lds, int voff, int soff) {
+#if defined(__HIP_DEVICE_COMPILE__)
+    __builtin_amdgcn_raw_ptr_buffer_load_lds(t, (__attribute__((address_space(3))) void *)lds, 4, voff, soff, 0, 0);
 #endif
 }
 
@@ -52,38 +62,38 @@ struct MxPlace {
         rb = t % a.row_blocks;
         cb = t / a.row_blocks % a.col_blocks;
         kp = t / (a.row_blocks * a.col_blocks);
-        u0 = (int)((int64_t)a.units * kp / a.ks);
-        u1 = (int)((int64_t)a.units * (kp + 1) / a.ks);
+        const int64_t pairs = (a.units + 1) / 2;  // parts of K are whole pairs of units
+        u0 = (int)(pairs * kp / a.ks) * 2;
+        u1 = min((int)(pairs * (kp + 1) / a.ks) * 2, a.units);
     }
 };
 
-// A wave's weights of a unit, NT * 32 columns: lane 32h + 16b + r holds row r of tile b, its blocks h and 2 + h.
+// A wave's weights, NT * 32 columns: lane 32h + 16b + r holds row r of tile b of a pair of tiles.
 template <int NT>
-struct MxB {
-    u32x4 q[NT][2];
-    uint32_t s[NT][2];
-};
-template <int NT>
-struct MxBLoad {
+struct MxW {
     __amdgpu_buffer_rsrc_t buf[NT];
-    int off[NT];  // the lane's; tiles past the last are read as the last (not stored)
-    __device__ __forceinline__ MxBLoad(const MxGemmArgs &a, int tile0, int lane) {
+    int off[NT];  // of the lane's tile; tiles past the last are read as the last (not stored)
+    int slot;
+    __device__ __forceinline__ MxW(const MxGemmArgs &a, int tile0, int lane) {
+        slot = 16 * (lane >> 5) + (lane & 15);
+        const int bytes = (a.units + 1) / 2 * kMxPair;
 #pragma unroll
         for (int nt = 0; nt < NT; nt++) {
-            const int t = min(tile0 + 2 * nt, a.ntile - 1), bytes = a.units * kMxRecord;
-            buf[nt] = rsrc(a.w + (size_t)t * bytes, (int64_t)min(2, a.ntile - t) * bytes);
+            const int t = min(tile0 + 2 * nt, a.ntile - 1);
+            buf[nt] = rsrc(a.w + (int64_t)t * bytes, (int64_t)min(2, a.ntile - t) * bytes);
             off[nt] = (lane & 16) && t + 1 < a.ntile ? bytes : 0;
         }
     }
-    __device__ __forceinline__ void load(int u, int lane, MxB<NT> &o) const {
-        const int slot = 16 * (lane >> 5) + (lane & 15);
-#pragma unroll
-        for (int nt = 0; nt < NT; nt++)
-#pragma unroll
-            for (int i = 0; i < 2; i++) {
-                o.q[nt][i] = __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(buf[nt], off[nt] + 16 * slot + 512 * i, u * kMxRecord, 0));
-                o.s[nt][i] = __builtin_amdgcn_raw_buffer_load_b8(buf[nt], off[nt] + 1024 + slot + 32 * i, u * kMxRecord, 0);
-            }
+    // blocks 2s + h of a pair of units (s from 0 to 3), and the word of their scales (byte s)
+    __device__ __forceinline__ u32x4 codes(int nt, int pair, int s) const {
+        return __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(buf[nt], off[nt] + 16 * slot, pair * kMxPair + 512 * s, 0));
+    }
+    __device__ __forceinline__ uint32_t scales(int nt, int pair) const {
+        return __builtin_amdgcn_raw_buffer_load_b32(buf[nt], off[nt] + 4 * slot, pair * kMxPair + 2048, 0);
+    }
+    // of one unit: bytes i for blocks 2i + h
+    __device__ __forceinline__ uint32_t scales16(int nt, int u) const {
+        return __builtin_amdgcn_raw_buffer_load_b16(buf[nt], off[nt] + 4 * slot, (u >> 1) * kMxPair + 2048 + 2 * (u & 1), 0);
     }
 };
 
@@ -93,31 +103,46 @@ __device__ __forceinline__ void arrive() {
     __builtin_amdgcn_sched_barrier(0);
 }
 
-// lane: column lane % 32 of each 32, rows 8 i + 4h + e of each 32-row tile.  The bias is read before the first store:
-// a wait for a load waits for the stores before it, too.
+// lane: column lane % 32 of each 32, rows 8 i + 4h + e of each 32-row tile.  The bias is read and added before the first
+// store: a wait for a load waits for the stores before it, too.
 template <int MT, int NT>
 __device__ __forceinline__ void mx_store(const MxGemmArgs &a, const MxPlace &at, int tile0, int lane, floatx16 (&acc)[MT][NT]) {
     const bool slab = a.ks > 1;
     const int h = lane >> 5;
-    float bias[NT];
+    if (a.bias && !slab) {
 #pragma unroll
-    for (int nt = 0; nt < NT; nt++) {
-        const int64_t col = (int64_t)(tile0 + 2 * nt) * kTile + (lane & 31);
-        bias[nt] = a.bias && !slab && col < a.n ? a.bias[col] : 0.f;
+        for (int nt = 0; nt < NT; nt++) {
+            const int64_t col = (int64_t)(tile0 + 2 * nt) * kTile + (lane & 31);
+            const float bias = a.bias[min(col, a.n - 1)];
+#pragma unroll
+            for (int mt = 0; mt < MT; mt++)
+#pragma unroll
+                for (int e = 0; e < 16; e++) acc[mt][nt][e] += bias;
+        }
     }
     auto store = [&](auto *y, auto &&as) {
 #pragma unroll
         for (int mt = 0; mt < MT; mt++) {
-            const int row0 = (at.rb * MT + mt) * 32 + 4 * h;
+            const int first = (at.rb * MT + mt) * 32, row0 = first + 4 * h;
+            if (first >= a.m) return;
+            const bool whole = first + 32 <= a.m;
 #pragma unroll
             for (int nt = 0; nt < NT; nt++) {
                 const int64_t col = (int64_t)(tile0 + 2 * nt) * kTile + (lane & 31);
                 if (col >= a.n) continue;
                 auto *p = y + (int64_t)row0 * a.n + col;
+                if (whole) {  // uniform: no branch a store
 #pragma unroll
-                for (int e = 0; e < 16; e++) {
-                    if (row0 + 8 * (e / 4) + e % 4 < a.m) *p = as(acc[mt][nt][e] + bias[nt]);
-                    p += e % 4 == 3 ? 5 * a.n : a.n;
+                    for (int e = 0; e < 16; e++) {
+                        *p = as(acc[mt][nt][e]);
+                        p += e % 4 == 3 ? 5 * a.n : a.n;
+                    }
+                } else {
+#pragma unroll
+                    for (int e = 0; e < 16; e++) {
+                        if (row0 + 8 * (e / 4) + e % 4 < a.m) *p = as(acc[mt][nt][e]);
+                        p += e % 4 == 3 ? 5 * a.n : a.n;
+                    }
                 }
             }
         }
@@ -149,7 +174,7 @@ __global__ __launch_bounds__(W * 64, 2) void mx_gemm16_kernel(MxGemmArgs a) {
     const int wv = __builtin_amdgcn_readfirstlane(tid >> 6);
     const MxPlace at(a);
     const int tile0 = (at.cb * W + wv) * 2 * NT;
-    const MxBLoad<NT> bl(a, tile0, lane);
+    const MxW<NT> w(a, tile0, lane);
     // Copy i of a wave: rows 4 (i W + wv) .. + 3 of the pieces [plane][row tile][32 rows].  Rows past m belong to the
     // next plane or lie past the buffer (zeros); they are not stored.
     const int k = (int)a.k;
@@ -168,15 +193,24 @@ __global__ __launch_bounds__(W * 64, 2) void mx_gemm16_kernel(MxGemmArgs a) {
     const int c32 = lane & 31, h = lane >> 5;
     floatx16 acc[MT][NT];
     mx_clear(acc);
-    MxB<NT> b[2];
+    u32x4 bq[2][NT][2];
+    uint32_t bs[2][NT];
+    auto load_b = [&](int u, int buf) {
+#pragma unroll
+        for (int nt = 0; nt < NT; nt++) {
+#pragma unroll
+            for (int i = 0; i < 2; i++) bq[buf][nt][i] = w.codes(nt, u >> 1, 2 * (u & 1) + i);
+            bs[buf][nt] = w.scales16(nt, u);
+        }
+    };
     copy_a(at.u0, 0);
-    bl.load(at.u0, lane, b[0]);
+    load_b(at.u0, 0);
     auto unit = [&](auto parity, int u) {
         constexpr int buf = decltype(parity)::value;
         arrive();
         const int next = min(u + 1, at.u1 - 1);
         copy_a(next, buf ^ 1);
-        bl.load(next, lane, b[buf ^ 1]);
+        load_b(next, buf ^ 1);
 #pragma unroll
         for (int s = 0; s < 8; s++) {
             // step s: word s / 2 of blocks 2 (s % 2) + h
@@ -188,7 +222,7 @@ __global__ __launch_bounds__(W * 64, 2) void mx_gemm16_kernel(MxGemmArgs a) {
                 for (int mt = 0; mt < MT; mt++)
                     af[p][mt] = *reinterpret_cast<const u32x4 *>(lds + buf * BUF + (p * MT + mt) * kPiece + c32 * 256 + ((chunk ^ (c32 & 15)) << 4));
 #pragma unroll
-            for (int nt = 0; nt < NT; nt++) bf[nt] = mx_codes_bf16(b[buf].q[nt][s & 1][s >> 1], mx_scale(b[buf].s[nt][s & 1]));
+            for (int nt = 0; nt < NT; nt++) bf[nt] = mx_codes_bf16(bq[buf][nt][s & 1][s >> 1], mx_scale((bs[buf][nt] >> (8 * (s & 1))) & 0xFFu));
             // (the lo plane first: added to a finished hi sum its low bits would be cut off)
 #pragma unroll
             for (int p = P - 1; p >= 0; p--)
@@ -207,68 +241,94 @@ __global__ __launch_bounds__(W * 64, 2) void mx_gemm16_kernel(MxGemmArgs a) {
     mx_store(a, at, tile0, lane, acc);
 }
 
+// A stage is a pair of units (256 k).  A wave's B operands are loaded for the next stage as soon as a step has used them;
+// the A records are copied to the other LDS buffer.  Copies are issued before the loads of a stage, so that the wait for
+// them at the next one leaves the loads in flight.
 template <int MT, int NT>
 __global__ __launch_bounds__(W * 64, 2) void mx_gemm4_kernel(MxGemmArgs a) {
-    constexpr int REC = 2 * MT;                   // records (16-row tiles) of a unit
-    constexpr int SC = (REC + 3) / 4 * 256;       // their scales: a copy holds four records'
-    constexpr int BUF = REC * 1024 + SC;
+    constexpr int REC = 2 * MT;                // 16-row tiles
+    constexpr int BUF = mx_gemm4_stage(MT);    // codes [REC][2048], then scales [REC][128] (at least 1 KB of them)
     extern __shared__ __attribute__((aligned(16))) uint8_t lds[];
     const int tid = threadIdx.x, lane = tid & 63;
     const int wv = __builtin_amdgcn_readfirstlane(tid >> 6);
     const MxPlace at(a);
     const int tile0 = (at.cb * W + wv) * 2 * NT;
-    const MxBLoad<NT> bl(a, tile0, lane);
-    const int mtiles = (a.m + 15) / 16, bytes = a.units * kMxRecord;
+    const MxW<NT> w(a, tile0, lane);
+    const int mtiles = (a.m + 15) / 16, bytes = (a.units + 1) / 2 * kMxPair;
     const __amdgpu_buffer_rsrc_t xb = rsrc(a.x, (int64_t)mtiles * bytes);
     // (row tiles past the last: the last one again, not stored)
-    auto copy_a = [&](int u, int buf) {
+    auto copy_a = [&](int pair, int buf) {
 #pragma unroll
-        for (int i = 0; i < (REC + W - 1) / W; i++) {
-            const int rec = i * W + wv;
-            if (rec < REC)
-                copy16_lds(xb, lds + buf * BUF + rec * 1024, 16 * lane, min(at.rb * REC + rec, mtiles - 1) * bytes + u * kMxRecord);
+        for (int i = 0; i < MT; i++) {  // 2 REC pieces of 1 KB
+            const int piece = i * W + wv;
+            copy16_lds(xb, lds + buf * BUF + piece * 1024, 16 * lane,
+                       min(at.rb * REC + piece / 2, mtiles - 1) * bytes + pair * kMxPair + piece % 2 * 1024);
         }
-        if (wv < SC / 256) {
-            const int rec = min(at.rb * REC + min(4 * wv + (lane >> 4), REC - 1), mtiles - 1);
-#if defined(__HIP_DEVICE_COMPILE__)
-            __builtin_amdgcn_raw_ptr_buffer_load_lds(xb, (__attribute__((address_space(3))) void *)(lds + buf * BUF + REC * 1024 + wv * 256), 4,
-                                                     rec * bytes + 1024 + 4 * (lane & 15), u * kMxRecord, 0, 0);
-#endif
-        }
+        // two tiles' scales a wave
+        const int rec = min(at.rb * REC + (2 * wv + (lane >> 5)) % REC, mtiles - 1);
+        copy4_lds(xb, lds + buf * BUF + REC * 2048 + wv * 256, rec * bytes + 4 * (lane & 31), pair * kMxPair + 2048);
     };
-    const int b16 = (lane >> 4) & 1, slot = 16 * (lane >> 5) + (lane & 15);
+    const int b16 = (lane >> 4) & 1;
     floatx16 acc[MT][NT];
     mx_clear(acc);
-    MxB<NT> b[2];
-    copy_a(at.u0, 0);
-    bl.load(at.u0, lane, b[0]);
-    auto unit = [&](auto parity, int u) {
+    u32x4 bq[NT][4];
+    uint32_t bs[2][NT];
+    auto load_scales = [&](int pair, int buf) {
+#pragma unroll
+        for (int nt = 0; nt < NT; nt++) bs[buf][nt] = w.scales(nt, pair);
+    };
+    const int v0 = at.u0 / 2, v1 = (at.u1 + 1) / 2;  // (parts of K are whole pairs)
+    copy_a(v0, 0);
+    load_scales(v0, 0);
+#pragma unroll
+    for (int s = 0; s < 4; s++)
+#pragma unroll
+        for (int nt = 0; nt < NT; nt++) bq[nt][s] = w.codes(nt, v0, s);
+    auto stage = [&](auto parity, int v) {
         constexpr int buf = decltype(parity)::value;
-        arrive();
-        const int next = min(u + 1, at.u1 - 1);
+        wait_vmcnt<5 * NT>();  // this stage's copies have landed
+        __builtin_amdgcn_s_barrier();
+        __builtin_amdgcn_sched_barrier(0);
+        const int next = min(v + 1, v1 - 1);
         copy_a(next, buf ^ 1);
-        bl.load(next, lane, b[buf ^ 1]);
+        load_scales(next, buf ^ 1);
+        __builtin_amdgcn_sched_barrier(0);
+        uint32_t as[MT];
 #pragma unroll
-        for (int i = 0; i < 2; i++) {
-            u32x4 af[MT];
-            uint32_t as[MT];
+        for (int mt = 0; mt < MT; mt++)
+            as[mt] = *reinterpret_cast<const uint32_t *>(lds + buf * BUF + REC * 2048 + (2 * mt + b16) * 128 + 4 * w.slot);
+        // The next step's A is read, and this step's B loaded anew, between the MFMAs: left to itself the scheduler moves
+        // all the loads to the stage's end, where the next stage waits for them.
+        u32x4 af[2][MT];
+        auto read_a = [&](int s) {
 #pragma unroll
-            for (int mt = 0; mt < MT; mt++) {
-                af[mt] = *reinterpret_cast<const u32x4 *>(lds + buf * BUF + (2 * mt + b16) * 1024 + 512 * i + 16 * slot);
-                as[mt] = lds[buf * BUF + REC * 1024 + (2 * mt + b16) * 64 + 32 * i + slot];
-            }
+            for (int mt = 0; mt < MT; mt++)
+                af[s & 1][mt] = *reinterpret_cast<const u32x4 *>(lds + buf * BUF + (2 * mt + b16) * 2048 + 512 * s + 16 * w.slot);
+        };
+        read_a(0);
+        auto step = [&](auto which) {
+            constexpr int s = decltype(which)::value;
+            if constexpr (s < 3) read_a(s + 1);
 #pragma unroll
             for (int mt = 0; mt < MT; mt++)
 #pragma unroll
-                for (int nt = 0; nt < NT; nt++) acc[mt][nt] = mfma32_mx(af[mt], as[mt], b[buf].q[nt][i], b[buf].s[nt][i], acc[mt][nt]);
-        }
+                for (int nt = 0; nt < NT; nt++) acc[mt][nt] = mfma32_mx<s>(af[s & 1][mt], as[mt], bq[nt][s], bs[buf][nt], acc[mt][nt]);
+#pragma unroll
+            for (int nt = 0; nt < NT; nt++) bq[nt][s] = w.codes(nt, next, s);
+            __builtin_amdgcn_sched_barrier(0);
+        };
+        step(std::integral_constant<int, 0>());
+        step(std::integral_constant<int, 1>());
+        step(std::integral_constant<int, 2>());
+        step(std::integral_constant<int, 3>());
+        __builtin_amdgcn_sched_barrier(0);
     };
-    int u = at.u0;
-    for (; u + 1 < at.u1; u += 2) {
-        unit(std::integral_constant<int, 0>(), u);
-        unit(std::integral_constant<int, 1>(), u + 1);
+    int v = v0;
+    for (; v + 1 < v1; v += 2) {
+        stage(std::integral_constant<int, 0>(), v);
+        stage(std::integral_constant<int, 1>(), v + 1);
     }
-    if (u < at.u1) unit(std::integral_constant<int, 0>(), u);
+    if (v < v1) stage(std::integral_constant<int, 0>(), v);
     mx_store(a, at, tile0, lane, acc);
 }
 
@@ -283,7 +343,8 @@ int launch16(const MxGemmArgs &a, void *stream) {
 }
 template <int MT, int NT>
 int launch4(const MxGemmArgs &a, void *stream) {
-    constexpr size_t lds = 2 * (2 * MT * 1024 + (2 * MT + 3) / 4 * 256);
+    constexpr size_t lds = 2 * mx_gemm4_stage(MT);
+    static_assert(lds <= 65536, "LDS of a launch without an attribute");
     hipLaunchKernelGGL((mx_gemm4_kernel<MT, NT>), dim3((unsigned)(a.row_blocks * a.col_blocks * a.ks)), dim3(W * 64), lds,
                        (hipStream_t)stream, a);
     return (int)hipGetLastError();

@@ -153,7 +153,7 @@ MxGemmPlan mx_gemm_plan(int64_t m, int64_t n, int64_t k, int x_kind) {
     p.ks = 1;
     p.row_blocks = (int)((tiles + p.mt - 1) / p.mt);
     p.col_blocks = (int)((n + 128 * p.nt - 1) / (128 * p.nt));
-    const size_t x = four ? (size_t)(mx_tiles(m) * mx_units(k)) * kMxRecord : x_kind == kMxF32 ? (size_t)m * (size_t)k * 6 : 0;
+    const size_t x = four ? (size_t)(mx_tiles(m) * mx_pairs(k)) * kMxPair : x_kind == kMxF32 ? (size_t)m * (size_t)k * 6 : 0;
     p.slabs = align256(x);
     p.bytes = p.slabs + (p.ks > 1 ? (size_t)p.ks * (size_t)m * (size_t)n * 4 : 0);
     return p;

@@ -101,7 +101,7 @@ bool make_layout_mxfp4(int64_t n, int64_t k, Layout *L, const char **err) {
     L->k = k;
     L->ntile = mx_tiles(n);
     L->nblk = mx_units(k);
-    L->qs_bytes = (size_t)L->ntile * L->nblk * kMxRecord;
+    L->qs_bytes = (size_t)L->ntile * mx_pairs(k) * kMxPair;
     return true;
 }
 
