@@ -32,14 +32,18 @@ __device__ __forceinline__ floatx16 mfma32_mx(u32x4 a, uint32_t sa, u32x4 b, uin
 #endif
 }
 
-// bytes of a stage's A in LDS: 2 mt tiles' codes and the four waves' copies of scales
-constexpr int mx_gemm4_stage(int mt) { return 2 * mt * 2048 + 1024; }
+// copies of scales of a wave and stage (the four waves' hold at least 8 tiles'), and the bytes of a stage's A in LDS
+constexpr int mx_gemm4_scale_copies(int mt) { return mt > 4 ? mt / 4 : 1; }
+constexpr int mx_gemm4_stage(int mt) { return 2 * mt * 2048 + 1024 * mx_gemm4_scale_copies(mt); }
 // 4 bytes a lane from a buffer straight into LDS
 __device__ __forceinline__ void copy4_lds(__amdgpu_buffer_rsrc_t t, uint8_t *lds, int voff, int soff) {
 #if defined(__HIP_DEVICE_COMPILE__)
     __builtin_amdgcn_raw_ptr_buffer_load_lds(t, (__attribute__((address_space(3))) void *)lds, 4, voff, soff, 0, 0);
 #endif
 }
+
+// a wave's LDS for 32 rows of 128 bytes of outputs
+constexpr int kOutRow = 144, kOutBuf = 32 * kOutRow;
 
 struct MxGemmArgs {
     const uint8_t *w, *x;  // x: bf16 planes [P][m][k], or the records of the quantized rows
@@ -48,6 +52,7 @@ struct MxGemmArgs {
     int y_bf16;
     int m, units, ntile, ks;
     int row_blocks, col_blocks;
+    int wide;              // rows of y (or the slabs) are whole aligned 16-byte pieces
     int64_t n, k;
 };
 
@@ -106,7 +111,8 @@ __device__ __forceinline__ void arrive() {
 // lane: column lane % 32 of each 32, rows 8 i + 4h + e of each 32-row tile.  The bias is read and added before the first
 // store: a wait for a load waits for the stores before it, too.
 template <int MT, int NT>
-__device__ __forceinline__ void mx_store(const MxGemmArgs &a, const MxPlace &at, int tile0, int lane, floatx16 (&acc)[MT][NT]) {
+__device__ __forceinline__ void mx_store(const MxGemmArgs &a, const MxPlace &at, int tile0, int wv, int lane, uint8_t *lds,
+                                         floatx16 (&acc)[MT][NT]) {
     const bool slab = a.ks > 1;
     const int h = lane >> 5;
     if (a.bias && !slab) {
@@ -120,37 +126,73 @@ __device__ __forceinline__ void mx_store(const MxGemmArgs &a, const MxPlace &at,
                 for (int e = 0; e < 16; e++) acc[mt][nt][e] += bias;
         }
     }
+    const bool bf16 = !slab && a.y_bf16;
+    float *slabs = reinterpret_cast<float *>(a.y) + (slab ? (int64_t)at.kp * a.m * a.n : 0);
+    if (a.wide) {
+        // Through LDS, 32 rows of 128 bytes at a time, so that a store is eight rows' 16 bytes a lane.  The wave's own
+        // part of what held A (every wave is past it), whose accesses stay in order.
+        __syncthreads();
+        uint8_t *mine = lds + wv * kOutBuf;
+        const int row8 = lane >> 3, at16 = lane & 7;
+        auto flush = [&](int mt, uint8_t *y, int64_t col0, int elem) {  // y: of element [0][0]
+            __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+            __builtin_amdgcn_wave_barrier();
+            __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+            const int64_t col = col0 + at16 * (16 / elem);
+#pragma unroll
+            for (int i = 0; i < 4; i++) {
+                const u32x4 v = *reinterpret_cast<const u32x4 *>(mine + (8 * i + row8) * kOutRow + at16 * 16);
+                const int64_t row = (at.rb * MT + mt) * 32 + 8 * i + row8;
+                if (row < a.m && col < a.n) *reinterpret_cast<u32x4 *>(y + (row * a.n + col) * elem) = v;
+            }
+            __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+            __builtin_amdgcn_wave_barrier();
+            __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+        };
+#pragma unroll
+        for (int mt = 0; mt < MT; mt++) {
+            if ((at.rb * MT + mt) * 32 >= a.m) return;
+            const int64_t col0 = (int64_t)tile0 * kTile;
+            uint8_t *p = mine + 4 * h * kOutRow;
+            if (bf16) {
+                static_assert(NT == 2, "128 bytes of bf16");
+#pragma unroll
+                for (int nt = 0; nt < NT; nt++)
+#pragma unroll
+                    for (int e = 0; e < 16; e++)
+                        *reinterpret_cast<__bf16 *>(p + (8 * (e / 4) + e % 4) * kOutRow + (32 * nt + (lane & 31)) * 2) = (__bf16)acc[mt][nt][e];
+                flush(mt, reinterpret_cast<uint8_t *>(a.y), col0, 2);
+            } else {
+#pragma unroll
+                for (int nt = 0; nt < NT; nt++) {
+#pragma unroll
+                    for (int e = 0; e < 16; e++)
+                        *reinterpret_cast<float *>(p + (8 * (e / 4) + e % 4) * kOutRow + (lane & 31) * 4) = acc[mt][nt][e];
+                    flush(mt, reinterpret_cast<uint8_t *>(slabs), col0 + 32 * nt, 4);
+                }
+            }
+        }
+        return;
+    }
     auto store = [&](auto *y, auto &&as) {
 #pragma unroll
         for (int mt = 0; mt < MT; mt++) {
-            const int first = (at.rb * MT + mt) * 32, row0 = first + 4 * h;
-            if (first >= a.m) return;
-            const bool whole = first + 32 <= a.m;
+            const int row0 = (at.rb * MT + mt) * 32 + 4 * h;
 #pragma unroll
             for (int nt = 0; nt < NT; nt++) {
                 const int64_t col = (int64_t)(tile0 + 2 * nt) * kTile + (lane & 31);
                 if (col >= a.n) continue;
                 auto *p = y + (int64_t)row0 * a.n + col;
-                if (whole) {  // uniform: no branch a store
 #pragma unroll
-                    for (int e = 0; e < 16; e++) {
-                        *p = as(acc[mt][nt][e]);
-                        p += e % 4 == 3 ? 5 * a.n : a.n;
-                    }
-                } else {
-#pragma unroll
-                    for (int e = 0; e < 16; e++) {
-                        if (row0 + 8 * (e / 4) + e % 4 < a.m) *p = as(acc[mt][nt][e]);
-                        p += e % 4 == 3 ? 5 * a.n : a.n;
-                    }
+                for (int e = 0; e < 16; e++) {
+                    if (row0 + 8 * (e / 4) + e % 4 < a.m) *p = as(acc[mt][nt][e]);
+                    p += e % 4 == 3 ? 5 * a.n : a.n;
                 }
             }
         }
     };
-    if (!slab && a.y_bf16)
-        store(reinterpret_cast<uint16_t *>(a.y), [](float v) { return (uint16_t)f32_to_bf16_bits(v); });
-    else
-        store(reinterpret_cast<float *>(a.y) + (slab ? (int64_t)at.kp * a.m * a.n : 0), [](float v) { return v; });
+    if (bf16) store(reinterpret_cast<__bf16 *>(a.y), [](float v) { return (__bf16)v; });
+    else store(slabs, [](float v) { return v; });
 }
 
 template <int MT, int NT>
@@ -238,15 +280,16 @@ __global__ __launch_bounds__(W * 64, 2) void mx_gemm16_kernel(MxGemmArgs a) {
         unit(std::integral_constant<int, 1>(), u + 1);
     }
     if (u < at.u1) unit(std::integral_constant<int, 0>(), u);
-    mx_store(a, at, tile0, lane, acc);
+    mx_store(a, at, tile0, wv, lane, lds, acc);
 }
 
 // A stage is a pair of units (256 k).  A wave's B operands are loaded for the next stage as soon as a step has used them;
 // the A records are copied to the other LDS buffer.  Copies are issued before the loads of a stage, so that the wait for
 // them at the next one leaves the loads in flight.
 template <int MT, int NT>
-__global__ __launch_bounds__(W * 64, 2) void mx_gemm4_kernel(MxGemmArgs a) {
+__global__ __launch_bounds__(W * 64, MT > 4 ? 1 : 2) void mx_gemm4_kernel(MxGemmArgs a) {
     constexpr int REC = 2 * MT;                // 16-row tiles
+    constexpr int SC = mx_gemm4_scale_copies(MT);
     constexpr int BUF = mx_gemm4_stage(MT);    // codes [REC][2048], then scales [REC][128] (at least 1 KB of them)
     extern __shared__ __attribute__((aligned(16))) uint8_t lds[];
     const int tid = threadIdx.x, lane = tid & 63;
@@ -265,8 +308,11 @@ __global__ __launch_bounds__(W * 64, 2) void mx_gemm4_kernel(MxGemmArgs a) {
                        min(at.rb * REC + piece / 2, mtiles - 1) * bytes + pair * kMxPair + piece % 2 * 1024);
         }
         // two tiles' scales a wave
-        const int rec = min(at.rb * REC + (2 * wv + (lane >> 5)) % REC, mtiles - 1);
-        copy4_lds(xb, lds + buf * BUF + REC * 2048 + wv * 256, rec * bytes + 4 * (lane & 31), pair * kMxPair + 2048);
+#pragma unroll
+        for (int i = 0; i < SC; i++) {
+            const int rec = min(at.rb * REC + (2 * (i * W + wv) + (lane >> 5)) % REC, mtiles - 1);
+            copy4_lds(xb, lds + buf * BUF + REC * 2048 + (i * W + wv) * 256, rec * bytes + 4 * (lane & 31), pair * kMxPair + 2048);
+        }
     };
     const int b16 = (lane >> 4) & 1;
     floatx16 acc[MT][NT];
@@ -329,12 +375,12 @@ __global__ __launch_bounds__(W * 64, 2) void mx_gemm4_kernel(MxGemmArgs a) {
         stage(std::integral_constant<int, 1>(), v + 1);
     }
     if (v < v1) stage(std::integral_constant<int, 0>(), v);
-    mx_store(a, at, tile0, lane, acc);
+    mx_store(a, at, tile0, wv, lane, lds, acc);
 }
 
 template <int MT, int NT, int P>
 int launch16(const MxGemmArgs &a, void *stream) {
-    constexpr size_t lds = 2 * MT * P * kPiece;
+    constexpr size_t lds = std::max(2 * MT * P * kPiece, W * kOutBuf);
     auto *kernel = mx_gemm16_kernel<MT, NT, P>;
     hipError_t e = allow_lds(reinterpret_cast<const void *>(kernel), lds);
     if (e != hipSuccess) return (int)e;
@@ -343,10 +389,11 @@ int launch16(const MxGemmArgs &a, void *stream) {
 }
 template <int MT, int NT>
 int launch4(const MxGemmArgs &a, void *stream) {
-    constexpr size_t lds = 2 * mx_gemm4_stage(MT);
-    static_assert(lds <= 65536, "LDS of a launch without an attribute");
-    hipLaunchKernelGGL((mx_gemm4_kernel<MT, NT>), dim3((unsigned)(a.row_blocks * a.col_blocks * a.ks)), dim3(W * 64), lds,
-                       (hipStream_t)stream, a);
+    constexpr size_t lds = std::max(2 * mx_gemm4_stage(MT), W * kOutBuf);
+    auto *kernel = mx_gemm4_kernel<MT, NT>;
+    hipError_t e = allow_lds(reinterpret_cast<const void *>(kernel), lds);
+    if (e != hipSuccess) return (int)e;
+    hipLaunchKernelGGL(kernel, dim3((unsigned)(a.row_blocks * a.col_blocks * a.ks)), dim3(W * 64), lds, (hipStream_t)stream, a);
     return (int)hipGetLastError();
 }
 
@@ -371,6 +418,7 @@ int launch_mx_gemm(const MxArgs &a, void *scratch, void *stream) {
     g.col_blocks = p.col_blocks;
     g.n = a.n;
     g.k = a.k;
+    g.wide = a.n % (p.ks > 1 || !a.y_bf16 ? 4 : 8) == 0 && (uintptr_t)g.y % 16 == 0;
     int e = 0;
     if (a.x_kind != kMxBf16) {
         if (a.x_kind == kMxF32) e = launch_mx_split(reinterpret_cast<const float *>(a.x), a.m * a.k, reinterpret_cast<uint16_t *>(base), stream);
@@ -381,7 +429,7 @@ int launch_mx_gemm(const MxArgs &a, void *scratch, void *stream) {
     }
     if (a.x_kind == kMxBf16) e = p.mt == 1 ? launch16<1, 2, 1>(g, stream) : launch16<2, 2, 1>(g, stream);
     else if (a.x_kind == kMxF32) e = launch16<1, 2, 3>(g, stream);
-    else e = p.mt == 1 ? launch4<1, 2>(g, stream) : p.mt == 2 ? launch4<2, 2>(g, stream) : launch4<4, 2>(g, stream);
+    else e = p.mt == 1 ? launch4<1, 2>(g, stream) : p.mt == 2 ? launch4<2, 2>(g, stream) : p.mt == 4 ? launch4<4, 2>(g, stream) : launch4<8, 2>(g, stream);
     if (e || p.ks == 1) return e;
     return launch_int4_sum(slabs, p.ks, a.m, a.n, a.bias, a.y, a.y_bf16, stream);
 }
