@@ -4,8 +4,8 @@
 //   v = s_j + l_t - log sum_i e^(l_i),
 // and the `keep` largest of an item's values are wanted.  Within a beam v has the order of l, so the keep largest
 // logits of every beam hold them.  Two launches:
-//   beam_seg_kernel   one wave per 2048 logits of a beam: the maximum, the sum of e^(l - maximum) over the other
-//                     elements, and the candidates (nnq_logits.h).  Beams that offer nothing by themselves (ended
+//   beam_seg_kernel   one wave per 2048 logits of a beam: the maximum, the sum of e^(l - maximum), and the candidates
+//                     (nnq_logits.h).  Beams that offer nothing by themselves (ended
 //                     ones, scores of -inf) are not read.
 //   beam_join_kernel  one workgroup per item: log sum e^l of each beam from its segments, in 64 bits and in a fixed
 //                     order, and the largest values of the beams' candidates, compared in 64 bits.
@@ -24,11 +24,11 @@ namespace {
 constexpr int kBeamWaves = 4;
 constexpr int kBeamThreads = 1024;
 constexpr int kBeamList = 1024;  // candidates that the join ranks in LDS
+constexpr int kStats = 2;        // segments that a lane of it holds
+constexpr int kHeld = 8;         // candidates that a thread of it holds
 
 struct BeamStat {
-    float mx, r;   // a segment's maximum, the sum of e^(l - mx) over its elements below it
-    uint32_t cnt;  // elements equal to it
-    uint32_t pad;
+    float mx, r;  // a segment's maximum, the sum of e^(l - mx)
 };
 
 struct BeamDev {
@@ -80,20 +80,17 @@ __global__ __launch_bounds__(kBeamWaves * 64) void beam_seg_kernel(BeamDev g) {
     const float mx = max64(lm);
     const float ref = mx == kNegInf ? 0.f : mx;
     float r = 0.f;
-    int cnt = kSeg;
 #pragma unroll
     for (int e = 0; e < kPer; e++) {
-        const float d = __builtin_elementwise_maximum(x[e] - ref, -1e30f);  // (-inf: its e^d is 0; NaN stays)
-        const float ex = exp_of(d);
-        const bool below = d != 0.f;  // (or NaN)
-        cnt -= __popcll(__ballot(below));
-        r += below ? ex : 0.f;
+        // e^d: d log2(e) with the constant in two parts and one rounding (-inf: 0)
+        const float d = x[e] - ref;
+        r += __builtin_amdgcn_exp2f(fmaf(d, 1.44269502162933349609f, d * 1.92596299112661746887e-8f));
     }
     r = sum64(r);
     const int64_t at = rl * g.nseg + seg;
-    if (lane == 0) g.stat[at] = BeamStat{mx, r, (uint32_t)cnt, 0};
+    if (lane == 0) g.stat[at] = BeamStat{mx, r};
     __shared__ uint64_t list[kBeamWaves][64];
-    segment_candidates<V>(x, lm, base, a.keep, g.slots, lane, list[wv], g.cand + at * g.slots);
+    segment_candidates<V, sizeof(T) == 4 ? 24 : 16>(x, lm, base, a.keep, g.slots, lane, list[wv], g.cand + at * g.slots);
 }
 
 // larger values have larger ones (v is a number)
@@ -103,6 +100,20 @@ __device__ __forceinline__ uint64_t ord64(double v) {
 }
 __device__ __forceinline__ double unord64(uint64_t o) {
     return __longlong_as_double((long long)(o >> 63 ? o & 0x7FFFFFFFFFFFFFFFull : ~o));
+}
+
+__device__ __forceinline__ double sum64d(double v) {  // as sum64
+    auto with = [&](auto &&f) {
+        const uint64_t u = (uint64_t)__double_as_longlong(v);
+        const uint32_t lo = f((uint32_t)u), hi = f((uint32_t)(u >> 32));
+        v += __longlong_as_double((long long)((uint64_t)hi << 32 | lo));
+    };
+    with([](uint32_t x) { return lane_of<0xB1>(x); });
+    with([](uint32_t x) { return lane_of<0x4E>(x); });
+    with([](uint32_t x) { return lane_of<0x141>(x); });
+    with([](uint32_t x) { return lane_of<0x140>(x); });
+    for (int o = 16; o < 64; o += o) v += __shfl_xor(v, o, 64);
+    return v;
 }
 
 // a candidate: its value's order (0: none), its beam and its key (logit, then index)
@@ -133,33 +144,40 @@ __global__ __launch_bounds__(kBeamThreads) void beam_join_kernel(BeamDev g) {
     const uint64_t *cand = g.cand + (int64_t)blockIdx.x * a.beams * g.nseg * g.slots;
     const int64_t keys = g.nseg * g.slots;
     const double nan = __longlong_as_double(0x7FF8000000000000ll);
+    // A beam's keys belong to `share` waves (beams over the number of waves: to one, which has several beams); a wave's
+    // beams are first, first + step, ..  The first kHeld keys of a lane are loaded at once, before the sums that they
+    // wait for (beams that were not read leave what the scratch held: not looked at).
+    const int share = a.beams >= NW ? 1 : NW / a.beams, step = NW / share;
+    const int first = wv / share, at0 = (wv % share) * 64 + lane;
+    uint64_t held[kHeld];
+#pragma unroll
+    for (int i = 0; i < kHeld; i++) {
+        const int64_t at = at0 + i * 64 * share;
+        held[i] = first < a.beams && at < keys ? cand[first * keys + at] : 0ull;
+    }
     if (tid == 0) listed = 0;
     for (int b = wv; b < a.beams; b += NW) {
         const float score = a.scores[item * a.beams + b];
+        const uint8_t end = a.finished ? a.finished[item * a.beams + b] : 0;
+        const BeamStat *st = stat + b * g.nseg;
+        BeamStat q[kStats];  // (the first of a lane's segments stay)
+#pragma unroll
+        for (int i = 0; i < kStats; i++) q[i] = lane + 64 * i < g.nseg ? st[lane + 64 * i] : BeamStat{kNegInf, 0.f};
+        const bool fin = finite_score(score);
         float mx = kNegInf;
-        const bool fin = finite_score(score), end = beam_ended(a, item * a.beams + b);
         double o = nan;
         if (fin && !end) {
-            const BeamStat *st = stat + b * g.nseg;
-            for (int64_t i = lane; i < g.nseg; i += 64) mx = fmaxf(mx, st[i].mx);
+#pragma unroll
+            for (int i = 0; i < kStats; i++) mx = fmaxf(mx, q[i].mx);
+            for (int64_t i = lane + 64 * kStats; i < g.nseg; i += 64) mx = fmaxf(mx, st[i].mx);
             mx = max64(mx);
-            double r = 0.0, cnt = 0.0;  // everything but the elements equal to the maximum, and their number
-            for (int64_t i = lane; i < g.nseg; i += 64) {
-                const BeamStat q = st[i];
-                if (q.mx == mx) {
-                    cnt += (double)q.cnt;
-                    r += (double)q.r;
-                } else {
-                    const double f = exp((double)q.mx - (double)mx);
-                    r += f * ((double)q.cnt + (double)q.r);
-                }
-            }
-            for (int s = 32; s > 0; s >>= 1) {
-                r += __shfl_xor(r, s, 64);
-                cnt += __shfl_xor(cnt, s, 64);
-            }
+            double r = 0.0;
+            auto add = [&](const BeamStat &t) { r = fma(exp((double)t.mx - (double)mx), (double)t.r, r); };
+#pragma unroll
+            for (int i = 0; i < kStats; i++) add(q[i]);
+            for (int64_t i = lane + 64 * kStats; i < g.nseg; i += 64) add(st[i]);
             // (a row without a logit above -inf: mx = -inf)
-            o = mx == kNegInf ? nan : (double)score - log1p(r + (cnt - 1.0));
+            o = mx == kNegInf ? nan : (double)score - log(sum64d(r));
         }
         if (lane == 0) {
             off[b] = o;
@@ -169,43 +187,60 @@ __global__ __launch_bounds__(kBeamThreads) void beam_join_kernel(BeamDev g) {
     }
     __syncthreads();
 
-    auto value = [&](double o, float mx, uint64_t key) -> uint64_t {
-        return key ? ord64(o + ((double)unord((uint32_t)(key >> 32)) - (double)mx)) : 0;
-    };
-    auto each = [&](auto &&f) {  // the thread's candidates
-        for (int b = 0; b < a.beams; b++) {
-            const double o = off[b];
-            const float mx = top[b];
-            if (ended[b]) {
-                if (tid == b) f(Cand{ended[b], 1, b});
-            } else if (o == o) {
-                for (int64_t i = tid; i < keys; i += kBeamThreads) {
-                    const uint64_t k = cand[b * keys + i];
-                    f(Cand{value(o, mx, k), k, b});
-                }
-            }
+    auto value = [&](int b, uint64_t key) { return ord64(off[b] + ((double)unord((uint32_t)(key >> 32)) - (double)top[b])); };
+    auto each = [&](int b, auto &&f) {  // the lane's keys of beam b (0: none)
+        if (b == first) {
+#pragma unroll
+            for (int i = 0; i < kHeld; i++) f(held[i]);
+        }
+        for (int64_t i = at0 + (b == first ? kHeld : 0) * 64 * share; i < keys; i += 4 * 64 * share) {
+            uint64_t k[4];
+#pragma unroll
+            for (int e = 0; e < 4; e++) k[e] = i + e * 64 * share < keys ? cand[b * keys + i + e * 64 * share] : 0ull;
+#pragma unroll
+            for (int e = 0; e < 4; e++) f(k[e]);
         }
     };
-    uint64_t best = 0;
-    each([&](const Cand &c) { best = max(best, c.v); });
+    // candidates of a value of at least `low`: within a beam they are the logits from some bound on, and only what is near
+    // it needs its value
+    auto from = [&](uint64_t low, auto &&f) {
+        for (int b = first; b < a.beams; b += step) {
+            if (off[b] != off[b]) continue;
+            const double lv = unord64(low), at = lv - off[b] + (double)top[b];  // (NaN where low is no value's)
+            const float near = (float)(at - 1e-6 * fabs(at) - 1e-9 * (fabs(lv) + fabs(off[b]) + fabs((double)top[b])));
+            const uint32_t bound = near > -3e38f ? ord(near) : 0u;
+            each(b, [&](uint64_t k) {
+                if (k && (uint32_t)(k >> 32) >= bound) {
+                    const uint64_t v = value(b, k);
+                    if (v >= low) f(Cand{v, k, b});
+                }
+            });
+        }
+        if (tid < a.beams && ended[tid] && ended[tid] >= low) f(Cand{ended[tid], 1, tid});
+    };
+    uint64_t best = tid < a.beams ? ended[tid] : 0;
+    for (int b = first; b < a.beams; b += step) {
+        if (off[b] != off[b]) continue;
+        uint64_t k = 0;
+        each(b, [&](uint64_t x) { k = max(k, x); });
+        if (k) best = max(best, value(b, k));
+    }
     maxima[tid] = best;
     __syncthreads();
     if (wv == 0) {
-        // the keep-th largest of the maxima of 64 parts is a lower bound of the keep-th largest value (its leading 32 bits)
+        // the keep-th largest of the maxima of 64 parts is a lower bound of the keep-th largest value (its leading 24 bits)
         uint64_t m = maxima[lane];
 #pragma unroll
         for (int w = 1; w < NW; w++) m = max(m, maxima[64 * w + lane]);
         const uint32_t v = (uint32_t)(m >> 32);
-        const uint32_t b = largest_with<32>(a.keep, [&](uint32_t k) { return __popcll(__ballot(v >= k)); });
+        const uint32_t b = largest_with<24>(a.keep, [&](uint32_t k) { return __popcll(__ballot(v >= k)); });
         if (lane == 0) bound = max((uint64_t)b << 32, (uint64_t)1);
     }
     __syncthreads();
     const uint64_t low = bound;
-    each([&](const Cand &c) {
-        if (c.v >= low) {
-            const uint32_t at = atomicAdd(&listed, 1u);
-            if (at < kBeamList) list[at] = c;
-        }
+    from(low, [&](const Cand &c) {
+        const uint32_t at = atomicAdd(&listed, 1u);
+        if (at < kBeamList) list[at] = c;
     });
     __syncthreads();
     auto put = [&](int place, const Cand &c) {
@@ -215,6 +250,25 @@ __global__ __launch_bounds__(kBeamThreads) void beam_join_kernel(BeamDev g) {
         a.tokens[at] = !c.v ? -1 : ended[c.beam] ? a.end_token : (int64_t)(0xFFFFFFFFu - (uint32_t)c.key);
     };
     const int got = (int)min(listed, (uint32_t)kBeamList);
+    if (got <= 64) {  // as a rule: one wave, a candidate a lane
+        if (wv) return;
+        const Cand c = lane < got ? list[lane] : Cand{0, 0, kBeams};
+        int place = 0;
+        auto lane_u64 = [&](uint64_t v, int j) {
+            return (uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)(v >> 32), j) << 32 | (uint32_t)__builtin_amdgcn_readlane((int)v, j);
+        };
+        for (int j = 0; j < got; j++) {
+            const uint64_t v = lane_u64(c.v, j);
+            place += v > c.v;
+            if (__ballot(v == c.v) & ~(1ull << j)) {  // uniform
+                const Cand o{v, lane_u64(c.key, j), __builtin_amdgcn_readlane(c.beam, j)};
+                place += v == c.v && ahead(o, c);
+            }
+        }
+        if (lane < got && place < a.keep) put(place, c);
+        if (lane >= got && lane < a.keep) put(lane, Cand{0, 0, 0});
+        return;
+    }
     if (listed <= kBeamList) {
         for (int i = tid; i < got; i += kBeamThreads) {
             const Cand c = list[i];
@@ -229,8 +283,8 @@ __global__ __launch_bounds__(kBeamThreads) void beam_join_kernel(BeamDev g) {
     Cand last{~0ull, ~0ull, -1};
     for (int place = 0; place < a.keep; place++) {
         Cand c{0, 0, kBeams};
-        each([&](const Cand &x) {
-            if (x.v && ahead(last, x) && ahead(x, c)) c = x;
+        from(1, [&](const Cand &x) {
+            if (ahead(last, x) && ahead(x, c)) c = x;
         });
         for (int s = 32; s > 0; s >>= 1) {
             const Cand o = shfl_cand(c, s);

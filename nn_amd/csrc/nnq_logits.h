@@ -104,14 +104,14 @@ __device__ __forceinline__ uint32_t largest_with(int want, F &&count) {
 
 // The candidates of the `want` largest of a segment, as keys, at cand[0 .. slots) (0: none).  Element e of a lane is
 // logit base + (e / V) * 64 V + e % V; lm: the lane's largest, -inf where there is no logit; list: 64 keys of LDS of the
-// wave's own.
-template <int V>
+// wave's own.  BITS: how many leading bits of the bound are settled; bf16 has 16.
+template <int V, int BITS = 24>
 __device__ __forceinline__ void segment_candidates(const float (&x)[kPer], float lm, int64_t base, int want, int slots, int lane,
                                                    uint64_t *list, uint64_t *cand) {
     const uint32_t mine = lm == lm ? ord(lm) : 0;  // (no number in the lane)
     // (its leading 24 bits do: a bound 2^-15 of its size below lets hardly more candidates in, also for
     // logits far from 0; with 16 bits 301 x 151936 logits around 300 took 114 us, 43 with 24)
-    const uint32_t lanes = largest_with<24>(want, [&](uint32_t k) { return __popcll(__ballot(mine >= k)); });
+    const uint32_t lanes = largest_with<BITS>(want, [&](uint32_t k) { return __popcll(__ballot(mine >= k)); });
     float t = unord(max(lanes, kOrdNegInf + 1));  // (-inf is no candidate)
     // the lane's candidates as bits, element 0 the highest
     uint32_t bits = 0;

@@ -180,7 +180,7 @@ BeamPlan beam_plan(int64_t batch, int beams, int64_t n, int keep) {
     BeamPlan p{};
     p.nseg = ((n + 2047) / 2048 + 3) / 4 * 4;
     p.slots = std::min(64, (keep + keep / 2 + 6 + 3) / 4 * 4);
-    const int64_t per = beams * p.nseg * (16 + 8 * (int64_t)p.slots);
+    const int64_t per = beams * p.nseg * (8 + 8 * (int64_t)p.slots);
     p.items = std::max<int64_t>(1, std::min({batch, ((int64_t)64 << 20) / per, (int64_t)65535 / beams}));
     p.bytes = (size_t)(p.items * per);
     return p;
