@@ -297,14 +297,17 @@ struct MxArgs {
     int64_t ntile, units;
     unsigned long long *argmax_partial;  // optional (m = 1): argmax keys, at most ntile of them
     int64_t *argmax_count;               //   and how many the launch writes
-    int ks;                              // (set by the launch: parts of K, their sums in slabs [ks][m][n])
+    int ks, kw, nw;                      // (set by the launch: MxRowsPlan's; the sums of ks parts of K in slabs [ks][m][n])
     float *slabs;
 };
-// how m rows run (nnq_plan.cpp), with the scratch's offsets
+// how up to kMxRows rows run (nnq_plan.cpp): parts of K, waves along K and along the tiles, pairs of units of a
+// wave at a time, workgroups a part, LDS and scratch bytes
 struct MxRowsPlan {
-    int ks, planes;  // planes: f32 x goes through its bf16 planes in the scratch
+    int ks, kw, nw, pp, groups, lds;
+    int first;  // x is quantized by a launch of its own (to the scratch's start)
     size_t slabs, bytes;
 };
+constexpr int kMxTriRows = 5;  // f32 rows whose three planes share one MFMA
 MxRowsPlan mx_rows_plan(int64_t m, int64_t n, int64_t k, int x_kind);
 struct MxGemmPlan {
     int mt, nt, ks;              // 32-row tiles of a workgroup, 32-column tiles of its waves, K split

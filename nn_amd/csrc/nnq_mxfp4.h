@@ -29,10 +29,11 @@ __device__ __forceinline__ float mx_scale(uint32_t byte) { return __uint_as_floa
 
 // 16x16x128: lane 16p + r supplies block p (32 columns) of A's row r and of B's column r with their scales; lane l
 // receives D[4 (l / 16) + i][l % 16].  32x32x64: lane 32h + r block h of row r; D[8 (i / 4) + 4h + i % 4][l % 32].
+template <int BYTE>  // of the words of scales
 __device__ __forceinline__ floatx4 mfma_mx16(u32x4 a, uint32_t sa, u32x4 b, uint32_t sb, floatx4 c) {
 #if defined(__HIP_DEVICE_COMPILE__)
     const i32x8 av = {(int)a[0], (int)a[1], (int)a[2], (int)a[3], 0, 0, 0, 0}, bv = {(int)b[0], (int)b[1], (int)b[2], (int)b[3], 0, 0, 0, 0};
-    return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(av, bv, c, 4, 4, 0, (int)sa, 0, (int)sb);
+    return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(av, bv, c, 4, 4, BYTE, (int)sa, BYTE, (int)sb);
 #else
     return c;
 #endif

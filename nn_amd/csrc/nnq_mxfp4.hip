@@ -192,24 +192,19 @@ __global__ __launch_bounds__(256) void mx_split_kernel(const float *x, int64_t c
 
 // ---- one to sixteen token rows ----------------------------------------------------------
 // Bound: the weight stream from HBM (17 / 32 of a byte for each weight), read once for all token rows.  A workgroup of
-// up to 16 waves owns blocks of R tiles; wave w takes units w, w + waves, ..; the next step's loads are in flight
-// while the current one is computed.  The waves' sums meet in LDS, one barrier per block of tiles.
+// kw * nw waves takes nw tiles at a time; wave (i, j) sums pairs of units i, i + kw, .. of tile j, a step's pairs all
+// in its registers, loaded for the next step as soon as they have been used.  x of the workgroup's
+// part of K lies in LDS, as MFMA operands read it; the waves' sums meet there too, one barrier a step.
 // x: X_BF16 bf16 rows; X_TRI up to five f32 rows, row t as the MFMA's rows 3t .. 3t + 2 (the three bf16 planes above);
-// X_PLANES three planes of bf16 rows; X_Q16 / X_Q32 rows to be quantized, each lane its own block; X_CODES codes and
-// scales given.
+// X_PLANES more f32 rows, an MFMA for each plane; X_Q16 / X_Q32 rows to be quantized; X_CODES codes and scales given.
 enum { X_BF16, X_TRI, X_PLANES, X_Q16, X_Q32, X_CODES };
 constexpr bool mx_both(int xf) { return xf >= X_Q16; }
-constexpr int kTriRow = 272;  // LDS bytes of a plane's row of a unit (256 and a shift of the banks)
-constexpr int kTriBuf = 16 * kTriRow;
+constexpr int kSumRow = 20;                       // floats of an MFMA row's 16 sums (and a shift of the banks)
+constexpr int kSumWave = 16 * kSumRow * 4;        // bytes of a wave's sums of a tile
 
-__device__ __forceinline__ void wave_sync() {
-    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
-    __builtin_amdgcn_wave_barrier();
-    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
-}
 template <int CTRL>
-__device__ __forceinline__ float row_add(float v) {
-    return v + __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(v), CTRL, 0xF, 0xF, true));
+__device__ __forceinline__ uint32_t row_lane(uint32_t v) {
+    return (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, CTRL, 0xF, 0xF, true);
 }
 __device__ __forceinline__ uint64_t mx_argmax_key(float v, uint32_t idx) {
     if (v != v) return ~0ull;
@@ -217,184 +212,230 @@ __device__ __forceinline__ uint64_t mx_argmax_key(float v, uint32_t idx) {
     return ((uint64_t)((b & 0x80000000u) ? ~b : (b | 0x80000000u)) << 32) | (0xFFFFFFFFu - idx);
 }
 
-// the operands of a unit
+// x in LDS.  bf16 rows (X_BF16: of the tokens, f32: 3t + plane) of `pairs` pairs of units and 16 bytes, so that the same
+// columns of 16 rows lie in 16 different places of the banks; or rows of codes, 16 bytes a block and 16 more, and
+// behind them words of scales in the image's order, [row][pair][2].
 template <int XF>
-struct XOp {
-    static constexpr int P = XF == X_PLANES ? 3 : 1;
-    u32x4 a[mx_both(XF) ? 1 : P][mx_both(XF) ? 1 : 4];
-    uint32_t s;
+struct XStage {
+    static constexpr bool BOTH = mx_both(XF), F32 = XF == X_TRI || XF == X_PLANES;
+    static constexpr int U = XF == X_BF16 ? 8 : F32 ? 3 : XF == X_Q16 ? 2 : XF == X_Q32 ? 1 : 4;  // pieces of a thread at a time
+    static constexpr int L = XF == X_BF16 || XF == X_CODES ? 1 : F32 ? 2 : XF == X_Q16 ? 4 : 8;   // loads of a piece
+    int pitch, pieces, row_pieces, k0;
+    uint8_t *lds, *words;
+    __amdgpu_buffer_rsrc_t rx, rs;
+    u32x4 v[U][L];
+    uint32_t s[XF == X_CODES ? U : 1];
+    __device__ __forceinline__ XStage(const MxArgs &a, uint8_t *at) {
+        const int64_t xel = a.m * a.k;
+        rx = rsrc(a.x, XF == X_CODES ? xel / 2 : XF == X_BF16 || XF == X_Q16 ? 2 * xel : 4 * xel);
+        rs = rsrc(a.xs, XF == X_CODES ? xel / 32 : 0);
+        lds = at;
+    }
+    __device__ __forceinline__ void part(const MxArgs &a, int pair0, int pairs) {
+        row_pieces = pairs * (BOTH ? 8 : 32);  // blocks, or 8 columns
+        pieces = (int)a.m * row_pieces;
+        pitch = pairs * (BOTH ? 128 : 512) + 16;
+        k0 = pair0 * 2 * kMxUnit;
+        words = lds + (int)a.m * pitch;
+    }
+    // (columns from K on: zeros)
+    __device__ __forceinline__ void load(const MxArgs &a, int first) {
+#pragma unroll
+        for (int i = 0; i < U; i++) {
+            const int at = first + i * (int)blockDim.x, row = at / row_pieces, k = k0 + (at - row * row_pieces) * (BOTH ? 32 : 8);
+            const int el = at < pieces && k < (int)a.k ? row * (int)a.k + k : -1;
+            const int off = el < 0 ? 0x7FFFFFF0 : XF == X_CODES ? el / 2 : XF == X_BF16 || XF == X_Q16 ? 2 * el : 4 * el;
+#pragma unroll
+            for (int l = 0; l < L; l++) v[i][l] = __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(rx, off, 16 * l, 0));
+            if constexpr (XF == X_CODES) s[i] = __builtin_amdgcn_raw_buffer_load_b8(rs, el < 0 ? 0x7FFFFFF0 : el / 32, 0, 0);
+        }
+    }
+    __device__ __forceinline__ void store(const MxArgs &a, int first) {
+#pragma unroll
+        for (int i = 0; i < U; i++) {
+            const int at = first + i * (int)blockDim.x, row = at / row_pieces, piece = at - row * row_pieces;
+            if (at >= pieces) continue;
+            if constexpr (XF == X_BF16) {
+                *reinterpret_cast<u32x4 *>(lds + row * pitch + 16 * piece) = v[i][0];
+            } else if constexpr (F32) {
+                u32x4 h, m, l;
+#pragma unroll
+                for (int e = 0; e < 4; e++) {
+                    uint32_t c[3];
+                    split3(__uint_as_float(v[i][e / 2][2 * (e & 1)]), __uint_as_float(v[i][e / 2][2 * (e & 1) + 1]), c[0], c[1], c[2]);
+                    h[e] = c[0];
+                    m[e] = c[1];
+                    l[e] = c[2];
+                }
+                uint8_t *o = lds + 3 * row * pitch + 16 * piece;
+                *reinterpret_cast<u32x4 *>(o) = h;
+                *reinterpret_cast<u32x4 *>(o + pitch) = m;
+                *reinterpret_cast<u32x4 *>(o + 2 * pitch) = l;
+            } else {
+                u32x4 q = v[i][0];
+                uint32_t byte = 0;
+                if constexpr (XF == X_CODES) byte = s[i];
+                else q = mx_quantize_block<XF == X_Q16>(v[i], a.floor_rule, byte);
+                *reinterpret_cast<u32x4 *>(lds + row * pitch + 16 * piece) = q;
+                // block 4 (unit) + 2i + h of a pair: word h, byte 2 (unit) + i
+                words[row * row_pieces + (piece & ~7) + 4 * (piece & 1) + 2 * ((piece >> 2) & 1) + ((piece >> 1) & 1)] = (uint8_t)byte;
+            }
+        }
+    }
+    __device__ __forceinline__ void rest(const MxArgs &a, int first) {  // what one load does not hold
+        for (int i = first + U * (int)blockDim.x; i < pieces; i += U * (int)blockDim.x) {
+            load(a, i);
+            store(a, i);
+        }
+    }
 };
 
-// (columns from k on, and rows past m: zeros)
-template <int XF>
-__device__ __forceinline__ void load_operand(const MxArgs &a, __amdgpu_buffer_rsrc_t rx, __amdgpu_buffer_rsrc_t rs, int u,
-                                             int ue, int lane, uint8_t *buf, XOp<XF> &x) {
-    const int r = lane & 15, k0 = u * kMxUnit + 32 * (lane >> 4);
-    const bool in = r < (int)a.m && k0 < (int)a.k && u < ue;
-    const int el = r * (int)a.k + k0;
-    auto ld = [&](int off, int at) { return __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(rx, off, at, 0)); };
-    if constexpr (XF == X_BF16 || XF == X_PLANES) {
-#pragma unroll
-        for (int p = 0; p < XOp<XF>::P; p++)
-#pragma unroll
-            for (int q = 0; q < 4; q++) x.a[p][q] = ld(in ? 2 * el : 0x7FFFFFF0, 2 * p * (int)(a.m * a.k) + 16 * q);
-    } else if constexpr (XF == X_TRI) {
-        // lane l splits columns 2l, 2l + 1 of every row; row 3t + p of the buffer is plane p of token t
-        const int c = u * kMxUnit + 2 * lane;
-#pragma unroll
-        for (int t = 0; t < 5; t++) {
-            if (t >= (int)a.m) break;
-            const u32x2 v = __builtin_bit_cast(u32x2, __builtin_amdgcn_raw_buffer_load_b64(rx, c < (int)a.k && u < ue ? 4 * (t * (int)a.k + c) : 0x7FFFFFF0, 0, 0));
-            uint32_t h, m, l;
-            split3(__uint_as_float(v[0]), __uint_as_float(v[1]), h, m, l);
-            uint32_t *o = reinterpret_cast<uint32_t *>(buf + 3 * t * kTriRow) + lane;
-            o[0] = h;
-            o[kTriRow / 4] = m;
-            o[kTriRow / 2] = l;
-        }
-        wave_sync();
-        // (rows past the tokens' read what the buffer holds: rows are independent, theirs are not stored)
-#pragma unroll
-        for (int q = 0; q < 4; q++) x.a[0][q] = *reinterpret_cast<const u32x4 *>(buf + r * kTriRow + 64 * (lane >> 4) + 16 * q);
-        wave_sync();
-    } else if constexpr (XF == X_CODES) {
-        x.a[0][0] = ld(in ? el / 2 : 0x7FFFFFF0, 0);
-        x.s = __builtin_amdgcn_raw_buffer_load_b8(rs, in ? el / 32 : 0x7FFFFFF0, 0, 0);
-    } else {
-        constexpr bool B = XF == X_Q16;
-        u32x4 v[B ? 4 : 8];
-#pragma unroll
-        for (int i = 0; i < (B ? 4 : 8); i++) v[i] = ld(in ? el * (B ? 2 : 4) : 0x7FFFFFF0, 16 * i);
-        x.a[0][0] = mx_quantize_block<B>(v, a.floor_rule, x.s);
-    }
-}
-
-// Part kp = blockIdx.x % ks of the units, in passes of waves * UPW units, over blocks blockIdx.x / ks, + gridDim.x / ks,
-// .. of R tiles.
-template <int XF, int R, int UPW>
+// Part kp = blockIdx.x % ks of the pairs, in chunks that LDS holds (as a rule one), over blocks blockIdx.x / ks, + gridDim.x
+// / ks, .. of nw tiles.
+template <int XF, int PP>
 __global__ __launch_bounds__(1024) void mx_rows_kernel(MxArgs a) {
     constexpr bool BOTH = mx_both(XF);
-    constexpr int P = XOp<XF>::P;
+    constexpr int P = XF == X_PLANES ? 3 : 1;
     const int tid = threadIdx.x, lane = tid & 63;
-    const int wv = __builtin_amdgcn_readfirstlane(tid >> 6), waves = (int)(blockDim.x >> 6);
-    // LDS: (X_TRI) a staging buffer a wave, then two reduction buffers [tile][MFMA row][column][17 waves]
+    const int wv = __builtin_amdgcn_readfirstlane(tid >> 6), kw = a.kw, nw = a.nw, wi = wv % kw, wj = wv / kw;
+    // LDS: the sums of two steps, then x
     extern __shared__ __attribute__((aligned(16))) uint8_t lds[];
-    uint8_t *buf = lds + wv * kTriBuf;
-    float *red = reinterpret_cast<float *>(lds + (XF == X_TRI ? waves * kTriBuf : 0));
-    const int m = (int)a.m, units = (int)a.units;
-    const int rows = XF == X_TRI ? 3 * m : m;  // MFMA rows that count
+    const int sums = kw * nw * kSumWave;
+    const int m = (int)a.m, rows = XF == X_TRI ? 3 * m : m;  // MFMA rows that count
+    const int all = ((int)a.units + 1) / 2;
     const int ks = a.ks, kp = (int)blockIdx.x % ks, step = (int)gridDim.x / ks;
-    const int ub = (int)((int64_t)units * kp / ks), ue = (int)((int64_t)units * (kp + 1) / ks);
-    const int npass = (ue - ub + waves * UPW - 1) / (waves * UPW);
-    const int nblock = (int)((a.ntile + R - 1) / R);
+    const int pb = (int)((int64_t)all * kp / ks), pe = (int)((int64_t)all * (kp + 1) / ks);
+    const int chunks = (pe - pb + kw * PP - 1) / (kw * PP);
+    const int nblock = (int)((a.ntile + nw - 1) / nw);
     const int c = lane & 15, p4 = lane >> 4;
-    const int64_t xel = a.m * a.k;
-    const __amdgpu_buffer_rsrc_t rx = rsrc(a.x, XF == X_CODES ? xel / 2 : XF == X_PLANES ? 6 * xel : XF == X_BF16 || XF == X_Q16 ? 2 * xel : 4 * xel);
-    const __amdgpu_buffer_rsrc_t rs = rsrc(a.xs, XF == X_CODES ? xel / 32 : 0);
-    XOp<XF> x[UPW];
-    u32x4 wq[R][UPW];
-    uint32_t ws[R][UPW];
-    const int64_t tile_bytes = (int64_t)((units + 1) / 2) * kMxPair;
-    const int ls = 2048 + 4 * (16 * (p4 & 1) + c) + (p4 >> 1);
-    // a unit that does not exist is read at the last that does (its x is zeros), a tile that does not exist as a
-    // buffer of no bytes
-    auto tile_buffer = [&](int b, int r) {
-        const int64_t tile = (int64_t)b * R + r;
+    const int64_t tile_bytes = (int64_t)all * kMxPair;
+    XStage<XF> x(a, lds + 2 * sums);
+    u32x4 wq[PP][2];
+    uint32_t ws[PP];
+    // a pair that does not exist is read at the last that does (and not used), a tile that does not exist as a buffer of
+    // no bytes
+    auto tile_buffer = [&](int b) {
+        const int64_t tile = (int64_t)b * nw + wj;
         return rsrc(a.w + min(tile, a.ntile - 1) * tile_bytes, tile < a.ntile ? tile_bytes : 0);
     };
-    auto load_w = [&](__amdgpu_buffer_rsrc_t t, int pass, int r, int j) {
-        const int u = min(ub + (pass * UPW + j) * waves + wv, ue - 1), at = (u >> 1) * kMxPair;
-        wq[r][j] = __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(t, 16 * lane, at + (u & 1) * 1024, 2));
-        ws[r][j] = __builtin_amdgcn_raw_buffer_load_b8(t, ls, at + 2 * (u & 1), 2);
-    };
-    auto load_x = [&](int pass) {
+    auto load_w = [&](__amdgpu_buffer_rsrc_t t, int chunk, int j) {
+        const int at = min(pb + (chunk * PP + j) * kw + wi, pe - 1) * kMxPair;
 #pragma unroll
-        for (int j = 0; j < UPW; j++) load_operand<XF>(a, rx, rs, ub + (pass * UPW + j) * waves + wv, ue, lane, buf, x[j]);
+        for (int h = 0; h < 2; h++) wq[j][h] = __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(t, 16 * lane, at + 1024 * h, 2));
+        ws[j] = __builtin_amdgcn_raw_buffer_load_b32(t, 2048 + 4 * (16 * (p4 & 1) + c), at, 2);
+    };
+    auto stage_part = [&](int chunk) {
+        const int p0 = pb + chunk * kw * PP;
+        x.part(a, p0, min(kw * PP, pe - p0));
     };
     uint64_t key = 0;
     int b = (int)blockIdx.x / ks, par = 0;
+    // x before the weights: loads return in order, and x comes from L2
+    stage_part(0);
+    x.load(a, tid);
+    {
+        const __amdgpu_buffer_rsrc_t t = tile_buffer(b);
 #pragma unroll
-    for (int r = 0; r < R; r++) {
-        const __amdgpu_buffer_rsrc_t t = tile_buffer(b, r);
-#pragma unroll
-        for (int j = 0; j < UPW; j++) load_w(t, 0, r, j);
+        for (int j = 0; j < PP; j++) load_w(t, 0, j);
     }
-    load_x(0);
+    x.store(a, tid);
+    x.rest(a, tid);
+    __syncthreads();
+    const int xrow = min(XF == X_PLANES ? 3 * c : c, (XF == X_PLANES ? 3 * m - 3 : rows - 1));  // (MFMA rows past the last: the last again, not stored)
     for (; b < nblock; b += step) {
-        floatx4 acc[R];
+        floatx4 acc = {0.f, 0.f, 0.f, 0.f};
+        for (int chunk = 0; chunk < chunks; chunk++) {
+            // the next step: the next chunk, or the next block's first
+            const bool last = chunk + 1 == chunks;
+            const int nb = last ? b + step : b, nc = last ? 0 : chunk + 1;
+            const __amdgpu_buffer_rsrc_t t = tile_buffer(nb);
 #pragma unroll
-        for (int r = 0; r < R; r++) acc[r] = floatx4{0.f, 0.f, 0.f, 0.f};
-        for (int pass = 0; pass < npass; pass++) {
-            // the next step: the next pass, or the next block's first; a unit's registers are loaded for it as soon as
-            // they have been used
-            const bool last = pass + 1 == npass;
-            const int nb = last ? b + step : b, np = last ? 0 : pass + 1;
+            for (int j = 0; j < PP; j++) {
+                const bool there = pb + (chunk * PP + j) * kw + wi < pe;
+                const int local = j * kw + wi;  // pair of the chunk
+                if constexpr (BOTH) {
+                    if (there) {
+                        const uint32_t xs = *reinterpret_cast<const uint32_t *>(x.words + xrow * x.row_pieces + 8 * local + 4 * (p4 & 1)) >> (8 * (p4 >> 1));
+                        const uint32_t s = ws[j] >> (8 * (p4 >> 1));
+                        const uint8_t *xa = x.lds + xrow * x.pitch + 128 * local + 16 * p4;
+                        acc = mfma_mx16<0>(*reinterpret_cast<const u32x4 *>(xa), xs, wq[j][0], s, acc);
+                        acc = mfma_mx16<2>(*reinterpret_cast<const u32x4 *>(xa + 64), xs, wq[j][1], s, acc);
+                    }
+                } else if (there) {
 #pragma unroll
-            for (int r = 0; r < R; r++) {
-                const __amdgpu_buffer_rsrc_t t = tile_buffer(nb, r);
-#pragma unroll
-                for (int j = 0; j < UPW; j++) {
-                    if constexpr (BOTH) {
-                        acc[r] = mfma_mx16(x[j].a[0][0], x[j].s, wq[r][j], ws[r][j], acc[r]);
-                    } else {
-                        const float s = mx_scale(ws[r][j]);
+                    for (int h = 0; h < 2; h++)
 #pragma unroll
                         for (int q = 0; q < 4; q++) {
-                            const u32x4 bq = mx_codes_bf16(wq[r][j][q], s);
+                            u32x4 xa[P];
+#pragma unroll
+                            for (int p = 0; p < P; p++)
+                                xa[p] = *reinterpret_cast<const u32x4 *>(x.lds + (xrow + p) * x.pitch + 512 * local + 256 * h + 64 * p4 + 16 * q);
+                            const u32x4 bq = mx_codes_bf16(wq[j][h][q], mx_scale((ws[j] >> (8 * (p4 >> 1) + 16 * h)) & 0xFFu));
                             // (the lo plane first: added to a finished hi sum its low bits would be cut off)
 #pragma unroll
-                            for (int p = P - 1; p >= 0; p--) acc[r] = mfma16x16x32_bf16(x[j].a[p][q], bq, acc[r]);
+                            for (int p = P - 1; p >= 0; p--) acc = mfma16x16x32_bf16(xa[p], bq, acc);
                         }
-                    }
-                    load_w(t, np, r, j);
                 }
+                load_w(t, nc, j);
             }
-            if (npass > 1 && nb < nblock) load_x(np);
+            if (chunks > 1 && nb < nblock) {
+                __syncthreads();
+                stage_part(nc);
+                x.load(a, tid);
+                x.store(a, tid);
+                x.rest(a, tid);
+                __syncthreads();
+            }
         }
-        float *rb = red + par * R * 16 * 272;
+        // lane 16p + c: rows 4p .. 4p + 3 of output column c -> [tile][wave along K][row][column]
+        float *sb = reinterpret_cast<float *>(lds + par * sums);
 #pragma unroll
-        for (int r = 0; r < R; r++)
-#pragma unroll
-            for (int i = 0; i < 4; i++)
-                if (4 * p4 + i < rows) rb[((r * 16 + 4 * p4 + i) * 16 + c) * 17 + wv] = acc[r][i];
+        for (int i = 0; i < 4; i++)
+            if (4 * p4 + i < rows) sb[(wj * kw + wi) * (kSumWave / 4) + (4 * p4 + i) * kSumRow + c] = acc[i];
         __syncthreads();  // also: every wave is past its reads of the other buffer
-        // a wave takes four outputs at a time, a wave's part of each to a lane of 16
-        for (int i = wv; i < R * m * 4; i += waves) {
-            int r = 0, t = i >> 2;
-#pragma unroll
-            for (int q = 1; q < R; q++)
-                if (t >= m) r++, t -= m;
-            const int col = 4 * (i & 3) + p4;
-            const float *o = rb + (r * 16 * 16 + col) * 17 + c;
+        const int outs = nw * m * 16;
+        auto put = [&](int i, float v) {
+            const int col = i & 15, t = (i >> 4) % m, tile = (i >> 4) / m;
+            const int64_t row = ((int64_t)b * nw + tile) * kTile + col;
+            if (row >= a.n) return;
+            if (ks > 1) {
+                a.slabs[((int64_t)kp * m + t) * a.n + row] = v;
+                return;
+            }
+            if (a.bias) v += a.bias[row];
+            if (a.y_bf16) reinterpret_cast<__bf16 *>(a.y)[t * a.n + row] = (__bf16)v;
+            else reinterpret_cast<float *>(a.y)[t * a.n + row] = v;
+            if (a.argmax_partial) key = max(key, mx_argmax_key(v, (uint32_t)row));
+        };
+        // waves w0, w0 + dw, .. of output i (three planes: the lo ones first)
+        auto sum = [&](int i, int w0, int dw) {
+            const int col = i & 15, t = (i >> 4) % m, tile = (i >> 4) / m;
+            const float *o = sb + tile * kw * (kSumWave / 4) + (XF == X_TRI ? 3 * t : t) * kSumRow + col;
             float v = 0.f;
-            if (c < waves) {
-                if constexpr (XF == X_TRI) v = (o[(3 * t + 2) * 272] + o[(3 * t + 1) * 272]) + o[3 * t * 272];
-                else v = o[t * 272];
+#pragma unroll
+            for (int p = XF == X_TRI ? 2 : 0; p >= 0; p--) {
+                float u = 0.f;
+                for (int w = w0; w < kw; w += dw) u += o[w * (kSumWave / 4) + p * kSumRow];
+                v += u;
             }
-            v = row_add<0xB1>(v);
-            v = row_add<0x4E>(v);
-            v = row_add<0x141>(v);
-            v = row_add<0x140>(v);
-            const int64_t row = ((int64_t)b * R + r) * kTile + col;
-            if (c == 0 && row < a.n) {
-                if (ks > 1) {
-                    a.slabs[((int64_t)kp * m + t) * a.n + row] = v;
-                    continue;
-                }
-                if (a.bias) v += a.bias[row];
-                if (a.y_bf16)
-                    reinterpret_cast<uint16_t *>(a.y)[t * a.n + row] = (uint16_t)f32_to_bf16_bits(v);
-                else
-                    reinterpret_cast<float *>(a.y)[t * a.n + row] = v;
-                if (a.argmax_partial) key = max(key, mx_argmax_key(v, (uint32_t)row));
-            }
+            return v;
+        };
+        if (outs * 8 <= (int)blockDim.x) {  // few outputs: eight lanes each
+            const int i = tid >> 3;
+            float v = i < outs ? sum(i, tid & 7, 8) : 0.f;
+            v += __uint_as_float(row_lane<0xB1>(__float_as_uint(v)));
+            v += __uint_as_float(row_lane<0x4E>(__float_as_uint(v)));
+            v += __uint_as_float(row_lane<0x141>(__float_as_uint(v)));
+            if (i < outs && (tid & 7) == 0) put(i, v);
+        } else {
+            for (int i = tid; i < outs; i += (int)blockDim.x) put(i, sum(i, 0, 1));
         }
         par ^= 1;
     }
     if (a.argmax_partial) {
-        // m = 1: lanes that stored outputs hold keys (0 elsewhere); one key per workgroup
+        // m = 1: threads that stored outputs hold keys (0 elsewhere); one key per workgroup
         __syncthreads();
-        unsigned long long *kr = reinterpret_cast<unsigned long long *>(red);
+        unsigned long long *kr = reinterpret_cast<unsigned long long *>(lds);
         for (int o = 32; o > 0; o >>= 1) {
             const uint64_t other = __shfl_xor((unsigned long long)key, o, 64);
             key = other > key ? other : key;
@@ -402,52 +443,32 @@ __global__ __launch_bounds__(1024) void mx_rows_kernel(MxArgs a) {
         if (lane == 0) kr[wv] = key;
         __syncthreads();
         if (tid == 0) {
-            for (int w = 1; w < waves; w++) key = max(key, (uint64_t)kr[w]);
+            for (int w = 1; w < kw * nw; w++) key = max(key, (uint64_t)kr[w]);
             a.argmax_partial[blockIdx.x] = key;
         }
     }
 }
 
-int cus() {
-    static int n[64] = {0};
-    int dev = 0;
-    if (hipGetDevice(&dev) != hipSuccess || dev < 0 || dev >= 64) return 256;
-    if (n[dev] == 0) {
-        int c = 0;
-        if (hipDeviceGetAttribute(&c, hipDeviceAttributeMultiprocessorCount, dev) != hipSuccess || c <= 0) c = 256;
-        n[dev] = c;  // concurrent first calls store the same value
-    }
-    return n[dev];
-}
-
-// a wave for every unit of a part of K, 4 to 16
-int rows_waves(const MxArgs &a) {
-    const int64_t part = (a.units + a.ks - 1) / a.ks;
-    int waves = 16;
-    while (waves > 4 && waves / 2 >= part) waves /= 2;
-    return waves;
-}
-
-template <int XF, int R, int UPW>
-int launch_rows_t(const MxArgs &a, void *stream) {
-    const int waves = rows_waves(a);  // the chip holds 16 / waves workgroups per CU
-    const int64_t blocks = (a.ntile + R - 1) / R;
-    const int64_t grid = std::min<int64_t>(blocks, std::max<int64_t>(1, (int64_t)cus() * (16 / waves) / a.ks)) * a.ks;
-    const size_t lds = (size_t)(XF == X_TRI ? waves * kTriBuf : 0) + 2 * R * 16 * 272 * 4;
+template <int XF, int PP>
+int launch_rows_t(const MxArgs &a, const MxRowsPlan &p, void *stream) {
+    const int64_t blocks = (a.ntile + p.nw - 1) / p.nw;
+    const int64_t grid = std::min<int64_t>(blocks, std::max(1, p.groups)) * p.ks;
     if (a.argmax_count) *a.argmax_count = grid;
-    auto *kernel = mx_rows_kernel<XF, R, UPW>;
-    hipError_t e = allow_lds(reinterpret_cast<const void *>(kernel), lds);
+    auto *kernel = mx_rows_kernel<XF, PP>;
+    hipError_t e = allow_lds(reinterpret_cast<const void *>(kernel), (size_t)p.lds);
     if (e != hipSuccess) return (int)e;
-    hipLaunchKernelGGL(kernel, dim3((unsigned)grid), dim3(waves * 64), lds, (hipStream_t)stream, a);
+    hipLaunchKernelGGL(kernel, dim3((unsigned)grid), dim3((unsigned)(p.kw * p.nw * 64)), (size_t)p.lds, (hipStream_t)stream, a);
     return (int)hipGetLastError();
 }
 
 template <int XF>
-int launch_rows_x(const MxArgs &a, void *stream) {
-    const bool two = a.ntile > 2 * (int64_t)cus() * (16 / rows_waves(a));
-    // (two units of three planes have no registers)
-    if (XF == X_PLANES || (a.units + a.ks - 1) / a.ks <= 16) return two ? launch_rows_t<XF, 2, 1>(a, stream) : launch_rows_t<XF, 1, 1>(a, stream);
-    if constexpr (XF != X_PLANES) return two ? launch_rows_t<XF, 2, 2>(a, stream) : launch_rows_t<XF, 1, 2>(a, stream);
+int launch_rows_x(const MxArgs &a, const MxRowsPlan &p, void *stream) {
+    switch (p.pp) {
+    case 1: return launch_rows_t<XF, 1>(a, p, stream);
+    case 2: return launch_rows_t<XF, 2>(a, p, stream);
+    case 3: return launch_rows_t<XF, 3>(a, p, stream);
+    case 4: return launch_rows_t<XF, 4>(a, p, stream);
+    }
     return (int)hipErrorInvalidValue;
 }
 
@@ -515,19 +536,23 @@ int launch_mx_rows(const MxArgs &g, void *scratch, void *stream) {
     if (a.m < 1 || a.m > kMxRows || a.units < 1 || a.ntile < 1 || (a.argmax_partial && (a.m != 1 || p.ks != 1)) || (p.bytes && !scratch))
         return (int)hipErrorInvalidValue;
     a.ks = p.ks;
-    a.slabs = reinterpret_cast<float *>(reinterpret_cast<uint8_t *>(scratch) + p.slabs);
+    a.kw = p.kw;
+    a.nw = p.nw;
+    uint8_t *base = reinterpret_cast<uint8_t *>(scratch);
+    a.slabs = reinterpret_cast<float *>(base + p.slabs);
     int e = 0;
-    if (a.x_kind == kMxF32 && p.planes) {
-        e = launch_mx_split(reinterpret_cast<const float *>(a.x), a.m * a.k, reinterpret_cast<uint16_t *>(scratch), stream);
+    if (p.first) {  // quantized once, not by every workgroup
+        uint8_t *scales = base + (size_t)a.m * a.k / 2;
+        e = launch_mx_quantize(a.x, a.x_kind == kMxQuantBf16, a.m, a.k, a.k, a.floor_rule, base, scales, stream);
         if (e) return e;
-        a.x = scratch;
-        e = launch_rows_x<X_PLANES>(a, stream);
-    } else {
-        e = a.x_kind == kMxBf16  ? launch_rows_x<X_BF16>(a, stream)
-            : a.x_kind == kMxF32 ? launch_rows_x<X_TRI>(a, stream)
-            : a.x_kind == kMxQuantBf16 ? launch_rows_x<X_Q16>(a, stream)
-            : a.x_kind == kMxQuantF32  ? launch_rows_x<X_Q32>(a, stream) : launch_rows_x<X_CODES>(a, stream);
+        a.x = base;
+        a.xs = scales;
+        a.x_kind = kMxCodes;
     }
+    e = a.x_kind == kMxBf16          ? launch_rows_x<X_BF16>(a, p, stream)
+                  : a.x_kind == kMxF32         ? (a.m <= kMxTriRows ? launch_rows_x<X_TRI>(a, p, stream) : launch_rows_x<X_PLANES>(a, p, stream))
+                  : a.x_kind == kMxQuantBf16   ? launch_rows_x<X_Q16>(a, p, stream)
+                  : a.x_kind == kMxQuantF32    ? launch_rows_x<X_Q32>(a, p, stream) : launch_rows_x<X_CODES>(a, p, stream);
     if (e || a.ks == 1) return e;
     return launch_int4_sum(a.slabs, a.ks, a.m, a.n, a.bias, a.y, a.y_bf16, stream);
 }

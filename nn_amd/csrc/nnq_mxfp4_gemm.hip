@@ -238,41 +238,67 @@ __global__ __launch_bounds__(W * 64, 2) void mx_gemm16_kernel(MxGemmArgs a) {
     mx_clear(acc);
     u32x4 bq[2][NT][2];
     uint32_t bs[2][NT];
-    auto load_b = [&](int u, int buf) {
+    auto load_codes = [&](int u, int par, int i) {
 #pragma unroll
-        for (int nt = 0; nt < NT; nt++) {
-#pragma unroll
-            for (int i = 0; i < 2; i++) bq[buf][nt][i] = w.codes(nt, u >> 1, 2 * (u & 1) + i);
-            bs[buf][nt] = w.scales16(nt, u);
-        }
+        for (int nt = 0; nt < NT; nt++) bq[par][nt][i] = w.codes(nt, u >> 1, 2 * (u & 1) + i);
     };
-    copy_a(at.u0, 0);
-    load_b(at.u0, 0);
-    auto unit = [&](auto parity, int u) {
-        constexpr int buf = decltype(parity)::value;
-        arrive();
-        const int next = min(u + 1, at.u1 - 1);
-        copy_a(next, buf ^ 1);
-        load_b(next, buf ^ 1);
+    auto load_scales = [&](int u, int par) {
 #pragma unroll
-        for (int s = 0; s < 8; s++) {
-            // step s: word s / 2 of blocks 2 (s % 2) + h
-            const int chunk = (2 * (s & 1) + h) * 4 + (s >> 1);
-            u32x4 af[P][MT], bf[NT];
+        for (int nt = 0; nt < NT; nt++) bs[par][nt] = w.scales16(nt, u);
+    };
+#pragma unroll
+    for (int i = 0; i < 2; i++) {
+        const int u = min(at.u0 + i, at.u1 - 1);
+        copy_a(u, i);
+        __builtin_amdgcn_sched_barrier(0);
+        load_codes(u, i, 0);
+        load_codes(u, i, 1);
+        load_scales(u, i);
+        __builtin_amdgcn_sched_barrier(0);
+    }
+    int cur = 0;  // this unit's LDS buffer of three
+    // Operands are formed, and A read, a step ahead of the MFMAs; a unit's weights are loaded for the unit after next as soon
+    // as they have been used.
+    auto unit = [&](auto parity, int u) {
+        constexpr int par = decltype(parity)::value;
+        // this unit's copies have landed: behind them came its loads, and the next unit's copies and loads
+        wait_vmcnt<NA + 2 * 3 * NT>();
+        __builtin_amdgcn_s_barrier();
+        __builtin_amdgcn_sched_barrier(0);
+        const int next = min(u + 2, at.u1 - 1);
+        const uint8_t *from = lds + cur * BUF + c32 * 256;
+        copy_a(next, cur == 0 ? 2 : cur - 1);
+        cur = cur == 2 ? 0 : cur + 1;
+        __builtin_amdgcn_sched_barrier(0);
+        u32x4 af[2][P][MT], bf[2][NT];
+        auto form = [&](int s) {  // step s: word s % 4 of blocks 2 (s / 4) + h
+            const int chunk = (2 * (s >> 2) + h) * 4 + (s & 3);
 #pragma unroll
             for (int p = 0; p < P; p++)
 #pragma unroll
                 for (int mt = 0; mt < MT; mt++)
-                    af[p][mt] = *reinterpret_cast<const u32x4 *>(lds + buf * BUF + (p * MT + mt) * kPiece + c32 * 256 + ((chunk ^ (c32 & 15)) << 4));
+                    af[s & 1][p][mt] = *reinterpret_cast<const u32x4 *>(from + (p * MT + mt) * kPiece + ((chunk ^ (c32 & 15)) << 4));
 #pragma unroll
-            for (int nt = 0; nt < NT; nt++) bf[nt] = mx_codes_bf16(bq[buf][nt][s & 1][s >> 1], mx_scale((bs[buf][nt] >> (8 * (s & 1))) & 0xFFu));
+            for (int nt = 0; nt < NT; nt++)
+                bf[s & 1][nt] = mx_codes_bf16(bq[par][nt][s >> 2][s & 3], mx_scale((bs[par][nt] >> (8 * (s >> 2))) & 0xFFu));
+        };
+        form(0);
+#pragma unroll
+        for (int s = 0; s < 8; s++) {
+            if (s < 7) form(s + 1);
+            if (s == 3) load_codes(next, par, 0);
+            if (s == 7) {
+                load_codes(next, par, 1);
+                load_scales(next, par);
+            }
             // (the lo plane first: added to a finished hi sum its low bits would be cut off)
 #pragma unroll
             for (int p = P - 1; p >= 0; p--)
 #pragma unroll
                 for (int mt = 0; mt < MT; mt++)
 #pragma unroll
-                    for (int nt = 0; nt < NT; nt++) acc[mt][nt] = mfma32_bf16(af[p][mt], bf[nt], acc[mt][nt]);
+                    for (int nt = 0; nt < NT; nt++) acc[mt][nt] = mfma32_bf16(af[s & 1][p][mt], bf[s & 1][nt], acc[mt][nt]);
+            if (s == 3 || s == 7) __builtin_amdgcn_sched_barrier(0);
         }
     };
     int u = at.u0;
@@ -281,6 +307,7 @@ __global__ __launch_bounds__(W * 64, 2) void mx_gemm16_kernel(MxGemmArgs a) {
         unit(std::integral_constant<int, 1>(), u + 1);
     }
     if (u < at.u1) unit(std::integral_constant<int, 0>(), u);
+    wait_vmcnt<0>();  // (copies for units past the last)
     mx_store(a, at, tile0, wv, lane, lds, acc);
 }
 
@@ -381,7 +408,7 @@ __global__ __launch_bounds__(W * 64, MT > 4 ? 1 : 2) void mx_gemm4_kernel(MxGemm
 
 template <int MT, int NT, int P>
 int launch16(const MxGemmArgs &a, void *stream) {
-    constexpr size_t lds = std::max(2 * MT * P * kPiece, W * kOutBuf);
+    constexpr size_t lds = std::max(3 * MT * P * kPiece, W * kOutBuf);
     auto *kernel = mx_gemm16_kernel<MT, NT, P>;
     hipError_t e = allow_lds(reinterpret_cast<const void *>(kernel), lds);
     if (e != hipSuccess) return (int)e;
@@ -428,7 +455,7 @@ int launch_mx_gemm(const MxArgs &a, void *scratch, void *stream) {
         if (e) return e;
         g.x = base;
     }
-    if (a.x_kind == kMxBf16) e = p.mt == 1 ? launch16<1, 2, 1>(g, stream) : launch16<2, 2, 1>(g, stream);
+    if (a.x_kind == kMxBf16) e = p.mt == 1 ? launch16<1, 2, 1>(g, stream) : p.mt == 2 ? launch16<2, 2, 1>(g, stream) : launch16<4, 2, 1>(g, stream);
     else if (a.x_kind == kMxF32) e = launch16<1, 2, 3>(g, stream);
     else e = p.mt == 1 ? launch4<1, 2>(g, stream) : p.mt == 2 ? launch4<2, 2>(g, stream) : p.mt == 4 ? launch4<4, 2>(g, stream) : launch4<8, 2>(g, stream);
     if (e || p.ks == 1) return e;

@@ -5,6 +5,7 @@
 // (tests/sanitize) runs the same code on the CPU over ragged and extreme shapes.
 #include <algorithm>
 #include <cmath>
+#include <cstdio>
 #include <cstdlib>
 
 #include "nnq_internal.h"
@@ -135,13 +136,48 @@ int64_t int4_chunk_rows(int64_t m, int64_t k) {
 
 bool mx_takes_rows(int64_t m, int64_t n, int64_t k, int x_kind) { return m <= kMxRows; }
 
-// f32 x of up to five rows is split into its bf16 planes by the kernel that uses it, of more by one launch before it
+// LDS bytes of x of m rows and `pairs` pairs of units (XStage)
+static int64_t mx_stage_bytes(int64_t m, int64_t pairs, int x_kind) {
+    if (x_kind >= kMxQuantBf16) return m * (pairs * 128 + 16 + pairs * 8);
+    return m * (x_kind == kMxF32 ? 3 : 1) * (pairs * 512 + 16);
+}
+
+// x that every workgroup quantizes for itself: up to this many bytes of it.  Beyond, reading it in every workgroup costs more
+// than a launch before.
+constexpr int64_t kMxFirstBytes = 196608;
+
+// A wave along K for every two pairs of units (up to 16: three or four pairs), as many more along the tiles as make four
+// waves, and as many workgroups on a CU as its 16 waves and its LDS hold; where x leaves room for one only, more waves
+// along the tiles instead (their loads are what is in flight).  Swept on MI355X over 17 shapes of 1 to 16 rows (us, waves
+// along K x tiles): 1 x 4096 -> 4096 5.5 (8 x 1), 7.0 (16 x 1), 5.9 (4 x 1); 12 x 4096 -> 24576 16.0 (8 x 2), 16.5 (4 x 3),
+// 20 (16 x 1); 1 x 512 -> 151936 11.9 (1 x 4), 25 (2 x 1).
 MxRowsPlan mx_rows_plan(int64_t m, int64_t n, int64_t k, int x_kind) {
     MxRowsPlan p{};
-    p.ks = 1;
-    p.planes = x_kind == kMxF32 && m > 5;
-    p.slabs = p.planes ? align256((size_t)m * (size_t)k * 6) : 0;
-    p.bytes = p.slabs + (p.ks > 1 ? (size_t)p.ks * (size_t)m * (size_t)n * 4 : 0);
+    const int64_t all = mx_pairs(k), tiles = mx_tiles(n), cus = 256, cap = 163840;
+    // K goes over workgroups where its x does not fit (one row: in chunks, without a second launch)
+    int64_t ks = 1;
+    while (m > 1 && ks < 8 && ks < all && mx_stage_bytes(m, (all + ks - 1) / ks, x_kind) + 2 * 16 * 1280 > cap) ks++;
+    const int64_t part = (all + ks - 1) / ks, per_cu = (tiles * ks + cus - 1) / cus;  // tiles of a CU's part
+    p.ks = (int)ks;
+    p.kw = (int)std::min<int64_t>(16, (part + 1) / 2);
+    p.pp = (int)std::min<int64_t>(4, (part + p.kw - 1) / p.kw);
+    p.nw = (int)std::min<int64_t>(per_cu, std::max(1, 4 / p.kw));
+    auto bytes = [&] { return 2 * (int64_t)p.kw * p.nw * 1280 + mx_stage_bytes(m, std::min<int64_t>(part, p.kw * p.pp), x_kind); };
+    if (const char *e = getenv("MX_ROWS")) sscanf(e, "%d,%d,%d", &p.kw, &p.nw, &p.pp);
+    while (bytes() > cap && p.pp > 1) p.pp--;
+    while (bytes() > cap && p.kw > 1) p.kw--;
+    int64_t fit = std::min<int64_t>(16 / (p.kw * p.nw), cap / bytes());
+    if (fit < 2 && per_cu > 1 && p.nw == 1 && p.kw <= 8) {
+        const int64_t steps = (per_cu + 16 / p.kw - 1) / (16 / p.kw);
+        p.nw = (int)((per_cu + steps - 1) / steps);
+        while (bytes() > cap && p.nw > 1) p.nw--;
+        fit = 1;
+    }
+    p.lds = (int)bytes();
+    p.groups = (int)std::max<int64_t>(1, cus * std::max<int64_t>(1, fit) / ks);
+    p.first = x_kind >= kMxQuantBf16 && x_kind != kMxCodes && m * k * (x_kind == kMxQuantBf16 ? 2 : 4) > kMxFirstBytes;
+    p.slabs = p.first ? align256((size_t)m * (size_t)k / 2 + (size_t)m * (size_t)k / 32) : 0;
+    p.bytes = p.slabs + (ks > 1 ? (size_t)ks * (size_t)m * (size_t)n * 4 : 0);
     return p;
 }
 
@@ -152,7 +188,7 @@ MxGemmPlan mx_gemm_plan(int64_t m, int64_t n, int64_t k, int x_kind) {
     p.nt = 2;
     p.mt = x_kind == kMxF32 ? 1 : tiles == 1 ? 1 : four && tiles > 2 ? 4 : 2;
     p.ks = 1;
-    if (four && getenv("MX_MT")) p.mt = atoi(getenv("MX_MT"));
+    if ((four || x_kind == kMxBf16) && getenv("MX_MT")) p.mt = atoi(getenv("MX_MT"));
     p.row_blocks = (int)((tiles + p.mt - 1) / p.mt);
     p.col_blocks = (int)((n + 128 * p.nt - 1) / (128 * p.nt));
     const size_t x = four ? (size_t)(mx_tiles(m) * mx_pairs(k)) * kMxPair : x_kind == kMxF32 ? (size_t)m * (size_t)k * 6 : 0;
