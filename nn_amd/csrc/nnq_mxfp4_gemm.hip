@@ -134,16 +134,17 @@ __device__ __forceinline__ void mx_store(const MxGemmArgs &a, const MxPlace &at,
         // out the operands that the next workgroups share (2048 x 4096 -> 24576 in 4 bits: 109 us, 128 with plain stores).
         __syncthreads();
         uint8_t *mine = lds + wv * kOutBuf;
-        const int row8 = lane >> 3, at16 = lane & 7;
-        auto flush = [&](int mt, uint8_t *y, int64_t col0, int elem) {  // y: of element [0][0]
+        auto flush = [&](auto bytes, int mt, uint8_t *y, int64_t col0, int elem) {  // rows of so many bytes; y: of element [0][0]
+            constexpr int L = decltype(bytes)::value / 16;  // lanes of a row
             __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
             __builtin_amdgcn_wave_barrier();
             __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
-            const int64_t col = col0 + at16 * (16 / elem);
+            const int64_t col = col0 + lane % L * (16 / elem);
 #pragma unroll
-            for (int i = 0; i < 4; i++) {
-                const u32x4 v = *reinterpret_cast<const u32x4 *>(mine + (8 * i + row8) * kOutRow + at16 * 16);
-                const int64_t row = (at.rb * MT + mt) * 32 + 8 * i + row8;
+            for (int i = 0; i < L / 2; i++) {
+                const int r = 64 / L * i + lane / L;
+                const u32x4 v = *reinterpret_cast<const u32x4 *>(mine + r * kOutRow + lane % L * 16);
+                const int64_t row = (at.rb * MT + mt) * 32 + r;
                 if (row < a.m && col < a.n) __builtin_nontemporal_store(v, reinterpret_cast<u32x4 *>(y + (row * a.n + col) * elem));
             }
             __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
@@ -156,20 +157,21 @@ __device__ __forceinline__ void mx_store(const MxGemmArgs &a, const MxPlace &at,
             const int64_t col0 = (int64_t)tile0 * kTile;
             uint8_t *p = mine + 4 * h * kOutRow;
             if (bf16) {
-                static_assert(NT == 2, "128 bytes of bf16");
 #pragma unroll
-                for (int nt = 0; nt < NT; nt++)
+                for (int nt = 0; nt < NT; nt++) {
 #pragma unroll
                     for (int e = 0; e < 16; e++)
-                        *reinterpret_cast<__bf16 *>(p + (8 * (e / 4) + e % 4) * kOutRow + (32 * nt + (lane & 31)) * 2) = (__bf16)acc[mt][nt][e];
-                flush(mt, reinterpret_cast<uint8_t *>(a.y), col0, 2);
+                        *reinterpret_cast<__bf16 *>(p + (8 * (e / 4) + e % 4) * kOutRow + (32 * (nt & 1) + (lane & 31)) * 2) = (__bf16)acc[mt][nt][e];
+                    if (nt & 1) flush(std::integral_constant<int, 128>(), mt, reinterpret_cast<uint8_t *>(a.y), col0 + 32 * (nt - 1), 2);
+                    else if (nt == NT - 1) flush(std::integral_constant<int, 64>(), mt, reinterpret_cast<uint8_t *>(a.y), col0 + 32 * nt, 2);
+                }
             } else {
 #pragma unroll
                 for (int nt = 0; nt < NT; nt++) {
 #pragma unroll
                     for (int e = 0; e < 16; e++)
                         *reinterpret_cast<float *>(p + (8 * (e / 4) + e % 4) * kOutRow + (lane & 31) * 4) = acc[mt][nt][e];
-                    flush(mt, reinterpret_cast<uint8_t *>(slabs), col0 + 32 * nt, 4);
+                    flush(std::integral_constant<int, 128>(), mt, reinterpret_cast<uint8_t *>(slabs), col0 + 32 * nt, 4);
                 }
             }
         }
@@ -455,9 +457,22 @@ int launch_mx_gemm(const MxArgs &a, void *scratch, void *stream) {
         if (e) return e;
         g.x = base;
     }
-    if (a.x_kind == kMxBf16) e = p.mt == 1 ? launch16<1, 2, 1>(g, stream) : p.mt == 2 ? launch16<2, 2, 1>(g, stream) : launch16<4, 2, 1>(g, stream);
-    else if (a.x_kind == kMxF32) e = launch16<1, 2, 3>(g, stream);
-    else e = p.mt == 1 ? launch4<1, 2>(g, stream) : p.mt == 2 ? launch4<2, 2>(g, stream) : p.mt == 4 ? launch4<4, 2>(g, stream) : launch4<8, 2>(g, stream);
+    const int tile = 10 * p.mt + p.nt;
+    e = (int)hipErrorInvalidValue;
+    if (a.x_kind == kMxBf16)
+        e = tile == 12   ? launch16<1, 2, 1>(g, stream)
+            : tile == 13 ? launch16<1, 3, 1>(g, stream)
+            : tile == 22 ? launch16<2, 2, 1>(g, stream)
+            : tile == 23 ? launch16<2, 3, 1>(g, stream)
+            : tile == 42 ? launch16<4, 2, 1>(g, stream) : e;
+    else if (a.x_kind == kMxF32)
+        e = tile == 12 ? launch16<1, 2, 3>(g, stream) : tile == 13 ? launch16<1, 3, 3>(g, stream) : tile == 22 ? launch16<2, 2, 3>(g, stream) : e;
+    else
+        e = tile == 12   ? launch4<1, 2>(g, stream)
+            : tile == 13 ? launch4<1, 3>(g, stream)
+            : tile == 22 ? launch4<2, 2>(g, stream)
+            : tile == 23 ? launch4<2, 3>(g, stream)
+            : tile == 42 ? launch4<4, 2>(g, stream) : e;
     if (e || p.ks == 1) return e;
     return launch_int4_sum(slabs, p.ks, a.m, a.n, a.bias, a.y, a.y_bf16, stream);
 }

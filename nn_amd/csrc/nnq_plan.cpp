@@ -188,7 +188,7 @@ MxGemmPlan mx_gemm_plan(int64_t m, int64_t n, int64_t k, int x_kind) {
     p.nt = 2;
     p.mt = x_kind == kMxF32 ? 1 : tiles == 1 ? 1 : four && tiles > 2 ? 4 : 2;
     p.ks = 1;
-    if ((four || x_kind == kMxBf16) && getenv("MX_MT")) p.mt = atoi(getenv("MX_MT"));
+    if (const char *e = getenv("MX_CFG")) sscanf(e, "%d,%d,%d", &p.mt, &p.nt, &p.ks);
     p.row_blocks = (int)((tiles + p.mt - 1) / p.mt);
     p.col_blocks = (int)((n + 128 * p.nt - 1) / (128 * p.nt));
     const size_t x = four ? (size_t)(mx_tiles(m) * mx_pairs(k)) * kMxPair : x_kind == kMxF32 ? (size_t)m * (size_t)k * 6 : 0;
