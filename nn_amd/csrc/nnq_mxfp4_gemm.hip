@@ -42,6 +42,8 @@ __device__ __forceinline__ void copy4_lds(__amdgpu_buffer_rsrc_t t, uint8_t *lds
 #endif
 }
 
+typedef u32x4 u32x4_at4 __attribute__((aligned(4)));
+typedef u32x4 u32x4_at2 __attribute__((aligned(2)));
 // a wave's LDS for 32 rows of 128 bytes of outputs
 constexpr int kOutRow = 144, kOutBuf = 32 * kOutRow;
 
@@ -52,7 +54,6 @@ struct MxGemmArgs {
     int y_bf16;
     int m, units, ntile, ks;
     int row_blocks, col_blocks;
-    int wide;              // rows of y (or the slabs) are whole aligned 16-byte pieces
     int64_t n, k;
 };
 
@@ -128,74 +129,62 @@ __device__ __forceinline__ void mx_store(const MxGemmArgs &a, const MxPlace &at,
     }
     const bool bf16 = !slab && a.y_bf16;
     float *slabs = reinterpret_cast<float *>(a.y) + (slab ? (int64_t)at.kp * a.m * a.n : 0);
-    if (a.wide) {
-        // Through LDS, 32 rows of 128 bytes at a time, so that a store is eight rows' 16 bytes a lane.  The wave's own
-        // part of what held A (every wave is past it), whose accesses stay in order.  Non-temporal: outputs in L2 would push
-        // out the operands that the next workgroups share (2048 x 4096 -> 24576 in 4 bits: 109 us, 128 with plain stores).
-        __syncthreads();
-        uint8_t *mine = lds + wv * kOutBuf;
-        auto flush = [&](auto bytes, int mt, uint8_t *y, int64_t col0, int elem) {  // rows of so many bytes; y: of element [0][0]
-            constexpr int L = decltype(bytes)::value / 16;  // lanes of a row
-            __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
-            __builtin_amdgcn_wave_barrier();
-            __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
-            const int64_t col = col0 + lane % L * (16 / elem);
+    // Through LDS, 32 rows of 128 bytes at a time, so that a store is eight rows' 16 bytes a lane.  The wave's own
+    // part of what held A (every wave is past it), whose accesses stay in order.  Non-temporal: outputs in L2 would push
+    // out the operands that the next workgroups share (2048 x 4096 -> 24576 in 4 bits: 109 us, 128 with plain stores).
+    __syncthreads();
+    uint8_t *mine = lds + wv * kOutBuf;
+    auto flush = [&](auto bytes, int mt, uint8_t *y, int64_t col0, int elem) {  // rows of so many bytes; y: of element [0][0]
+        constexpr int L = decltype(bytes)::value / 16;  // lanes of a row
+        __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+        __builtin_amdgcn_wave_barrier();
+        __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+        const int64_t col = col0 + lane % L * (16 / elem);
 #pragma unroll
-            for (int i = 0; i < L / 2; i++) {
-                const int r = 64 / L * i + lane / L;
-                const u32x4 v = *reinterpret_cast<const u32x4 *>(mine + r * kOutRow + lane % L * 16);
-                const int64_t row = (at.rb * MT + mt) * 32 + r;
-                if (row < a.m && col < a.n) __builtin_nontemporal_store(v, reinterpret_cast<u32x4 *>(y + (row * a.n + col) * elem));
-            }
-            __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
-            __builtin_amdgcn_wave_barrier();
-            __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
-        };
-#pragma unroll
-        for (int mt = 0; mt < MT; mt++) {
-            if ((at.rb * MT + mt) * 32 >= a.m) return;
-            const int64_t col0 = (int64_t)tile0 * kTile;
-            uint8_t *p = mine + 4 * h * kOutRow;
-            if (bf16) {
-#pragma unroll
-                for (int nt = 0; nt < NT; nt++) {
-#pragma unroll
-                    for (int e = 0; e < 16; e++)
-                        *reinterpret_cast<__bf16 *>(p + (8 * (e / 4) + e % 4) * kOutRow + (32 * (nt & 1) + (lane & 31)) * 2) = (__bf16)acc[mt][nt][e];
-                    if (nt & 1) flush(std::integral_constant<int, 128>(), mt, reinterpret_cast<uint8_t *>(a.y), col0 + 32 * (nt - 1), 2);
-                    else if (nt == NT - 1) flush(std::integral_constant<int, 64>(), mt, reinterpret_cast<uint8_t *>(a.y), col0 + 32 * nt, 2);
-                }
+        for (int i = 0; i < L / 2; i++) {
+            const int r = 64 / L * i + lane / L;
+            const u32x4 v = *reinterpret_cast<const u32x4 *>(mine + r * kOutRow + lane % L * 16);
+            const int64_t row = (at.rb * MT + mt) * 32 + r;
+            uint8_t *o = y + (row * a.n + col) * elem;
+            if (row >= a.m || col >= a.n) continue;
+            if (col + 16 / elem <= a.n) {  // (16 bytes at the element's alignment: rows need not be whole pieces)
+                if (elem == 4) __builtin_nontemporal_store(v, reinterpret_cast<u32x4_at4 *>(o));
+                else __builtin_nontemporal_store(v, reinterpret_cast<u32x4_at2 *>(o));
             } else {
-#pragma unroll
-                for (int nt = 0; nt < NT; nt++) {
-#pragma unroll
-                    for (int e = 0; e < 16; e++)
-                        *reinterpret_cast<float *>(p + (8 * (e / 4) + e % 4) * kOutRow + (lane & 31) * 4) = acc[mt][nt][e];
-                    flush(std::integral_constant<int, 128>(), mt, reinterpret_cast<uint8_t *>(slabs), col0 + 32 * nt, 4);
+                for (int e = 0; e < 16 / elem && col + e < a.n; e++) {
+                    if (elem == 4) reinterpret_cast<uint32_t *>(o)[e] = v[e];
+                    else reinterpret_cast<uint16_t *>(o)[e] = (uint16_t)(v[e >> 1] >> (16 * (e & 1)));
                 }
             }
         }
-        return;
-    }
-    auto store = [&](auto *y, auto &&as) {
+        __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+        __builtin_amdgcn_wave_barrier();
+        __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+    };
 #pragma unroll
-        for (int mt = 0; mt < MT; mt++) {
-            const int row0 = (at.rb * MT + mt) * 32 + 4 * h;
+    for (int mt = 0; mt < MT; mt++) {
+        if ((at.rb * MT + mt) * 32 >= a.m) return;
+        const int64_t col0 = (int64_t)tile0 * kTile;
+        uint8_t *p = mine + 4 * h * kOutRow;
+        if (bf16) {
 #pragma unroll
             for (int nt = 0; nt < NT; nt++) {
-                const int64_t col = (int64_t)(tile0 + 2 * nt) * kTile + (lane & 31);
-                if (col >= a.n) continue;
-                auto *p = y + (int64_t)row0 * a.n + col;
 #pragma unroll
-                for (int e = 0; e < 16; e++) {
-                    if (row0 + 8 * (e / 4) + e % 4 < a.m) *p = as(acc[mt][nt][e]);
-                    p += e % 4 == 3 ? 5 * a.n : a.n;
-                }
+                for (int e = 0; e < 16; e++)
+                    *reinterpret_cast<__bf16 *>(p + (8 * (e / 4) + e % 4) * kOutRow + (32 * (nt & 1) + (lane & 31)) * 2) = (__bf16)acc[mt][nt][e];
+                if (nt & 1) flush(std::integral_constant<int, 128>(), mt, reinterpret_cast<uint8_t *>(a.y), col0 + 32 * (nt - 1), 2);
+                else if (nt == NT - 1) flush(std::integral_constant<int, 64>(), mt, reinterpret_cast<uint8_t *>(a.y), col0 + 32 * nt, 2);
+            }
+        } else {
+#pragma unroll
+            for (int nt = 0; nt < NT; nt++) {
+#pragma unroll
+                for (int e = 0; e < 16; e++)
+                    *reinterpret_cast<float *>(p + (8 * (e / 4) + e % 4) * kOutRow + (lane & 31) * 4) = acc[mt][nt][e];
+                flush(std::integral_constant<int, 128>(), mt, reinterpret_cast<uint8_t *>(slabs), col0 + 32 * nt, 4);
             }
         }
-    };
-    if (bf16) store(reinterpret_cast<__bf16 *>(a.y), [](float v) { return (__bf16)v; });
-    else store(slabs, [](float v) { return v; });
+    }
 }
 
 template <int MT, int NT>
@@ -448,7 +437,6 @@ int launch_mx_gemm(const MxArgs &a, void *scratch, void *stream) {
     g.col_blocks = p.col_blocks;
     g.n = a.n;
     g.k = a.k;
-    g.wide = a.n % (p.ks > 1 || !a.y_bf16 ? 4 : 8) == 0 && (uintptr_t)g.y % 16 == 0;
     int e = 0;
     if (a.x_kind != kMxBf16) {
         if (a.x_kind == kMxF32) e = launch_mx_split(reinterpret_cast<const float *>(a.x), a.m * a.k, reinterpret_cast<uint16_t *>(base), stream);
@@ -463,13 +451,11 @@ int launch_mx_gemm(const MxArgs &a, void *scratch, void *stream) {
         e = tile == 12   ? launch16<1, 2, 1>(g, stream)
             : tile == 13 ? launch16<1, 3, 1>(g, stream)
             : tile == 22 ? launch16<2, 2, 1>(g, stream)
-            : tile == 23 ? launch16<2, 3, 1>(g, stream)
-            : tile == 42 ? launch16<4, 2, 1>(g, stream) : e;
+            : tile == 23 ? launch16<2, 3, 1>(g, stream) : e;
     else if (a.x_kind == kMxF32)
         e = tile == 12 ? launch16<1, 2, 3>(g, stream) : tile == 13 ? launch16<1, 3, 3>(g, stream) : tile == 22 ? launch16<2, 2, 3>(g, stream) : e;
     else
         e = tile == 12   ? launch4<1, 2>(g, stream)
-            : tile == 13 ? launch4<1, 3>(g, stream)
             : tile == 22 ? launch4<2, 2>(g, stream)
             : tile == 23 ? launch4<2, 3>(g, stream)
             : tile == 42 ? launch4<4, 2>(g, stream) : e;

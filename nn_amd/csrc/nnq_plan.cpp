@@ -5,8 +5,6 @@
 // (tests/sanitize) runs the same code on the CPU over ragged and extreme shapes.
 #include <algorithm>
 #include <cmath>
-#include <cstdio>
-#include <cstdlib>
 
 #include "nnq_internal.h"
 
@@ -134,7 +132,11 @@ int64_t int4_chunk_rows(int64_t m, int64_t k) {
 
 // ---- MXFP4 rows ----
 
-bool mx_takes_rows(int64_t m, int64_t n, int64_t k, int x_kind) { return m <= kMxRows; }
+// Up to 16 rows the kernel for rows, unless over eight rows and many tiles K would go over workgroups (us, rows / GEMM: 16
+// bf16 rows of 4096 -> 24576 22.9 / 19.0, 12 f32 rows of 2048 -> 151936 99 / 69; 16 of 12288 -> 4096 16.1 / 17.6).
+bool mx_takes_rows(int64_t m, int64_t n, int64_t k, int x_kind) {
+    return m <= 8 || (m <= kMxRows && (mx_tiles(n) <= 256 || mx_rows_plan(m, n, k, x_kind).ks == 1));
+}
 
 // LDS bytes of x of m rows and `pairs` pairs of units (XStage)
 static int64_t mx_stage_bytes(int64_t m, int64_t pairs, int x_kind) {
@@ -142,9 +144,9 @@ static int64_t mx_stage_bytes(int64_t m, int64_t pairs, int x_kind) {
     return m * (x_kind == kMxF32 ? 3 : 1) * (pairs * 512 + 16);
 }
 
-// x that every workgroup quantizes for itself: up to this many bytes of it.  Beyond, reading it in every workgroup costs more
-// than a launch before.
-constexpr int64_t kMxFirstBytes = 196608;
+// The most values of x that every workgroup quantizes for itself; beyond, a launch before costs less (us, in the call /
+// before: 8 bf16 rows of 12288 -> 4096 12.6 / 12.7, of 4096 -> 4096 6.4 / 8.2; 8 f32 rows of 4096 -> 4096 12.6 / 8.7).
+constexpr int64_t kMxFirstBf16 = 98304, kMxFirstF32 = 16384;
 
 // A wave along K for every two pairs of units (up to 16: three or four pairs), as many more along the tiles as make four
 // waves, and as many workgroups on a CU as its 16 waves and its LDS hold; where x leaves room for one only, more waves
@@ -163,7 +165,6 @@ MxRowsPlan mx_rows_plan(int64_t m, int64_t n, int64_t k, int x_kind) {
     p.pp = (int)std::min<int64_t>(4, (part + p.kw - 1) / p.kw);
     p.nw = (int)std::min<int64_t>(per_cu, std::max(1, 4 / p.kw));
     auto bytes = [&] { return 2 * (int64_t)p.kw * p.nw * 1280 + mx_stage_bytes(m, std::min<int64_t>(part, p.kw * p.pp), x_kind); };
-    if (const char *e = getenv("MX_ROWS")) sscanf(e, "%d,%d,%d", &p.kw, &p.nw, &p.pp);
     while (bytes() > cap && p.pp > 1) p.pp--;
     while (bytes() > cap && p.kw > 1) p.kw--;
     int64_t fit = std::min<int64_t>(16 / (p.kw * p.nw), cap / bytes());
@@ -175,23 +176,47 @@ MxRowsPlan mx_rows_plan(int64_t m, int64_t n, int64_t k, int x_kind) {
     }
     p.lds = (int)bytes();
     p.groups = (int)std::max<int64_t>(1, cus * std::max<int64_t>(1, fit) / ks);
-    p.first = x_kind >= kMxQuantBf16 && x_kind != kMxCodes && m * k * (x_kind == kMxQuantBf16 ? 2 : 4) > kMxFirstBytes;
+    p.first = (x_kind == kMxQuantBf16 && m * k > kMxFirstBf16) || (x_kind == kMxQuantF32 && m * k > kMxFirstF32);
     p.slabs = p.first ? align256((size_t)m * (size_t)k / 2 + (size_t)m * (size_t)k / 32) : 0;
     p.bytes = p.slabs + (ks > 1 ? (size_t)ks * (size_t)m * (size_t)n * 4 : 0);
     return p;
 }
 
+// More rows: the workgroup tile (mt x 32 rows, nt x 128 columns) and the K split of the least estimated time.  c
+// workgroups on a CU take c * step + lag for each stage of K (128 k, products of 4-bit operands 256), fitted on MI355X to 15
+// shapes of 17 to 2048 rows with all tiles and splits: the choice takes 1% more than the best of them in the mean, 9% at
+// most.  With K split the slabs are written and read back at 4 TB/s by one launch more.
 MxGemmPlan mx_gemm_plan(int64_t m, int64_t n, int64_t k, int x_kind) {
+    struct Tile {
+        int mt, nt;
+        double step, lag;
+    };
+    static const Tile four[] = {{1, 2, 0.274, 0.057}, {2, 2, 0.348, 0.068}, {2, 3, 0.493, 0.084}, {4, 2, 0.66, 0.0}};
+    static const Tile bf16[] = {{1, 2, 0.306, 0.115}, {1, 3, 0.416, 0.184}, {2, 2, 0.445, 0.267}, {2, 3, 0.655, 0.358}};
+    static const Tile f32[] = {{1, 2, 0.847, 0.316}, {1, 3, 1.198, 0.329}, {2, 2, 2.12, 0.0}};
     MxGemmPlan p{};
-    const bool four = x_kind >= kMxQuantBf16;
-    const int64_t tiles = (m + 31) / 32;
-    p.nt = 2;
-    p.mt = x_kind == kMxF32 ? 1 : tiles == 1 ? 1 : four && tiles > 2 ? 4 : 2;
-    p.ks = 1;
-    if (const char *e = getenv("MX_CFG")) sscanf(e, "%d,%d,%d", &p.mt, &p.nt, &p.ks);
-    p.row_blocks = (int)((tiles + p.mt - 1) / p.mt);
+    const bool both = x_kind >= kMxQuantBf16;
+    const Tile *tiles = both ? four : x_kind == kMxBf16 ? bf16 : f32;
+    const int count = x_kind == kMxF32 ? 3 : 4;
+    const int64_t cus = 256, rows = (m + 31) / 32, pairs = mx_pairs(k), stages = both ? pairs : mx_units(k);
+    double best = 1e30;
+    for (int i = 0; i < count; i++)
+        for (int64_t s = 1; s <= 8 && (s == 1 || pairs / s >= 2); s++) {
+            const Tile &t = tiles[i];
+            const int64_t wg = (rows + t.mt - 1) / t.mt * ((n + 128 * t.nt - 1) / (128 * t.nt)) * s;
+            const double c = wg > 4 * cus ? (double)wg / cus : (double)((wg + cus - 1) / cus);
+            double us = (double)((stages + s - 1) / s) * (c * t.step + t.lag);
+            if (s > 1) us += 2.5 + (double)(2 * s) * (double)m * (double)n * 4 / 4.1e6;
+            if (us < best) {
+                best = us;
+                p.mt = t.mt;
+                p.nt = t.nt;
+                p.ks = (int)s;
+            }
+        }
+    p.row_blocks = (int)((rows + p.mt - 1) / p.mt);
     p.col_blocks = (int)((n + 128 * p.nt - 1) / (128 * p.nt));
-    const size_t x = four ? (size_t)(mx_tiles(m) * mx_pairs(k)) * kMxPair : x_kind == kMxF32 ? (size_t)m * (size_t)k * 6 : 0;
+    const size_t x = both ? (size_t)(mx_tiles(m) * pairs) * kMxPair : x_kind == kMxF32 ? (size_t)m * (size_t)k * 6 : 0;
     p.slabs = align256(x);
     p.bytes = p.slabs + (p.ks > 1 ? (size_t)p.ks * (size_t)m * (size_t)n * 4 : 0);
     return p;
