@@ -415,6 +415,11 @@ _SCALE_RULES = {"ceil": 0, "floor": 1}
 
 
 def _mxfp4_rows(codes, scales):
+    # (a small call is bound by its host side: what is right as a rule is looked at first, at once)
+    if (isinstance(codes, torch.Tensor) and isinstance(scales, torch.Tensor) and codes.dtype is torch.uint8 and
+            scales.dtype is torch.uint8 and codes.dim() and codes.shape[-1] % 16 == 0 and
+            scales.shape == (*codes.shape[:-1], codes.shape[-1] // 16)):
+        return codes, scales
     for t, what in ((codes, "codes"), (scales, "scales")):
         if not isinstance(t, torch.Tensor):
             raise Unsupported(f"{what} must be a tensor")
@@ -443,13 +448,14 @@ class Mxfp4Rows(NamedTuple):
         codes, scales = _mxfp4_rows(self.codes, self.scales)
         _device_input(codes, "codes")
         _device_input(scales, "scales", codes.device.index)
-        if dtype not in (torch.float32, torch.bfloat16):
+        if dtype is not torch.float32 and dtype is not torch.bfloat16:
             raise Unsupported(f"output dtype {dtype} (float32 or bfloat16)")
-        out = torch.empty((*codes.shape[:-1], 2 * codes.shape[-1]), dtype=dtype, device=codes.device)
-        if out.numel():
+        k = 2 * codes.shape[-1]
+        out = codes.new_empty((*codes.shape[:-1], k), dtype=dtype)
+        n = out.numel()
+        if n:
             c, s = _aligned(codes.contiguous(), 4), scales.contiguous()
-            k = out.shape[-1]
-            _launch(out, _lib.load().nnq_mxfp4_dequantize, _ptr(c), _ptr(s), out.numel() // k, k, _ptr(out), _DTYPE[dtype])
+            _launch(out, _lib.load().nnq_mxfp4_dequantize, c.data_ptr(), s.data_ptr(), n // k, k, out.data_ptr(), _DTYPE[dtype])
         return out
 
 
@@ -465,18 +471,19 @@ def quantize_mxfp4_rows(x: torch.Tensor, scale_rule: str = "ceil") -> Mxfp4Rows:
     nearest, halves to even.  A block with NaN or an infinity becomes NaN (scale 255).  No host synchronisation."""
     rule = _scale_rule(scale_rule)
     _device_input(x, "x")
-    if x.dim() < 1 or x.shape[-1] == 0 or x.shape[-1] % 32:
+    k = x.shape[-1] if x.dim() else 0
+    if k == 0 or k % 32:
         raise InvalidShape(f"x {list(x.shape)}: the last dimension must be a positive multiple of 32")
-    if x.dtype not in (torch.float32, torch.bfloat16):
+    if x.dtype is not torch.float32 and x.dtype is not torch.bfloat16:
         x = x.float()
-    k = x.shape[-1]
     v = x if x.dim() <= 2 else x.reshape(-1, k)
     if v.stride(-1) != 1:
         v = v.contiguous()
-    codes = torch.empty((*x.shape[:-1], k // 2), dtype=torch.uint8, device=x.device)
-    scales = torch.empty((*x.shape[:-1], k // 32), dtype=torch.uint8, device=x.device)
-    _launch(v, _lib.load().nnq_mxfp4_quantize, _ptr(v), _DTYPE[v.dtype], x.numel() // k, k, v.stride(0) if v.dim() == 2 else k,
-            rule, _ptr(codes), _ptr(scales))
+    batch = x.shape[:-1]
+    codes = x.new_empty((*batch, k // 2), dtype=torch.uint8)
+    scales = x.new_empty((*batch, k // 32), dtype=torch.uint8)
+    _launch(v, _lib.load().nnq_mxfp4_quantize, v.data_ptr(), _DTYPE[v.dtype], x.numel() // k, k,
+            v.stride(0) if v.dim() == 2 else k, rule, codes.data_ptr(), scales.data_ptr())
     return Mxfp4Rows(codes, scales)
 
 
@@ -758,7 +765,7 @@ def beam_select(logits: torch.Tensor, scores: torch.Tensor, keep: Optional[int] 
     batch, beams, n = logits.shape[:-2], logits.shape[-2], logits.shape[-1]
     if not isinstance(scores, torch.Tensor) or scores.shape != logits.shape[:-1]:
         raise ShapeMismatch(f"scores must be a tensor {[*batch, beams]}, one per row of logits")
-    if scores.is_complex():
+    if scores.dtype is not torch.float32 and scores.is_complex():
         raise Unsupported(f"scores must be real, got {scores.dtype}")
     keep = beams if keep is None else int(keep)
     if not 1 <= beams <= 32 or not 1 <= keep <= 32:
@@ -775,8 +782,9 @@ def beam_select(logits: torch.Tensor, scores: torch.Tensor, keep: Optional[int] 
     if v.stride(-1) != 1 and n > 1:
         v = v.contiguous()
     items = v.shape[0] if v.dim() == 3 else 1
-    out = torch.empty((*batch, keep), dtype=torch.float32, device=v.device)
-    parents, tokens = torch.empty((2, *batch, keep), dtype=torch.int64, device=v.device).unbind(0)
+    shape = (*batch, keep)
+    out = s.new_empty(shape)
+    parents, tokens = s.new_empty(shape, dtype=torch.int64), s.new_empty(shape, dtype=torch.int64)
     _launch(v, _lib.load().nnq_beam_select, _ptr(v), _DTYPE[v.dtype], items, beams, n, v.stride(0) if v.dim() == 3 else 0,
             v.stride(-2), _ptr(s), _ptr(f), int(end_token), keep, _ptr(out), _ptr(parents), _ptr(tokens))
     return BeamSelection(out, parents, tokens)
@@ -801,29 +809,30 @@ def beam_reorder(states, parents: torch.Tensor, dim: int = 0) -> None:
     if not 1 <= beams <= 32:
         raise InvalidShape(f"{beams} beams (1 to 32)")
     alike = {}
+    device, slots = parents.device, batch * beams
     for t in states:
-        _device_input(t, "state")
-        if t.device != parents.device:
-            raise Unsupported(f"state is on {t.device}, parents on {parents.device}")
-        if not -t.dim() <= dim < t.dim():
-            raise RankMismatch(f"a state of rank {t.dim()} has no dimension {dim}")
-        d = dim % t.dim()
-        if t.shape[d] != batch * beams:
-            raise ShapeMismatch(f"state {list(t.shape)} must have {batch} x {beams} slots along dimension {d}")
+        if not isinstance(t, torch.Tensor) or t.device != device:
+            raise Unsupported(f"a state must be a tensor on {device}, as parents are")
+        shape = t.shape
+        if not -len(shape) <= dim < len(shape):
+            raise RankMismatch(f"a state of rank {len(shape)} has no dimension {dim}")
+        if shape[dim] != slots:
+            raise ShapeMismatch(f"state {list(shape)} must have {batch} x {beams} slots along dimension {dim}")
         if t.numel():
-            alike.setdefault((t.shape, t.stride(), t.element_size(), d), []).append(t.data_ptr())
+            alike.setdefault((shape, t.stride(), t.dtype), []).append(t.data_ptr())
     for ptrs in alike.values():
         if len(set(ptrs)) != len(ptrs):
             raise TensorError("a state is given twice")
     p = parents if parents.dtype is torch.int64 else parents.long()
     p = p.contiguous()
-    for (shape, stride, elem, d), ptrs in alike.items():
+    for (shape, stride, dtype), ptrs in alike.items():
+        d = dim % len(shape)
         sizes, strides = [*shape[:d], *shape[d + 1:]], [*stride[:d], *stride[d + 1:]]
         if len(sizes) > 8:
             raise Unsupported(f"a state of rank {len(shape)} (at most 9)")
         i64s = ctypes.c_int64 * len(sizes)
         _launch(p, _lib.load().nnq_beam_reorder, (ctypes.c_void_p * len(ptrs))(*ptrs), len(ptrs), batch, beams, stride[d], len(sizes),
-                i64s(*sizes), i64s(*strides), elem, _ptr(p))
+                i64s(*sizes), i64s(*strides), dtype.itemsize, p.data_ptr())
 
 
 # ---------------------------------------------------------------------------------
