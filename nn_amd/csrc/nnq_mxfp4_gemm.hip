@@ -2,9 +2,19 @@
 //  * mx_gemm16_kernel: x in bf16 (f32 x: three bf16 planes that sum to it), 32x32x16 bf16 MFMAs.  A code times its
 //    scale is exact in bf16, one conversion for two of them, so nothing is scaled afterwards.
 //  * mx_gemm4_kernel: x quantized to MXFP4, 32x32x64 block-scaled MFMAs on the codes and scales as they are.
-// A workgroup of four waves takes MT * 32 rows and NT * 128 columns.  The A pieces of a unit (128 k) are copied
-// straight to one of two LDS buffers, a unit ahead, with one barrier a unit; a wave's weights go from memory into its
-// registers, a unit ahead too.  With too few workgroups K is split: f32 slabs, added in order.
+// A workgroup of four waves takes MT * 32 rows and NT * 128 columns.  The A pieces of a stage of K are copied straight to
+// LDS (three buffers, two stages ahead, in the bf16 kernel with stages of 128 k; two buffers with stages of 256 k), with one
+// barrier a stage; a wave's weights go from memory into its registers as far ahead, and none passes through LDS.  With too
+// few workgroups K is split: f32 slabs, added in order.
+// Measured (MI355X, in a graph over copies of the weight that pass the Infinity Cache; the library's bf16 product of 8192^3
+// reaches 1.14 PFLOP/s; the MFMAs alone from registers, on random data, 1.61 in bf16 and 6.4 in 4 bits):
+//  * 512 bf16 rows of 4096 -> 12288 46 to 51 us, 1.0 to 1.1 PFLOP/s; 2048 rows 172 us, 1.2: bound by the MFMAs at the clock that
+//    they leave.  300 f32 rows cost three times as much.
+//  * 2048 rows of 4096 -> 24576 in 4 bits 104 to 113 us with 7 of quantization, 3.7 to 3.9 PFLOP/s.  Variants that leave work
+//    out say what of the kernel's 103: the MFMAs alone 60, with the LDS reads 65, the copies of A 72, the loads of B 91, the
+//    stores 103.  The loads are 98 KB a stage and CU, 85% of what its L1 delivers beside the MFMAs.  One wave a SIMD with
+//    256 rows a workgroup (122 us), a third buffer (112) and eight waves that share A (115 / 115) were no faster.
+//  * 301 f32 rows of 2880 -> 5751 in 4 bits 18 us: latency of two launches, 12 stages and the first loads.
 #include <algorithm>
 #include <type_traits>
 
@@ -32,9 +42,8 @@ __device__ __forceinline__ floatx16 mfma32_mx(u32x4 a, uint32_t sa, u32x4 b, uin
 #endif
 }
 
-// copies of scales of a wave and stage (the four waves' hold at least 8 tiles'), and the bytes of a stage's A in LDS
-constexpr int mx_gemm4_scale_copies(int mt) { return mt > 4 ? mt / 4 : 1; }
-constexpr int mx_gemm4_stage(int mt) { return 2 * mt * 2048 + 1024 * mx_gemm4_scale_copies(mt); }
+// bytes of a stage's A in LDS: 2 mt tiles' codes, and two tiles' scales of each of the four waves
+constexpr int mx_gemm4_stage(int mt) { return 2 * mt * 2048 + 1024; }
 // 4 bytes a lane from a buffer straight into LDS
 __device__ __forceinline__ void copy4_lds(__amdgpu_buffer_rsrc_t t, uint8_t *lds, int voff, int soff) {
 #if defined(__HIP_DEVICE_COMPILE__)
@@ -103,9 +112,12 @@ struct MxW {
     }
 };
 
+// every wave's copies into LDS, but for the N youngest loads and copies of each, have landed and can be read
+template <int N>
 __device__ __forceinline__ void arrive() {
-    __builtin_amdgcn_s_waitcnt(0x0070);  // vmcnt(0) lgkmcnt(0)
+    wait_vmcnt<N>();
     __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");
     __builtin_amdgcn_sched_barrier(0);
 }
 
@@ -129,6 +141,7 @@ __device__ __forceinline__ void mx_store(const MxGemmArgs &a, const MxPlace &at,
     }
     const bool bf16 = !slab && a.y_bf16;
     float *slabs = reinterpret_cast<float *>(a.y) + (slab ? (int64_t)at.kp * a.m * a.n : 0);
+    wait_vmcnt<0>();  // (copies into LDS for stages past the last)
     // Through LDS, 32 rows of 128 bytes at a time, so that a store is eight rows' 16 bytes a lane.  The wave's own
     // part of what held A (every wave is past it), whose accesses stay in order.  Non-temporal: outputs in L2 would push
     // out the operands that the next workgroups share (2048 x 4096 -> 24576 in 4 bits: 109 us, 128 with plain stores).
@@ -253,9 +266,7 @@ __global__ __launch_bounds__(W * 64, 2) void mx_gemm16_kernel(MxGemmArgs a) {
     auto unit = [&](auto parity, int u) {
         constexpr int par = decltype(parity)::value;
         // this unit's copies have landed: behind them came its loads, and the next unit's copies and loads
-        wait_vmcnt<NA + 2 * 3 * NT>();
-        __builtin_amdgcn_s_barrier();
-        __builtin_amdgcn_sched_barrier(0);
+        arrive<NA + 2 * 3 * NT>();
         const int next = min(u + 2, at.u1 - 1);
         const uint8_t *from = lds + cur * BUF + c32 * 256;
         copy_a(next, cur == 0 ? 2 : cur - 1);
@@ -298,7 +309,6 @@ __global__ __launch_bounds__(W * 64, 2) void mx_gemm16_kernel(MxGemmArgs a) {
         unit(std::integral_constant<int, 1>(), u + 1);
     }
     if (u < at.u1) unit(std::integral_constant<int, 0>(), u);
-    wait_vmcnt<0>();  // (copies for units past the last)
     mx_store(a, at, tile0, wv, lane, lds, acc);
 }
 
@@ -306,9 +316,8 @@ __global__ __launch_bounds__(W * 64, 2) void mx_gemm16_kernel(MxGemmArgs a) {
 // the A records are copied to the other LDS buffer.  Copies are issued before the loads of a stage, so that the wait for
 // them at the next one leaves the loads in flight.
 template <int MT, int NT>
-__global__ __launch_bounds__(W * 64, MT > 4 ? 1 : 2) void mx_gemm4_kernel(MxGemmArgs a) {
+__global__ __launch_bounds__(W * 64, 2) void mx_gemm4_kernel(MxGemmArgs a) {
     constexpr int REC = 2 * MT;                // 16-row tiles
-    constexpr int SC = mx_gemm4_scale_copies(MT);
     constexpr int BUF = mx_gemm4_stage(MT);    // codes [REC][2048], then scales [REC][128] (at least 1 KB of them)
     extern __shared__ __attribute__((aligned(16))) uint8_t lds[];
     const int tid = threadIdx.x, lane = tid & 63;
@@ -327,11 +336,8 @@ __global__ __launch_bounds__(W * 64, MT > 4 ? 1 : 2) void mx_gemm4_kernel(MxGemm
                        min(at.rb * REC + piece / 2, mtiles - 1) * bytes + pair * kMxPair + piece % 2 * 1024);
         }
         // two tiles' scales a wave
-#pragma unroll
-        for (int i = 0; i < SC; i++) {
-            const int rec = min(at.rb * REC + (2 * (i * W + wv) + (lane >> 5)) % REC, mtiles - 1);
-            copy4_lds(xb, lds + buf * BUF + REC * 2048 + (i * W + wv) * 256, rec * bytes + 4 * (lane & 31), pair * kMxPair + 2048);
-        }
+        const int rec = min(at.rb * REC + (2 * wv + (lane >> 5)) % REC, mtiles - 1);
+        copy4_lds(xb, lds + buf * BUF + REC * 2048 + wv * 256, rec * bytes + 4 * (lane & 31), pair * kMxPair + 2048);
     };
     const int b16 = (lane >> 4) & 1;
     floatx16 acc[MT][NT];
@@ -351,9 +357,7 @@ __global__ __launch_bounds__(W * 64, MT > 4 ? 1 : 2) void mx_gemm4_kernel(MxGemm
         for (int nt = 0; nt < NT; nt++) bq[nt][s] = w.codes(nt, v0, s);
     auto stage = [&](auto parity, int v) {
         constexpr int buf = decltype(parity)::value;
-        wait_vmcnt<5 * NT>();  // this stage's copies have landed
-        __builtin_amdgcn_s_barrier();
-        __builtin_amdgcn_sched_barrier(0);
+        arrive<5 * NT>();  // this stage's copies: behind them came its loads
         const int next = min(v + 1, v1 - 1);
         copy_a(next, buf ^ 1);
         load_scales(next, buf ^ 1);
