@@ -25,7 +25,7 @@ constexpr int kBeamWaves = 4;
 constexpr int kBeamThreads = 1024;
 constexpr int kBeamList = 1024;  // candidates that the join ranks in LDS
 constexpr int kStats = 2;        // segments that a lane of it holds
-constexpr int kHeld = 8;         // candidates that a thread of it holds
+constexpr int kHeld = 4;         // pairs of candidates that a thread of it holds
 
 struct BeamStat {
     float mx, r;  // a segment's maximum, the sum of e^(l - mx)
@@ -149,12 +149,15 @@ __global__ __launch_bounds__(kBeamThreads) void beam_join_kernel(BeamDev g) {
     // wait for (beams that were not read leave what the scratch held: not looked at).
     const int share = a.beams >= NW ? 1 : NW / a.beams, step = NW / share;
     const int first = wv / share, at0 = (wv % share) * 64 + lane;
-    uint64_t held[kHeld];
+    const int64_t pieces = keys / 2;  // of 16 bytes (nseg and slots are multiples of 4)
+    auto load2 = [&](int b, int64_t at, uint64_t(&k)[2]) {
+        const u32x4 v = at < pieces ? *reinterpret_cast<const u32x4 *>(cand + b * keys + 2 * at) : u32x4{0, 0, 0, 0};
+        k[0] = (uint64_t)v[1] << 32 | v[0];
+        k[1] = (uint64_t)v[3] << 32 | v[2];
+    };
+    uint64_t held[kHeld][2];
 #pragma unroll
-    for (int i = 0; i < kHeld; i++) {
-        const int64_t at = at0 + i * 64 * share;
-        held[i] = first < a.beams && at < keys ? cand[first * keys + at] : 0ull;
-    }
+    for (int i = 0; i < kHeld; i++) load2(min(first, a.beams - 1), at0 + i * 64 * share, held[i]);
     if (tid == 0) listed = 0;
     for (int b = wv; b < a.beams; b += NW) {
         const float score = a.scores[item * a.beams + b];
@@ -191,14 +194,16 @@ __global__ __launch_bounds__(kBeamThreads) void beam_join_kernel(BeamDev g) {
     auto each = [&](int b, auto &&f) {  // the lane's keys of beam b (0: none)
         if (b == first) {
 #pragma unroll
-            for (int i = 0; i < kHeld; i++) f(held[i]);
+            for (int i = 0; i < kHeld; i++) f(held[i][0]), f(held[i][1]);
         }
-        for (int64_t i = at0 + (b == first ? kHeld : 0) * 64 * share; i < keys; i += 4 * 64 * share) {
-            uint64_t k[4];
+        // (many at once: a workgroup's reads of a long list wait for one another otherwise)
+        constexpr int N = 8;
+        for (int64_t i = at0 + (b == first ? kHeld : 0) * 64 * share; i < pieces; i += N * 64 * share) {
+            uint64_t k[N][2];
 #pragma unroll
-            for (int e = 0; e < 4; e++) k[e] = i + e * 64 * share < keys ? cand[b * keys + i + e * 64 * share] : 0ull;
+            for (int e = 0; e < N; e++) load2(b, i + e * 64 * share, k[e]);
 #pragma unroll
-            for (int e = 0; e < 4; e++) f(k[e]);
+            for (int e = 0; e < N; e++) f(k[e][0]), f(k[e][1]);
         }
     };
     // candidates of a value of at least `low`: within a beam they are the logits from some bound on, and only what is near

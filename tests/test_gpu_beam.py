@@ -68,7 +68,7 @@ def inputs(batch, beams, n, dtype=F32, seed=0, spread=3.0):
 @pytest.mark.parametrize("dtype", [F32, BF16, F16])
 @pytest.mark.parametrize("batch,beams,n,keep", [(1, 1, 1, 1), (1, 2, 3, 4), (2, 3, 7, 32), (1, 4, 2047, 8), (3, 5, 2049, 5),
                                                 (2, 4, 8193, 8), (7, 8, 5000, 16), (1, 32, 3001, 32), (2, 16, 50257, 32),
-                                                (1, 1, 151936, 1), (1, 4, 151936, 8)])
+                                                (1, 1, 151936, 1), (1, 4, 151936, 8), (1, 16, 90001, 32), (2, 23, 40000, 17), (9, 6, 32000, 12)])
 def test_select(batch, beams, n, keep, dtype):
     import nn_amd
     logits, scores = inputs(batch, beams, n, dtype)

@@ -172,9 +172,12 @@ def check_linear(y, x, w, bias, out):
     assert over.max().item() <= 0, f"over the bar by {over.max().item():.2e}"
 
 
+# (every tile of the GEMMs and every pairing of waves of the rows kernel is among them: few and many columns, K in one to
+# several parts, units that end inside a pair, f32 rows whose planes share an MFMA and those that do not)
 SHAPES = [(1, 1, 32), (1, 16, 128), (2, 33, 96), (3, 300, 2880), (5, 129, 4128), (6, 257, 2112), (8, 512, 8192), (13, 40, 224),
           (16, 1000, 512), (17, 64, 32), (31, 129, 160), (33, 300, 2880), (64, 255, 384), (65, 513, 1056), (130, 70, 4096),
-          (200, 1025, 640), (301, 384, 2208)]
+          (200, 1025, 640), (301, 384, 2208), (4, 9000, 288), (12, 6001, 1024), (7, 5000, 5152), (9, 4100, 9216), (16, 8200, 4096),
+          (40, 13000, 1024), (260, 6200, 512), (520, 4200, 256)]
 
 
 @pytest.mark.parametrize("m,n,k", SHAPES)
@@ -328,6 +331,28 @@ def test_the_weight_in_the_calls_beside_the_linear():
     check_linear(r.logits, xs, decode(codes, scales), bias, F32)
     for a, b in zip(r[:5], t[:5]):
         assert torch.equal(a, b)
+
+
+def test_the_head_with_nan_and_without_allocation():
+    import ctypes
+
+    import nn_amd
+    from nn_amd import _lib
+    n, k = 3000, 12288 + 8192  # (x of a long row passes through LDS in chunks)
+    codes, scales = weight(n, k, 13)
+    w = nn_amd.QuantizedWeight.from_mxfp4_rows(codes, scales)
+    x = torch.randn(k, generator=torch.Generator().manual_seed(9)).cuda() * 0.2
+    logits, tok = nn_amd.linear_sample(x, w, seed=5, top_k=8)
+    check_linear(logits[None], x[None], decode(codes, scales), None, F32)
+    out, t = torch.empty(n, device="cuda"), torch.empty(1, dtype=torch.int32, device="cuda")
+    cfg = _lib.Sampling(0.7, 8, 1, 0.9, 1.0, 0.0, 5)
+    rc = _lib.load().nnq_linear_sample_noalloc(w.handle, x.data_ptr(), k, None, 0, out.data_ptr(), None, 0, ctypes.byref(cfg),
+                                               t.data_ptr(), torch.cuda.current_stream().cuda_stream)
+    assert rc == _lib.OK
+    assert torch.equal(out, logits) and int(t) == int(tok)
+    x[77] = NAN
+    with pytest.raises(nn_amd.NonFiniteData):
+        nn_amd.linear_argmax(x, w)
 
 
 def test_linears_captured_in_a_graph():
