@@ -3,7 +3,7 @@
 Hand-written HIP kernels behind a C ABI (``include/nnq.h``, ``libnnq.so``) for
 the dequant-fused matmul over GGUF Q8_0 / Q4_K / Q6_K blocks and the GPT-OSS
 MXFP4 mixture-of-experts layer (GPT-OSS and nn-core OCP MXFP4 layouts); ``nn_amd.quantized`` mirrors the reference's
-operator surface in Python.
+operator surface in Python.  Beside it: 4-bit group-scaled and MXFP4 linears, token log probabilities, beam search.
 """
 from .quantized import (  # noqa: F401
     BeamSelection, BiasMismatch, DataLengthMismatch, InvalidShape, Layout, Mxfp4Rows, NonFiniteData, NotQuantized, QuantizedMatmulError,
