@@ -16,6 +16,7 @@
 // the segments); sixteen beams of 151936 with 32 kept, whose 68000 candidates one workgroup reads, 29 in all.  Of the join
 // 1 us each are the loads, the exponentials and logarithm in 64 bits, the bound of the keep-th value, and the ranking.
 #include <algorithm>
+#include <type_traits>
 
 #include "nnq_device.h"
 #include "nnq_internal.h"
@@ -94,7 +95,7 @@ __global__ __launch_bounds__(kBeamWaves * 64) void beam_seg_kernel(BeamDev g) {
     const int64_t at = rl * g.nseg + seg;
     if (lane == 0) g.stat[at] = BeamStat{mx, r};
     __shared__ uint64_t list[kBeamWaves][64];
-    segment_candidates<V, sizeof(T) == 4 ? 24 : 16>(x, lm, base, a.keep, g.slots, lane, list[wv], g.cand + at * g.slots);
+    segment_candidates<V, std::is_same<T, Bf16>::value ? 16 : 24>(x, lm, base, a.keep, g.slots, lane, list[wv], g.cand + at * g.slots);
 }
 
 // larger values have larger ones (v is a number)
@@ -396,6 +397,7 @@ int launch_reorder(const ReorderArgs &a, int tensors, void *stream) {
     const dim3 grid((unsigned)std::min<int64_t>((a.pieces + 255) / 256, 65536), (unsigned)std::min<int64_t>(a.batch, 65535), (unsigned)tensors);
     if (a.beams <= 4) hipLaunchKernelGGL((beam_reorder_kernel<VEC, 4>), grid, dim3(256), 0, (hipStream_t)stream, a);
     else if (a.beams <= 8) hipLaunchKernelGGL((beam_reorder_kernel<VEC, 8>), grid, dim3(256), 0, (hipStream_t)stream, a);
+    else if (a.beams <= 16) hipLaunchKernelGGL((beam_reorder_kernel<VEC, 16>), grid, dim3(256), 0, (hipStream_t)stream, a);
     else hipLaunchKernelGGL((beam_reorder_kernel<VEC, 32>), grid, dim3(256), 0, (hipStream_t)stream, a);
     return (int)hipGetLastError();
 }
