@@ -347,9 +347,14 @@ struct Bytes<16> {
     typedef u32x4 type;
 };
 
+// Pieces of a thread at a time: two where a thread may have a single one to read (us, one / two / four: 16 items of 2 slots, 480
+// MB 135 / 106 / 108; 8 of 4 slots, 787 MB 162 / 153 / 157; 0.6 MB 3.0 / 3.4 / 4.2).
+constexpr int reorder_pieces(int most) { return most <= 4 ? 2 : 1; }
+
 template <int VEC, int MOST>
 __global__ __launch_bounds__(256) void beam_reorder_kernel(ReorderArgs a) {
     typedef typename Bytes<VEC>::type T;
+    constexpr int PER = reorder_pieces(MOST);
     __shared__ int from[MOST];
     __shared__ int moves;
     const int tid = threadIdx.x;
@@ -367,23 +372,47 @@ __global__ __launch_bounds__(256) void beam_reorder_kernel(ReorderArgs a) {
             int f[MOST];
 #pragma unroll
             for (int j = 0; j < MOST; j++) f[j] = j < a.beams ? __builtin_amdgcn_readfirstlane(from[j]) : -1;
-            for (int64_t i = (int64_t)blockIdx.x * 256 + tid; i < a.pieces; i += (int64_t)gridDim.x * 256) {
-                uint8_t *p = a.state[blockIdx.z] + item * a.beams * a.slot_stride;
-                int64_t left = i;
+            uint8_t *base = a.state[blockIdx.z] + item * a.beams * a.slot_stride;
+            auto place = [&](int64_t i) {  // of piece i (as a rule in 32 bits)
+                int64_t at = 0;
+                if (a.pieces <= 0xFFFFFFFFll) {
+                    uint32_t left = (uint32_t)i;
 #pragma unroll
-                for (int d = kReorderDims - 1; d >= 0; d--) {
-                    if (a.size[d] == 1) continue;
-                    const int64_t q = left / a.size[d];
-                    p += (left - q * a.size[d]) * a.stride[d];
-                    left = q;
+                    for (int d = kReorderDims - 1; d >= 0; d--) {
+                        if (a.size[d] == 1) continue;
+                        const uint32_t q = left / (uint32_t)a.size[d];
+                        at += (int64_t)(left - q * (uint32_t)a.size[d]) * a.stride[d];
+                        left = q;
+                    }
+                } else {
+                    int64_t left = i;
+#pragma unroll
+                    for (int d = kReorderDims - 1; d >= 0; d--) {
+                        if (a.size[d] == 1) continue;
+                        const int64_t q = left / a.size[d];
+                        at += (left - q * a.size[d]) * a.stride[d];
+                        left = q;
+                    }
                 }
-                T v[MOST];
+                return base + at;
+            };
+            for (int64_t i = (int64_t)blockIdx.x * (256 * PER) + tid; i < a.pieces; i += (int64_t)gridDim.x * (256 * PER)) {
+                uint8_t *p[PER];
+                T v[PER][MOST];
+#pragma unroll
+                for (int e = 0; e < PER; e++) p[e] = i + e * 256 < a.pieces ? place(i + e * 256) : nullptr;
 #pragma unroll
                 for (int j = 0; j < MOST; j++)
-                    if (f[j] >= 0) v[j] = *reinterpret_cast<const T *>(p + f[j] * a.slot_stride);
+                    if (f[j] >= 0)
+#pragma unroll
+                        for (int e = 0; e < PER; e++)
+                            if (p[e]) v[e][j] = *reinterpret_cast<const T *>(p[e] + f[j] * a.slot_stride);
 #pragma unroll
                 for (int j = 0; j < MOST; j++)
-                    if (f[j] >= 0) *reinterpret_cast<T *>(p + j * a.slot_stride) = v[j];
+                    if (f[j] >= 0)
+#pragma unroll
+                        for (int e = 0; e < PER; e++)
+                            if (p[e]) __builtin_nontemporal_store(v[e][j], reinterpret_cast<T *>(p[e] + j * a.slot_stride));
             }
         }
         __syncthreads();
@@ -394,7 +423,8 @@ __global__ __launch_bounds__(256) void beam_reorder_kernel(ReorderArgs a) {
 
 template <int VEC>
 int launch_reorder(const ReorderArgs &a, int tensors, void *stream) {
-    const dim3 grid((unsigned)std::min<int64_t>((a.pieces + 255) / 256, 65536), (unsigned)std::min<int64_t>(a.batch, 65535), (unsigned)tensors);
+    const int64_t per = reorder_pieces(a.beams);
+    const dim3 grid((unsigned)std::min<int64_t>((a.pieces + 256 * per - 1) / (256 * per), 65536), (unsigned)std::min<int64_t>(a.batch, 65535), (unsigned)tensors);
     if (a.beams <= 4) hipLaunchKernelGGL((beam_reorder_kernel<VEC, 4>), grid, dim3(256), 0, (hipStream_t)stream, a);
     else if (a.beams <= 8) hipLaunchKernelGGL((beam_reorder_kernel<VEC, 8>), grid, dim3(256), 0, (hipStream_t)stream, a);
     else if (a.beams <= 16) hipLaunchKernelGGL((beam_reorder_kernel<VEC, 16>), grid, dim3(256), 0, (hipStream_t)stream, a);
