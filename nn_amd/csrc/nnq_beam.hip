@@ -347,14 +347,12 @@ struct Bytes<16> {
     typedef u32x4 type;
 };
 
-// Pieces of a thread at a time: two where a thread may have a single one to read (us, one / two / four: 16 items of 2 slots, 480
-// MB 135 / 106 / 108; 8 of 4 slots, 787 MB 162 / 153 / 157; 0.6 MB 3.0 / 3.4 / 4.2).
-constexpr int reorder_pieces(int most) { return most <= 4 ? 2 : 1; }
-
-template <int VEC, int MOST>
+// PER: pieces of a thread at a time, two where a thread may have a single one to read and the card has many rounds of
+// workgroups all the same (us, one / two: 0.6 MB in 76 workgroups of one 3.0 / 3.4; 105 MB in 6400 19.6 / 21.2; 210 MB in
+// 12800 36.8 / 37.8; 787 MB in 48000 151 / 138; 480 MB of two slots in 59000 135 / 106, of four pieces 108).
+template <int VEC, int MOST, int PER>
 __global__ __launch_bounds__(256) void beam_reorder_kernel(ReorderArgs a) {
     typedef typename Bytes<VEC>::type T;
-    constexpr int PER = reorder_pieces(MOST);
     __shared__ int from[MOST];
     __shared__ int moves;
     const int tid = threadIdx.x;
@@ -421,15 +419,19 @@ __global__ __launch_bounds__(256) void beam_reorder_kernel(ReorderArgs a) {
     }
 }
 
+template <int VEC, int MOST, int PER>
+int launch_reorder_as(const ReorderArgs &a, int tensors, void *stream) {
+    const dim3 grid((unsigned)std::min<int64_t>((a.pieces + 256 * PER - 1) / (256 * PER), 65536), (unsigned)std::min<int64_t>(a.batch, 65535), (unsigned)tensors);
+    hipLaunchKernelGGL((beam_reorder_kernel<VEC, MOST, PER>), grid, dim3(256), 0, (hipStream_t)stream, a);
+    return (int)hipGetLastError();
+}
 template <int VEC>
 int launch_reorder(const ReorderArgs &a, int tensors, void *stream) {
-    const int64_t per = reorder_pieces(a.beams);
-    const dim3 grid((unsigned)std::min<int64_t>((a.pieces + 256 * per - 1) / (256 * per), 65536), (unsigned)std::min<int64_t>(a.batch, 65535), (unsigned)tensors);
-    if (a.beams <= 4) hipLaunchKernelGGL((beam_reorder_kernel<VEC, 4>), grid, dim3(256), 0, (hipStream_t)stream, a);
-    else if (a.beams <= 8) hipLaunchKernelGGL((beam_reorder_kernel<VEC, 8>), grid, dim3(256), 0, (hipStream_t)stream, a);
-    else if (a.beams <= 16) hipLaunchKernelGGL((beam_reorder_kernel<VEC, 16>), grid, dim3(256), 0, (hipStream_t)stream, a);
-    else hipLaunchKernelGGL((beam_reorder_kernel<VEC, 32>), grid, dim3(256), 0, (hipStream_t)stream, a);
-    return (int)hipGetLastError();
+    if (a.beams > 16) return launch_reorder_as<VEC, 32, 1>(a, tensors, stream);
+    if (a.beams > 8) return launch_reorder_as<VEC, 16, 1>(a, tensors, stream);
+    if (a.beams > 4) return launch_reorder_as<VEC, 8, 1>(a, tensors, stream);
+    const double groups = (double)((a.pieces + 255) / 256) * (double)a.batch * tensors;
+    return groups >= 24576 ? launch_reorder_as<VEC, 4, 2>(a, tensors, stream) : launch_reorder_as<VEC, 4, 1>(a, tensors, stream);
 }
 
 }  // namespace

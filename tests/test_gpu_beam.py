@@ -295,6 +295,20 @@ def test_reorder_several_states_and_integer_types():
     assert torch.equal(d.cpu(), moved(ts[1], p, 0))
 
 
+@pytest.mark.parametrize("batch,beams,shape,dtype", [(12300, 2, (300, 8), BF16), (12300, 4, (3, 211), torch.uint8),
+                                                     (70001, 3, (5,), BF16), (40, 4, (8, 5000, 6), F32)])
+def test_reorder_many_pieces(batch, beams, shape, dtype):
+    import nn_amd
+    p = parents_of(batch, beams, 6)
+    cache = torch.randint(0, 100, (batch * beams, *shape[:-1], shape[-1] + 4), generator=torch.Generator().manual_seed(2)).to(dtype)
+    for used in (shape[-1] + 4, shape[-1]):
+        got = cache.cuda()
+        nn_amd.beam_reorder(got[..., :used], p.cuda())
+        want = cache.cuda()
+        want[..., :used] = moved(want[..., :used], p, 0)
+        assert torch.equal(got, want)
+
+
 def test_reorder_beyond_32_bit_offsets():
     import nn_amd
     state = torch.zeros(4, 3, 1 << 30, dtype=torch.uint8, device="cuda")  # 12 GiB, one item a leading index
