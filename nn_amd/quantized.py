@@ -808,24 +808,28 @@ def beam_reorder(states, parents: torch.Tensor, dim: int = 0) -> None:
     batch = parents.shape[0] if parents.dim() == 2 else 1
     if not 1 <= beams <= 32:
         raise InvalidShape(f"{beams} beams (1 to 32)")
-    alike = {}
-    device, slots = parents.device, batch * beams
+    alike, last = {}, None
+    index, slots = parents.get_device(), batch * beams
     for t in states:
-        if not isinstance(t, torch.Tensor) or t.device != device:
-            raise Unsupported(f"a state must be a tensor on {device}, as parents are")
-        shape = t.shape
-        if not -len(shape) <= dim < len(shape):
-            raise RankMismatch(f"a state of rank {len(shape)} has no dimension {dim}")
-        if shape[dim] != slots:
-            raise ShapeMismatch(f"state {list(shape)} must have {batch} x {beams} slots along dimension {dim}")
-        if t.numel():
-            alike.setdefault((shape, t.stride(), t.dtype), []).append(t.data_ptr())
-    for ptrs in alike.values():
-        if len(set(ptrs)) != len(ptrs):
+        if not isinstance(t, torch.Tensor) or t.get_device() != index:
+            raise Unsupported(f"a state must be a tensor on {parents.device}, as parents are")
+        key = (t.shape, t.stride(), t.dtype)
+        if key != last:  # (as a rule the states are alike)
+            shape = t.shape
+            if not -len(shape) <= dim < len(shape):
+                raise RankMismatch(f"a state of rank {len(shape)} has no dimension {dim}")
+            if shape[dim] != slots:
+                raise ShapeMismatch(f"state {list(shape)} must have {batch} x {beams} slots along dimension {dim}")
+            last, ptrs = key, alike.setdefault(key, [])
+        ptrs.append(t.data_ptr())
+    for (shape, _, _), ptrs in alike.items():
+        if len(set(ptrs)) != len(ptrs) and 0 not in shape:
             raise TensorError("a state is given twice")
     p = parents if parents.dtype is torch.int64 else parents.long()
     p = p.contiguous()
     for (shape, stride, dtype), ptrs in alike.items():
+        if 0 in shape:
+            continue
         d = dim % len(shape)
         sizes, strides = [*shape[:d], *shape[d + 1:]], [*stride[:d], *stride[d + 1:]]
         if len(sizes) > 8:
