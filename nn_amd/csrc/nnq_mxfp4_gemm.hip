@@ -13,7 +13,8 @@
 //  * 2048 rows of 4096 -> 24576 in 4 bits 104 to 113 us with 7 of quantization, 3.7 to 3.9 PFLOP/s.  Variants that leave work
 //    out say what of the kernel's 103: the MFMAs alone 60, with the LDS reads 65, the copies of A 72, the loads of B 91, the
 //    stores 103.  The loads are 98 KB a stage and CU, 85% of what its L1 delivers beside the MFMAs.  One wave a SIMD with
-//    256 rows a workgroup (122 us), a third buffer (112) and eight waves that share A (115 / 115) were no faster.
+//    256 rows a workgroup (122 us) or 256 x 256 and both operands through LDS (126), a third buffer (112) and eight waves
+//    that share A (115 / 115) were no faster.
 //  * 301 f32 rows of 2880 -> 5751 in 4 bits 18 us: latency of two launches, 12 stages and the first loads.
 #include <algorithm>
 #include <type_traits>
