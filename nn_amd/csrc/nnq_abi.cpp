@@ -1051,20 +1051,20 @@ int nnq_beam_reorder(void *const *states, int64_t n_states, int64_t batch, int64
     if (batch > INT64_MAX / kBeams || slot_stride > (int64_t)1 << 56) return size_fail();
     for (int i = 0; i < ndim; i++)
         if (strides[i] > (int64_t)1 << 56) return size_fail();
-    if (n_states == 0 || batch == 0 || beams == 1) return NNQ_OK;
-    if (!states || !parents) return fail(NNQ_ERR_INVALID_ARGUMENT, "null pointer");
-    if ((uintptr_t)parents & 7) return fail(NNQ_ERR_INVALID_ARGUMENT, "parents must be 8-byte aligned");
-    uintptr_t bits = 0;
-    for (int64_t i = 0; i < n_states; i++) {
-        if (!states[i]) return fail(NNQ_ERR_INVALID_ARGUMENT, "state %lld is null", (long long)i);
-        bits |= (uintptr_t)states[i];
-    }
+    if (n_states && !states) return fail(NNQ_ERR_INVALID_ARGUMENT, "null pointer");
     ReorderArgs a{};
+    uintptr_t bits = 0;
+    for (int64_t i = 0; i < n_states; i++) bits |= (uintptr_t)states[i];
+    const char *err = reorder_geometry(batch * beams, slot_stride, ndim, sizes, strides, elem_bytes, bits, &a);
+    if (err) return fail(a.dims < 0 ? NNQ_ERR_UNSUPPORTED : NNQ_ERR_INVALID_ARGUMENT, "state tensors have %s", err);
+    if (n_states == 0 || batch == 0 || beams == 1) return NNQ_OK;
+    if (!parents) return fail(NNQ_ERR_INVALID_ARGUMENT, "null pointer");
+    if ((uintptr_t)parents & 7) return fail(NNQ_ERR_INVALID_ARGUMENT, "parents must be 8-byte aligned");
+    for (int64_t i = 0; i < n_states; i++)
+        if (!states[i]) return fail(NNQ_ERR_INVALID_ARGUMENT, "state %lld is null", (long long)i);
     a.parents = parents;
     a.batch = batch;
     a.beams = (int)beams;
-    const char *err = reorder_geometry(batch * beams, slot_stride, ndim, sizes, strides, elem_bytes, bits, &a);
-    if (err) return fail(a.dims < 0 ? NNQ_ERR_UNSUPPORTED : NNQ_ERR_INVALID_ARGUMENT, "state tensors have %s", err);
     if (a.pieces == 0) return NNQ_OK;
     for (int64_t i = 0; i < n_states; i += kReorderTensors) {
         const int count = (int)std::min<int64_t>(kReorderTensors, n_states - i);

@@ -794,8 +794,8 @@ def beam_reorder(states, parents: torch.Tensor, dim: int = 0) -> None:
     """The states that follow a step: slot b * beams + j along ``dim`` of each state becomes a copy of slot
     b * beams + parents[b, j], in place, whatever the parents are (all reads come before the writes).
 
-    states: a device tensor or several on one device, of any dtypes, which must not overlap; strided ones are written where
-    they lie, so ``cache[..., :used, :]`` moves the used part only.  parents: integers [batch, beams] or [beams] (beams
+    states: a device tensor or several on one device, of any dtypes, which must overlap neither one another nor parents;
+    strided ones are written where they lie, so ``cache[..., :used, :]`` moves the used part only.  parents: integers [batch, beams] or [beams] (beams
     up to 32) on that device; a slot whose parent is itself, or outside [0, beams) as the -1 of ``beam_select``, stays as it
     is, and only slots that move are read and written.  No host synchronisation."""
     states = [states] if isinstance(states, torch.Tensor) else list(states)
@@ -827,16 +827,23 @@ def beam_reorder(states, parents: torch.Tensor, dim: int = 0) -> None:
             raise TensorError("a state is given twice")
     p = parents if parents.dtype is torch.int64 else parents.long()
     p = p.contiguous()
+    calls = []
     for (shape, stride, dtype), ptrs in alike.items():
+        d = dim % len(shape)
         if 0 in shape:
             continue
-        d = dim % len(shape)
-        sizes, strides = [*shape[:d], *shape[d + 1:]], [*stride[:d], *stride[d + 1:]]
-        if len(sizes) > 8:
+        if len(shape) > 9:
             raise Unsupported(f"a state of rank {len(shape)} (at most 9)")
-        i64s = ctypes.c_int64 * len(sizes)
-        _launch(p, _lib.load().nnq_beam_reorder, (ctypes.c_void_p * len(ptrs))(*ptrs), len(ptrs), batch, beams, stride[d], len(sizes),
-                i64s(*sizes), i64s(*strides), dtype.itemsize, p.data_ptr())
+        i64s = ctypes.c_int64 * (len(shape) - 1)
+        sizes, strides = list(shape), list(stride)
+        del sizes[d]
+        calls.append((ptrs, (batch, beams, strides.pop(d), len(sizes), i64s(*sizes), i64s(*strides), dtype.itemsize, p.data_ptr())))
+    fn = _lib.load().nnq_beam_reorder
+    if len(calls) > 1:  # (a state that is refused is refused before another has moved)
+        for _, args in calls:
+            _launch(p, fn, None, 0, *args)
+    for ptrs, args in calls:
+        _launch(p, fn, (ctypes.c_void_p * len(ptrs))(*ptrs), len(ptrs), *args)
 
 
 # ---------------------------------------------------------------------------------

@@ -359,6 +359,18 @@ def test_refusals():
         nn_amd.beam_reorder(torch.zeros(6, 3, 3, 3, 3, 3, device="cuda")[:, :2, :2, :2, :2, :2], p)
 
 
+def test_reorder_moves_all_states_or_none():
+    import nn_amd
+    p = torch.tensor([[1, 2, 0], [0, 0, 0]], device="cuda")
+    for bad in (torch.randn(1, 4, device="cuda").expand(6, 4), torch.zeros(6, 3, 3, 3, 3, 3, device="cuda")[:, :2, :2, :2, :2, :2],
+                torch.zeros(6, *(1,) * 9, device="cuda")):
+        good = torch.randn(6, 5, device="cuda")
+        was = good.clone()
+        with pytest.raises((nn_amd.TensorError, nn_amd.Unsupported)):
+            nn_amd.beam_reorder([good, bad], p)
+        assert torch.equal(good, was)
+
+
 # ---- together -------------------------------------------------------------------------------
 
 

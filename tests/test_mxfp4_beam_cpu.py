@@ -104,6 +104,12 @@ def test_beam_reorder_refusals(lib):
     assert reorder(lib, (0, 8), (8, 1)) == _lib.OK
 
 
+def test_beam_reorder_checks_the_geometry_first(lib):
+    for states, batch, beams in (((), 2, 3), ((4096,), 2, 1), ((4096,), 1, 3)):
+        assert reorder(lib, (4, 8), (7, 1), states=states, batch=batch, beams=beams) == _lib.ERR_INVALID_ARGUMENT
+        assert reorder(lib, (2,) * 5, (1000, 300, 90, 20, 3), slot=4000, states=states, batch=batch, beams=beams) == _lib.ERR_UNSUPPORTED
+
+
 def test_python_refusals_without_a_device():
     import nn_amd
     codes, scales = torch.zeros(4, 32, dtype=torch.uint8), torch.zeros(4, 2, dtype=torch.uint8)
