@@ -41,7 +41,8 @@ __global__ __launch_bounds__(256) void mx_quantize_kernel(const uint8_t *x, int6
         const int64_t at = first + i * 256;
         v[i] = u32x4{0, 0, 0, 0};
         if (at >= pieces) continue;  // (whole blocks: pieces is a multiple of G)
-        const int64_t row = row_pieces ? at / row_pieces : 0;
+        // (quotients in 64 bits: 64 rows of 4096 apart from one another 3.0 us, 2.7 in 32)
+        const int64_t row = !row_pieces ? 0 : pieces >> 32 ? at / row_pieces : (uint32_t)at / (uint32_t)row_pieces;
         const uint8_t *p = x + row * row_bytes + (at - row * row_pieces) * 16;
         if constexpr (BF16) v[i] = *reinterpret_cast<const u32x4_2 *>(p);
         else v[i] = *reinterpret_cast<const u32x4_4 *>(p);
