@@ -77,14 +77,14 @@ __device__ __forceinline__ int64_t mx_scale_at(int64_t job, int lane) {
 }
 
 // x rows (whole units) to the records of the image, for a product of 4-bit operands: lane 16p + r quantizes block p
-// of row r, so that nothing crosses lanes.  (2048 x 4096 bf16 6.7 us, 301 x 2880 f32 3.7: the latter is one wave a CU.)
+// of row r, so that nothing crosses lanes.  One wave a workgroup, so that few of them lie on all CUs (four: 0.3 to 0.5 us
+// more).  (2048 x 4096 bf16 6.7 us, 301 x 2880 f32 3.4: the latter is two waves a CU.)
 template <bool BF16>
-__global__ __launch_bounds__(256) void mx_quantize_image_kernel(const uint8_t *x, int64_t m, int64_t k, int64_t units,
-                                                                int64_t jobs, int floor_rule, uint8_t *image) {
+__global__ __launch_bounds__(64) void mx_quantize_image_kernel(const uint8_t *x, int64_t m, int64_t k, int64_t units,
+                                                               int floor_rule, uint8_t *image) {
     constexpr int L = BF16 ? 4 : 8;
-    const int64_t job = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
-    if (job >= jobs) return;
-    const int lane = threadIdx.x & 63;
+    const int64_t job = (int64_t)blockIdx.x;
+    const int lane = threadIdx.x;
     const int64_t row = job / units * kTile + (lane & 15), k0 = job % units * kMxUnit + 32 * (lane >> 4);
     u32x4 v[L];
 #pragma unroll
@@ -518,12 +518,12 @@ int launch_mx_dequantize(const uint8_t *codes, const uint8_t *scales, int64_t co
 
 int launch_mx_quantize_image(const void *x, int x_bf16, int64_t m, int64_t k, int floor_rule, uint8_t *image, void *stream) {
     const int64_t units = 2 * mx_pairs(k), jobs = mx_tiles(m) * units;
-    if ((jobs + 3) / 4 > INT32_MAX) return (int)hipErrorInvalidValue;
+    if (jobs > INT32_MAX) return (int)hipErrorInvalidValue;
     const uint8_t *p = reinterpret_cast<const uint8_t *>(x);
     if (x_bf16)
-        hipLaunchKernelGGL(mx_quantize_image_kernel<true>, dim3(wave_jobs(jobs)), dim3(256), 0, (hipStream_t)stream, p, m, k, units, jobs, floor_rule, image);
+        hipLaunchKernelGGL(mx_quantize_image_kernel<true>, dim3((unsigned)jobs), dim3(64), 0, (hipStream_t)stream, p, m, k, units, floor_rule, image);
     else
-        hipLaunchKernelGGL(mx_quantize_image_kernel<false>, dim3(wave_jobs(jobs)), dim3(256), 0, (hipStream_t)stream, p, m, k, units, jobs, floor_rule, image);
+        hipLaunchKernelGGL(mx_quantize_image_kernel<false>, dim3((unsigned)jobs), dim3(64), 0, (hipStream_t)stream, p, m, k, units, floor_rule, image);
     return (int)hipGetLastError();
 }
 
