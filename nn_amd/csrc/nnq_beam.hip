@@ -66,16 +66,29 @@ __global__ __launch_bounds__(kBeamWaves * 64) void beam_seg_kernel(BeamDev g) {
     const int64_t seg = (int64_t)blockIdx.x * kBeamWaves + wv;
     if (!finite_score(a.scores[item * a.beams + beam]) || beam_ended(a, item * a.beams + beam)) return;
     const T *p = reinterpret_cast<const T *>(a.logits) + item * a.batch_stride + beam * a.beam_stride;
-    const int64_t base = seg * kSeg + (int64_t)lane * V;  // logit of element 0
+    // 16 bytes at a time; fewer logits than all lanes' first loads one at a time, so that as many lanes as can be have
+    // some: with fewer lanes than `keep` their maxima bound nothing, and the exact search behind that takes 13 us
+    // (7 x 16 f16 beams of 80084 = 39 segments and 212 with 31 kept: 44 us the call, so 30)
+    const int64_t start = seg * kSeg;
+    const bool few = a.n - start < 64 * V;
+    const int64_t base = start + (few ? lane : lane * V);  // logit of element 0
     float x[kPer];
+    if (few) {
 #pragma unroll
-    for (int v = 0; v < kPer / V; v++) {
-        const int64_t i = base + v * 64 * V;
-        if (i + V <= a.n) {
-            widen16<T>(load16(p + i), x + v * V);
-        } else {
+        for (int e = 0; e < kPer; e++) x[e] = kNegInf;
 #pragma unroll
-            for (int e = 0; e < V; e++) x[v * V + e] = i + e < a.n ? widen<T>(p[i + e]) : kNegInf;
+        for (int e = 0; e < V; e++)
+            if (base + 64 * e < a.n) x[e] = widen<T>(p[base + 64 * e]);
+    } else {
+#pragma unroll
+        for (int v = 0; v < kPer / V; v++) {
+            const int64_t i = base + v * 64 * V;
+            if (i + V <= a.n) {
+                widen16<T>(load16(p + i), x + v * V);
+            } else {
+#pragma unroll
+                for (int e = 0; e < V; e++) x[v * V + e] = i + e < a.n ? widen<T>(p[i + e]) : kNegInf;
+            }
         }
     }
     // (fmaxf passes over NaN; a NaN reaches the sum through its difference)
@@ -95,7 +108,9 @@ __global__ __launch_bounds__(kBeamWaves * 64) void beam_seg_kernel(BeamDev g) {
     const int64_t at = rl * g.nseg + seg;
     if (lane == 0) g.stat[at] = BeamStat{mx, r};
     __shared__ uint64_t list[kBeamWaves][64];
-    segment_candidates<V, std::is_same<T, Bf16>::value ? 16 : 24>(x, lm, base, a.keep, g.slots, lane, list[wv], g.cand + at * g.slots);
+    constexpr int BITS = std::is_same<T, Bf16>::value ? 16 : 24;
+    if (!few) segment_candidates<V, BITS>(x, lm, base, a.keep, g.slots, lane, list[wv], g.cand + at * g.slots);
+    else segment_candidates<1, BITS>(x, lm, base, a.keep, g.slots, lane, list[wv], g.cand + at * g.slots);
 }
 
 // larger values have larger ones (v is a number)
@@ -238,10 +253,12 @@ __global__ __launch_bounds__(kBeamThreads) void beam_join_kernel(BeamDev g) {
     maxima[tid] = best;
     __syncthreads();
     if (wv == 0) {
-        // the keep-th largest of the maxima of 64 parts is a lower bound of the keep-th largest value (its leading 24 bits)
+        // The keep-th largest of the maxima of 64 parts is a lower bound of the keep-th largest value (its leading 24 bits).
+        // A part takes another lane of every wave: of short rows only the first lanes hold candidates (2 x 15 beams of
+        // 1621 with 30 kept 16 us, 61 with the same lane of all; 4 x 32 of 1000 with 32 21 and 170)
         uint64_t m = maxima[lane];
 #pragma unroll
-        for (int w = 1; w < NW; w++) m = max(m, maxima[64 * w + lane]);
+        for (int w = 1; w < NW; w++) m = max(m, maxima[64 * w + ((lane + 64 / NW * w) & 63)]);
         const uint32_t v = (uint32_t)(m >> 32);
         const uint32_t b = largest_with<24>(a.keep, [&](uint32_t k) { return __popcll(__ballot(v >= k)); });
         if (lane == 0) bound = max((uint64_t)b << 32, (uint64_t)1);

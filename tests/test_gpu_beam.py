@@ -77,6 +77,17 @@ def test_select(batch, beams, n, keep, dtype):
     check(r, plain(logits, scores, keep))
 
 
+@pytest.mark.parametrize("dtype", [F32, BF16, F16])
+@pytest.mark.parametrize("beams,keep", [(2, 31), (15, 30), (32, 32)])
+@pytest.mark.parametrize("n", [63, 64, 200, 255, 257, 511, 512, 1000, 1621, 2048 + 40, 2048 + 212, 4096 + 500])
+def test_select_rows_that_end_early(n, beams, keep, dtype):
+    """few lanes of a row's last segment hold logits, and few of the join's candidates; also with equal logits"""
+    import nn_amd
+    logits, scores = inputs(2, beams, n, dtype)
+    logits[1] = logits[1].float().round().to(dtype)
+    check(nn_amd.beam_select(logits.cuda(), scores.cuda(), keep), plain(logits, scores, keep))
+
+
 @pytest.mark.parametrize("n", [5, 3000, 20000])
 def test_select_ties_go_by_beam_then_token(n):
     """identical beams: every continuation of one ties with the others'; whole-number logits tie within a beam"""
