@@ -102,6 +102,7 @@ int nnq_rule_gemm_ring(int64_t m, int64_t ntile, int64_t nblk, int x_bf16, int *
 int nnq_rule_gemm_wide(int64_t m, int64_t ntile, int64_t nblk, int x_bf16, int h_out, int *ks);
 int nnq_rule_gemm_wide6(int64_t m, int64_t ntile, int64_t nblk);
 int nnq_rule_moe_few(int64_t experts, int64_t hidden, int64_t inter, int64_t tokens, int top_k, int x_bf16);
+int nnq_rule_mx_x_offset(int row, int m, int k, int u, int col);  // mx_x_offset, the address of a copy
 }
 
 // ---- kernel launch parameters ------------------------------------------------------
@@ -317,6 +318,13 @@ struct MxGemmPlan {
 MxGemmPlan mx_gemm_plan(int64_t m, int64_t n, int64_t k, int x_kind);
 bool mx_takes_rows(int64_t m, int64_t n, int64_t k, int x_kind);  // or launch_mx_gemm
 int64_t mx_chunk_rows(int64_t m, int64_t k);
+// Byte of column col of unit u of row `row` in a bf16 plane of m rows of k, without the unit (its bytes and the plane's are the
+// instruction's scalar offset, which a buffer's range check may leave out): for rows and columns that do not exist a place
+// outside every buffer, so that no more than the planes is read whatever the check counts.
+constexpr int kMxNowhere = 0x7FFFFFF0;
+constexpr int mx_x_offset(int row, int m, int k, int u, int col) {
+    return row < m && u * kMxUnit + col < k ? (row * k + col) * 2 : kMxNowhere;
+}
 size_t mx_linear_scratch(int64_t m, int64_t n, int64_t k, int x_kind);  // of a call in chunks
 int launch_mx_rows(const MxArgs &a, void *scratch, void *stream);
 int launch_mx_gemm(const MxArgs &a, void *scratch, void *stream);

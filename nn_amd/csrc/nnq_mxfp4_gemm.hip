@@ -223,19 +223,18 @@ __global__ __launch_bounds__(W * 64, 2) void mx_gemm16_kernel(MxGemmArgs a) {
     const MxPlace at(a);
     const int tile0 = (at.cb * W + wv) * 2 * NT;
     const MxW<NT> w(a, tile0, lane);
-    // Copy i of a wave: rows 4 (i W + wv) .. + 3 of the pieces [plane][row tile][32 rows].  Rows past m belong to the
-    // next plane or lie past the buffer (zeros); they are not stored.
+    // Copy i of a wave: rows 4 (i W + wv) .. + 3 of the pieces [plane][row tile][32 rows].  Rows past m are not read (zeros);
+    // they are not stored.
     const int k = (int)a.k;
     const int64_t plane = (int64_t)a.m * k * 2;
     const __amdgpu_buffer_rsrc_t xb = rsrc(a.x, P * plane);
     const int l16 = lane >> 4, swz = ((lane & 15) ^ ((4 * wv + l16) & 15)) * 8;  // (W = 4: row % 16 is the same for every i)
     auto copy_a = [&](int u, int buf) {
-        const bool in = u * kMxUnit + swz < k;
 #pragma unroll
         for (int i = 0; i < NA; i++) {
             const int row = 4 * (i * W + wv), pl = row / (MT * 32);
-            const int off = ((at.rb * MT * 32 + row % (MT * 32) + l16) * k + swz) * 2;
-            copy16_lds(xb, lds + buf * BUF + (i * W + wv) * 1024, in ? off : 0x7FFFFFF0, pl * (int)plane + u * kMxUnit * 2);
+            const int off = mx_x_offset(at.rb * MT * 32 + row % (MT * 32) + l16, a.m, k, u, swz);
+            copy16_lds(xb, lds + buf * BUF + (i * W + wv) * 1024, off, pl * (int)plane + u * kMxUnit * 2);
         }
     };
     const int c32 = lane & 31, h = lane >> 5;

@@ -222,6 +222,8 @@ MxGemmPlan mx_gemm_plan(int64_t m, int64_t n, int64_t k, int x_kind) {
     return p;
 }
 
+int nnq_rule_mx_x_offset(int row, int m, int k, int u, int col) { return mx_x_offset(row, m, k, u, col); }
+
 // launches whose x the kernels reach with 32-bit offsets (three bf16 planes: 6 bytes a value), whole 128-row tiles
 int64_t mx_chunk_rows(int64_t m, int64_t k) {
     const int64_t rows = ((int64_t)1 << 30) / (6 * (k + kMxUnit)) / 128 * 128;
