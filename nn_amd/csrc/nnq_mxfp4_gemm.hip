@@ -350,6 +350,7 @@ __global__ __launch_bounds__(W * 64, 2) void mx_gemm4_kernel(MxGemmArgs a) {
     };
     const int v0 = at.u0 / 2, v1 = (at.u1 + 1) / 2;  // (parts of K are whole pairs)
     copy_a(v0, 0);
+    __builtin_amdgcn_sched_barrier(0);
     load_scales(v0, 0);
 #pragma unroll
     for (int s = 0; s < 4; s++)
@@ -360,6 +361,7 @@ __global__ __launch_bounds__(W * 64, 2) void mx_gemm4_kernel(MxGemmArgs a) {
         arrive<5 * NT>();  // this stage's copies: behind them came its loads
         const int next = min(v + 1, v1 - 1);
         copy_a(next, buf ^ 1);
+        __builtin_amdgcn_sched_barrier(0);
         load_scales(next, buf ^ 1);
         __builtin_amdgcn_sched_barrier(0);
         uint32_t as[MT];
