@@ -344,8 +344,8 @@ int nnq_linear_logprobs(const nnq_weight *w, const void *x, nnq_dtype x_dtype, i
  * logits at element b * batch_stride + j * beam_stride (n of them; NNQ_F32, NNQ_BF16 or NNQ_F16).  Its continuation by
  * token t is worth scores[b][j] + log(softmax(row)[t]); of all the item's continuations the `keep` largest go to
  *   out_scores [batch, keep] f32, parents [batch, keep] (the beam j) and tokens [batch, keep], device i64,
- * in descending order, equal ones by beam, then token.  Values are compared before they are rounded to f32: the sum over
- * a row in f32 (its exponentials to 2^-22), the rest in 64 bits.
+ * in descending order, equal ones by beam, then token.  Values are compared before they are rounded to f32: the sums over
+ * 2048 logits in f32 (exponentials to 2^-22; at most 2.5e-6 of the sum off, 1e-7 as a rule), the rest in 64 bits.
  * finished [batch, beams] (device bytes, may be NULL): a beam that is not 0 there has one continuation, by end_token
  * (any non-negative token) with its score unchanged; its logits are not read.  A beam whose score is not finite has none
  * (-inf: unused beams, as all but one at the first step), nor has one whose row holds NaN or +inf or nothing above

@@ -100,9 +100,12 @@ __global__ __launch_bounds__(kBeamWaves * 64) void beam_seg_kernel(BeamDev g) {
     float r = 0.f;
 #pragma unroll
     for (int e = 0; e < kPer; e++) {
-        // e^d: d log2(e) with the constant in two parts and one rounding (-inf: 0)
-        const float d = x[e] - ref;
-        r += __builtin_amdgcn_exp2f(fmaf(d, 1.44269502162933349609f, d * 1.92596299112661746887e-8f));
+        // e^d as exp_of has it, but for the constant's second part, 2^-29 of p: to 2^-22, and to 2^-21 where 2048 of them weigh
+        // less than 2^-19 (d < -21).  2^p alone is off by 2^-21 ln 2 at d = -5.6, to the same side for equal logits, and row
+        // sums by 2.8e-7 (24 x 8 bf16 beams of 50257 20.4 us, so 21.1; with the second part 21.4).
+        const float d = __builtin_elementwise_maximum(x[e] - ref, -1e30f);  // (-inf: its e^d is 0; NaN stays)
+        const float p = d * 1.44269504088896340736f, ex = __builtin_amdgcn_exp2f(p);
+        r += fmaf(ex, fmaf(p, -0x1.62e43p-1f, d), ex);
     }
     r = sum64(r);
     const int64_t at = rl * g.nseg + seg;
