@@ -103,6 +103,9 @@ int nnq_rule_gemm_wide(int64_t m, int64_t ntile, int64_t nblk, int x_bf16, int h
 int nnq_rule_gemm_wide6(int64_t m, int64_t ntile, int64_t nblk);
 int nnq_rule_moe_few(int64_t experts, int64_t hidden, int64_t inter, int64_t tokens, int top_k, int x_bf16);
 int nnq_rule_mx_x_offset(int row, int m, int k, int u, int col);  // mx_x_offset, the address of a copy
+// the form of one launch over MXFP4 rows, x of kind MxInput: 1: launch_mx_rows, f[] = {pp, kw, nw, ks}; 0: launch_mx_gemm,
+// f[] = {mt, nt, ks, stages of a part}
+int nnq_rule_mx(int64_t m, int64_t n, int64_t k, int x_kind, int *f);
 }
 
 // ---- kernel launch parameters ------------------------------------------------------

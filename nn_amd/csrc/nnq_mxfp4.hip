@@ -480,11 +480,11 @@ int launch_rows_t(const MxArgs &a, const MxRowsPlan &p, void *stream) {
 
 template <int XF>
 int launch_rows_x(const MxArgs &a, const MxRowsPlan &p, void *stream) {
-    switch (p.pp) {
-    case 1: return launch_rows_t<XF, 1>(a, p, stream);
-    case 2: return launch_rows_t<XF, 2>(a, p, stream);
-    case 3: return launch_rows_t<XF, 3>(a, p, stream);
-    case 4: return launch_rows_t<XF, 4>(a, p, stream);
+    if (p.pp == 1) return launch_rows_t<XF, 1>(a, p, stream);
+    if (p.pp == 2) return launch_rows_t<XF, 2>(a, p, stream);
+    if constexpr (XF != X_PLANES) {  // (the planes of six rows leave LDS for 17 pairs: two a wave)
+        if (p.pp == 3) return launch_rows_t<XF, 3>(a, p, stream);
+        if (p.pp == 4) return launch_rows_t<XF, 4>(a, p, stream);
     }
     return (int)hipErrorInvalidValue;
 }

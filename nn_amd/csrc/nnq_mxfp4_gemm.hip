@@ -459,7 +459,7 @@ int launch_mx_gemm(const MxArgs &a, void *scratch, void *stream) {
             : tile == 22 ? launch16<2, 2, 1>(g, stream)
             : tile == 23 ? launch16<2, 3, 1>(g, stream) : e;
     else if (a.x_kind == kMxF32)
-        e = tile == 12 ? launch16<1, 2, 3>(g, stream) : tile == 13 ? launch16<1, 3, 3>(g, stream) : tile == 22 ? launch16<2, 2, 3>(g, stream) : e;
+        e = tile == 12 ? launch16<1, 2, 3>(g, stream) : tile == 13 ? launch16<1, 3, 3>(g, stream) : e;
     else
         e = tile == 12   ? launch4<1, 2>(g, stream)
             : tile == 22 ? launch4<2, 2>(g, stream)

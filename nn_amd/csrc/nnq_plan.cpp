@@ -193,11 +193,11 @@ MxGemmPlan mx_gemm_plan(int64_t m, int64_t n, int64_t k, int x_kind) {
     };
     static const Tile four[] = {{1, 2, 0.274, 0.057}, {2, 2, 0.348, 0.068}, {2, 3, 0.493, 0.084}, {4, 2, 0.66, 0.0}};
     static const Tile bf16[] = {{1, 2, 0.306, 0.115}, {1, 3, 0.416, 0.184}, {2, 2, 0.445, 0.267}, {2, 3, 0.655, 0.358}};
-    static const Tile f32[] = {{1, 2, 0.847, 0.316}, {1, 3, 1.198, 0.329}, {2, 2, 2.12, 0.0}};
+    static const Tile f32[] = {{1, 2, 0.847, 0.316}, {1, 3, 1.198, 0.329}};  // (64 x 256: 2.12 a stage, two of 32 x 256 less)
     MxGemmPlan p{};
     const bool both = x_kind >= kMxQuantBf16;
     const Tile *tiles = both ? four : x_kind == kMxBf16 ? bf16 : f32;
-    const int count = x_kind == kMxF32 ? 3 : 4;
+    const int count = x_kind == kMxF32 ? 2 : 4;
     const int64_t cus = 256, rows = (m + 31) / 32, pairs = mx_pairs(k), stages = both ? pairs : mx_units(k);
     double best = 1e30;
     for (int i = 0; i < count; i++)
@@ -220,6 +220,23 @@ MxGemmPlan mx_gemm_plan(int64_t m, int64_t n, int64_t k, int x_kind) {
     p.slabs = align256(x);
     p.bytes = p.slabs + (p.ks > 1 ? (size_t)p.ks * (size_t)m * (size_t)n * 4 : 0);
     return p;
+}
+
+int nnq_rule_mx(int64_t m, int64_t n, int64_t k, int x_kind, int *f) {
+    if (mx_takes_rows(m, n, k, x_kind)) {
+        const MxRowsPlan p = mx_rows_plan(m, n, k, x_kind);
+        f[0] = p.pp;
+        f[1] = p.kw;
+        f[2] = p.nw;
+        f[3] = p.ks;
+        return 1;
+    }
+    const MxGemmPlan p = mx_gemm_plan(m, n, k, x_kind);
+    f[0] = p.mt;
+    f[1] = p.nt;
+    f[2] = p.ks;
+    f[3] = (int)((x_kind >= kMxQuantBf16 ? mx_pairs(k) : mx_units(k)) / p.ks);
+    return 0;
 }
 
 int nnq_rule_mx_x_offset(int row, int m, int k, int u, int col) { return mx_x_offset(row, m, k, u, col); }

@@ -15,6 +15,48 @@ def lib():
     return _lib.load()
 
 
+# ---- which form a shape takes -----------------------------------------------------------
+
+BF16, F32, QUANT_BF16, QUANT_F32, CODES = range(5)  # kinds of x (MxInput)
+
+
+def form(lib, m, n, k, x):
+    """("rows", kind, pairs of a wave) or ("gemm", operands, 32-row tiles, 128-column tiles)"""
+    lib.nnq_rule_mx.argtypes = [ctypes.c_int64] * 3 + [ctypes.c_int, ctypes.POINTER(ctypes.c_int)]
+    f = (ctypes.c_int * 4)()
+    if lib.nnq_rule_mx(m, n, k, x, f):
+        kind = {BF16: "X_BF16", F32: "X_TRI" if m <= 5 else "X_PLANES", QUANT_BF16: "X_Q16", QUANT_F32: "X_Q32", CODES: "X_CODES"}[x]
+        return "rows", kind, f[0]
+    return ("gemm16", f[0], f[1], 3 if x == F32 else 1) if x in (BF16, F32) else ("gemm4", f[0], f[1])
+
+
+def built_forms():
+    """the kernels' instantiations, from the calls that launch them"""
+    gemm = open(os.path.join(build.CSRC, "nnq_mxfp4_gemm.hip")).read()
+    rows = open(os.path.join(build.CSRC, "nnq_mxfp4.hip")).read()
+    forms = {("gemm16", *map(int, g)) for g in re.findall(r"launch16<(\d), (\d), (\d)>\(", gemm)}
+    forms |= {("gemm4", *map(int, g)) for g in re.findall(r"launch4<(\d), (\d)>\(", gemm)}
+    counts = [int(c) for c in re.findall(r"launch_rows_t<XF, (\d)>\(", rows)]
+    for kind in re.findall(r"launch_rows_x<(X_\w+)>\(", rows):
+        forms |= {("rows", kind, c) for c in counts if kind != "X_PLANES" or c <= 2}
+    assert "if constexpr (XF != X_PLANES)" in rows
+    return forms
+
+
+def test_every_built_form_is_some_shapes(lib):
+    """and every shape's form is built"""
+    rng = random.Random(5)
+    log = lambda lo, hi: round(lo * (hi / lo) ** rng.random())
+    seen = set()
+    for _ in range(150000):
+        m = rng.choice((log(1, 16), log(17, 9000)))
+        seen.add(form(lib, m, log(1, 300000), 32 * log(1, 1 << 15), rng.randrange(5)))
+    assert seen == built_forms(), (seen ^ built_forms())
+
+
+# ---- addresses ----------------------------------------------------------------------------
+
+
 @pytest.mark.parametrize("planes", [1, 3])
 def test_copies_of_x_stay_in_its_planes(lib, planes):
     """The GEMM with bf16 operands copies 16 bytes at (offset of a lane) + (plane and unit, a scalar offset).  A buffer's range
@@ -114,7 +156,7 @@ def test_gemm_waits_cover_their_copies(tmp_path):
                     os.path.join(build.CSRC, "nnq_mxfp4_gemm.hip"), "-o", out], check=True, stdout=subprocess.DEVNULL,
                    stderr=subprocess.DEVNULL)
     kernels = list(kernel_blocks(open(out).read()))
-    assert {k[0] for k, _ in kernels} == {16, 4} and len(kernels) >= 8
+    assert {k[0] for k, _ in kernels} == {16, 4} and len(kernels) >= 10
     for kernel, blocks in kernels:
         assert early_reads(kernel, blocks) == []
         # a load in front of the copies of a stage would be seen
