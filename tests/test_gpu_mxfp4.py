@@ -172,8 +172,8 @@ def check_linear(y, x, w, bias, out):
     assert over.max().item() <= 0, f"over the bar by {over.max().item():.2e}"
 
 
-# (every tile of the GEMMs and every pairing of waves of the rows kernel is among them: few and many columns, K in one to
-# several parts, units that end inside a pair, f32 rows whose planes share an MFMA and those that do not)
+# (few and many columns, K in one to several parts, units that end inside a pair, f32 rows whose planes share an MFMA and
+# those that do not; the larger tiles and longer rows that test_mxfp4_forms.py lists are not among them)
 SHAPES = [(1, 1, 32), (1, 16, 128), (2, 33, 96), (3, 300, 2880), (5, 129, 4128), (6, 257, 2112), (8, 512, 8192), (13, 40, 224),
           (16, 1000, 512), (17, 64, 32), (31, 129, 160), (33, 300, 2880), (64, 255, 384), (65, 513, 1056), (130, 70, 4096),
           (200, 1025, 640), (301, 384, 2208), (4, 9000, 288), (12, 6001, 1024), (7, 5000, 5152), (9, 4100, 9216), (16, 8200, 4096),
