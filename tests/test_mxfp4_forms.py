@@ -1,6 +1,6 @@
 """Every form of the linears over MXFP4 rows (tiles of the GEMMs, pairs of units of the rows kernel, K in one or several
 parts) on operands whose products and sums are exact in f32 in any order, so that the outputs are equal to the
-definition's.
+definition's, and f32 x in its norm.
 
 Exactness: a weight row has up to 16 values of +-0.5, 1 or 2 (codes and scales vary) and is zero elsewhere.  x: f32 odd
 integers of 17 bits (all three bf16 parts of each count), bf16 integers of 8, or, where it is quantized, blocks that the
@@ -134,3 +134,24 @@ def test_every_form_is_exact(kind, shape):
             want = (ref if b is None else ref + b.double()).float().to(out)
             y = call(b, out_dtype=out)
             assert y.dtype is out and torch.equal(y, want), (out, (y != want).nonzero()[:4].tolist())
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("m,n,k", [(1, 301, 4096), (3, 77, 8224), (5, 261, 3872), (6, 64, 288), (11, 500, 2880), (16, 71, 1056),
+                                   (20, 65, 288), (33, 300, 2880), (393, 1027, 2016), (1156, 1549, 288)])
+def test_f32_rows_in_their_norm(m, n, k):
+    """Dense random operands: 3 K / 16 + 40 roundings to 2^-24 of a partial sum, whose size grows as a random walk's, are
+    2^-24 sqrt(N / 6) of the result in the mean; allowed is twice that.  x without its third part would be off by more."""
+    import nn_amd
+    g = torch.Generator().manual_seed(m + n + k)
+    codes = torch.randint(0, 256, (n, k // 2), generator=g, dtype=torch.uint8).cuda()
+    scales = torch.randint(121, 124, (n, k // 32), generator=g).to(torch.uint8).cuda()
+    w = nn_amd.QuantizedWeight.from_mxfp4_rows(codes, scales)
+    x = torch.randn(m, k, generator=g).cuda()
+    full = w.dequantize().double()
+    ref = x.double() @ full.t()
+    bar = 2 * 2.0 ** -24 * math.sqrt((3 * k / 16 + 40) / 6)
+    cut = (x.view(torch.int32) & ~0xFF).view(torch.float32)
+    assert (cut.double() @ full.t() - ref).norm() > bar * ref.norm()
+    y = nn_amd.quantized_linear(x, w)
+    assert (y.double() - ref).norm() <= bar * ref.norm(), ((y.double() - ref).norm() / ref.norm()).item()
