@@ -12,8 +12,8 @@
 // A row's segments begin at its multiples of 2048 wherever it lies, so that equal rows have equal sums and their
 // continuations tie exactly.
 // Bound: one read of the logits; small calls by the latency of two launches.  Measured (MI355X): four beams of 151936 with 8
-// kept 5.6 + 6.2 us, 24 x 8 bf16 beams of 50257 with 16 kept 11.1 + 8.8, 64 x 5 f32 beams of 151936 38 + 8.8 (5.1 TB/s in
-// the segments); sixteen beams of 151936 with 32 kept, whose 68000 candidates one workgroup reads, 29 in all.  Of the join
+// kept 5.6 + 6.1 us, 24 x 8 bf16 beams of 50257 with 16 kept 11.8 + 8.1, 64 x 5 f32 beams of 151936 38 + 9.4 (5.2 TB/s in
+// the segments); sixteen beams of 151936 with 32 kept, whose 68000 candidates one workgroup reads, 30 in all.  Of the join
 // 1 us each are the loads, the exponentials and logarithm in 64 bits, the bound of the keep-th value, and the ranking.
 #include <algorithm>
 #include <type_traits>
@@ -346,6 +346,9 @@ int launch_select(const BeamDev &g, int64_t items, void *stream) {
 // Bound: the bytes of the slots that move, written once, and of their parents, read once.  A thread takes one piece (up
 // to 16 bytes) of all slots of an item: it reads the pieces of the parents of all slots that move before it writes any,
 // so that the copy is in place whatever the parents are, and a parent of several slots comes from HBM once.
+// Measured (MI355X): 787 MB of 4 beams 135 to 142 us, 5.6 TB/s; of more beams, all but one slot moving / half of them, each
+// from a parent of its own: 8 beams 140 / 158, 16 beams 146 / 165, 32 beams 168 / 167; small ones: 1.8 MB of 6 beams 4.0, 9.7 MB of
+// 32 beams 9.7 (19 workgroups a tensor, 16 loads a thread).
 template <int N>
 struct Bytes {
     typedef uint8_t type;

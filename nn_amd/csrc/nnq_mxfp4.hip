@@ -100,7 +100,8 @@ __global__ __launch_bounds__(64) void mx_quantize_image_kernel(const uint8_t *x,
     image[mx_scale_at(job, lane)] = (uint8_t)byte;
 }
 
-// The image of codes and scales that are on the device; one wave per (tile, unit).  Rows and columns past the end:
+// The image of codes and scales that are on the device: of a weight, and of quantized rows in each product of more than 16
+// (2048 of 4096 -> 4096 28.2 us the call, 29.4 with x to be quantized); one wave per (tile, unit).  Rows and columns past the end:
 // zeros.  bad (start: all ones; null: not asked): the lowest index of a scale byte over 252.
 __global__ __launch_bounds__(256) void mx_repack_kernel(const uint8_t *codes, const uint8_t *scales, int64_t n, int64_t k,
                                                         int64_t units, int64_t jobs, uint8_t *image, unsigned long long *bad) {

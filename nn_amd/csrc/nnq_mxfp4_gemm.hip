@@ -9,12 +9,14 @@
 // Measured (MI355X, in a graph over copies of the weight that pass the Infinity Cache; the library's bf16 product of 8192^3
 // reaches 1.14 PFLOP/s; the MFMAs alone from registers, on random data, 1.61 in bf16 and 6.4 in 4 bits):
 //  * 512 bf16 rows of 4096 -> 12288 46 to 51 us, 1.0 to 1.1 PFLOP/s; 2048 rows 172 us, 1.2: bound by the MFMAs at the clock that
-//    they leave.  300 f32 rows cost three times as much.
-//  * 2048 rows of 4096 -> 24576 in 4 bits 104 to 113 us with 7 of quantization, 3.7 to 3.9 PFLOP/s.  Variants that leave work
-//    out say what of the kernel's 103: the MFMAs alone 60, with the LDS reads 65, the copies of A 72, the loads of B 91, the
-//    stores 103.  The loads are 98 KB a stage and CU, 85% of what its L1 delivers beside the MFMAs.  One wave a SIMD with
-//    256 rows a workgroup (122 us) or 256 x 256 and both operands through LDS (126), a third buffer (112) and eight waves
-//    that share A (115 / 115) were no faster.
+//    they leave.  f32 rows take three MFMAs for one: 512 of them 120 to 130 us, 1.2 PFLOP/s of MFMAs, 2048 469.
+//  * 2048 rows of 4096 -> 24576 in 4 bits 104 to 113 us with 7 of quantization, 3.7 to 3.9 PFLOP/s (125 to 129 in
+//    graphs of three such calls in later runs).  Variants that leave work out say what of the kernel's 103: the MFMAs alone 60, with
+//    the LDS reads 65, the copies of A 72, the loads of B 91, the stores 103.  Counters: L1's address unit busy 83% of the
+//    cycles, its data return 96%, the matrix pipe 50%, one 64-byte access in 46%: the loads' path, or what two waves a SIMD hide of
+//    it.  256 x 256 outputs a CU with both operands through LDS have a third less loads, but one wave a SIMD (126 us), so they
+//    do not tell these apart; 256 rows with the weights in registers (122), a third buffer (112) and eight waves that share A
+//    (115 / 115) were no faster.
 //  * 301 f32 rows of 2880 -> 5751 in 4 bits 18 us: latency of two launches, 12 stages and the first loads.
 #include <algorithm>
 #include <type_traits>

@@ -133,7 +133,10 @@ int64_t int4_chunk_rows(int64_t m, int64_t k) {
 // ---- MXFP4 rows ----
 
 // Up to 16 rows the kernel for rows, unless over eight rows and many tiles K would go over workgroups (us, rows / GEMM: 16
-// bf16 rows of 4096 -> 24576 22.9 / 19.0, 12 f32 rows of 2048 -> 151936 99 / 69; 16 of 12288 -> 4096 16.1 / 17.6).
+// bf16 rows of 4096 -> 24576 21.7 / 20.0, 16 f32 rows of 4096 -> 151936 184 / 111; 16 bf16 of 12288 -> 4096 14.5 / 16.8, 9 f32 of
+// 1024 -> 24576 10.3 / 14.4).  Over 170 shapes of 9 to 16 rows, K of 1024 to 12288 and n of 4096 to 151936, this takes 0.2% more
+// than the better of both in the mean for products of 4-bit operands (at most 5%), 5% for bf16 x (25%: 16 x 1024 -> 50304
+// 12.6 / 10.1) and 7% for f32 x (48%: 12 x 1024 -> 151936 52 / 35, and the other way 31%: 9 x 4096 -> 8192 13.7 / 18.0).
 bool mx_takes_rows(int64_t m, int64_t n, int64_t k, int x_kind) {
     return m <= 8 || (m <= kMxRows && (mx_tiles(n) <= 256 || mx_rows_plan(m, n, k, x_kind).ks == 1));
 }
@@ -144,8 +147,11 @@ static int64_t mx_stage_bytes(int64_t m, int64_t pairs, int x_kind) {
     return m * (x_kind == kMxF32 ? 3 : 1) * (pairs * 512 + 16);
 }
 
-// The most values of x that every workgroup quantizes for itself; beyond, a launch before costs less (us, in the call /
-// before: 8 bf16 rows of 12288 -> 4096 12.6 / 12.7, of 4096 -> 4096 6.4 / 8.2; 8 f32 rows of 4096 -> 4096 12.6 / 8.7).
+// The most values of x that every workgroup quantizes for itself; beyond, a launch before costs less.  us, in the call /
+// before, -> 4096: bf16 rows 4 x 8192 8.4 / 10.1, 8 x 8192 9.9 / 11.2, 12 x 8192 11.4 / 11.7, 8 x 12288 12.4 / 13.1; 16 x 8192 12.4 /
+// 12.0, 12 x 12288 14.4 / 13.8, 8 x 24576 21.0 / 20.4, 16 x 12288 16.1 / 14.5.  f32 rows 2 x 4096 6.3 / 7.1, 8 x 2048 6.9 / 7.0, 4 x
+// 4096 7.6 / 8.2, 2 x 8192 8.9 / 9.8; 2 x 12288 12.0 / 12.1, 8 x 4096 10.1 / 8.7, 4 x 8192 11.7 / 10.6, 8 x 12288 21.1 / 12.8.
+// (n of 16384 moves the change to half of that, n of 1024 hardly.)
 constexpr int64_t kMxFirstBf16 = 98304, kMxFirstF32 = 16384;
 
 // A wave along K for every two pairs of units (up to 16: three or four pairs), as many more along the tiles as make four
@@ -288,7 +294,7 @@ const char *reorder_geometry(int64_t slots, int64_t slot_stride, int ndim, const
     int64_t span = elem;
     for (int i = 0; i <= n; i++) {
         if (all[i].size <= 1) continue;
-        if (all[i].stride < span) return "elements that overlap";
+        if (all[i].stride < span) return "elements that overlap or interleave";
         if (__builtin_mul_overflow(all[i].stride, all[i].size - 1, &all[i].size) || __builtin_add_overflow(span, all[i].size, &span))
             return "a span beyond 2^63 bytes";
     }
