@@ -363,8 +363,9 @@ int nnq_beam_select(const void *logits, nnq_dtype dtype, int64_t batch, int64_t 
  * dimension has stride slot_stride, the other ndim (up to 8) sizes[] and strides[], all in elements of elem_bytes; e.g.
  * the used part of a cache.  Bytes between the elements are neither read nor written.  Elements of one tensor that
  * overlap, or strides that do not each cover what the smaller ones span, are NNQ_ERR_INVALID_ARGUMENT (tensors that overlap
- * one another or parents are the caller's to avoid), more than four dimensions that do not follow one another NNQ_ERR_UNSUPPORTED.  beams from 1 to 32.  Only slots that move are
- * read and written.  With n_states = 0 the geometry is checked and nothing else happens. */
+ * one another or parents are the caller's to avoid), more than four dimensions that do not follow one another
+ * NNQ_ERR_UNSUPPORTED.  beams from 1 to 32.  Only slots that move are read and written.  With n_states = 0 the geometry is
+ * checked and nothing else happens. */
 int nnq_beam_reorder(void *const *states, int64_t n_states, int64_t batch, int64_t beams, int64_t slot_stride, int ndim,
                      const int64_t *sizes, const int64_t *strides, int64_t elem_bytes, const int64_t *parents, void *stream);
 

@@ -322,8 +322,9 @@ MxGemmPlan mx_gemm_plan(int64_t m, int64_t n, int64_t k, int x_kind);
 bool mx_takes_rows(int64_t m, int64_t n, int64_t k, int x_kind);  // or launch_mx_gemm
 int64_t mx_chunk_rows(int64_t m, int64_t k);
 // Byte of column col of unit u of row `row` in a bf16 plane of m rows of k, without the unit (its bytes and the plane's are the
-// instruction's scalar offset, which a buffer's range check may leave out): for rows and columns that do not exist a place
-// outside every buffer, so that no more than the planes is read whatever the check counts.
+// instruction's scalar offset): for rows and columns that do not exist a place outside every buffer, so that no more than the
+// planes is read whether or not a buffer's range check counts the scalar offset (LLVM documents it as not counted; MI355X
+// counts it, measured).
 constexpr int kMxNowhere = 0x7FFFFFF0;
 constexpr int mx_x_offset(int row, int m, int k, int u, int col) {
     return row < m && u * kMxUnit + col < k ? (row * k + col) * 2 : kMxNowhere;

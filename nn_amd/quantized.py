@@ -799,11 +799,11 @@ def beam_reorder(states, parents: torch.Tensor, dim: int = 0) -> None:
     b * beams + parents[b, j], in place, whatever the parents are (all reads come before the writes).
 
     states: a device tensor or several on one device, of any dtypes, which must overlap neither one another nor parents;
-    strided ones are written where they lie, so ``cache[..., :used, :]`` moves the used part only.  The move has no gradient: where
+    strided ones are written where they lie, so ``cache[..., :used, :]`` moves the used part only.  parents: integers
+    [batch, beams] or [beams] (beams up to 32) on that device; a slot whose parent is itself, or outside [0, beams) as the -1
+    of ``beam_select``, stays as it is, and only slots that move are read and written.  The move has no gradient: where
     gradients are recorded a state that requires one is refused, and a backward pass over a state saved before raises, as
-    after torch's own writes in place.  parents: integers [batch, beams] or [beams] (beams
-    up to 32) on that device; a slot whose parent is itself, or outside [0, beams) as the -1 of ``beam_select``, stays as it
-    is, and only slots that move are read and written.  No host synchronisation."""
+    after torch's own writes in place.  No host synchronisation."""
     states = [states] if isinstance(states, torch.Tensor) else list(states)
     if not isinstance(parents, torch.Tensor) or parents.dim() not in (1, 2):
         raise ShapeMismatch("parents must be a tensor [batch, beams] or [beams]")

@@ -60,7 +60,7 @@ def test_every_built_form_is_some_shapes(lib):
 @pytest.mark.parametrize("planes", [1, 3])
 def test_copies_of_x_stay_in_its_planes(lib, planes):
     """The GEMM with bf16 operands copies 16 bytes at (offset of a lane) + (plane and unit, a scalar offset).  A buffer's range
-    check is only sure to count the lane's offset, so that one has to keep every copy in the planes by itself: of all rows of
+    check is only documented to count the lane's offset, so that one has to keep every copy in the planes by itself: of all rows of
     the last row block, those past m too, and all columns of a unit that K ends in."""
     lib.nnq_rule_mx_x_offset.argtypes = [ctypes.c_int] * 5
     rng = random.Random(planes)
